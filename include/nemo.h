@@ -248,6 +248,152 @@ nemo_status nemo_dequantize(int32_t ggml_type, const void* d_raw, int64_t n_valu
 nemo_status nemo_probe_stream(const void* d_src, size_t bytes, int32_t loads_per_thread, uint32_t* d_sink,
                               void* stream);
 
+/* ---- attention block operators -------------------------------------------
+ * The reference has these only inside its encoder pass (src/webgpu/ops.ts:21-56,
+ * 168-362), in one form each; here they are operators on device buffers of
+ * any layout, for callers that build a layer from nemo_weight_matmul and
+ * these. All are enqueued on `stream` (NULL: the default stream) and return;
+ * nothing is allocated, so they can be captured into a HIP graph after one
+ * eager call of the same kind. Strides count elements. */
+
+#define NEMO_TYPE_I8 24        /* GGML's code */
+#define NEMO_TYPE_BF16 30      /* GGML's code */
+#define NEMO_TYPE_F8_E4M3 259  /* 8-bit floats, largest 448; not a GGML type code */
+
+/* Rotary positions. A head's first rotary_dim values are r / 2 pairs, pair i
+ * of which is turned by the angle position * f_i and scaled by `magnitude`:
+ *   (a, b) -> m (a cos - b sin, a sin + b cos).
+ * The head's other values are copied. f_i = theta^(-2i / r), and then by
+ * `scaling`: LINEAR f_i / factor; YARN f_i / factor for pairs that turn less
+ * than beta_slow times in original_positions, f_i for those that turn more
+ * than beta_fast times, a linear ramp over the pair index between (the
+ * table of src/webgpu/model.ts:95-106 is YARN with factor 16, 16384, 32, 1,
+ * interleaved, magnitude 1); BANDS f_i / factor for wavelengths longer than
+ * original_positions / low_band, f_i for those shorter than
+ * original_positions / high_band, between them linear in the number of
+ * turns. */
+#define NEMO_ROPE_INTERLEAVED 0 /* pair i: values 2i and 2i + 1 */
+#define NEMO_ROPE_HALF 1        /* pair i: values i and i + r / 2 */
+#define NEMO_ROPE_NONE 0
+#define NEMO_ROPE_LINEAR 1
+#define NEMO_ROPE_YARN 2
+#define NEMO_ROPE_BANDS 3
+
+typedef struct nemo_rope nemo_rope;
+typedef struct nemo_rope_config {
+  int32_t head_dim;           /* 2..1024, even */
+  int32_t rotary_dim;         /* 2..head_dim, even; 0: head_dim */
+  int32_t layout;             /* NEMO_ROPE_INTERLEAVED or _HALF */
+  int32_t scaling;            /* NEMO_ROPE_NONE.._BANDS */
+  double theta;               /* > 1 */
+  double factor;              /* > 0; LINEAR, YARN, BANDS */
+  int32_t original_positions; /* >= 1; YARN, BANDS */
+  double beta_fast, beta_slow; /* YARN: beta_fast >= beta_slow > 0 */
+  double low_band, high_band;  /* BANDS: high_band > low_band > 0 */
+  double magnitude;            /* 0: 1, for YARN 0.1 ln(factor) + 1 (factor > 1) */
+} nemo_rope_config;
+
+/* head_dim 128, whole heads, interleaved, theta 1e6, no scaling (its factor
+ * 1, 16384 positions, betas 32 and 1, bands 1 and 4), magnitude 0. */
+void nemo_rope_config_default(nemo_rope_config* out);
+
+/* The frequencies are computed in 64 bits on the host and held on the
+ * context's device. */
+nemo_status nemo_rope_create(nemo_ctx* ctx, const nemo_rope_config* config, nemo_rope** out);
+/* Waits for the device, then frees it. */
+nemo_status nemo_rope_destroy(nemo_rope* rope);
+
+/* `heads` heads of each row: head h of row t starts at x + t x_row + h x_head
+ * and goes to y + t y_row + h y_head. y may be x with the same strides (the
+ * heads are turned in place); other overlap of an input and an output is not
+ * allowed. */
+typedef struct nemo_rope_heads {
+  const void* x;
+  void* y;
+  int64_t x_row, x_head, y_row, y_head;
+  int32_t heads;
+} nemo_rope_heads;
+
+/* Turn the heads of `rows` tokens, `type` F32, F16 or BF16 (arithmetic in 32
+ * bits, one rounding), of q and, unless it is NULL, of k in the same launch.
+ * Row t has position base + d_positions[t] (device; NULL: base + t). Angles
+ * are position * f_i in 64 bits, reduced there: their error is about 2^-53 of
+ * the angle. Negative positions turn back. */
+nemo_status nemo_rope_apply(nemo_rope* rope, int32_t type, const nemo_rope_heads* q, const nemo_rope_heads* k,
+                            int64_t rows, const int64_t* d_positions, int64_t base, void* stream);
+
+/* Attention with a sliding window and sinks. Request b has query rows
+ * q_start[b] .. q_start[b + 1] - 1 of q and out and kv_len[b] key and value rows
+ * from kv_start[b] on. Its queries are its last positions: query i of n stands at
+ * p = kv_len - n + i, and sees key j when
+ *   j <= p + right  and  (j >= p - left  or  j < sinks)
+ * (left or right -1: no bound on that side; right 0 is causal). out = softmax(scale q.k) v
+ * over the keys it sees, 0 when it sees none. Query head h reads key and
+ * value head h / (q_heads / kv_heads). Keys and values that no query of a
+ * request sees may hold anything, NaN included; one that some queries see
+ * reaches no other query's result. Softmax sums and the output are
+ * accumulated in 32 bits; the probabilities are rounded to `type` for the
+ * product with v. */
+typedef struct nemo_attention_config {
+  int32_t q_heads, kv_heads; /* q_heads a multiple of kv_heads, at most 1024 */
+  int32_t head_dim;          /* 64 or 128 */
+  int32_t type;              /* F16 or BF16 */
+  int32_t left, right;       /* >= 0, or -1: unbounded */
+  int32_t sinks;             /* >= 0 */
+  float scale;               /* > 0, or 0: head_dim^-1/2 */
+} nemo_attention_config;
+
+/* Buffers are 16-byte aligned, strides multiples of 8. The index arrays are
+ * read on the device when the work runs (a captured graph may be replayed
+ * with other lengths); entries outside the buffers are cut to q_rows and
+ * kv_rows. Rows of `out` that belong to no request are left as they were. */
+typedef struct nemo_attention_batch {
+  int32_t count;             /* requests */
+  int64_t q_rows, kv_rows;   /* rows of q and out, of k and v */
+  int64_t max_kv;            /* the longest kv_len, or more: a hint for the split of the keys over the chip */
+  const int32_t* q_start;    /* device [count + 1], ascending */
+  const int64_t* kv_start;   /* device [count] */
+  const int32_t* kv_len;     /* device [count] */
+  const void *q, *k, *v;
+  void* out;
+  int64_t q_row, q_head, k_row, k_head, v_row, v_head, out_row, out_head;
+  void* workspace;           /* device, 16-byte aligned; NULL: the keys of a query are not split */
+  size_t workspace_bytes;    /* at least nemo_window_attention_workspace's when workspace is given */
+} nemo_attention_batch;
+
+/* Bytes of workspace for a batch of these sizes (0: none is used). Its
+ * content carries nothing from one call to the next; calls that may overlap,
+ * graphs among them, need one each. */
+nemo_status nemo_window_attention_workspace(const nemo_attention_config* config, int32_t count, int64_t q_rows,
+                                            int64_t max_kv, size_t* bytes);
+nemo_status nemo_window_attention(nemo_ctx* ctx, const nemo_attention_config* config,
+                                  const nemo_attention_batch* batch, void* stream);
+
+/* Residual addition, RMSNorm and 8-bit output in one pass, for each row:
+ *   h = x + delta,  y = h / sqrt(mean(h^2) + epsilon) * weight
+ * in 32 bits from the unrounded h; sum = h and y in `type`; and
+ *   scales = max |y| / 127 (I8) or / 448 (F8_E4M3), y8 = round(y / scale)
+ * of the unrounded y over a whole row or over each `group` columns (scale 0,
+ * and y8 0, where y is 0; NaN where y holds a NaN; to even on ties). */
+typedef struct nemo_norm_args {
+  int32_t type;              /* of x, delta, sum, y: F32, F16 or BF16 */
+  int32_t hidden;            /* >= 1 */
+  int64_t rows;
+  const void* x;
+  const void* delta;         /* NULL: h = x */
+  const float* weight;       /* [hidden]; NULL: 1 */
+  void* sum;                 /* NULL: not written; may be x or delta */
+  void* y;                   /* NULL: not written; may be x or delta */
+  void* y8;                  /* NULL: not written */
+  float* scales;             /* rows of 1, or of hidden / group; with y8 */
+  int64_t x_row, delta_row, sum_row, y_row, y8_row, scales_row;
+  int32_t type8;             /* I8 or F8_E4M3, with y8 */
+  int32_t group;             /* 0 (a row), 32, 64 or 128, which divides hidden */
+  float epsilon;             /* >= 0 */
+} nemo_norm_args;
+
+nemo_status nemo_rmsnorm(nemo_ctx* ctx, const nemo_norm_args* args, void* stream);
+
 /* ---- offline requantization (src/gguf/quantization.ts:77-131) ------------ */
 
 /* requantizeMatrixToQ40 (src/gguf/quantization.ts:101-131) on the GPU: the

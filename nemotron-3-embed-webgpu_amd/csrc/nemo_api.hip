@@ -16,6 +16,7 @@
 
 #include "../../include/nemo.h"
 #include "nemo_common.h"
+#include "nemo_operators.h"
 #include "nemo_ops.h"
 #include "nemo_quant.h"
 #include "nemo_synth.h"
@@ -1429,5 +1430,196 @@ nemo_status nemo_requantize_q40(nemo_ctx* ctx, int32_t src_type, const void* src
     hip_check(launch_requant_q40(src_type, (const uint8_t*)d_src.get(), k, n, (uint8_t*)d_out.get(), nullptr),
               "requantize");
     hip_check(hipMemcpy(out, d_out.get(), need, hipMemcpyDeviceToHost), "download");
+  });
+}
+
+// ---------------------------------------------------------------------------
+// Attention block operators
+// ---------------------------------------------------------------------------
+
+struct nemo_rope {
+  nemo_ctx* ctx = nullptr;
+  DevPtr turns;
+  RopeAngles angles{};
+};
+
+// Whole turns a position of each pair (formulas at nemo_rope_config).
+static std::vector<double> rope_turns(const nemo_rope_config& c, int rotary) {
+  const double two_pi = 2 * 3.14159265358979323846;
+  const int pairs = rotary / 2;
+  auto edge = [&](double turns) { return rotary * log(c.original_positions / (turns * two_pi)) / (2 * log(c.theta)); };
+  const double lo = fmax(0.0, floor(edge(c.beta_fast))), hi = fmin(rotary - 1.0, ceil(edge(c.beta_slow)));
+  std::vector<double> v(pairs);
+  for (int i = 0; i < pairs; ++i) {
+    const double f = pow(c.theta, -2.0 * i / rotary) / two_pi;
+    double slow = 0;  // the share of f / factor
+    if (c.scaling == NEMO_ROPE_LINEAR) slow = 1;
+    if (c.scaling == NEMO_ROPE_YARN) slow = fmin(1.0, fmax(0.0, (i - lo) / fmax(0.001, hi - lo)));
+    if (c.scaling == NEMO_ROPE_BANDS)
+      slow = 1 - fmin(1.0, fmax(0.0, (c.original_positions * f - c.low_band) / (c.high_band - c.low_band)));
+    v[i] = slow * f / c.factor + (1 - slow) * f;
+    if (slow == 0) v[i] = f;
+  }
+  return v;
+}
+
+static void validate_rope(const nemo_rope_config& c) {
+  if (c.head_dim < 2 || c.head_dim > 1024 || c.head_dim % 2)
+    fail(NEMO_ERR_INVALID, "rope head_dim must be even and in [2, 1024]");
+  if (c.rotary_dim < 0 || c.rotary_dim > c.head_dim || c.rotary_dim % 2)
+    fail(NEMO_ERR_INVALID, "rotary_dim must be even and in [0, head_dim]");
+  if (c.layout != NEMO_ROPE_INTERLEAVED && c.layout != NEMO_ROPE_HALF) fail(NEMO_ERR_INVALID, "unknown rope layout");
+  if (c.scaling < NEMO_ROPE_NONE || c.scaling > NEMO_ROPE_BANDS) fail(NEMO_ERR_INVALID, "unknown rope scaling");
+  if (!(c.theta > 1) || !isfinite(c.theta)) fail(NEMO_ERR_INVALID, "rope theta must be finite and above 1");
+  if (c.scaling != NEMO_ROPE_NONE && (!(c.factor > 0) || !isfinite(c.factor)))
+    fail(NEMO_ERR_INVALID, "rope factor must be finite and positive");
+  if (c.scaling >= NEMO_ROPE_YARN && c.original_positions < 1)
+    fail(NEMO_ERR_INVALID, "rope original_positions must be positive");
+  if (c.scaling == NEMO_ROPE_YARN && !(c.beta_slow > 0 && c.beta_fast >= c.beta_slow && isfinite(c.beta_fast)))
+    fail(NEMO_ERR_INVALID, "rope betas must be positive, beta_fast at least beta_slow");
+  if (c.scaling == NEMO_ROPE_BANDS && !(c.low_band > 0 && c.high_band > c.low_band && isfinite(c.high_band)))
+    fail(NEMO_ERR_INVALID, "rope bands must be positive, high_band above low_band");
+  if (!isfinite(c.magnitude)) fail(NEMO_ERR_INVALID, "rope magnitude must be finite");
+}
+
+void nemo_rope_config_default(nemo_rope_config* out) {
+  if (!out) return;
+  *out = nemo_rope_config{128, 0, NEMO_ROPE_INTERLEAVED, NEMO_ROPE_NONE, 1e6, 1.0, 16384, 32.0, 1.0, 1.0, 4.0, 0.0};
+}
+
+nemo_status nemo_rope_create(nemo_ctx* ctx, const nemo_rope_config* config, nemo_rope** out) {
+  return guarded([&] {
+    if (!ctx || !config || !out) fail(NEMO_ERR_INVALID, "null argument");
+    const nemo_rope_config& c = *config;
+    validate_rope(c);
+    set_device(ctx);
+    auto r = std::make_unique<nemo_rope>();
+    r->ctx = ctx;
+    r->angles.head_dim = c.head_dim;
+    r->angles.rotary = c.rotary_dim ? c.rotary_dim : c.head_dim;
+    r->angles.half = c.layout == NEMO_ROPE_HALF;
+    const double yarn = c.scaling == NEMO_ROPE_YARN && c.factor > 1 ? 0.1 * log(c.factor) + 1 : 1.0;
+    r->angles.magnitude = (float)(c.magnitude != 0 ? c.magnitude : yarn);
+    const std::vector<double> turns = rope_turns(c, r->angles.rotary);
+    r->turns = dev_alloc(turns.size() * 8, "rope frequencies");
+    hip_check(hipMemcpy(r->turns.get(), turns.data(), turns.size() * 8, hipMemcpyHostToDevice), "upload");
+    r->angles.turns = (const double*)r->turns.get();
+    *out = r.release();
+  });
+}
+
+nemo_status nemo_rope_destroy(nemo_rope* rope) {
+  return guarded([&] {
+    if (!rope) return;
+    set_device(rope->ctx);
+    hip_check(hipDeviceSynchronize(), "sync");
+    delete rope;
+  });
+}
+
+// Largest stride, in elements, and largest numbers of rows: they keep every
+// offset within 63 bits, a tile's within 31, and grids within 2^32 threads.
+constexpr int64_t kMaxStride = 1 << 23, kMaxRows = 1 << 23, kMaxKeys = 1 << 30, kMaxQueries = 1 << 26;
+
+static void validate_stride(int64_t v, const char* what) {
+  if (v < 0 || v > kMaxStride) fail(NEMO_ERR_INVALID, std::string(what) + " must be in [0, 2^23]");
+}
+
+static void validate_rope_heads(const nemo_rope_heads& s) {
+  if (s.heads < 0 || s.heads > 65536) fail(NEMO_ERR_INVALID, "rope heads must be in [0, 65536]");
+  if (s.heads && (!s.x || !s.y)) fail(NEMO_ERR_INVALID, "null argument");
+  for (int64_t v : {s.x_row, s.x_head, s.y_row, s.y_head}) validate_stride(v, "rope strides");
+}
+
+nemo_status nemo_rope_apply(nemo_rope* rope, int32_t type, const nemo_rope_heads* q, const nemo_rope_heads* k,
+                            int64_t rows, const int64_t* d_positions, int64_t base, void* stream) {
+  return guarded([&] {
+    if (!rope || !q) fail(NEMO_ERR_INVALID, "null argument");
+    if (type != kF32 && type != kF16 && type != NEMO_TYPE_BF16)
+      fail(NEMO_ERR_UNSUPPORTED, "rope takes F32, F16 or BF16");
+    if (rows < 0 || rows > kMaxRows) fail(NEMO_ERR_INVALID, "rows must be in [0, 2^23]");
+    validate_rope_heads(*q);
+    if (k) validate_rope_heads(*k);
+    set_device(rope->ctx);
+    hip_check(launch_rope_apply(rope->angles, type, *q, k, rows, d_positions, base, (hipStream_t)stream), "rope");
+  });
+}
+
+static void validate_attention(const nemo_attention_config& c) {
+  if (c.q_heads < 1 || c.q_heads > 1024 || c.kv_heads < 1 || c.q_heads % c.kv_heads)
+    fail(NEMO_ERR_INVALID, "q_heads must be a positive multiple of kv_heads, at most 1024");
+  if (c.head_dim != 64 && c.head_dim != 128) fail(NEMO_ERR_UNSUPPORTED, "head_dim must be 64 or 128");
+  if (c.type != kF16 && c.type != NEMO_TYPE_BF16) fail(NEMO_ERR_UNSUPPORTED, "attention takes F16 or BF16");
+  if (c.left < -1 || c.right < -1 || c.sinks < 0)
+    fail(NEMO_ERR_INVALID, "left and right must be -1 or more, sinks 0 or more");
+  if (!(c.scale >= 0) || !isfinite(c.scale)) fail(NEMO_ERR_INVALID, "scale must be finite and 0 or more");
+}
+
+static void validate_attention_sizes(const nemo_attention_config& c, int32_t count, int64_t q_rows, int64_t max_kv) {
+  if (count < 0 || count > (1 << 20)) fail(NEMO_ERR_INVALID, "count must be in [0, 2^20]");
+  if (q_rows < 0 || q_rows > kMaxQueries / c.q_heads)
+    fail(NEMO_ERR_INVALID, "q_rows times q_heads must be in [0, 2^26]");
+  if (max_kv < 0) fail(NEMO_ERR_INVALID, "max_kv must be 0 or more");
+}
+
+nemo_status nemo_window_attention_workspace(const nemo_attention_config* config, int32_t count, int64_t q_rows,
+                                            int64_t max_kv, size_t* bytes) {
+  return guarded([&] {
+    if (!config || !bytes) fail(NEMO_ERR_INVALID, "null argument");
+    validate_attention(*config);
+    validate_attention_sizes(*config, count, q_rows, max_kv);
+    *bytes = window_workspace(*config, count, q_rows, max_kv);
+  });
+}
+
+nemo_status nemo_window_attention(nemo_ctx* ctx, const nemo_attention_config* config,
+                                  const nemo_attention_batch* batch, void* stream) {
+  return guarded([&] {
+    if (!ctx || !config || !batch) fail(NEMO_ERR_INVALID, "null argument");
+    const nemo_attention_batch& b = *batch;
+    validate_attention(*config);
+    validate_attention_sizes(*config, b.count, b.q_rows, b.max_kv);
+    if (b.kv_rows < 0 || b.kv_rows > kMaxKeys) fail(NEMO_ERR_INVALID, "kv_rows must be in [0, 2^30]");
+    if (b.count == 0 || b.q_rows == 0) return;
+    if (!b.q_start || !b.kv_start || !b.kv_len || !b.q || !b.out || (b.kv_rows && (!b.k || !b.v)))
+      fail(NEMO_ERR_INVALID, "null argument");
+    for (int64_t v : {b.q_row, b.q_head, b.k_row, b.k_head, b.v_row, b.v_head, b.out_row, b.out_head}) {
+      validate_stride(v, "attention strides");
+      if (v % 8) fail(NEMO_ERR_INVALID, "attention strides must be multiples of 8");
+    }
+    for (const void* p : {b.q, b.k, b.v, (const void*)b.out, (const void*)b.workspace})
+      if ((uintptr_t)p & 15) fail(NEMO_ERR_INVALID, "attention buffers must be 16-byte aligned");
+    const size_t need = b.workspace ? window_workspace(*config, b.count, b.q_rows, b.max_kv) : 0;
+    if (b.workspace && b.workspace_bytes < need)
+      fail(NEMO_ERR_INVALID, "workspace has " + std::to_string(b.workspace_bytes) + " bytes; this batch needs " +
+                                 std::to_string(need));
+    set_device(ctx);
+    hip_check(launch_window_attention(*config, b, (hipStream_t)stream), "window attention");
+  });
+}
+
+nemo_status nemo_rmsnorm(nemo_ctx* ctx, const nemo_norm_args* args, void* stream) {
+  return guarded([&] {
+    if (!ctx || !args) fail(NEMO_ERR_INVALID, "null argument");
+    const nemo_norm_args& a = *args;
+    if (a.type != kF32 && a.type != kF16 && a.type != NEMO_TYPE_BF16)
+      fail(NEMO_ERR_UNSUPPORTED, "the norm takes F32, F16 or BF16");
+    if (a.hidden < 1) fail(NEMO_ERR_INVALID, "hidden must be positive");
+    if (a.rows < 0 || a.rows > kMaxRows) fail(NEMO_ERR_INVALID, "rows must be in [0, 2^23]");
+    if (!(a.epsilon >= 0) || !isfinite(a.epsilon)) fail(NEMO_ERR_INVALID, "epsilon must be finite and 0 or more");
+    for (int64_t v : {a.x_row, a.delta_row, a.sum_row, a.y_row, a.y8_row, a.scales_row})
+      validate_stride(v, "norm strides");
+    if (a.y8) {
+      if (a.type8 != NEMO_TYPE_I8 && a.type8 != NEMO_TYPE_F8_E4M3)
+        fail(NEMO_ERR_UNSUPPORTED, "the 8-bit output is I8 or F8_E4M3");
+      if (a.group != 0 && a.group != 32 && a.group != 64 && a.group != 128)
+        fail(NEMO_ERR_INVALID, "group must be 0, 32, 64 or 128");
+      if (a.group && a.hidden % a.group) fail(NEMO_ERR_INVALID, "group must divide hidden");
+      if (!a.scales) fail(NEMO_ERR_INVALID, "8-bit output needs scales");
+    }
+    if (a.rows == 0) return;
+    if (!a.x || (!a.sum && !a.y && !a.y8)) fail(NEMO_ERR_INVALID, "null argument");
+    set_device(ctx);
+    hip_check(launch_norm8(a, (hipStream_t)stream), "rmsnorm");
   });
 }
