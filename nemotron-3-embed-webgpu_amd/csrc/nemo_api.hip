@@ -1556,7 +1556,8 @@ static void validate_attention(const nemo_attention_config& c) {
 }
 
 static void validate_attention_sizes(const nemo_attention_config& c, int32_t count, int64_t q_rows, int64_t max_kv) {
-  if (count < 0 || count > (1 << 20)) fail(NEMO_ERR_INVALID, "count must be in [0, 2^20]");
+  if (count < 0 || count > (1 << 20) || (int64_t)count * c.kv_heads > (1 << 22))
+    fail(NEMO_ERR_INVALID, "count must be in [0, 2^20], count times kv_heads at most 2^22");
   if (q_rows < 0 || q_rows > kMaxQueries / c.q_heads)
     fail(NEMO_ERR_INVALID, "q_rows times q_heads must be in [0, 2^26]");
   if (max_kv < 0) fail(NEMO_ERR_INVALID, "max_kv must be 0 or more");

@@ -1,6 +1,17 @@
 // Attention with a sliding window and sinks for gfx950 (include/nemo.h
 // nemo_window_attention): softmax(scale q.k) v over the keys j <= p + right
 // that have j >= p - left or j < sinks.
+//
+// Rows are (query, head of the group) pairs of one request and KV head, query
+// by query, so 32 rows fill an MFMA operand whatever the group and the number
+// of queries. A tile of rows attends a list of N key slots: the sinks before
+// its first window key, then the keys of its rows' windows together; no other
+// key is read. Scores are taken transposed, S^T = K Q^T (32 keys x 32 rows per
+// v_mfma_f32_32x32x16), so a lane holds one row, its softmax is per-lane
+// arithmetic in fp32, and its score registers are the B operand of O^T = V^T
+// P^T: the MFMA's k slots of a 16-key chunk are taken in the order that the
+// score registers have. K and V go row-major into LDS by DMA; K fragments are
+// 16-byte reads, V^T fragments transposed reads (ds_read_b64_tr_b16).
 #include <algorithm>
 
 #include "nemo_operators.h"
@@ -11,7 +22,7 @@ namespace {
 
 struct WindowArgs {
   nemo_attention_batch b;
-  int group, left, right, sinks;
+  int kv_heads, group, left, right, sinks;
   float scale2;  // of the scores, in units of log2
 };
 
@@ -85,28 +96,346 @@ struct OneRow {
       }
     }
   }
+  __device__ __forceinline__ void store(T* out) const {
+    for (int i = 0; i < HD / 64; ++i) out[(threadIdx.x & 63) + 64 * i] = (T)(l == 0.f ? 0.f : o[i] / l);
+  }
 };
 
-// One wave a (query, head) row.
+// ---------------------------------------------------------------------------
+// Fragments
+// ---------------------------------------------------------------------------
+
+typedef short short4v __attribute__((ext_vector_type(4)));
+typedef short short8v __attribute__((ext_vector_type(8)));
+typedef bf16_t bf16x8 __attribute__((ext_vector_type(8)));
+typedef float float8v __attribute__((ext_vector_type(8)));
+typedef __attribute__((address_space(3))) void lds_void;
+typedef __attribute__((address_space(3))) short4v lds_short4v;
+
+template <typename T>
+struct Mma;
+template <>
+struct Mma<half_t> {
+  typedef half8v frag;
+  static __device__ __forceinline__ float16v mma(frag a, frag b, float16v c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+  }
+};
+template <>
+struct Mma<bf16_t> {
+  typedef bf16x8 frag;
+  static __device__ __forceinline__ float16v mma(frag a, frag b, float16v c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+  }
+};
+
+// LDS images of 32 keys, row-major, HD / 8 chunks of 16 bytes a row, chunk c of
+// row r at c ^ swizzle: K's spreads the 32 rows that a fragment read touches
+// over the banks, V's the four rows of 64 bytes of a transposed read.
+constexpr int kKeys = 32;
+template <int HD>
+__device__ __forceinline__ int k_swizzle(int row) {
+  return HD == 128 ? row & 15 : (row & 7) ^ ((row >> 3) & 1);
+}
+template <int HD>
+__device__ __forceinline__ int v_swizzle(int row) {
+  return HD == 128 ? 4 * (row & 3) : 4 * ((row >> 1) & 1);
+}
+
+// Copies of ROWS key rows into an image by one wave, 1 KB an instruction:
+// rows first .. first + ROWS of a 32-row image (or of two that follow each
+// other). lane_off: the lane's byte offsets from the address of slot row 0 of
+// the image, for rows that lie `stride` bytes apart.
+template <int HD, int ROWS, bool VALUES>
+struct Stager {
+  static constexpr int kChunks = HD / 8, kPer = 64 / kChunks, kN = ROWS / kPer;
+  uint32_t off[kN];
+  int row, chunk[kN];
+  __device__ __forceinline__ Stager(int first, int64_t stride) {
+    const int lane = threadIdx.x & 63;
+    row = first + lane / kChunks;
+#pragma unroll
+    for (int i = 0; i < kN; ++i) {
+      const int r = row + kPer * i;
+      chunk[i] = 16 * ((lane % kChunks) ^ (VALUES ? v_swizzle<HD>(r) : k_swizzle<HD>(r)));
+      off[i] = (uint32_t)(r * stride) + chunk[i];
+    }
+  }
+  // Slots t0 .. of the list, all of them window keys: consecutive rows from `at`.
+  __device__ __forceinline__ void rows(const uint8_t* at, uint8_t* image) const {
+#pragma unroll
+    for (int i = 0; i < kN; ++i)
+      __builtin_amdgcn_global_load_lds((const void*)(at + off[i]), (lds_void*)(image + 1024 * i), 16, 0, 0);
+  }
+  // Any slots: key(t) of each, the last slot's from there on.
+  template <typename Key>
+  __device__ __forceinline__ void slots(const uint8_t* base, int64_t stride, int t0, int n, Key&& key,
+                                        uint8_t* image) const {
+#pragma unroll
+    for (int i = 0; i < kN; ++i) {
+      const int64_t j = key(min(t0 + row + kPer * i, n - 1));
+      __builtin_amdgcn_global_load_lds((const void*)(base + j * stride + chunk[i]), (lds_void*)(image + 1024 * i), 16,
+                                       0, 0);
+    }
+  }
+};
+
+// The tile of 32 rows of a wave, or the larger one of a workgroup: its key
+// list, and in list coordinates what the row of a lane sees: t < hi and (t >= lo
+// or t < sinks).
+struct KeyList {
+  int sinks, lo, n;  // slots t < sinks are keys t, others lo + t - sinks
+  __device__ __forceinline__ KeyList(const WindowArgs& a, int p0, int p1, int keys) {
+    const Seen first(a, p0, keys), last(a, p1, keys);
+    lo = first.lo;
+    sinks = min(a.sinks, lo);
+    n = sinks + last.hi - lo;
+  }
+  __device__ __forceinline__ int key(int t) const { return t < sinks ? t : lo + t - sinks; }
+};
+
+// A wave's 32 rows: row l % 32 in lane l, whose half hl = l / 32 holds the
+// output columns 32 db + 8 j + 4 hl + 0..3 in registers 4j.. of o[db], and the
+// sum of its own keys' probabilities.
 template <typename T, int HD>
-__global__ __launch_bounds__(256) void window_row_kernel(WindowArgs a) {
-  constexpr int R = 4;
-  const nemo_attention_batch& b = a.b;
-  const int i = tile_request(b, a.group, R, blockIdx.x);
-  if (i < 0) return;
-  const Request r(b, i);
-  const int row = (blockIdx.x - tile_base(b, a.group, R, i)) * R + (threadIdx.x >> 6);
-  if (row >= r.queries * a.group) return;
-  const int qi = row / a.group, h = blockIdx.y * a.group + row % a.group, lane = threadIdx.x & 63;
-  const T* q = (const T*)b.q + (int64_t)(r.q0 + qi) * b.q_row + h * b.q_head;
-  const T* k = (const T*)b.k + r.kv0 * b.k_row + blockIdx.y * b.k_head;
-  const T* v = (const T*)b.v + r.kv0 * b.v_row + blockIdx.y * b.v_head;
-  T* out = (T*)b.out + (int64_t)(r.q0 + qi) * b.out_row + h * b.out_head;
-  const Seen seen(a, r.keys - r.queries + qi, r.keys);
+struct Rows {
+  static constexpr int DC = HD / 16, DB = HD / 32;
+  typedef typename Mma<T>::frag frag;
+  frag q[DC];
+  float16v o[DB];
+  float m, l;
+
+  __device__ __forceinline__ void clear() {
+    m = -INFINITY;
+    l = 0.f;
+#pragma unroll
+    for (int db = 0; db < DB; ++db)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) o[db][r] = 0.f;
+  }
+  __device__ __forceinline__ void load(const T* row, int hl) {
+#pragma unroll
+    for (int c = 0; c < DC; ++c) q[c] = *(const frag*)(row + 16 * c + 8 * hl);
+  }
+  __device__ __forceinline__ float16v scores(const uint8_t* image, int lane) const {
+    const int row = lane & 31, hl = lane >> 5, sw = k_swizzle<HD>(row);
+    float16v s = {};
+#pragma unroll
+    for (int c = 0; c < DC; ++c)
+      s = Mma<T>::mma(*(const frag*)(image + row * 2 * HD + 16 * ((2 * c + hl) ^ sw)), q[c], s);
+    return s;
+  }
+  // Probabilities against a reference maximum that is raised only when a row
+  // exceeds it by 2^8 (a wave vote): p <= 256 then, far from overflow, and
+  // most blocks need no exchange between lanes and no rescaling; numerator
+  // and denominator share the reference, so the result is the softmax. A row
+  // that has seen nothing yet has the reference 0.
+  __device__ __forceinline__ void probabilities(const float16v& s, float scale2, frag (&p)[2]) {
+    float most = s[0];
+#pragma unroll
+    for (int r = 1; r < 16; ++r) most = fmaxf(most, s[r]);
+    most *= scale2;
+    if (__builtin_amdgcn_ballot_w64(most > m + 8.0f)) {
+      asm volatile("");  // keeps the rare path a branch
+      const float mn = fmaxf(m, fmaxf(most, __shfl_xor(most, 32, 64)));
+      const float alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn);
+      l *= alpha;
+#pragma unroll
+      for (int db = 0; db < DB; ++db)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[db][r] *= alpha;
+      m = mn;
+    }
+    const float ref = m == -INFINITY ? 0.f : m;
+    float e[16];
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      e[r] = __builtin_amdgcn_exp2f(fmaf(s[r], scale2, -ref));
+      l += e[r];
+    }
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      float8v f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) f[i] = e[8 * c + i];
+      p[c] = __builtin_convertvector(f, frag);
+    }
+  }
+  // O^T += V^T P^T: k slot 8 hl + e of chunk c is key 16 c + 8 (e / 4) + 4 hl + e
+  // % 4, score register 8 c + e. A transposed read gives the 16 lanes of a
+  // group 4 keys of 16 columns; lane i of it reads key i / 4's columns 4 (i % 4)...
+  __device__ __forceinline__ void values(const uint8_t* image, int lane, const frag (&p)[2]) {
+    const int i = lane & 15, hl = lane >> 5;
+    const int key = 4 * hl + (i >> 2), half = (lane >> 4) & 1;
+#pragma unroll
+    for (int c = 0; c < 2; ++c)
+#pragma unroll
+      for (int db = 0; db < DB; ++db) {
+        const int chunk = 4 * db + 2 * half + ((i >> 1) & 1);
+        short8v a;
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const int r = 16 * c + 8 * u + key;
+          const short4v v = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+              (lds_short4v*)(image + r * 2 * HD + 16 * (chunk ^ v_swizzle<HD>(r)) + 8 * (i & 1)));
+#pragma unroll
+          for (int e = 0; e < 4; ++e) a[4 * u + e] = v[e];
+        }
+        o[db] = Mma<T>::mma(__builtin_bit_cast(frag, a), p[c], o[db]);
+      }
+  }
+  __device__ __forceinline__ void store(T* out, int hl) const {
+    typedef T vec __attribute__((ext_vector_type(4)));
+    const float inv = l == 0.f ? 0.f : 1.0f / l;
+#pragma unroll
+    for (int db = 0; db < DB; ++db)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        vec v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = (T)(o[db][4 * j + e] * inv);
+        *(vec*)(out + 32 * db + 8 * j + 4 * hl) = v;
+      }
+  }
+  // Whether a value of the lane's row is not finite.
+  __device__ __forceinline__ bool spoilt() const {
+    float z = l * 0.f;
+#pragma unroll
+    for (int db = 0; db < DB; ++db)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) z = fmaf(o[db][r], 0.f, z);
+    return z != 0.f;
+  }
+};
+
+// Scores of hidden slots of the block at t0 become -infinity.
+__device__ __forceinline__ void hide(float16v& s, int t0, int hl, int lo, int hi, int sinks) {
+#pragma unroll
+  for (int r = 0; r < 16; ++r) {
+    const int t = t0 + 8 * (r >> 2) + 4 * hl + (r & 3);
+    if (!(t < hi && (t >= lo || t < sinks))) s[r] = -INFINITY;
+  }
+}
+
+// Addresses of one request and KV head.
+template <typename T>
+struct Heads {
+  const T *q, *k, *v;
+  T* out;
+  int64_t q_row, q_head, out_row, out_head;
+  int group;
+  __device__ __forceinline__ Heads(const WindowArgs& a, const Request& r, int kvh)
+      : q_row(a.b.q_row), q_head(a.b.q_head), out_row(a.b.out_row), out_head(a.b.out_head), group(a.group) {
+    q = (const T*)a.b.q + r.q0 * q_row + (int64_t)kvh * group * q_head;
+    k = (const T*)a.b.k + r.kv0 * a.b.k_row + kvh * a.b.k_head;
+    v = (const T*)a.b.v + r.kv0 * a.b.v_row + kvh * a.b.v_head;
+    out = (T*)a.b.out + r.q0 * out_row + (int64_t)kvh * group * out_head;
+  }
+  __device__ __forceinline__ const T* query(int row) const {
+    return q + (row / group) * q_row + (row % group) * q_head;
+  }
+  __device__ __forceinline__ T* output(int row) const {
+    return out + (row / group) * out_row + (row % group) * out_head;
+  }
+};
+
+// A row over the slots [t0, t1) that it sees, key by key.
+template <typename T, int HD>
+__device__ __forceinline__ OneRow<T, HD> one_row(const WindowArgs& a, const Heads<T>& h, const KeyList& list,
+                                                 const Request& r, int row, int t0, int t1) {
+  const Seen seen(a, r.keys - r.queries + row / h.group, r.keys);
+  const int lo = seen.lo - list.lo + list.sinks, hi = seen.hi - list.lo + list.sinks, first = min(a.sinks, hi);
   OneRow<T, HD> acc;
-  acc.keys(q, k, b.k_row, v, b.v_row, 0, seen.sinks, a.scale2);
-  acc.keys(q, k, b.k_row, v, b.v_row, seen.lo, seen.hi, a.scale2);
-  for (int c = 0; c < HD / 64; ++c) out[lane + 64 * c] = (T)(acc.l == 0.f ? 0.f : acc.o[c] / acc.l);
+  acc.keys(h.query(row), h.k, a.b.k_row, h.v, a.b.v_row, t0, min(t1, first), a.scale2);
+  const int from = max(max(t0, lo), first), to = min(t1, hi);
+  if (from < to) acc.keys(h.query(row), h.k, a.b.k_row, h.v, a.b.v_row, list.key(from), list.key(to - 1) + 1, a.scale2);
+  return acc;
+}
+
+// ---------------------------------------------------------------------------
+// Many rows: a workgroup of 4 waves takes 128 rows, 32 a wave, and stages 64
+// keys a round for all of them, two rounds deep.
+// ---------------------------------------------------------------------------
+
+constexpr int kTileRows = 128;
+
+template <typename T, int HD>
+__global__ __launch_bounds__(256, HD == 128 ? 2 : 4) void window_tile_kernel(WindowArgs a) {
+  constexpr int IMG = 2 * kKeys * HD;  // bytes of an image of 32 keys
+  __shared__ __attribute__((aligned(16))) uint8_t lds[2][4 * IMG];  // [stage]: K, K, V, V
+  const nemo_attention_batch& b = a.b;
+  const int kvh = blockIdx.x % a.kv_heads, tile_no = blockIdx.x / a.kv_heads;  // an XCD's L2 keeps to one KV head of 8
+  const int request = tile_request(b, a.group, kTileRows, tile_no);
+  if (request < 0) return;
+  const Request r(b, request);
+  const int rows = r.queries * a.group, row0 = (tile_no - tile_base(b, a.group, kTileRows, request)) * kTileRows;
+  if (row0 >= rows) return;
+  const Heads<T> heads(a, r, kvh);
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), hl = lane >> 5;
+  const int behind = r.keys - r.queries;  // position of query 0
+  const KeyList list(a, behind + row0 / a.group, behind + min(row0 + kTileRows - 1, rows - 1) / a.group, r.keys);
+  const int w0 = row0 + 32 * wave, w1 = min(w0 + 31, rows - 1);
+  const bool active = w0 < rows;
+  const int row = min(w0 + (lane & 31), rows - 1);
+  auto window = [&](int at) {
+    Seen s(a, behind + at / a.group, r.keys);
+    s.lo += list.sinks - list.lo;
+    s.hi += list.sinks - list.lo;
+    return s;
+  };
+  const Seen mine = window(row), first = window(min(w0, rows - 1)), last = window(w1);
+  const int rounds = (list.n + 63) >> 6;
+
+  const int64_t k_stride = 2 * b.k_row, v_stride = 2 * b.v_row;
+  const Stager<HD, 16, false> ks(16 * wave, k_stride);
+  const Stager<HD, 16, true> vs(16 * wave, v_stride);
+  auto stage = [&](int at) {
+    uint8_t* ki = lds[at & 1] + 16 * wave * 2 * HD;
+    uint8_t* vi = ki + 2 * IMG;
+    const int t0 = 64 * at;
+    if (t0 >= list.sinks && t0 + 64 <= list.n) {
+      const int64_t j = list.key(t0);
+      ks.rows((const uint8_t*)heads.k + j * k_stride, ki);
+      vs.rows((const uint8_t*)heads.v + j * v_stride, vi);
+    } else {
+      auto key = [&](int t) { return list.key(t); };
+      ks.slots((const uint8_t*)heads.k, k_stride, t0, list.n, key, ki);
+      vs.slots((const uint8_t*)heads.v, v_stride, t0, list.n, key, vi);
+    }
+  };
+  if (rounds) stage(0);
+  Rows<T, HD> acc;
+  acc.load(heads.query(row), hl);
+  acc.clear();
+  for (int at = 0; at < rounds; ++at) {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();  // this round has landed, and every wave has left the other stage
+    if (at + 1 < rounds) stage(at + 1);
+    if (!active) continue;
+    const uint8_t* image = lds[at & 1];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int t0 = 64 * at + 32 * u;
+      if (t0 >= last.hi || (t0 + 32 <= first.lo && t0 >= a.sinks)) continue;  // no row sees it
+      float16v s = acc.scores(image + u * IMG, lane);
+      if (t0 + 32 > first.hi || (t0 < last.lo && t0 + 32 > a.sinks)) hide(s, t0, hl, mine.lo, mine.hi, a.sinks);
+      typename Mma<T>::frag p[2];
+      acc.probabilities(s, a.scale2, p);
+      acc.values(image + (2 + u) * IMG, lane, p);
+    }
+  }
+  if (!active) return;
+  acc.l += __shfl_xor(acc.l, 32, 64);
+  // A value that some rows of the wave do not see meets their probability 0;
+  // where it is not finite, their sums are not, and they are taken again. (One
+  // query's rows see the same keys.)
+  const uint64_t bad = w0 / a.group == w1 / a.group ? 0 : __builtin_amdgcn_ballot_w64(acc.spoilt());
+  const uint32_t again = (uint32_t)(bad | bad >> 32);
+  if (w0 + (lane & 31) < rows && !(again >> (lane & 31) & 1)) acc.store(heads.output(row), hl);
+  for (uint32_t todo = again; todo; todo &= todo - 1) {
+    const int at = w0 + __builtin_ctz(todo);
+    if (at < rows) one_row<T, HD>(a, heads, list, r, at, 0, list.n).store(heads.output(at));
+  }
 }
 
 }  // namespace
@@ -117,20 +446,24 @@ size_t window_workspace(const nemo_attention_config& c, int count, int64_t q_row
 
 hipError_t launch_window_attention(const nemo_attention_config& c, const nemo_attention_batch& b, hipStream_t stream) {
   if (b.count == 0 || b.q_rows == 0) return hipSuccess;
-  WindowArgs a{b, c.q_heads / c.kv_heads, 0, 0, 0, 0.f};
+  WindowArgs a{b, c.kv_heads, c.q_heads / c.kv_heads, 0, 0, 0, 0.f};
   auto bound = [](int v) { return v < 0 ? kUnbounded : std::min(v, kUnbounded); };
   a.left = bound(c.left);
   a.right = bound(c.right);
   a.sinks = std::min(c.sinks, kUnbounded);
   a.scale2 = (c.scale > 0.f ? c.scale : 1.0f / sqrtf((float)c.head_dim)) * 1.4426950408889634f;
-  const dim3 grid((unsigned)(b.q_rows * a.group / 4 + b.count), c.kv_heads);
-  if (c.type == NEMO_TYPE_F16) {
-    if (c.head_dim == 64) window_row_kernel<half_t, 64><<<grid, 256, 0, stream>>>(a);
-    else window_row_kernel<half_t, 128><<<grid, 256, 0, stream>>>(a);
-  } else {
-    if (c.head_dim == 64) window_row_kernel<bf16_t, 64><<<grid, 256, 0, stream>>>(a);
-    else window_row_kernel<bf16_t, 128><<<grid, 256, 0, stream>>>(a);
-  }
+  auto launch = [&](auto type, auto hd) {
+    constexpr int HD = decltype(hd)::value;
+    typedef decltype(type) T;
+    const unsigned tiles = (unsigned)(b.q_rows * a.group / kTileRows + b.count);
+    window_tile_kernel<T, HD><<<tiles * c.kv_heads, 256, 0, stream>>>(a);
+  };
+  auto typed = [&](auto type) {
+    if (c.head_dim == 64) launch(type, std::integral_constant<int, 64>{});
+    else launch(type, std::integral_constant<int, 128>{});
+  };
+  if (c.type == NEMO_TYPE_F16) typed(half_t{});
+  else typed(bf16_t{});
   return hipGetLastError();
 }
 
