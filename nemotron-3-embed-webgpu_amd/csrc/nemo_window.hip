@@ -438,11 +438,228 @@ __global__ __launch_bounds__(256, HD == 128 ? 2 : 4) void window_tile_kernel(Win
   }
 }
 
+// ---------------------------------------------------------------------------
+// Few rows: the 4 waves of a workgroup take the same 32 rows and every fourth
+// block of 32 keys each, staged by the wave for itself two blocks deep (no
+// barrier in the loop), and add up in LDS. With `splits` above 1 the blocks are
+// dealt out to that many workgroups as well, whose sums a second kernel joins.
+// ---------------------------------------------------------------------------
+
+constexpr int kFewWaves = 4;
+
+// Sums of a split: the row's reference maximum and sum, and its output values.
+struct Partials {
+  float2* ml;  // [split][row], null: not split
+  float* o;    // [split][row][HD]
+  int64_t rows;
+  int splits;
+};
+
+template <typename T, int HD>
+__global__ __launch_bounds__(64 * kFewWaves) void window_few_kernel(WindowArgs a, Partials part) {
+  constexpr int IMG = 2 * kKeys * HD;
+  constexpr int OP = HD + 4;  // row of the sums in LDS, in floats
+  __shared__ __attribute__((aligned(16))) uint8_t lds[kFewWaves][2][2 * IMG];
+  __shared__ float2 sums[kFewWaves][32];
+  __shared__ uint32_t spoilt;
+  static_assert(kFewWaves * 32 * OP * 4 <= sizeof(lds), "the sums fit in the keys' place");
+  const nemo_attention_batch& b = a.b;
+  const int kvh = blockIdx.x % a.kv_heads, tile_no = blockIdx.x / a.kv_heads, split = blockIdx.y;
+  const int request = tile_request(b, a.group, 32, tile_no);
+  if (request < 0) return;
+  const Request r(b, request);
+  const int rows = r.queries * a.group, row0 = (tile_no - tile_base(b, a.group, 32, request)) * 32;
+  if (row0 >= rows) return;
+  const Heads<T> heads(a, r, kvh);
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), hl = lane >> 5;
+  const int behind = r.keys - r.queries, row1 = min(row0 + 31, rows - 1);
+  const KeyList list(a, behind + row0 / a.group, behind + row1 / a.group, r.keys);
+  const int row = min(row0 + (lane & 31), rows - 1);
+  auto window = [&](int at) {
+    Seen s(a, behind + at / a.group, r.keys);
+    s.lo += list.sinks - list.lo;
+    s.hi += list.sinks - list.lo;
+    return s;
+  };
+  const Seen mine = window(row), first = window(row0), last = window(row1);
+  const int blocks = (list.n + 31) >> 5;
+  const int block0 = (int)((int64_t)blocks * split / part.splits);
+  const int block1 = (int)((int64_t)blocks * (split + 1) / part.splits);
+
+  const int64_t k_stride = 2 * b.k_row, v_stride = 2 * b.v_row;
+  const Stager<HD, 32, false> ks(0, k_stride);
+  const Stager<HD, 32, true> vs(0, v_stride);
+  auto stage = [&](int at, int buffer) {
+    uint8_t* ki = lds[wave][buffer];
+    const int t0 = 32 * at;
+    if (t0 >= list.sinks && t0 + 32 <= list.n) {
+      const int64_t j = list.key(t0);
+      ks.rows((const uint8_t*)heads.k + j * k_stride, ki);
+      vs.rows((const uint8_t*)heads.v + j * v_stride, ki + IMG);
+    } else {
+      auto key = [&](int t) { return list.key(t); };
+      ks.slots((const uint8_t*)heads.k, k_stride, t0, list.n, key, ki);
+      vs.slots((const uint8_t*)heads.v, v_stride, t0, list.n, key, ki + IMG);
+    }
+  };
+  Rows<T, HD> acc;
+  acc.load(heads.query(row), hl);
+  acc.clear();
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the queries: from here on only copies are counted
+  int at = block0 + wave;
+  if (at < block1) stage(at, 0);
+  for (int buffer = 0; at < block1; at += kFewWaves, buffer ^= 1) {
+    if (at + kFewWaves < block1) {
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the other buffer's reads are done
+      stage(at + kFewWaves, buffer ^ 1);
+      asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * IMG / 1024) : "memory");
+    } else {
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    }
+    const int t0 = 32 * at;
+    if (t0 >= last.hi || (t0 + 32 <= first.lo && t0 >= a.sinks)) continue;
+    float16v s = acc.scores(lds[wave][buffer], lane);
+    if (t0 + 32 > first.hi || (t0 < last.lo && t0 + 32 > a.sinks)) hide(s, t0, hl, mine.lo, mine.hi, a.sinks);
+    typename Mma<T>::frag p[2];
+    acc.probabilities(s, a.scale2, p);
+    acc.values(lds[wave][buffer] + IMG, lane, p);
+  }
+  // The waves' sums: row-major in LDS, in place of the keys.
+  acc.l += __shfl_xor(acc.l, 32, 64);
+  if (threadIdx.x == 0) spoilt = 0;
+  __syncthreads();
+  float* o = (float*)lds;
+  if (row0 + (lane & 31) < rows) {
+    if (hl == 0) sums[wave][lane] = make_float2(acc.m, acc.l);
+#pragma unroll
+    for (int db = 0; db < HD / 32; ++db)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float4v v = {acc.o[db][4 * j], acc.o[db][4 * j + 1], acc.o[db][4 * j + 2], acc.o[db][4 * j + 3]};
+        *(float4v*)(o + (wave * 32 + (lane & 31)) * OP + 32 * db + 8 * j + 4 * hl) = v;
+      }
+  }
+  __syncthreads();
+  // Thread: HD / 8 columns of one row.
+  constexpr int C = HD / 8;
+  const int mrow = threadIdx.x >> 3, c0 = (threadIdx.x & 7) * C;
+  const bool valid = row0 + mrow < rows;
+  float m = -INFINITY, l = 0.f, v[C] = {};
+  if (valid) {
+#pragma unroll
+    for (int w = 0; w < kFewWaves; ++w) m = fmaxf(m, sums[w][mrow].x);
+#pragma unroll
+    for (int w = 0; w < kFewWaves; ++w) {
+      const float2 ml = sums[w][mrow];
+      if (ml.x == -INFINITY && ml.y == 0.f) continue;  // saw nothing
+      const float f = ml.x == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(ml.x - m);
+      l = fmaf(f, ml.y, l);
+#pragma unroll
+      for (int c = 0; c < C; ++c) v[c] = fmaf(f, o[(w * 32 + mrow) * OP + c0 + c], v[c]);
+    }
+    if (row0 / a.group != row1 / a.group) {
+      float z = l * 0.f;
+#pragma unroll
+      for (int c = 0; c < C; ++c) z = fmaf(v[c], 0.f, z);
+      if (z != 0.f) atomicOr(&spoilt, 1u << mrow);
+    }
+  }
+  __syncthreads();
+  const int64_t out_row = (int64_t)r.q0 * a.kv_heads * a.group + kvh * a.group;  // of row 0's first head, [query][head]
+  auto partial = [&](int at) {
+    return part.rows * split + out_row + (int64_t)(at / a.group) * a.kv_heads * a.group + at % a.group;
+  };
+  const uint32_t again = spoilt;
+  if (valid && !(again >> mrow & 1)) {
+    if (part.ml) {
+      const int64_t at = partial(row0 + mrow);
+      if (c0 == 0) part.ml[at] = make_float2(m, l);
+#pragma unroll
+      for (int c = 0; c < C; c += 4) *(float4v*)(part.o + at * HD + c0 + c) = float4v{v[c], v[c + 1], v[c + 2], v[c + 3]};
+    } else {
+      typedef T vec __attribute__((ext_vector_type(8)));
+      const float inv = l == 0.f ? 0.f : 1.0f / l;
+      T* out = heads.output(row0 + mrow) + c0;
+#pragma unroll
+      for (int c = 0; c < C; c += 8) {
+        vec t;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) t[e] = (T)(v[c + e] * inv);
+        *(vec*)(out + c) = t;
+      }
+    }
+  }
+  // As in window_tile_kernel: rows spoilt by values that they do not see.
+  uint32_t todo = again;
+  for (int n = 0; todo; todo &= todo - 1, ++n) {
+    if (n % kFewWaves != wave) continue;
+    const int at = row0 + __builtin_ctz(todo);
+    const OneRow<T, HD> one = one_row<T, HD>(a, heads, list, r, at, 32 * block0, min(32 * block1, list.n));
+    if (part.ml) {
+      if (lane == 0) part.ml[partial(at)] = make_float2(one.m, one.l);
+#pragma unroll
+      for (int c = 0; c < HD / 64; ++c) part.o[partial(at) * HD + lane + 64 * c] = one.o[c];
+    } else {
+      one.store(heads.output(at));
+    }
+  }
+}
+
+// Joins the splits: a wave a row, lane z the weight of split z (at most 64).
+template <typename T, int HD>
+__global__ __launch_bounds__(256) void window_join_kernel(WindowArgs a, Partials part) {
+  constexpr int R = 4;
+  const nemo_attention_batch& b = a.b;
+  const int kvh = blockIdx.x % a.kv_heads, tile_no = blockIdx.x / a.kv_heads;
+  const int request = tile_request(b, a.group, R, tile_no);
+  if (request < 0) return;
+  const Request r(b, request);
+  const int row = (tile_no - tile_base(b, a.group, R, request)) * R + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+  if (row >= r.queries * a.group) return;
+  const int64_t at = (int64_t)(r.q0 + row / a.group) * a.kv_heads * a.group + kvh * a.group + row % a.group;
+  const float2 ml = lane < part.splits ? part.ml[part.rows * lane + at] : make_float2(-INFINITY, 0.f);
+  float m = ml.x;
+#pragma unroll
+  for (int x = 32; x > 0; x >>= 1) m = fmaxf(m, __shfl_xor(m, x, 64));
+  const bool empty = ml.x == -INFINITY && ml.y == 0.f;
+  const float f = empty ? 0.f : ml.x == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(ml.x - m);
+  float l = empty ? 0.f : f * ml.y;
+#pragma unroll
+  for (int x = 32; x > 0; x >>= 1) l += __shfl_xor(l, x, 64);
+  const uint64_t full = ~__builtin_amdgcn_ballot_w64(empty);
+  float v[HD / 64] = {};
+  for (int z = 0; z < part.splits; ++z) {
+    if (!(full >> z & 1)) continue;
+    const float fz = __shfl(f, z, 64);
+#pragma unroll
+    for (int c = 0; c < HD / 64; ++c) v[c] = fmaf(fz, part.o[(part.rows * z + at) * HD + lane + 64 * c], v[c]);
+  }
+  T* out = (T*)b.out + (int64_t)(r.q0 + row / a.group) * b.out_row + (kvh * a.group + row % a.group) * b.out_head;
+#pragma unroll
+  for (int c = 0; c < HD / 64; ++c) out[lane + 64 * c] = (T)(l == 0.f ? 0.f : v[c] / l);
+}
+
+// Whether the keys are dealt out to the waves of a workgroup, not the rows:
+// when tiles of 128 rows would leave CUs without one.
+bool few_rows(const nemo_attention_config& c, int64_t q_rows) {
+  return q_rows * c.q_heads < 256 * kTileRows;
+}
+
 }  // namespace
 
-int window_splits(const nemo_attention_config& c, int count, int64_t q_rows, int64_t max_kv) { return 1; }
+int window_splits(const nemo_attention_config& c, int count, int64_t q_rows, int64_t max_kv) {
+  if (count == 0 || q_rows == 0 || !few_rows(c, q_rows)) return 1;
+  const int64_t tiles = std::max<int64_t>(q_rows * (c.q_heads / c.kv_heads) / 32, count) * c.kv_heads;
+  int64_t keys = max_kv;
+  if (c.left >= 0 && c.right >= 0)
+    keys = std::min(keys, (int64_t)c.left + c.right + c.sinks + (q_rows + count - 1) / count);
+  return (int)std::max<int64_t>(1, std::min<int64_t>({(512 + tiles - 1) / tiles, keys / 256, 64}));
+}
 
-size_t window_workspace(const nemo_attention_config& c, int count, int64_t q_rows, int64_t max_kv) { return 0; }
+size_t window_workspace(const nemo_attention_config& c, int count, int64_t q_rows, int64_t max_kv) {
+  const int splits = window_splits(c, count, q_rows, max_kv);
+  return splits == 1 ? 0 : (size_t)splits * q_rows * c.q_heads * (c.head_dim * 4 + 8);
+}
 
 hipError_t launch_window_attention(const nemo_attention_config& c, const nemo_attention_batch& b, hipStream_t stream) {
   if (b.count == 0 || b.q_rows == 0) return hipSuccess;
@@ -452,11 +669,23 @@ hipError_t launch_window_attention(const nemo_attention_config& c, const nemo_at
   a.right = bound(c.right);
   a.sinks = std::min(c.sinks, kUnbounded);
   a.scale2 = (c.scale > 0.f ? c.scale : 1.0f / sqrtf((float)c.head_dim)) * 1.4426950408889634f;
+  const int splits = b.workspace ? window_splits(c, b.count, b.q_rows, b.max_kv) : 1;
+  const int64_t rows = b.q_rows * c.q_heads;
+  Partials part{nullptr, nullptr, rows, splits};
+  if (splits > 1) {
+    part.o = (float*)b.workspace;
+    part.ml = (float2*)(part.o + splits * rows * c.head_dim);
+  }
+  auto tiles = [&](int r) { return (unsigned)(b.q_rows * a.group / r + b.count) * c.kv_heads; };
   auto launch = [&](auto type, auto hd) {
     constexpr int HD = decltype(hd)::value;
     typedef decltype(type) T;
-    const unsigned tiles = (unsigned)(b.q_rows * a.group / kTileRows + b.count);
-    window_tile_kernel<T, HD><<<tiles * c.kv_heads, 256, 0, stream>>>(a);
+    if (!few_rows(c, b.q_rows)) {
+      window_tile_kernel<T, HD><<<tiles(kTileRows), 256, 0, stream>>>(a);
+      return;
+    }
+    window_few_kernel<T, HD><<<dim3(tiles(32), splits), 64 * kFewWaves, 0, stream>>>(a, part);
+    if (splits > 1) window_join_kernel<T, HD><<<tiles(4), 256, 0, stream>>>(a, part);
   };
   auto typed = [&](auto type) {
     if (c.head_dim == 64) launch(type, std::integral_constant<int, 64>{});
