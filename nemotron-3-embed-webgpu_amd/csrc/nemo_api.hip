@@ -1588,6 +1588,8 @@ nemo_status nemo_window_attention(nemo_ctx* ctx, const nemo_attention_config* co
       validate_stride(v, "attention strides");
       if (v % 8) fail(NEMO_ERR_INVALID, "attention strides must be multiples of 8");
     }
+    if (b.kv_rows > 1 && (b.k_row < config->head_dim || b.v_row < config->head_dim))
+      fail(NEMO_ERR_INVALID, "rows of k and v must not overlap");
     for (const void* p : {b.q, b.k, b.v, (const void*)b.out, (const void*)b.workspace})
       if ((uintptr_t)p & 15) fail(NEMO_ERR_INVALID, "attention buffers must be 16-byte aligned");
     const size_t need = b.workspace ? window_workspace(*config, b.count, b.q_rows, b.max_kv) : 0;

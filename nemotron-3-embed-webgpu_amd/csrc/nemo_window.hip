@@ -24,48 +24,58 @@ struct WindowArgs {
   nemo_attention_batch b;
   int kv_heads, group, left, right, sinks;
   float scale2;  // of the scores, in units of log2
+  // row / group for rows below 2^31: (row + the high half of row * magic) >> shift
+  uint32_t magic;
+  int shift;
+  __device__ __forceinline__ int query(int row) const {
+    return (int)((__umulhi((uint32_t)row, magic) + (uint32_t)row) >> shift);
+  }
 };
 
-// The keys that a query at p sees of a request's n: [0, sinks) and [lo, hi).
+// The window of a query at p over a request's n keys: [lo, hi).
 struct Seen {
-  int sinks, lo, hi;
+  int lo, hi;
   __device__ __forceinline__ Seen(const WindowArgs& a, int p, int n) {
     hi = max(0, min(n, a.right >= kUnbounded ? n : p + a.right + 1));
     lo = a.left >= kUnbounded ? 0 : min(hi, max(0, p - a.left));
-    sinks = min(a.sinks, lo);
   }
 };
 
-// A request as it lies in the buffers, whatever the index arrays hold.
+// A request as it lies in the buffers, whatever the index arrays hold, and the
+// number of its first tile. Tiles of ROWS (query, head of the group) rows are
+// numbered through a batch without a table: request i's first number is
+// floor(q_start[i] group / ROWS) + i, which leaves it at least as many numbers
+// as it has tiles. The request of tile number t is the last whose first is not
+// above t; none (i = -1) before the first request. Each lane looks at one
+// request and has its whole entry at hand when it is the one.
+template <int ROWS>
 struct Request {
-  int q0, queries, keys;
+  int i, tile, q0, queries, keys;
   int64_t kv0;
-  __device__ __forceinline__ Request(const nemo_attention_batch& b, int i) {
-    q0 = min(max(b.q_start[i], 0), (int)b.q_rows);
-    queries = max(min(b.q_start[i + 1], (int)b.q_rows) - q0, 0);
-    kv0 = min(max(b.kv_start[i], (int64_t)0), b.kv_rows);
-    keys = (int)min((int64_t)max(b.kv_len[i], 0), b.kv_rows - kv0);
+  __device__ __forceinline__ Request(const WindowArgs& a, int t) {
+    const nemo_attention_batch& b = a.b;
+    i = -1;
+    for (int i0 = 0; i0 < b.count; i0 += 64) {
+      const int at = min(i0 + (int)(threadIdx.x & 63), b.count - 1);
+      const int begin = min(max(b.q_start[at], 0), (int)b.q_rows);
+      const int end = min(b.q_start[at + 1], (int)b.q_rows);
+      const int64_t kv = min(max(b.kv_start[at], (int64_t)0), b.kv_rows);
+      const int len = (int)min((int64_t)max(b.kv_len[at], 0), b.kv_rows - kv);
+      const int first = (int)((int64_t)begin * a.group / ROWS) + at;
+      const int n = (int)__popcll(__builtin_amdgcn_ballot_w64(i0 + (int)(threadIdx.x & 63) < b.count && first <= t));
+      if (n) {
+        i = i0 + n - 1;
+        tile = __builtin_amdgcn_readlane(first, n - 1);
+        q0 = __builtin_amdgcn_readlane(begin, n - 1);
+        queries = max(__builtin_amdgcn_readlane(end, n - 1) - q0, 0);
+        keys = __builtin_amdgcn_readlane(len, n - 1);
+        kv0 = (int64_t)(uint32_t)__builtin_amdgcn_readlane((int)kv, n - 1) |
+              (int64_t)__builtin_amdgcn_readlane((int)(kv >> 32), n - 1) << 32;
+      }
+      if (n < 64) break;
+    }
   }
 };
-
-// Tiles of `rows` (query, head of the group) rows are numbered through a
-// batch without a table: request i's first is floor(q_start[i] group / rows)
-// + i, which leaves it at least as many numbers as it has tiles. The request
-// of tile number t, -1 if it is none's.
-__device__ __forceinline__ int tile_base(const nemo_attention_batch& b, int group, int rows, int i) {
-  const int q0 = min(max(b.q_start[i], 0), (int)b.q_rows);
-  return (int)((int64_t)q0 * group / rows) + i;
-}
-__device__ __forceinline__ int tile_request(const nemo_attention_batch& b, int group, int rows, int t) {
-  int found = 0;
-  for (int i0 = 0; i0 < b.count; i0 += 64) {
-    const int i = i0 + (int)(threadIdx.x & 63);
-    const uint64_t at = __builtin_amdgcn_ballot_w64(i < b.count && tile_base(b, group, rows, i) <= t);
-    found += (int)__popcll(at);
-    if (at != ~0ull) break;
-  }
-  return found - 1;
-}
 
 // One query head over keys [j0, j1), by a wave: its running maximum, sum and
 // output columns lane, lane + 64.
@@ -117,6 +127,10 @@ struct Mma;
 template <>
 struct Mma<half_t> {
   typedef half8v frag;
+  typedef half2v pair;
+  static __device__ __forceinline__ float add(pair p, float sum) {
+    return __builtin_amdgcn_fdot2(p, pair{(half_t)1.f, (half_t)1.f}, sum, false);
+  }
   static __device__ __forceinline__ float16v mma(frag a, frag b, float16v c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
   }
@@ -124,6 +138,10 @@ struct Mma<half_t> {
 template <>
 struct Mma<bf16_t> {
   typedef bf16x8 frag;
+  typedef bf16_t pair __attribute__((ext_vector_type(2)));
+  static __device__ __forceinline__ float add(pair p, float sum) {
+    return __builtin_amdgcn_fdot2_f32_bf16(p, pair{(bf16_t)1.f, (bf16_t)1.f}, sum, false);
+  }
   static __device__ __forceinline__ float16v mma(frag a, frag b, float16v c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
   }
@@ -142,56 +160,74 @@ __device__ __forceinline__ int v_swizzle(int row) {
   return HD == 128 ? 4 * (row & 3) : 4 * ((row >> 1) & 1);
 }
 
+// Copies of 16 bytes a lane into LDS at `to` + 16 lane, from a buffer's range
+// (zeros past its end). The compiler, which knows of the builtin for this that
+// it writes LDS, waits for every copy in flight before each transposed read;
+// written as here it has no register to be waited for, and the loops wait
+// for their images themselves.
+__device__ __forceinline__ uint32_t lds_address(const uint8_t* to) { return (uint32_t)(uintptr_t)(lds_void*)to; }
+__device__ __forceinline__ void copy_range(u32x4 range, uint32_t offset, const uint8_t* to) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+               :
+               : "s"(lds_address(to)), "v"(offset), "s"(range)
+               : "memory");
+}
 // Copies of ROWS key rows into an image by one wave, 1 KB an instruction:
 // rows first .. first + ROWS of a 32-row image (or of two that follow each
-// other). lane_off: the lane's byte offsets from the address of slot row 0 of
-// the image, for rows that lie `stride` bytes apart.
+// other). off: the lane's byte offsets from row 0 of the image, for rows that
+// lie `stride` bytes apart.
 template <int HD, int ROWS, bool VALUES>
 struct Stager {
   static constexpr int kChunks = HD / 8, kPer = 64 / kChunks, kN = ROWS / kPer;
   uint32_t off[kN];
-  int row, chunk[kN];
+  int row;
   __device__ __forceinline__ Stager(int first, int64_t stride) {
     const int lane = threadIdx.x & 63;
     row = first + lane / kChunks;
 #pragma unroll
     for (int i = 0; i < kN; ++i) {
       const int r = row + kPer * i;
-      chunk[i] = 16 * ((lane % kChunks) ^ (VALUES ? v_swizzle<HD>(r) : k_swizzle<HD>(r)));
-      off[i] = (uint32_t)(r * stride) + chunk[i];
+      off[i] = (uint32_t)(r * stride) + 16 * ((lane % kChunks) ^ (VALUES ? v_swizzle<HD>(r) : k_swizzle<HD>(r)));
     }
   }
-  // Slots t0 .. of the list, all of them window keys: consecutive rows from `at`.
-  __device__ __forceinline__ void rows(const uint8_t* at, uint8_t* image) const {
-#pragma unroll
-    for (int i = 0; i < kN; ++i)
-      __builtin_amdgcn_global_load_lds((const void*)(at + off[i]), (lds_void*)(image + 1024 * i), 16, 0, 0);
+  // The image of the rows from `at` on, of which `valid` are copied and the
+  // others zero.
+  static __device__ __forceinline__ u32x4 range(const uint8_t* at, int64_t stride, int valid) {
+    const int bytes = (int)stride * max(0, min(valid, kKeys));
+    return u32x4{(uint32_t)(uintptr_t)at, (uint32_t)((uintptr_t)at >> 32) & 0xffffu,
+                 (uint32_t)__builtin_amdgcn_readfirstlane(bytes), 0x00020000u};
   }
-  // Any slots: key(t) of each, the last slot's from there on.
-  template <typename Key>
-  __device__ __forceinline__ void slots(const uint8_t* base, int64_t stride, int t0, int n, Key&& key,
-                                        uint8_t* image) const {
+  __device__ __forceinline__ void copy(u32x4 range, int i, const uint8_t* image) const {
+    copy_range(range, off[i], image + 1024 * i);
+  }
+  __device__ __forceinline__ void copy(u32x4 range, const uint8_t* image) const {
 #pragma unroll
-    for (int i = 0; i < kN; ++i) {
-      const int64_t j = key(min(t0 + row + kPer * i, n - 1));
-      __builtin_amdgcn_global_load_lds((const void*)(base + j * stride + chunk[i]), (lds_void*)(image + 1024 * i), 16,
-                                       0, 0);
-    }
+    for (int i = 0; i < kN; ++i) copy(range, i, image);
   }
 };
 
-// The tile of 32 rows of a wave, or the larger one of a workgroup: its key
-// list, and in list coordinates what the row of a lane sees: t < hi and (t >= lo
-// or t < sinks).
+// The key list of the rows of queries at p0 .. p1: slots t < sinks are keys t,
+// slots from `pad`, a multiple of 32, on the keys from lo on, and those between
+// are empty, so an image of 32 slots holds rows that follow each other. In
+// list coordinates a row sees t < hi with t >= lo or t < sinks.
 struct KeyList {
-  int sinks, lo, n;  // slots t < sinks are keys t, others lo + t - sinks
+  int pad, lo, n, all_sinks;
   __device__ __forceinline__ KeyList(const WindowArgs& a, int p0, int p1, int keys) {
     const Seen first(a, p0, keys), last(a, p1, keys);
-    lo = first.lo;
-    sinks = min(a.sinks, lo);
-    n = sinks + last.hi - lo;
+    all_sinks = a.sinks;
+    lo = a.sinks < first.lo ? first.lo : 0;  // sinks that reach the window: keys from 0 on
+    pad = lo ? (a.sinks + 31) & ~31 : 0;
+    n = pad + last.hi - lo;
   }
-  __device__ __forceinline__ int key(int t) const { return t < sinks ? t : lo + t - sinks; }
+  __device__ __forceinline__ int key(int t) const { return t < pad ? t : lo + t - pad; }
+  // Rows that the image of the slots t0 .. t0 + 31 has.
+  __device__ __forceinline__ int rows(int t0) const { return t0 < 0 ? 0 : (t0 < pad ? all_sinks : n) - t0; }
+  __device__ __forceinline__ Seen window(const WindowArgs& a, int p, int keys) const {
+    Seen s(a, p, keys);
+    s.lo += pad - lo;
+    s.hi += pad - lo;
+    return s;
+  }
 };
 
 // A wave's 32 rows: row l % 32 in lane l, whose half hl = l / 32 holds the
@@ -203,7 +239,7 @@ struct Rows {
   typedef typename Mma<T>::frag frag;
   frag q[DC];
   float16v o[DB];
-  float m, l;
+  float m, l;  // reference and sum of the probabilities
 
   __device__ __forceinline__ void clear() {
     m = -INFINITY;
@@ -217,72 +253,137 @@ struct Rows {
 #pragma unroll
     for (int c = 0; c < DC; ++c) q[c] = *(const frag*)(row + 16 * c + 8 * hl);
   }
+  __device__ __forceinline__ frag key(const uint8_t* image, int lane, int c) const {
+    const int row = lane & 31;
+    return *(const frag*)(image + row * 2 * HD + 16 * ((2 * c + (lane >> 5)) ^ k_swizzle<HD>(row)));
+  }
   __device__ __forceinline__ float16v scores(const uint8_t* image, int lane) const {
-    const int row = lane & 31, hl = lane >> 5, sw = k_swizzle<HD>(row);
     float16v s = {};
 #pragma unroll
-    for (int c = 0; c < DC; ++c)
-      s = Mma<T>::mma(*(const frag*)(image + row * 2 * HD + 16 * ((2 * c + hl) ^ sw)), q[c], s);
+    for (int c = 0; c < DC; ++c) s = Mma<T>::mma(key(image, lane, c), q[c], s);
     return s;
   }
-  // Probabilities against a reference maximum that is raised only when a row
-  // exceeds it by 2^8 (a wave vote): p <= 256 then, far from overflow, and
-  // most blocks need no exchange between lanes and no rescaling; numerator
-  // and denominator share the reference, so the result is the softmax. A row
-  // that has seen nothing yet has the reference 0.
-  __device__ __forceinline__ void probabilities(const float16v& s, float scale2, frag (&p)[2]) {
-    float most = s[0];
+  // Probabilities 2^(s - m) are taken against a reference m that is the row's
+  // largest score so far only when it was last raised: it is raised when the
+  // sum of a lane's 16 says that one may have passed 2^15 (or is not a
+  // number, as for a row that has seen nothing, whose m is -infinity), and
+  // they are taken again. So the common block needs no maximum, no exchange
+  // between lanes and no rescaling, and one wave vote. Numerator and
+  // denominator share the reference, so the result is the softmax; the sum is
+  // that of the rounded probabilities.
+  static __device__ __forceinline__ float sum(const frag (&p)[2]) {
+    float v = 0.f;
 #pragma unroll
-    for (int r = 1; r < 16; ++r) most = fmaxf(most, s[r]);
-    most *= scale2;
-    if (__builtin_amdgcn_ballot_w64(most > m + 8.0f)) {
+    for (int i = 0; i < 8; ++i)
+      v = Mma<T>::add(typename Mma<T>::pair{p[i >> 2][2 * (i & 3)], p[i >> 2][2 * (i & 3) + 1]}, v);
+    return v;
+  }
+  static __device__ __forceinline__ void exponentials(const float16v& s, float scale2, float m, frag (&p)[2]) {
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      float8v e;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) e[i] = __builtin_amdgcn_exp2f(fmaf(s[8 * c + i], scale2, -m));
+      p[c] = __builtin_convertvector(e, frag);
+    }
+  }
+  // Adds the sum of p, the probabilities of s, to the row's, after raising the
+  // reference where it has to be.
+  __device__ __forceinline__ void settle(const float16v& s, float scale2, frag (&p)[2]) {
+    float add = sum(p);
+    if (__builtin_amdgcn_ballot_w64(!(add <= 0x1p15f))) {
       asm volatile("");  // keeps the rare path a branch
-      const float mn = fmaxf(m, fmaxf(most, __shfl_xor(most, 32, 64)));
-      const float alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn);
+      float top = s[0];
+#pragma unroll
+      for (int r = 1; r < 16; ++r) top = fmaxf(top, s[r]);
+      top *= scale2;
+      const float raised = fmaxf(m, fmaxf(top, __shfl_xor(top, 32, 64)));
+      const float alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - raised);
       l *= alpha;
 #pragma unroll
       for (int db = 0; db < DB; ++db)
 #pragma unroll
         for (int r = 0; r < 16; ++r) o[db][r] *= alpha;
-      m = mn;
+      m = raised;
+      exponentials(s, scale2, m == -INFINITY ? 0.f : m, p);
+      add = sum(p);
     }
-    const float ref = m == -INFINITY ? 0.f : m;
-    float e[16];
-#pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      e[r] = __builtin_amdgcn_exp2f(fmaf(s[r], scale2, -ref));
-      l += e[r];
-    }
-#pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      float8v f;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) f[i] = e[8 * c + i];
-      p[c] = __builtin_convertvector(f, frag);
-    }
+    l += add;
   }
-  // O^T += V^T P^T: k slot 8 hl + e of chunk c is key 16 c + 8 (e / 4) + 4 hl + e
-  // % 4, score register 8 c + e. A transposed read gives the 16 lanes of a
-  // group 4 keys of 16 columns; lane i of it reads key i / 4's columns 4 (i % 4)...
+  // V^T fragment of 16 keys (chunk c) and 32 columns (block db): k slot 8 hl +
+  // e is key 16 c + 8 (e / 4) + 4 hl + e % 4, that of score register 8 c + e. A
+  // transposed read gives the 16 lanes of a group 4 keys of 16 columns; lane i
+  // of it reads key i / 4's columns 4 (i % 4)...
+  __device__ __forceinline__ frag value(const uint8_t* image, int lane, int c, int db) const {
+    const int i = lane & 15, key = 4 * (lane >> 5) + (i >> 2);
+    const int chunk = (4 * db + 2 * ((lane >> 4) & 1) + ((i >> 1) & 1)) ^ v_swizzle<HD>(key);
+    const uint8_t* at = image + key * 2 * HD + 16 * chunk + 8 * (i & 1);
+    short8v a;
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const short4v v = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4v*)(at + (16 * c + 8 * u) * 2 * HD));
+#pragma unroll
+      for (int e = 0; e < 4; ++e) a[4 * u + e] = v[e];
+    }
+    return __builtin_bit_cast(frag, a);
+  }
+  // O^T += V^T P^T
   __device__ __forceinline__ void values(const uint8_t* image, int lane, const frag (&p)[2]) {
-    const int i = lane & 15, hl = lane >> 5;
-    const int key = 4 * hl + (i >> 2), half = (lane >> 4) & 1;
 #pragma unroll
     for (int c = 0; c < 2; ++c)
 #pragma unroll
-      for (int db = 0; db < DB; ++db) {
-        const int chunk = 4 * db + 2 * half + ((i >> 1) & 1);
-        short8v a;
+      for (int db = 0; db < DB; ++db) o[db] = Mma<T>::mma(value(image, lane, c, db), p[c], o[db]);
+  }
+  // One block of the pipelined loop: its probabilities from its scores s; in
+  // the same stream of instructions the scores of the next block, from the
+  // keys at k_image, and the product of the block before, whose
+  // probabilities are p, with its values at v_image. Then s and p are those of
+  // the next step. The matrix cores' work does not wait for the vector
+  // units' that way, and a wave issues both in turn.
+  // Copies (c), c < DC, are issued among the MFMAs too: a wave waits for the
+  // memory pipe at each.
+  template <typename Copies>
+  __device__ __forceinline__ void step(float16v& s, frag (&p)[2], const uint8_t* v_image, const uint8_t* k_image,
+                                       int lane, float scale2, Copies&& copies) {
+    frag kf[DC], vf[DC], next[2];
+    float16v n = {};
+    auto exponentials = [&](int from, int to) {
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const int r = 16 * c + 8 * u + key;
-          const short4v v = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-              (lds_short4v*)(image + r * 2 * HD + 16 * (chunk ^ v_swizzle<HD>(r)) + 8 * (i & 1)));
+      for (int r = from; r < to; r += 2) {
+        float v[2];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) a[4 * u + e] = v[e];
+        for (int i = 0; i < 2; ++i) {
+          v[i] = __builtin_amdgcn_exp2f(fmaf(s[r + i], scale2, -m));
+          asm volatile("" : "+v"(v[i]));  // here, not together where they are used
         }
-        o[db] = Mma<T>::mma(__builtin_bit_cast(frag, a), p[c], o[db]);
+        next[r >> 3][r & 7] = (T)v[0];
+        next[r >> 3][(r & 7) + 1] = (T)v[1];
       }
+    };
+    constexpr int AHEAD = DC / 2;  // fragments are read that many MFMAs before they are used
+    auto fragment = [&](int c) {
+      kf[c] = key(k_image, lane, c);
+      vf[c] = value(v_image, lane, c / DB, c % DB);
+    };
+#pragma unroll
+    for (int c = 0; c < AHEAD; ++c) fragment(c);
+    __builtin_amdgcn_sched_barrier(0);
+    exponentials(0, 4);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int c = 0; c < DC; ++c) {
+      n = Mma<T>::mma(kf[c], q[c], n);
+      exponentials(4 + 2 * (6 * c / DC), 4 + 2 * (6 * (c + 1) / DC));
+      __builtin_amdgcn_sched_barrier(0);
+      o[c % DB] = Mma<T>::mma(vf[c], p[c / DB], o[c % DB]);
+      if (c + AHEAD < DC) fragment(c + AHEAD);
+      copies(c);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    settle(s, scale2, next);
+    s = n;
+    p[0] = next[0];
+    p[1] = next[1];
   }
   __device__ __forceinline__ void store(T* out, int hl) const {
     typedef T vec __attribute__((ext_vector_type(4)));
@@ -324,117 +425,143 @@ struct Heads {
   T* out;
   int64_t q_row, q_head, out_row, out_head;
   int group;
-  __device__ __forceinline__ Heads(const WindowArgs& a, const Request& r, int kvh)
+  __device__ __forceinline__ Heads(const WindowArgs& a, int q0, int64_t kv0, int kvh)
       : q_row(a.b.q_row), q_head(a.b.q_head), out_row(a.b.out_row), out_head(a.b.out_head), group(a.group) {
-    q = (const T*)a.b.q + r.q0 * q_row + (int64_t)kvh * group * q_head;
-    k = (const T*)a.b.k + r.kv0 * a.b.k_row + kvh * a.b.k_head;
-    v = (const T*)a.b.v + r.kv0 * a.b.v_row + kvh * a.b.v_head;
-    out = (T*)a.b.out + r.q0 * out_row + (int64_t)kvh * group * out_head;
+    q = (const T*)a.b.q + q0 * q_row + (int64_t)kvh * group * q_head;
+    k = (const T*)a.b.k + kv0 * a.b.k_row + kvh * a.b.k_head;
+    v = (const T*)a.b.v + kv0 * a.b.v_row + kvh * a.b.v_head;
+    out = (T*)a.b.out + q0 * out_row + (int64_t)kvh * group * out_head;
   }
-  __device__ __forceinline__ const T* query(int row) const {
-    return q + (row / group) * q_row + (row % group) * q_head;
+  // Row `row`, of query i.
+  __device__ __forceinline__ const T* query(int row, int i) const {
+    return q + i * q_row + (row - i * group) * q_head;
   }
-  __device__ __forceinline__ T* output(int row) const {
-    return out + (row / group) * out_row + (row % group) * out_head;
+  __device__ __forceinline__ T* output(int row, int i) const {
+    return out + i * out_row + (row - i * group) * out_head;
   }
 };
 
 // A row over the slots [t0, t1) that it sees, key by key.
 template <typename T, int HD>
 __device__ __forceinline__ OneRow<T, HD> one_row(const WindowArgs& a, const Heads<T>& h, const KeyList& list,
-                                                 const Request& r, int row, int t0, int t1) {
-  const Seen seen(a, r.keys - r.queries + row / h.group, r.keys);
-  const int lo = seen.lo - list.lo + list.sinks, hi = seen.hi - list.lo + list.sinks, first = min(a.sinks, hi);
+                                                 int queries, int keys, int row, int t0, int t1) {
+  const int i = a.query(row);
+  const Seen seen = list.window(a, keys - queries + i, keys);
+  const int first = min(a.sinks, seen.hi);
   OneRow<T, HD> acc;
-  acc.keys(h.query(row), h.k, a.b.k_row, h.v, a.b.v_row, t0, min(t1, first), a.scale2);
-  const int from = max(max(t0, lo), first), to = min(t1, hi);
-  if (from < to) acc.keys(h.query(row), h.k, a.b.k_row, h.v, a.b.v_row, list.key(from), list.key(to - 1) + 1, a.scale2);
+  acc.keys(h.query(row, i), h.k, a.b.k_row, h.v, a.b.v_row, t0, min(t1, first), a.scale2);
+  const int from = max(max(t0, seen.lo), first), to = min(t1, seen.hi);
+  if (from < to) acc.keys(h.query(row, i), h.k, a.b.k_row, h.v, a.b.v_row, list.key(from), list.key(to - 1) + 1, a.scale2);
   return acc;
 }
 
 // ---------------------------------------------------------------------------
 // Many rows: a workgroup of 4 waves takes 128 rows, 32 a wave, and stages 64
-// keys a round for all of them, two rounds deep.
+// keys a round for all of them. A block's scores are taken one block ahead and
+// its product with V one behind, so the K rows of a round begin 64 slots after
+// its V rows, which begin at the last block of the round before.
 // ---------------------------------------------------------------------------
 
 constexpr int kTileRows = 128;
 
 template <typename T, int HD>
-__global__ __launch_bounds__(256, HD == 128 ? 2 : 4) void window_tile_kernel(WindowArgs a) {
+__global__ __launch_bounds__(256, HD == 128 ? 2 : 3) void window_tile_kernel(WindowArgs a) {
   constexpr int IMG = 2 * kKeys * HD;  // bytes of an image of 32 keys
-  __shared__ __attribute__((aligned(16))) uint8_t lds[2][4 * IMG];  // [stage]: K, K, V, V
+  __shared__ __attribute__((aligned(16))) uint8_t lds[2][2][2 * IMG];  // [K, V][round & 1]
   const nemo_attention_batch& b = a.b;
   const int kvh = blockIdx.x % a.kv_heads, tile_no = blockIdx.x / a.kv_heads;  // an XCD's L2 keeps to one KV head of 8
-  const int request = tile_request(b, a.group, kTileRows, tile_no);
-  if (request < 0) return;
-  const Request r(b, request);
-  const int rows = r.queries * a.group, row0 = (tile_no - tile_base(b, a.group, kTileRows, request)) * kTileRows;
+  const Request<kTileRows> r(a, tile_no);
+  if (r.i < 0) return;
+  const int rows = r.queries * a.group, row0 = (tile_no - r.tile) * kTileRows;
   if (row0 >= rows) return;
-  const Heads<T> heads(a, r, kvh);
+  const Heads<T> heads(a, r.q0, r.kv0, kvh);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), hl = lane >> 5;
   const int behind = r.keys - r.queries;  // position of query 0
-  const KeyList list(a, behind + row0 / a.group, behind + min(row0 + kTileRows - 1, rows - 1) / a.group, r.keys);
+  const KeyList list(a, behind + a.query(row0), behind + a.query(min(row0 + kTileRows - 1, rows - 1)), r.keys);
   const int w0 = row0 + 32 * wave, w1 = min(w0 + 31, rows - 1);
-  const bool active = w0 < rows;
-  const int row = min(w0 + (lane & 31), rows - 1);
-  auto window = [&](int at) {
-    Seen s(a, behind + at / a.group, r.keys);
-    s.lo += list.sinks - list.lo;
-    s.hi += list.sinks - list.lo;
-    return s;
-  };
+  const int row = min(w0 + (lane & 31), rows - 1);  // (a wave past the rows takes the last one's)
+  auto window = [&](int at) { return list.window(a, behind + a.query(at), r.keys); };
   const Seen mine = window(row), first = window(min(w0, rows - 1)), last = window(w1);
   const int rounds = (list.n + 63) >> 6;
 
+  // A wave copies 16 rows of K and of V a round: half of one of the two images
+  // of each. V's first image of round `at` is the block before the round's.
   const int64_t k_stride = 2 * b.k_row, v_stride = 2 * b.v_row;
-  const Stager<HD, 16, false> ks(16 * wave, k_stride);
-  const Stager<HD, 16, true> vs(16 * wave, v_stride);
-  auto stage = [&](int at) {
-    uint8_t* ki = lds[at & 1] + 16 * wave * 2 * HD;
-    uint8_t* vi = ki + 2 * IMG;
-    const int t0 = 64 * at;
-    if (t0 >= list.sinks && t0 + 64 <= list.n) {
-      const int64_t j = list.key(t0);
-      ks.rows((const uint8_t*)heads.k + j * k_stride, ki);
-      vs.rows((const uint8_t*)heads.v + j * v_stride, vi);
-    } else {
-      auto key = [&](int t) { return list.key(t); };
-      ks.slots((const uint8_t*)heads.k, k_stride, t0, list.n, key, ki);
-      vs.slots((const uint8_t*)heads.v, v_stride, t0, list.n, key, vi);
+  const Stager<HD, 16, false> ks(16 * (wave & 1), k_stride);
+  const Stager<HD, 16, true> vs(16 * (wave & 1), v_stride);
+  auto v_image = [&](int odd) { return lds[1][odd] + 16 * wave * 2 * HD; };
+  auto k_image = [&](int odd) { return lds[0][odd] + 16 * wave * 2 * HD; };
+  auto v_range = [&](int at) {
+    const int t0 = 64 * at - 32 + 32 * (wave >> 1);
+    return vs.range((const uint8_t*)heads.v + list.key(t0) * v_stride, v_stride, list.rows(t0));
+  };
+  auto k_range = [&](int at) {
+    const int t0 = 64 * at + 32 + 32 * (wave >> 1);
+    return ks.range((const uint8_t*)heads.k + list.key(t0) * k_stride, k_stride, list.rows(t0));
+  };
+  Rows<T, HD> acc;
+  acc.clear();
+  float16v s;
+  auto hidden = [&](int t0) {
+    if (t0 + 32 > first.hi || (t0 < last.lo && t0 + 32 > a.sinks)) {
+      asm volatile("");
+      hide(s, t0, hl, mine.lo, mine.hi, a.sinks);
     }
   };
-  if (rounds) stage(0);
-  Rows<T, HD> acc;
-  acc.load(heads.query(row), hl);
-  acc.clear();
-  for (int at = 0; at < rounds; ++at) {
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();  // this round has landed, and every wave has left the other stage
-    if (at + 1 < rounds) stage(at + 1);
-    if (!active) continue;
-    const uint8_t* image = lds[at & 1];
+  if (rounds) {
+    // K of the first block, in the place of the second round's V
+    const Stager<HD, 8, false> k0(8 * wave, k_stride);
+    k0.copy(k0.range((const uint8_t*)heads.k + list.key(0) * k_stride, k_stride, list.rows(0)),
+            lds[1][1] + 8 * wave * 2 * HD);
+    acc.load(heads.query(row, a.query(row)), hl);
+    vs.copy(v_range(0), v_image(0));
+    ks.copy(k_range(0), k_image(0));
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(IMG / 1024) : "memory");
+    __builtin_amdgcn_s_barrier();
+    s = acc.scores(lds[1][1], lane);
+    hidden(0);
+  }
+  typename Mma<T>::frag p[2] = {};
+  const bool tail = 64 * rounds - 32 < list.n;  // the last round's second block has slots
+  auto landed = [&] {
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();  // the round has landed, and every wave has left the other buffers
+  };
+  auto steps = [&](int at, const uint8_t* v, const uint8_t* k, auto&& copies) {
+    acc.step(s, p, v, k, lane, a.scale2, [&](int c) { copies(c); });
+    hidden(64 * at + 32);
+    acc.step(s, p, v + IMG, k + IMG, lane, a.scale2, [&](int c) { copies(HD / 16 + c); });
+    hidden(64 * at + 64);
+  };
+  // (No round behind the last is staged but as zeros, which nobody reads.)
+  for (int at = 0; at < rounds; at += 2) {
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      const int t0 = 64 * at + 32 * u;
-      if (t0 >= last.hi || (t0 + 32 <= first.lo && t0 >= a.sinks)) continue;  // no row sees it
-      float16v s = acc.scores(image + u * IMG, lane);
-      if (t0 + 32 > first.hi || (t0 < last.lo && t0 + 32 > a.sinks)) hide(s, t0, hl, mine.lo, mine.hi, a.sinks);
-      typename Mma<T>::frag p[2];
-      acc.probabilities(s, a.scale2, p);
-      acc.values(image + (2 + u) * IMG, lane, p);
+      if (at + u >= rounds) break;
+      landed();
+      const u32x4 v = v_range(at + u + 1), k = k_range(at + u + 1);
+      steps(at + u, lds[1][u], lds[0][u], [&](int c) {
+        constexpr int N = HD / 32;  // copies of each
+        if (c < N) vs.copy(v, c, v_image(1 - u));
+        else if (c < 2 * N) ks.copy(k, c - N, k_image(1 - u));
+      });
     }
   }
-  if (!active) return;
+  if (tail) {
+    landed();
+    acc.values(lds[1][rounds & 1], lane, p);
+  }
+  if (w0 >= rows) return;
   acc.l += __shfl_xor(acc.l, 32, 64);
   // A value that some rows of the wave do not see meets their probability 0;
   // where it is not finite, their sums are not, and they are taken again. (One
   // query's rows see the same keys.)
-  const uint64_t bad = w0 / a.group == w1 / a.group ? 0 : __builtin_amdgcn_ballot_w64(acc.spoilt());
+  const uint64_t bad = a.query(min(w0, w1)) == a.query(w1) ? 0 : __builtin_amdgcn_ballot_w64(acc.spoilt());
   const uint32_t again = (uint32_t)(bad | bad >> 32);
-  if (w0 + (lane & 31) < rows && !(again >> (lane & 31) & 1)) acc.store(heads.output(row), hl);
+  if (w0 + (lane & 31) < rows && !(again >> (lane & 31) & 1)) acc.store(heads.output(row, a.query(row)), hl);
   for (uint32_t todo = again; todo; todo &= todo - 1) {
     const int at = w0 + __builtin_ctz(todo);
-    if (at < rows) one_row<T, HD>(a, heads, list, r, at, 0, list.n).store(heads.output(at));
+    if (at < rows) one_row<T, HD>(a, heads, list, r.queries, r.keys, at, 0, list.n).store(heads.output(at, a.query(at)));
   }
 }
 
@@ -465,22 +592,16 @@ __global__ __launch_bounds__(64 * kFewWaves) void window_few_kernel(WindowArgs a
   static_assert(kFewWaves * 32 * OP * 4 <= sizeof(lds), "the sums fit in the keys' place");
   const nemo_attention_batch& b = a.b;
   const int kvh = blockIdx.x % a.kv_heads, tile_no = blockIdx.x / a.kv_heads, split = blockIdx.y;
-  const int request = tile_request(b, a.group, 32, tile_no);
-  if (request < 0) return;
-  const Request r(b, request);
-  const int rows = r.queries * a.group, row0 = (tile_no - tile_base(b, a.group, 32, request)) * 32;
+  const Request<32> r(a, tile_no);
+  if (r.i < 0) return;
+  const int rows = r.queries * a.group, row0 = (tile_no - r.tile) * 32;
   if (row0 >= rows) return;
-  const Heads<T> heads(a, r, kvh);
+  const Heads<T> heads(a, r.q0, r.kv0, kvh);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), hl = lane >> 5;
   const int behind = r.keys - r.queries, row1 = min(row0 + 31, rows - 1);
-  const KeyList list(a, behind + row0 / a.group, behind + row1 / a.group, r.keys);
+  const KeyList list(a, behind + a.query(row0), behind + a.query(row1), r.keys);
   const int row = min(row0 + (lane & 31), rows - 1);
-  auto window = [&](int at) {
-    Seen s(a, behind + at / a.group, r.keys);
-    s.lo += list.sinks - list.lo;
-    s.hi += list.sinks - list.lo;
-    return s;
-  };
+  auto window = [&](int at) { return list.window(a, behind + a.query(at), r.keys); };
   const Seen mine = window(row), first = window(row0), last = window(row1);
   const int blocks = (list.n + 31) >> 5;
   const int block0 = (int)((int64_t)blocks * split / part.splits);
@@ -490,20 +611,13 @@ __global__ __launch_bounds__(64 * kFewWaves) void window_few_kernel(WindowArgs a
   const Stager<HD, 32, false> ks(0, k_stride);
   const Stager<HD, 32, true> vs(0, v_stride);
   auto stage = [&](int at, int buffer) {
-    uint8_t* ki = lds[wave][buffer];
-    const int t0 = 32 * at;
-    if (t0 >= list.sinks && t0 + 32 <= list.n) {
-      const int64_t j = list.key(t0);
-      ks.rows((const uint8_t*)heads.k + j * k_stride, ki);
-      vs.rows((const uint8_t*)heads.v + j * v_stride, ki + IMG);
-    } else {
-      auto key = [&](int t) { return list.key(t); };
-      ks.slots((const uint8_t*)heads.k, k_stride, t0, list.n, key, ki);
-      vs.slots((const uint8_t*)heads.v, v_stride, t0, list.n, key, ki + IMG);
-    }
+    const int64_t j = list.key(32 * at);
+    const int valid = list.rows(32 * at);
+    ks.copy(ks.range((const uint8_t*)heads.k + j * k_stride, k_stride, valid), lds[wave][buffer]);
+    vs.copy(vs.range((const uint8_t*)heads.v + j * v_stride, v_stride, valid), lds[wave][buffer] + IMG);
   };
   Rows<T, HD> acc;
-  acc.load(heads.query(row), hl);
+  acc.load(heads.query(row, a.query(row)), hl);
   acc.clear();
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the queries: from here on only copies are counted
   int at = block0 + wave;
@@ -521,7 +635,8 @@ __global__ __launch_bounds__(64 * kFewWaves) void window_few_kernel(WindowArgs a
     float16v s = acc.scores(lds[wave][buffer], lane);
     if (t0 + 32 > first.hi || (t0 < last.lo && t0 + 32 > a.sinks)) hide(s, t0, hl, mine.lo, mine.hi, a.sinks);
     typename Mma<T>::frag p[2];
-    acc.probabilities(s, a.scale2, p);
+    acc.exponentials(s, a.scale2, acc.m, p);
+    acc.settle(s, a.scale2, p);
     acc.values(lds[wave][buffer] + IMG, lane, p);
   }
   // The waves' sums: row-major in LDS, in place of the keys.
@@ -557,7 +672,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void window_few_kernel(WindowArgs a
 #pragma unroll
       for (int c = 0; c < C; ++c) v[c] = fmaf(f, o[(w * 32 + mrow) * OP + c0 + c], v[c]);
     }
-    if (row0 / a.group != row1 / a.group) {
+    if (a.query(row0) != a.query(row1)) {
       float z = l * 0.f;
 #pragma unroll
       for (int c = 0; c < C; ++c) z = fmaf(v[c], 0.f, z);
@@ -567,7 +682,8 @@ __global__ __launch_bounds__(64 * kFewWaves) void window_few_kernel(WindowArgs a
   __syncthreads();
   const int64_t out_row = (int64_t)r.q0 * a.kv_heads * a.group + kvh * a.group;  // of row 0's first head, [query][head]
   auto partial = [&](int at) {
-    return part.rows * split + out_row + (int64_t)(at / a.group) * a.kv_heads * a.group + at % a.group;
+    const int i = a.query(at);
+    return part.rows * split + out_row + (int64_t)i * a.kv_heads * a.group + (at - i * a.group);
   };
   const uint32_t again = spoilt;
   if (valid && !(again >> mrow & 1)) {
@@ -579,7 +695,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void window_few_kernel(WindowArgs a
     } else {
       typedef T vec __attribute__((ext_vector_type(8)));
       const float inv = l == 0.f ? 0.f : 1.0f / l;
-      T* out = heads.output(row0 + mrow) + c0;
+      T* out = heads.output(row0 + mrow, a.query(row0 + mrow)) + c0;
 #pragma unroll
       for (int c = 0; c < C; c += 8) {
         vec t;
@@ -594,13 +710,13 @@ __global__ __launch_bounds__(64 * kFewWaves) void window_few_kernel(WindowArgs a
   for (int n = 0; todo; todo &= todo - 1, ++n) {
     if (n % kFewWaves != wave) continue;
     const int at = row0 + __builtin_ctz(todo);
-    const OneRow<T, HD> one = one_row<T, HD>(a, heads, list, r, at, 32 * block0, min(32 * block1, list.n));
+    const OneRow<T, HD> one = one_row<T, HD>(a, heads, list, r.queries, r.keys, at, 32 * block0, min(32 * block1, list.n));
     if (part.ml) {
       if (lane == 0) part.ml[partial(at)] = make_float2(one.m, one.l);
 #pragma unroll
       for (int c = 0; c < HD / 64; ++c) part.o[partial(at) * HD + lane + 64 * c] = one.o[c];
     } else {
-      one.store(heads.output(at));
+      one.store(heads.output(at, a.query(at)));
     }
   }
 }
@@ -611,12 +727,12 @@ __global__ __launch_bounds__(256) void window_join_kernel(WindowArgs a, Partials
   constexpr int R = 4;
   const nemo_attention_batch& b = a.b;
   const int kvh = blockIdx.x % a.kv_heads, tile_no = blockIdx.x / a.kv_heads;
-  const int request = tile_request(b, a.group, R, tile_no);
-  if (request < 0) return;
-  const Request r(b, request);
-  const int row = (tile_no - tile_base(b, a.group, R, request)) * R + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const Request<R> r(a, tile_no);
+  if (r.i < 0) return;
+  const int row = (tile_no - r.tile) * R + (threadIdx.x >> 6), lane = threadIdx.x & 63;
   if (row >= r.queries * a.group) return;
-  const int64_t at = (int64_t)(r.q0 + row / a.group) * a.kv_heads * a.group + kvh * a.group + row % a.group;
+  const int i = a.query(row), h = kvh * a.group + (row - i * a.group);
+  const int64_t at = (int64_t)(r.q0 + i) * a.kv_heads * a.group + h;
   const float2 ml = lane < part.splits ? part.ml[part.rows * lane + at] : make_float2(-INFINITY, 0.f);
   float m = ml.x;
 #pragma unroll
@@ -634,7 +750,7 @@ __global__ __launch_bounds__(256) void window_join_kernel(WindowArgs a, Partials
 #pragma unroll
     for (int c = 0; c < HD / 64; ++c) v[c] = fmaf(fz, part.o[(part.rows * z + at) * HD + lane + 64 * c], v[c]);
   }
-  T* out = (T*)b.out + (int64_t)(r.q0 + row / a.group) * b.out_row + (kvh * a.group + row % a.group) * b.out_head;
+  T* out = (T*)b.out + (int64_t)(r.q0 + i) * b.out_row + h * b.out_head;
 #pragma unroll
   for (int c = 0; c < HD / 64; ++c) out[lane + 64 * c] = (T)(l == 0.f ? 0.f : v[c] / l);
 }
@@ -663,7 +779,9 @@ size_t window_workspace(const nemo_attention_config& c, int count, int64_t q_row
 
 hipError_t launch_window_attention(const nemo_attention_config& c, const nemo_attention_batch& b, hipStream_t stream) {
   if (b.count == 0 || b.q_rows == 0) return hipSuccess;
-  WindowArgs a{b, c.kv_heads, c.q_heads / c.kv_heads, 0, 0, 0, 0.f};
+  WindowArgs a{b, c.kv_heads, c.q_heads / c.kv_heads, 0, 0, 0, 0.f, 0, 0};
+  while (1 << a.shift < a.group) ++a.shift;
+  a.magic = (uint32_t)((((uint64_t)1 << a.shift) - a.group) * ((uint64_t)1 << 32) / a.group + 1);
   auto bound = [](int v) { return v < 0 ? kUnbounded : std::min(v, kUnbounded); };
   a.left = bound(c.left);
   a.right = bound(c.right);
