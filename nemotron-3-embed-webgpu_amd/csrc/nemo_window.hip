@@ -161,7 +161,7 @@ __device__ __forceinline__ int v_swizzle(int row) {
 }
 
 // Copies of 16 bytes a lane into LDS at `to` + 16 lane, from a buffer's range
-// (zeros past its end). The compiler, which knows of the builtin for this that
+// (zeros past its end) or an address. The compiler, which knows of the builtin for this that
 // it writes LDS, waits for every copy in flight before each transposed read;
 // written as here it has no register to be waited for, and the loops wait
 // for their images themselves.
@@ -172,6 +172,13 @@ __device__ __forceinline__ void copy_range(u32x4 range, uint32_t offset, const u
                : "s"(lds_address(to)), "v"(offset), "s"(range)
                : "memory");
 }
+__device__ __forceinline__ void copy_address(const void* from, const uint8_t* to) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
+               :
+               : "s"(lds_address(to)), "v"(from)
+               : "memory");
+}
+
 // Copies of ROWS key rows into an image by one wave, 1 KB an instruction:
 // rows first .. first + ROWS of a 32-row image (or of two that follow each
 // other). off: the lane's byte offsets from row 0 of the image, for rows that
@@ -252,6 +259,11 @@ struct Rows {
   __device__ __forceinline__ void load(const T* row, int hl) {
 #pragma unroll
     for (int c = 0; c < DC; ++c) q[c] = *(const frag*)(row + 16 * c + 8 * hl);
+  }
+  // The same from an image of the rows.
+  __device__ __forceinline__ void load_image(const uint8_t* image, int lane) {
+#pragma unroll
+    for (int c = 0; c < DC; ++c) q[c] = key(image, lane, c);
   }
   __device__ __forceinline__ frag key(const uint8_t* image, int lane, int c) const {
     const int row = lane & 31;
@@ -385,7 +397,8 @@ struct Rows {
     p[0] = next[0];
     p[1] = next[1];
   }
-  __device__ __forceinline__ void store(T* out, int hl) const {
+  // The lane's row into an image, at that image row.
+  __device__ __forceinline__ void store(T* out, int row, int hl) const {
     typedef T vec __attribute__((ext_vector_type(4)));
     const float inv = l == 0.f ? 0.f : 1.0f / l;
 #pragma unroll
@@ -395,7 +408,7 @@ struct Rows {
         vec v;
 #pragma unroll
         for (int e = 0; e < 4; ++e) v[e] = (T)(o[db][4 * j + e] * inv);
-        *(vec*)(out + 32 * db + 8 * j + 4 * hl) = v;
+        *(vec*)(out + 8 * ((4 * db + j) ^ k_swizzle<HD>(row)) + 4 * hl) = v;
       }
   }
   // Whether a value of the lane's row is not finite.
@@ -409,12 +422,18 @@ struct Rows {
   }
 };
 
-// Scores of hidden slots of the block at t0 become -infinity.
+// Scores of hidden slots of the block at t0 become -infinity: bit c of `seen` is
+// whether slot t0 + c is t < hi with t >= lo or t < sinks.
 __device__ __forceinline__ void hide(float16v& s, int t0, int hl, int lo, int hi, int sinks) {
+  auto below = [&](int t) {  // bits of the slots before t
+    const int n = max(0, min(t - t0, 32));
+    return n == 32 ? ~0u : (1u << n) - 1;
+  };
+  const uint32_t seen = (below(hi) & (~below(lo) | below(sinks))) >> (4 * hl);
 #pragma unroll
   for (int r = 0; r < 16; ++r) {
-    const int t = t0 + 8 * (r >> 2) + 4 * hl + (r & 3);
-    if (!(t < hi && (t >= lo || t < sinks))) s[r] = -INFINITY;
+    const uint32_t keep = (uint32_t)((int)(seen << (31 - 8 * (r >> 2) - (r & 3))) >> 31);
+    s[r] = __uint_as_float((__float_as_uint(s[r]) & keep) | (0xff800000u & ~keep));
   }
 }
 
@@ -440,6 +459,15 @@ struct Heads {
     return out + i * out_row + (row - i * group) * out_head;
   }
 };
+
+// The rows of an image of 32, 16 bytes a lane: do(i, row, chunk) for row kPer i +
+// lane / kChunks of the image and its chunk, i < HD / 16.
+template <int HD, typename Do>
+__device__ __forceinline__ void image_rows(int lane, Do&& each) {
+  constexpr int kChunks = HD / 8, kPer = 64 / kChunks;
+#pragma unroll
+  for (int i = 0; i < kKeys / kPer; ++i) each(i, kPer * i + lane / kChunks, lane % kChunks);
+}
 
 // A row over the slots [t0, t1) that it sees, key by key.
 template <typename T, int HD>
@@ -508,17 +536,25 @@ __global__ __launch_bounds__(256, HD == 128 ? 2 : 3) void window_tile_kernel(Win
       hide(s, t0, hl, mine.lo, mine.hi, a.sinks);
     }
   };
+  uint8_t* const rows_image = lds[wave >> 1][1] + (wave & 1) * IMG;  // of this wave's queries, later outputs
   if (rounds) {
-    // K of the first block, in the place of the second round's V
+    // K of the first block, where V's block before the first would be (p is 0 for that)
     const Stager<HD, 8, false> k0(8 * wave, k_stride);
     k0.copy(k0.range((const uint8_t*)heads.k + list.key(0) * k_stride, k_stride, list.rows(0)),
-            lds[1][1] + 8 * wave * 2 * HD);
-    acc.load(heads.query(row, a.query(row)), hl);
-    vs.copy(v_range(0), v_image(0));
+            lds[1][0] + 8 * wave * 2 * HD);
+    image_rows<HD>(lane, [&](int i, int r, int chunk) {
+      const int at = min(w0 + r, rows - 1);
+      copy_address(heads.query(at, a.query(at)) + 8 * (chunk ^ k_swizzle<HD>(r)), rows_image + 1024 * i);
+    });
+    if (wave >> 1) vs.copy(v_range(0), v_image(0));
     ks.copy(k_range(0), k_image(0));
-    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(IMG / 1024) : "memory");
+    if (wave >> 1)
+      asm volatile("s_waitcnt vmcnt(%0)" ::"n"(IMG / 1024) : "memory");
+    else
+      asm volatile("s_waitcnt vmcnt(%0)" ::"n"(IMG / 2048) : "memory");
     __builtin_amdgcn_s_barrier();
-    s = acc.scores(lds[1][1], lane);
+    acc.load_image(rows_image, lane);
+    s = acc.scores(lds[1][0], lane);
     hidden(0);
   }
   typename Mma<T>::frag p[2] = {};
@@ -551,14 +587,21 @@ __global__ __launch_bounds__(256, HD == 128 ? 2 : 3) void window_tile_kernel(Win
     landed();
     acc.values(lds[1][rounds & 1], lane, p);
   }
-  if (w0 >= rows) return;
   acc.l += __shfl_xor(acc.l, 32, 64);
   // A value that some rows of the wave do not see meets their probability 0;
   // where it is not finite, their sums are not, and they are taken again. (One
   // query's rows see the same keys.)
   const uint64_t bad = a.query(min(w0, w1)) == a.query(w1) ? 0 : __builtin_amdgcn_ballot_w64(acc.spoilt());
   const uint32_t again = (uint32_t)(bad | bad >> 32);
-  if (w0 + (lane & 31) < rows && !(again >> (lane & 31) & 1)) acc.store(heads.output(row, a.query(row)), hl);
+  // Outputs go through LDS: whole rows to memory, 16 bytes a lane.
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  acc.store((T*)(rows_image + (lane & 31) * 2 * HD), lane & 31, hl);
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  image_rows<HD>(lane, [&](int i, int r, int chunk) {
+    const u32x4 v = *(const u32x4*)(rows_image + r * 2 * HD + 16 * (chunk ^ k_swizzle<HD>(r)));
+    if (w0 + r < rows && !(again >> r & 1)) *(u32x4*)(heads.output(w0 + r, a.query(w0 + r)) + 8 * chunk) = v;
+  });
   for (uint32_t todo = again; todo; todo &= todo - 1) {
     const int at = w0 + __builtin_ctz(todo);
     if (at < rows) one_row<T, HD>(a, heads, list, r.queries, r.keys, at, 0, list.n).store(heads.output(at, a.query(at)));
