@@ -28,9 +28,7 @@ hipError_t launch_norm8(const nemo_norm_args& args, hipStream_t stream);
 // Bounds of a window as the kernels take them: unbounded sides and larger
 // bounds are kUnbounded, which no sum of a position and a bound overflows.
 constexpr int kUnbounded = 1 << 30;
-// Pieces the keys of each query are split into when the caller gives a
-// workspace, and the bytes of it.
-int window_splits(const nemo_attention_config& c, int count, int64_t q_rows, int64_t max_kv);
+// Bytes of workspace with which the keys of a batch's queries are split.
 size_t window_workspace(const nemo_attention_config& c, int count, int64_t q_rows, int64_t max_kv);
 hipError_t launch_window_attention(const nemo_attention_config& c, const nemo_attention_batch& b, hipStream_t stream);
 

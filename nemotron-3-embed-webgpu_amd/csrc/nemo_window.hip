@@ -256,12 +256,7 @@ struct Rows {
 #pragma unroll
       for (int r = 0; r < 16; ++r) o[db][r] = 0.f;
   }
-  __device__ __forceinline__ void load(const T* row, int hl) {
-#pragma unroll
-    for (int c = 0; c < DC; ++c) q[c] = *(const frag*)(row + 16 * c + 8 * hl);
-  }
-  // The same from an image of the rows.
-  __device__ __forceinline__ void load_image(const uint8_t* image, int lane) {
+  __device__ __forceinline__ void load(const uint8_t* image, int lane) {
 #pragma unroll
     for (int c = 0; c < DC; ++c) q[c] = key(image, lane, c);
   }
@@ -553,7 +548,7 @@ __global__ __launch_bounds__(256, HD == 128 ? 2 : 3) void window_tile_kernel(Win
     else
       asm volatile("s_waitcnt vmcnt(%0)" ::"n"(IMG / 2048) : "memory");
     __builtin_amdgcn_s_barrier();
-    acc.load_image(rows_image, lane);
+    acc.load(rows_image, lane);
     s = acc.scores(lds[1][0], lane);
     hidden(0);
   }
@@ -609,13 +604,14 @@ __global__ __launch_bounds__(256, HD == 128 ? 2 : 3) void window_tile_kernel(Win
 }
 
 // ---------------------------------------------------------------------------
-// Few rows: the 4 waves of a workgroup take the same 32 rows and every fourth
-// block of 32 keys each, staged by the wave for itself two blocks deep (no
-// barrier in the loop), and add up in LDS. With `splits` above 1 the blocks are
-// dealt out to that many workgroups as well, whose sums a second kernel joins.
+// Few rows: the 8 waves of a workgroup take the same 32 rows and every eighth
+// block of 32 keys each, staged by the wave for itself (no barrier in the
+// loop), and add up in LDS. A wave's next K is copied while it works on V, its
+// next V while it works on K. With `splits` above 1 the blocks are dealt out
+// to that many workgroups as well, whose sums a second kernel joins.
 // ---------------------------------------------------------------------------
 
-constexpr int kFewWaves = 4;
+constexpr int kFewWaves = 8;
 
 // Sums of a split: the row's reference maximum and sum, and its output values.
 struct Partials {
@@ -628,11 +624,13 @@ struct Partials {
 template <typename T, int HD>
 __global__ __launch_bounds__(64 * kFewWaves) void window_few_kernel(WindowArgs a, Partials part) {
   constexpr int IMG = 2 * kKeys * HD;
-  constexpr int OP = HD + 4;  // row of the sums in LDS, in floats
-  __shared__ __attribute__((aligned(16))) uint8_t lds[kFewWaves][2][2 * IMG];
+  __shared__ __attribute__((aligned(16))) uint8_t lds[kFewWaves][2 * IMG];  // K, V; later the waves' sums
   __shared__ float2 sums[kFewWaves][32];
   __shared__ uint32_t spoilt;
-  static_assert(kFewWaves * 32 * OP * 4 <= sizeof(lds), "the sums fit in the keys' place");
+  // The float4 at column 4 c of a wave's row of sums.
+  auto sum_at = [&](int wave, int row, int c) {
+    return (float4v*)lds + (wave * 32 + row) * (HD / 4) + (c ^ (row & 15));
+  };
   const nemo_attention_batch& b = a.b;
   const int kvh = blockIdx.x % a.kv_heads, tile_no = blockIdx.x / a.kv_heads, split = blockIdx.y;
   const Request<32> r(a, tile_no);
@@ -653,40 +651,53 @@ __global__ __launch_bounds__(64 * kFewWaves) void window_few_kernel(WindowArgs a
   const int64_t k_stride = 2 * b.k_row, v_stride = 2 * b.v_row;
   const Stager<HD, 32, false> ks(0, k_stride);
   const Stager<HD, 32, true> vs(0, v_stride);
-  auto stage = [&](int at, int buffer) {
-    const int64_t j = list.key(32 * at);
-    const int valid = list.rows(32 * at);
-    ks.copy(ks.range((const uint8_t*)heads.k + j * k_stride, k_stride, valid), lds[wave][buffer]);
-    vs.copy(vs.range((const uint8_t*)heads.v + j * v_stride, v_stride, valid), lds[wave][buffer] + IMG);
+  uint8_t* const image = lds[wave];
+  auto stage_k = [&](int at) {
+    if (at >= block1) return;
+    ks.copy(ks.range((const uint8_t*)heads.k + list.key(32 * at) * k_stride, k_stride, list.rows(32 * at)), image);
+  };
+  auto stage_v = [&](int at) {
+    if (at >= block1) return;
+    vs.copy(vs.range((const uint8_t*)heads.v + list.key(32 * at) * v_stride, v_stride, list.rows(32 * at)),
+            image + IMG);
   };
   Rows<T, HD> acc;
-  acc.load(heads.query(row, a.query(row)), hl);
   acc.clear();
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the queries: from here on only copies are counted
   int at = block0 + wave;
-  if (at < block1) stage(at, 0);
-  for (int buffer = 0; at < block1; at += kFewWaves, buffer ^= 1) {
-    if (at + kFewWaves < block1) {
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the other buffer's reads are done
-      stage(at + kFewWaves, buffer ^ 1);
-      asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * IMG / 1024) : "memory");
-    } else {
-      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    }
+  if (at < block1) {
+    // the rows' image, where V goes next
+    image_rows<HD>(lane, [&](int i, int r, int chunk) {
+      const int qrow = min(row0 + r, rows - 1);
+      copy_address(heads.query(qrow, a.query(qrow)) + 8 * (chunk ^ k_swizzle<HD>(r)), image + IMG + 1024 * i);
+    });
+    stage_k(at);
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(IMG / 1024) : "memory");
+    acc.load(image + IMG, lane);
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    stage_v(at);
+  }
+  for (; at < block1; at += kFewWaves) {
     const int t0 = 32 * at;
-    if (t0 >= last.hi || (t0 + 32 <= first.lo && t0 >= a.sinks)) continue;
-    float16v s = acc.scores(lds[wave][buffer], lane);
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(IMG / 1024) : "memory");  // K, not yet V
+    float16v s = acc.scores(image, lane);
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    stage_k(at + kFewWaves);
     if (t0 + 32 > first.hi || (t0 < last.lo && t0 + 32 > a.sinks)) hide(s, t0, hl, mine.lo, mine.hi, a.sinks);
     typename Mma<T>::frag p[2];
     acc.exponentials(s, a.scale2, acc.m, p);
     acc.settle(s, a.scale2, p);
-    acc.values(lds[wave][buffer] + IMG, lane, p);
+    if (at + kFewWaves < block1)
+      asm volatile("s_waitcnt vmcnt(%0)" ::"n"(IMG / 1024) : "memory");  // V, not yet the next K
+    else
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    acc.values(image + IMG, lane, p);
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    stage_v(at + kFewWaves);
   }
   // The waves' sums: row-major in LDS, in place of the keys.
   acc.l += __shfl_xor(acc.l, 32, 64);
   if (threadIdx.x == 0) spoilt = 0;
   __syncthreads();
-  float* o = (float*)lds;
   if (row0 + (lane & 31) < rows) {
     if (hl == 0) sums[wave][lane] = make_float2(acc.m, acc.l);
 #pragma unroll
@@ -694,13 +705,13 @@ __global__ __launch_bounds__(64 * kFewWaves) void window_few_kernel(WindowArgs a
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const float4v v = {acc.o[db][4 * j], acc.o[db][4 * j + 1], acc.o[db][4 * j + 2], acc.o[db][4 * j + 3]};
-        *(float4v*)(o + (wave * 32 + (lane & 31)) * OP + 32 * db + 8 * j + 4 * hl) = v;
+        *sum_at(wave, lane & 31, 8 * db + 2 * j + hl) = v;
       }
   }
   __syncthreads();
-  // Thread: HD / 8 columns of one row.
-  constexpr int C = HD / 8;
-  const int mrow = threadIdx.x >> 3, c0 = (threadIdx.x & 7) * C;
+  // Thread: C columns of one row.
+  constexpr int C = HD / (2 * kFewWaves);
+  const int mrow = threadIdx.x / (2 * kFewWaves), c0 = threadIdx.x % (2 * kFewWaves) * C;
   const bool valid = row0 + mrow < rows;
   float m = -INFINITY, l = 0.f, v[C] = {};
   if (valid) {
@@ -713,7 +724,11 @@ __global__ __launch_bounds__(64 * kFewWaves) void window_few_kernel(WindowArgs a
       const float f = ml.x == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(ml.x - m);
       l = fmaf(f, ml.y, l);
 #pragma unroll
-      for (int c = 0; c < C; ++c) v[c] = fmaf(f, o[(w * 32 + mrow) * OP + c0 + c], v[c]);
+      for (int c = 0; c < C; c += 4) {
+        const float4v o = *sum_at(w, mrow, (c0 + c) / 4);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[c + e] = fmaf(f, o[e], v[c + e]);
+      }
     }
     if (a.query(row0) != a.query(row1)) {
       float z = l * 0.f;
@@ -736,16 +751,12 @@ __global__ __launch_bounds__(64 * kFewWaves) void window_few_kernel(WindowArgs a
 #pragma unroll
       for (int c = 0; c < C; c += 4) *(float4v*)(part.o + at * HD + c0 + c) = float4v{v[c], v[c + 1], v[c + 2], v[c + 3]};
     } else {
-      typedef T vec __attribute__((ext_vector_type(8)));
+      typedef T vec __attribute__((ext_vector_type(C)));
       const float inv = l == 0.f ? 0.f : 1.0f / l;
-      T* out = heads.output(row0 + mrow, a.query(row0 + mrow)) + c0;
+      vec t;
 #pragma unroll
-      for (int c = 0; c < C; c += 8) {
-        vec t;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) t[e] = (T)(v[c + e] * inv);
-        *(vec*)(out + c) = t;
-      }
+      for (int c = 0; c < C; ++c) t[c] = (T)(v[c] * inv);
+      *(vec*)(heads.output(row0 + mrow, a.query(row0 + mrow)) + c0) = t;
     }
   }
   // As in window_tile_kernel: rows spoilt by values that they do not see.
@@ -764,59 +775,84 @@ __global__ __launch_bounds__(64 * kFewWaves) void window_few_kernel(WindowArgs a
   }
 }
 
-// Joins the splits: a wave a row, lane z the weight of split z (at most 64).
+// Joins the splits, at most 64: a workgroup a row. Thread (g, c) adds columns 4
+// c.. of splits g, g + G, ..., and the G sums are added in order.
 template <typename T, int HD>
 __global__ __launch_bounds__(256) void window_join_kernel(WindowArgs a, Partials part) {
-  constexpr int R = 4;
+  constexpr int C = HD / 4, G = 256 / C;
+  __shared__ float weight[64];
+  __shared__ float4v sums[G][C];
   const nemo_attention_batch& b = a.b;
   const int kvh = blockIdx.x % a.kv_heads, tile_no = blockIdx.x / a.kv_heads;
-  const Request<R> r(a, tile_no);
+  const Request<1> r(a, tile_no);
   if (r.i < 0) return;
-  const int row = (tile_no - r.tile) * R + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int row = tile_no - r.tile, lane = threadIdx.x & 63;
   if (row >= r.queries * a.group) return;
   const int i = a.query(row), h = kvh * a.group + (row - i * a.group);
   const int64_t at = (int64_t)(r.q0 + i) * a.kv_heads * a.group + h;
+  // every wave: lane z's split
   const float2 ml = lane < part.splits ? part.ml[part.rows * lane + at] : make_float2(-INFINITY, 0.f);
   float m = ml.x;
 #pragma unroll
   for (int x = 32; x > 0; x >>= 1) m = fmaxf(m, __shfl_xor(m, x, 64));
-  const bool empty = ml.x == -INFINITY && ml.y == 0.f;
+  const bool empty = ml.x == -INFINITY && ml.y == 0.f;  // saw nothing; its values mean nothing
   const float f = empty ? 0.f : ml.x == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(ml.x - m);
   float l = empty ? 0.f : f * ml.y;
 #pragma unroll
   for (int x = 32; x > 0; x >>= 1) l += __shfl_xor(l, x, 64);
-  const uint64_t full = ~__builtin_amdgcn_ballot_w64(empty);
-  float v[HD / 64] = {};
-  for (int z = 0; z < part.splits; ++z) {
-    if (!(full >> z & 1)) continue;
-    const float fz = __shfl(f, z, 64);
+  if (threadIdx.x < 64) weight[lane] = empty ? -1.f : f;
+  __syncthreads();
+  const int c = threadIdx.x % C, g = threadIdx.x / C;
+  float4v v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int z = g; z < part.splits; z += G) {
+    const float4v o = *(const float4v*)(part.o + (part.rows * z + at) * HD + 4 * c);
+    const float w = weight[z];
 #pragma unroll
-    for (int c = 0; c < HD / 64; ++c) v[c] = fmaf(fz, part.o[(part.rows * z + at) * HD + lane + 64 * c], v[c]);
+    for (int e = 0; e < 4; ++e) v[e] = w == -1.f ? v[e] : fmaf(w, o[e], v[e]);
   }
-  T* out = (T*)b.out + (int64_t)(r.q0 + i) * b.out_row + h * b.out_head;
+  sums[g][c] = v;
+  __syncthreads();
+  if (threadIdx.x >= HD) return;
+  float sum = 0.f;
 #pragma unroll
-  for (int c = 0; c < HD / 64; ++c) out[lane + 64 * c] = (T)(l == 0.f ? 0.f : v[c] / l);
+  for (int k = 0; k < G; ++k) sum += sums[k][threadIdx.x / 4][threadIdx.x % 4];
+  T* out = (T*)b.out + (int64_t)(r.q0 + i) * b.out_row + h * b.out_head;
+  out[threadIdx.x] = (T)(l == 0.f ? 0.f : sum / l);
 }
 
-// Whether the keys are dealt out to the waves of a workgroup, not the rows:
-// when tiles of 128 rows would leave CUs without one.
-bool few_rows(const nemo_attention_config& c, int64_t q_rows) {
-  return q_rows * c.q_heads < 256 * kTileRows;
+// Which kernel a batch takes and how its keys are split, by its sizes alone.
+// `tiles` of 32 rows, of which window_few_kernel has `places` on the chip at a
+// time, and the keys that a query sees. Few rows: while the tiles fit (32
+// heads of 64, 8 KV heads, microseconds few : tile kernel: 500 tokens +-128 9.2
+// : 9.0, 1000 15.4 : 9.6; 512 behind 3000, window 512, 10.9 : 11.9), or nearly
+// and with many keys each (32 heads of 128: 512 tokens behind 8192 keys 106 :
+// 140, 4 x 128 of a 1024-key window 24.9 : 24.4, 64 single tokens of up to 4096
+// 174 : 185). A split costs a second launch, 3.5 us, and is taken from 1280 keys
+// (single token, 32 heads of 64, unsplit : split: 1100 keys 8.3 : 9.4, 1800 10.5
+// : 9.4, 8000 33.6 : 11.0), into pieces of 256 keys and more for more rows, whose
+// sums are written and read again (8 tokens over 8192 keys of 128: pieces of 256
+// 20.6, of 512 15.7).
+struct Plan {
+  bool few;
+  int splits;
+};
+Plan window_plan(const nemo_attention_config& c, int count, int64_t q_rows, int64_t max_kv) {
+  if (count == 0 || q_rows == 0) return {false, 1};
+  const int64_t rows = q_rows * (c.q_heads / c.kv_heads);
+  const int64_t tiles = std::max<int64_t>(rows / 32, count) * c.kv_heads, places = c.head_dim == 64 ? 512 : 256;
+  int64_t keys = max_kv;
+  if (c.left >= 0 && c.right >= 0) keys = std::min(keys, (int64_t)c.left + c.right + 1 + c.sinks);
+  if (tiles > places && (tiles > 2 * places || keys < 1024)) return {false, 1};
+  const int64_t piece = 256 + 8 * std::min<int64_t>(32, rows / count);
+  const int64_t splits = keys < 1280 ? 1 : std::min<int64_t>({places / tiles, keys / piece, 64});
+  return {true, (int)std::max<int64_t>(1, splits)};
 }
 
 }  // namespace
 
-int window_splits(const nemo_attention_config& c, int count, int64_t q_rows, int64_t max_kv) {
-  if (count == 0 || q_rows == 0 || !few_rows(c, q_rows)) return 1;
-  const int64_t tiles = std::max<int64_t>(q_rows * (c.q_heads / c.kv_heads) / 32, count) * c.kv_heads;
-  int64_t keys = max_kv;
-  if (c.left >= 0 && c.right >= 0)
-    keys = std::min(keys, (int64_t)c.left + c.right + c.sinks + (q_rows + count - 1) / count);
-  return (int)std::max<int64_t>(1, std::min<int64_t>({(512 + tiles - 1) / tiles, keys / 256, 64}));
-}
-
 size_t window_workspace(const nemo_attention_config& c, int count, int64_t q_rows, int64_t max_kv) {
-  const int splits = window_splits(c, count, q_rows, max_kv);
+  const int splits = window_plan(c, count, q_rows, max_kv).splits;
   return splits == 1 ? 0 : (size_t)splits * q_rows * c.q_heads * (c.head_dim * 4 + 8);
 }
 
@@ -830,7 +866,8 @@ hipError_t launch_window_attention(const nemo_attention_config& c, const nemo_at
   a.right = bound(c.right);
   a.sinks = std::min(c.sinks, kUnbounded);
   a.scale2 = (c.scale > 0.f ? c.scale : 1.0f / sqrtf((float)c.head_dim)) * 1.4426950408889634f;
-  const int splits = b.workspace ? window_splits(c, b.count, b.q_rows, b.max_kv) : 1;
+  const Plan plan = window_plan(c, b.count, b.q_rows, b.max_kv);
+  const int splits = b.workspace ? plan.splits : 1;
   const int64_t rows = b.q_rows * c.q_heads;
   Partials part{nullptr, nullptr, rows, splits};
   if (splits > 1) {
@@ -841,12 +878,12 @@ hipError_t launch_window_attention(const nemo_attention_config& c, const nemo_at
   auto launch = [&](auto type, auto hd) {
     constexpr int HD = decltype(hd)::value;
     typedef decltype(type) T;
-    if (!few_rows(c, b.q_rows)) {
+    if (!plan.few) {
       window_tile_kernel<T, HD><<<tiles(kTileRows), 256, 0, stream>>>(a);
       return;
     }
     window_few_kernel<T, HD><<<dim3(tiles(32), splits), 64 * kFewWaves, 0, stream>>>(a, part);
-    if (splits > 1) window_join_kernel<T, HD><<<tiles(4), 256, 0, stream>>>(a, part);
+    if (splits > 1) window_join_kernel<T, HD><<<tiles(1), 256, 0, stream>>>(a, part);
   };
   auto typed = [&](auto type) {
     if (c.head_dim == 64) launch(type, std::integral_constant<int, 64>{});

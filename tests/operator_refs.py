@@ -82,7 +82,12 @@ def attention(q, k, v, left, right, sinks, scale):
     A score is D products summed in 32 bits and scaled; its error is the
     probability's relative error, twice (the sum over the probabilities has
     it too). Probabilities are rounded to the type before the product with v,
-    which sums in 32 bits; the output is rounded once."""
+    which sums in 32 bits; the output is rounded once.
+
+    Half precision's probabilities below 2^-14 are rounded by up to 2^-25
+    whatever they are: the kernels take them against the row's largest score
+    at the time, whose own is 1, so their sum is at least 1 and the n seen
+    keys add 2^-25 (sum |v| + n |out|)."""
     n, H, D = q.shape
     m, K = k.shape[0], k.shape[1]
     out = torch.zeros(n, H, D, dtype=torch.float64)
@@ -106,4 +111,6 @@ def attention(q, k, v, left, right, sinks, scale):
         weight = p @ vv.abs()
         err = 2 * mag * (D + 4) * 2.0 ** -24 + HALF[q.dtype] + (m / 16 + 32) * 2.0 ** -24
         tol[:, h] = weight * err + HALF[q.dtype] * out[:, h].abs() + TINY[q.dtype]
+        seen = see.double()
+        tol[:, h] += TINY[q.dtype] * (seen @ vv.abs() + seen.sum(1, keepdim=True) * out[:, h].abs())
     return out, tol

@@ -298,10 +298,24 @@ WINDOWS = [(-1, -1, 0), (-1, 0, 0), (63, 0, 4), (0, 0, 0), (0, 0, 1), (130, 0, 7
            (-1, 5, 0), (5, -1, 3), (1000, 1000, 1), (0, 0, 1000)]
 
 
+# query and KV heads of batches that take the kernel for few rows and that for many
+FEW_MANY = [(4, 2), (64, 32)]
+
+
 @pytest.mark.parametrize("dtype,D", [(F16, 64), (F16, 128), (BF16, 64), (BF16, 128)])
 @pytest.mark.parametrize("left,right,sinks", WINDOWS)
-def test_attention_packed(torch_cuda, dtype, D, left, right, sinks):
-    Batch(dtype, 4, 2, D, left, right, sinks, [1, 200, 0, 33, 257, 64]).run().check()
+@pytest.mark.parametrize("H,K", FEW_MANY)
+def test_attention_packed(torch_cuda, H, K, dtype, D, left, right, sinks):
+    Batch(dtype, H, K, D, left, right, sinks, [1, 200, 0, 33, 257, 64]).run().check()
+
+
+@pytest.mark.parametrize("dtype,D", [(F16, 64), (BF16, 128)])
+def test_attention_many_requests(torch_cuda, dtype, D):
+    """More requests than a wave has lanes, many of them empty or of one token."""
+    lens = [(7 * i * i + 3 * i) % 23 for i in range(150)]
+    Batch(dtype, 4, 1, D, 9, 0, 2, lens).run().check()
+    Batch(dtype, 24, 8, D, 9, 2, 2, lens).run().check()
+    Batch(dtype, 8, 8, D, 50, 0, 2, [min(1, n) for n in lens], [n * 11 for n in lens]).run().check()
 
 
 @pytest.mark.parametrize("dtype,D", [(F16, 64), (BF16, 128)])
@@ -309,6 +323,8 @@ def test_attention_packed(torch_cuda, dtype, D, left, right, sinks):
 def test_attention_head_groups(torch_cuda, dtype, D, H, K):
     Batch(dtype, H, K, D, 40, 0, 2, [70, 1, 19]).run().check()
     Batch(dtype, H, K, D, 300, 0, 2, [1, 2, 1], [700, 350, 1]).run().check()
+    many = 520 * 32 // H  # rows for the kernel for many
+    Batch(dtype, H, K, D, 40, 7, 2, [many - 300, 300 if many > 300 else 0] if many > 300 else [many]).run().check()
 
 
 @pytest.mark.parametrize("dtype,D", [(F16, 64), (F16, 128), (BF16, 64), (BF16, 128)])
@@ -326,6 +342,7 @@ def test_attention_pieces(torch_cuda, dtype, D, left, right, sinks):
     """Several tokens behind a cache; requests without tokens, without keys,
     and with fewer keys than queries, whose first queries see nothing."""
     Batch(dtype, 4, 1, D, left, right, sinks, [5, 0, 100, 3, 40, 17], [900, 30, 700, 0, 25, 17]).run().check()
+    Batch(dtype, 64, 16, D, left, right, sinks, [5, 0, 100, 3, 240, 17], [900, 30, 700, 0, 25, 17]).run().check()
 
 
 @pytest.mark.parametrize("workspace", [True, False])
@@ -347,12 +364,28 @@ def test_attention_scale_and_extreme_scores(torch_cuda):
     b.check(scale=1.0)
 
 
+@pytest.mark.parametrize("H,K", FEW_MANY)
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_attention_scores_that_rise_and_fall(torch_cuda, H, K, dtype):
+    """Along the keys scores rise by thousands, fall and rise again, so that
+    the reference of the probabilities has to follow; a huge score that a
+    query does not see has no part in it."""
+    n = 300
+    b = Batch(dtype, H, K, 64, 150, 20, 3, [n], [n], poison=False)
+    size = torch.cat([torch.linspace(0.01, 40, 100), torch.linspace(40, 0.01, 100), torch.linspace(0.01, 90, 100)])
+    b.k = (b.k[:n] * size[:, None, None]).to(dtype)
+    b.v = b.v[:n]
+    b.dk, b.dv = b.k.cuda(), b.v.cuda()
+    b.run().check()
+
+
 @pytest.mark.parametrize("dtype,D", [(F16, 64), (BF16, 128)])
-def test_attention_hidden_values_reach_no_result(torch_cuda, dtype, D):
+@pytest.mark.parametrize("H,K", FEW_MANY)
+def test_attention_hidden_values_reach_no_result(torch_cuda, H, K, dtype, D):
     """Keys that some queries of a request see and others do not: NaN and
     infinities in them reach the results of the former alone."""
     left, right, sinks, n = 20, 0, 2, 300
-    b = Batch(dtype, 4, 2, D, left, right, sinks, [n], [n], poison=False)
+    b = Batch(dtype, H, K, D, left, right, sinks, [n], [n], poison=False)
     bad = [7, 150, 299]
     for j, value in zip(bad, (math.nan, math.inf, -math.inf)):
         b.v[j] = value
@@ -396,15 +429,16 @@ def test_attention_far_offsets(torch_cuda):
     b.run().check()
 
 
-def test_attention_strides(torch_cuda):
-    """Head-major caches and outputs, keys shared by every request (stride 0
-    over heads)."""
-    b = Batch(F16, 4, 2, 64, 100, 0, 3, [60, 9], [200, 120], poison=False)
-    b.dk = b.k.cuda().transpose(0, 1).contiguous().transpose(0, 1)
-    b.k[:, 1] = b.k[:, 0]
-    b.dk = b.k[:, :1].cuda().expand(-1, 2, -1)
+@pytest.mark.parametrize("H,K,n", [(4, 2, 60), (64, 32, 300)])
+def test_attention_strides(torch_cuda, H, K, n):
+    """Head-major caches, queries and outputs; keys that all heads share
+    (stride 0 over heads)."""
+    b = Batch(F16, H, K, 64, 100, 0, 3, [n, 9], [2 * n, 120], poison=False)
+    b.k[:, 1:] = b.k[:, :1]
+    b.dk = b.k[:, :1].cuda().expand(-1, K, -1)
     b.dv = b.v.cuda().transpose(0, 1).contiguous().transpose(0, 1)
-    b.out = torch.full((4, 72, 64), 7.0, dtype=F16, device="cuda").transpose(0, 1)
+    b.dq = b.dq.transpose(0, 1).contiguous().transpose(0, 1)
+    b.out = torch.full((H, n + 12, 64), 7.0, dtype=F16, device="cuda").transpose(0, 1)
     b.run().check()
 
 

@@ -88,10 +88,16 @@ def batch(**kw):
     (dict(v=None), "null"), (dict(q_start=None), "null"), (dict(kv_start=None), "null"), (dict(kv_len=None), "null"),
     (dict(q=AT + 2), "aligned"), (dict(k=AT + 8), "aligned"), (dict(out=AT + 4), "aligned"),
     (dict(workspace=AT + 1), "aligned"), (dict(q_row=-8), "strides"), (dict(k_row=1 << 24), "strides"),
-    (dict(v_head=60), "multiples of 8"), (dict(out_row=4), "multiples of 8"),
+    (dict(kv_rows=2, k_row=56), "overlap"), (dict(kv_rows=2, v_row=0), "overlap"),
+(dict(v_head=60), "multiples of 8"), (dict(out_row=4), "multiples of 8"),
 ])
 def test_attention_batches(fields, match):
     refused(_lib.load().nemo_window_attention, AT, config(), batch(**fields), None, match=match)
+
+
+def test_attention_of_too_many_heads():
+    refused(_lib.load().nemo_window_attention, AT, config(q_heads=8, kv_heads=8), batch(count=1 << 20), None,
+            match="count times kv_heads")
 
 
 def test_attention_of_nothing_needs_no_buffers():
