@@ -395,6 +395,32 @@ typedef struct nemo_norm_args {
 
 nemo_status nemo_rmsnorm(nemo_ctx* ctx, const nemo_norm_args* args, void* stream);
 
+/* Encoders of the same graph whose layers attend through a window, or whose
+ * rotary positions differ from the reference's: before nemo_model_finalize,
+ * the model's attention becomes nemo_rope_apply on the query and key heads
+ * (positions counted within a request, merged positions after the merge) and
+ * nemo_window_attention over each request's own keys, in place of the
+ * reference's rotation, key sampling and temperature. Every global_every-th
+ * layer (the global_every-th, the 2 global_every-th, ...; 0: none) has no left
+ * bound, and no right bound unless right is 0. rope.head_dim is taken from
+ * the model. A model without this call computes what the reference does. */
+typedef struct nemo_model_attention {
+  int32_t left, right, sinks; /* as in nemo_attention_config */
+  int32_t global_every;
+  nemo_rope_config rope;
+} nemo_model_attention;
+nemo_status nemo_model_set_attention(nemo_model* model, const nemo_model_attention* attention);
+
+/* The token states of the plan's last run in 8 bits, for indexes of one vector
+ * a token: the final RMSNorm of each request's merged rows, unpooled, as
+ * nemo_rmsnorm writes it (y8 [rows][hidden], scales [rows] or [rows][hidden /
+ * group]), request after request, max(1, ceil(0.64 length)) rows each. `rows`
+ * receives their number; more than `capacity`, and a plan that has not run or
+ * whose model merges after its last layer, are refused. Enqueued on `stream`
+ * (NULL: the plan's own) after the run. */
+nemo_status nemo_plan_token_states8(nemo_plan* plan, int32_t type8, int32_t group, void* d_y8, float* d_scales,
+                                    int64_t capacity, int64_t* rows, void* stream);
+
 /* ---- offline requantization (src/gguf/quantization.ts:77-131) ------------ */
 
 /* requantizeMatrixToQ40 (src/gguf/quantization.ts:101-131) on the GPU: the

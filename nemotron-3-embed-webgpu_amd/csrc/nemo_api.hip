@@ -294,6 +294,16 @@ struct nemo_model {
   int embedding_type = -1;
   const void* embedding = nullptr;
   std::atomic<int> live_plans{0};  // plans are created and destroyed from any thread
+  // nemo_model_set_attention: the layers rotate and attend by the operators.
+  bool windowed = false;
+  nemo_model_attention attention{};
+  RopeAngles angles{};
+  DevPtr turns;
+};
+
+// The index arrays of a ragged layout on the device, for the operators.
+struct RaggedIndex {
+  DevPtr positions, q_start, kv_start, kv_len;
 };
 
 struct nemo_weight {
@@ -326,6 +336,7 @@ struct nemo_plan {
   // (attention's preparation pass), room for attn_keys_cap keys per kv head.
   DevPtr attn_ks, attn_vts;
   int attn_keys_cap = 0;
+  RaggedIndex index_full, index_red;  // of a model with windowed attention
   uint32_t* h_ids = nullptr;   // pinned staging
   float* h_out = nullptr;
   // Recorded after every enqueue of the plan's work, on the stream it went
@@ -856,6 +867,13 @@ nemo_status nemo_plan_create(nemo_model* model, int32_t batch, int32_t sequence,
     p->wexp_gu_halves = gu;
     p->wexp_dn_halves = dn;
     p->out = dev_alloc((size_t)batch * H * 4, "embeddings");
+    if (model->windowed)
+      for (RaggedIndex* x : {&p->index_full, &p->index_red}) {
+        x->positions = dev_alloc((x == &p->index_full ? tf : tr) * 8, "positions");
+        x->q_start = dev_alloc((kMaxBatch + 1) * 4, "request rows");
+        x->kv_start = dev_alloc(kMaxBatch * 8, "request rows");
+        x->kv_len = dev_alloc(kMaxBatch * 4, "request rows");
+      }
     const std::vector<float> table = rope_table(sequence, d.head_dim, d.rope_theta);
     p->rope = dev_alloc(table.size() * 4, "RoPE sin/cos table");
     hip_check(hipMemcpy(p->rope.get(), table.data(), table.size() * 4, hipMemcpyHostToDevice), "upload");
@@ -912,10 +930,20 @@ nemo_status nemo_plan_read_buffer(nemo_plan* plan, const char* name, void* out, 
       // RoPE of the last layer's query and key heads, as the attention applied it.
       if (!plan->q) plan->q = dev_alloc(tf * QW * 2, "query rope");
       if (!plan->k) plan->k = dev_alloc(tf * KW * 2, "key rope");
-      hip_check(launch_rope((const uint16_t*)plan->qkv.get(), (int)QKV, plan->last_rows, (const float*)plan->rope.get(),
-                            d.q_heads, d.kv_heads, d.head_dim, (uint16_t*)plan->q.get(), (uint16_t*)plan->k.get(),
-                            plan->stream),
-                "rope");
+      const size_t done = plan->last_rows.start[plan->last_rows.count];
+      if (plan->model->windowed && done) {  // rotated where they are
+        hip_check(hipMemcpy2DAsync(plan->q.get(), QW * 2, plan->qkv.get(), QKV * 2, QW * 2, done,
+                                   hipMemcpyDeviceToDevice, plan->stream),
+                  "query heads");
+        hip_check(hipMemcpy2DAsync(plan->k.get(), KW * 2, (const uint16_t*)plan->qkv.get() + QW, QKV * 2, KW * 2, done,
+                                   hipMemcpyDeviceToDevice, plan->stream),
+                  "key heads");
+      } else {
+        hip_check(launch_rope((const uint16_t*)plan->qkv.get(), (int)QKV, plan->last_rows,
+                              (const float*)plan->rope.get(), d.q_heads, d.kv_heads, d.head_dim,
+                              (uint16_t*)plan->q.get(), (uint16_t*)plan->k.get(), plan->stream),
+                  "rope");
+      }
       src = n == "q" ? plan->q.get() : plan->k.get();
       bytes = tf * (n == "q" ? QW : KW) * 2;
     }
@@ -958,6 +986,35 @@ static void ragged_tables(nemo_plan* p, const uint32_t* lengths, size_t n_length
   }
 }
 
+// Layer l's rotary positions, in place in the QKV projection, and attention of
+// a model with windowed attention.
+static void windowed_attention(const nemo_model* m, int l, const RaggedIndex& x, int count, int rows, int longest,
+                               uint16_t* qkv, uint16_t* out, hipStream_t s) {
+  const nemo_dims& d = m->dims;
+  const nemo_model_attention& w = m->attention;
+  const int hd = d.head_dim, width = (d.q_heads + 2 * d.kv_heads) * hd;
+  const nemo_rope_heads heads{qkv, qkv, width, hd, width, hd, d.q_heads + d.kv_heads};
+  hip_check(launch_rope_apply(m->angles, kF16, heads, nullptr, rows, (const int64_t*)x.positions.get(), 0, s), "rope");
+  const bool global = w.global_every && (l + 1) % w.global_every == 0;
+  const nemo_attention_config c{d.q_heads, d.kv_heads, hd, kF16, global ? -1 : w.left,
+                                global && w.right ? -1 : w.right, w.sinks, 0.f};
+  nemo_attention_batch b{};
+  b.count = count;
+  b.q_rows = b.kv_rows = rows;
+  b.max_kv = longest;
+  b.q_start = (const int32_t*)x.q_start.get();
+  b.kv_start = (const int64_t*)x.kv_start.get();
+  b.kv_len = (const int32_t*)x.kv_len.get();
+  b.q = qkv;
+  b.k = qkv + d.q_heads * hd;
+  b.v = qkv + (d.q_heads + d.kv_heads) * hd;
+  b.out = out;
+  b.q_row = b.k_row = b.v_row = width;
+  b.q_head = b.k_head = b.v_head = b.out_head = hd;
+  b.out_row = d.q_heads * hd;
+  hip_check(launch_window_attention(c, b, s), "attention");
+}
+
 // Enqueue the whole graph (src/webgpu/model.ts:154-168). `mark(stage, begin)`
 // brackets stages for profiling.
 template <typename Mark>
@@ -979,7 +1036,13 @@ static void enqueue_graph(nemo_plan* p, const uint32_t* d_ids, const Ragged& src
   uint16_t* wexp = (uint16_t*)p->wexp.get();
   const float* rope = (const float*)p->rope.get();
 
+  auto write_index = [&](const RaggedIndex& x, const Ragged& rows) {
+    hip_check(launch_ragged_index(rows, (int64_t*)x.positions.get(), (int32_t*)x.q_start.get(),
+                                  (int64_t*)x.kv_start.get(), (int32_t*)x.kv_len.get(), s),
+              "request rows");
+  };
   mark(0, true);
+  if (m->windowed) write_index(p->index_full, src);
   hip_check(launch_embed_norm(d_ids, p->sequence, src, m->embedding_type, m->embedding, H, d.vocab, x_full,
                               m->layers[0].attn_norm, norm_full, d.rms_epsilon, s),
             "embedding");
@@ -997,6 +1060,7 @@ static void enqueue_graph(nemo_plan* p, const uint32_t* d_ids, const Ragged& src
     if (l == d.merge_after_layer) {
       mark(1, true);
       hip_check(launch_merge(norm_full, x_full, src, dst, H, norm_red, x_red, s), "token merge");
+      if (m->windowed) write_index(p->index_red, dst);
       mark(1, false);
     }
     const bool full = l < d.merge_after_layer;
@@ -1073,10 +1137,13 @@ static void enqueue_graph(nemo_plan* p, const uint32_t* d_ids, const Ragged& src
     // Every key before the merge under the README's rule (no request length
     // exceeds INT32_MAX); the plan's key buffers hold every key of a request.
     const int stride_threshold = d.kv_dense_before_merge && full ? INT32_MAX : d.kv_stride_threshold;
-    hip_check(launch_attention(qkv, QKV, rope, rows, d.q_heads, d.kv_heads, d.head_dim, stride_threshold,
-                               d.kv_stride, attn, s, prep ? (uint16_t*)p->attn_ks.get() : nullptr,
-                               prep ? (uint16_t*)p->attn_vts.get() : nullptr, p->attn_keys_cap),
-              "attention");
+    if (m->windowed)
+      windowed_attention(m, l, full ? p->index_full : p->index_red, rows.count, M, longest, qkv, attn, s);
+    else
+      hip_check(launch_attention(qkv, QKV, rope, rows, d.q_heads, d.kv_heads, d.head_dim, stride_threshold,
+                                 d.kv_stride, attn, s, prep ? (uint16_t*)p->attn_ks.get() : nullptr,
+                                 prep ? (uint16_t*)p->attn_vts.get() : nullptr, p->attn_keys_cap),
+                "attention");
     mark(3, false);
     // Residual projection (O or down) then x += delta; RMSNorm. With a K
     // split, the norm kernel sums the fp32 partials itself.
@@ -1482,6 +1549,21 @@ static void validate_rope(const nemo_rope_config& c) {
   if (!isfinite(c.magnitude)) fail(NEMO_ERR_INVALID, "rope magnitude must be finite");
 }
 
+// Angles of a checked configuration, their frequencies on the current device.
+static RopeAngles rope_angles(const nemo_rope_config& c, DevPtr& turns) {
+  RopeAngles a{};
+  a.head_dim = c.head_dim;
+  a.rotary = c.rotary_dim ? c.rotary_dim : c.head_dim;
+  a.half = c.layout == NEMO_ROPE_HALF;
+  const double yarn = c.scaling == NEMO_ROPE_YARN && c.factor > 1 ? 0.1 * log(c.factor) + 1 : 1.0;
+  a.magnitude = (float)(c.magnitude != 0 ? c.magnitude : yarn);
+  const std::vector<double> v = rope_turns(c, a.rotary);
+  turns = dev_alloc(v.size() * 8, "rope frequencies");
+  hip_check(hipMemcpy(turns.get(), v.data(), v.size() * 8, hipMemcpyHostToDevice), "upload");
+  a.turns = (const double*)turns.get();
+  return a;
+}
+
 void nemo_rope_config_default(nemo_rope_config* out) {
   if (!out) return;
   *out = nemo_rope_config{128, 0, NEMO_ROPE_INTERLEAVED, NEMO_ROPE_NONE, 1e6, 1.0, 16384, 32.0, 1.0, 1.0, 4.0, 0.0};
@@ -1495,15 +1577,7 @@ nemo_status nemo_rope_create(nemo_ctx* ctx, const nemo_rope_config* config, nemo
     set_device(ctx);
     auto r = std::make_unique<nemo_rope>();
     r->ctx = ctx;
-    r->angles.head_dim = c.head_dim;
-    r->angles.rotary = c.rotary_dim ? c.rotary_dim : c.head_dim;
-    r->angles.half = c.layout == NEMO_ROPE_HALF;
-    const double yarn = c.scaling == NEMO_ROPE_YARN && c.factor > 1 ? 0.1 * log(c.factor) + 1 : 1.0;
-    r->angles.magnitude = (float)(c.magnitude != 0 ? c.magnitude : yarn);
-    const std::vector<double> turns = rope_turns(c, r->angles.rotary);
-    r->turns = dev_alloc(turns.size() * 8, "rope frequencies");
-    hip_check(hipMemcpy(r->turns.get(), turns.data(), turns.size() * 8, hipMemcpyHostToDevice), "upload");
-    r->angles.turns = (const double*)r->turns.get();
+    r->angles = rope_angles(c, r->turns);
     *out = r.release();
   });
 }
@@ -1601,28 +1675,83 @@ nemo_status nemo_window_attention(nemo_ctx* ctx, const nemo_attention_config* co
   });
 }
 
+static void validate_norm(const nemo_norm_args& a) {
+  if (a.type != kF32 && a.type != kF16 && a.type != NEMO_TYPE_BF16)
+    fail(NEMO_ERR_UNSUPPORTED, "the norm takes F32, F16 or BF16");
+  if (a.hidden < 1) fail(NEMO_ERR_INVALID, "hidden must be positive");
+  if (a.rows < 0 || a.rows > kMaxRows) fail(NEMO_ERR_INVALID, "rows must be in [0, 2^23]");
+  if (!(a.epsilon >= 0) || !isfinite(a.epsilon)) fail(NEMO_ERR_INVALID, "epsilon must be finite and 0 or more");
+  for (int64_t v : {a.x_row, a.delta_row, a.sum_row, a.y_row, a.y8_row, a.scales_row})
+    validate_stride(v, "norm strides");
+  if (a.y8) {
+    if (a.type8 != NEMO_TYPE_I8 && a.type8 != NEMO_TYPE_F8_E4M3)
+      fail(NEMO_ERR_UNSUPPORTED, "the 8-bit output is I8 or F8_E4M3");
+    if (a.group != 0 && a.group != 32 && a.group != 64 && a.group != 128)
+      fail(NEMO_ERR_INVALID, "group must be 0, 32, 64 or 128");
+    if (a.group && a.hidden % a.group) fail(NEMO_ERR_INVALID, "group must divide hidden");
+    if (!a.scales) fail(NEMO_ERR_INVALID, "8-bit output needs scales");
+  }
+  if (a.rows && (!a.x || (!a.sum && !a.y && !a.y8))) fail(NEMO_ERR_INVALID, "null argument");
+}
+
 nemo_status nemo_rmsnorm(nemo_ctx* ctx, const nemo_norm_args* args, void* stream) {
   return guarded([&] {
     if (!ctx || !args) fail(NEMO_ERR_INVALID, "null argument");
-    const nemo_norm_args& a = *args;
-    if (a.type != kF32 && a.type != kF16 && a.type != NEMO_TYPE_BF16)
-      fail(NEMO_ERR_UNSUPPORTED, "the norm takes F32, F16 or BF16");
-    if (a.hidden < 1) fail(NEMO_ERR_INVALID, "hidden must be positive");
-    if (a.rows < 0 || a.rows > kMaxRows) fail(NEMO_ERR_INVALID, "rows must be in [0, 2^23]");
-    if (!(a.epsilon >= 0) || !isfinite(a.epsilon)) fail(NEMO_ERR_INVALID, "epsilon must be finite and 0 or more");
-    for (int64_t v : {a.x_row, a.delta_row, a.sum_row, a.y_row, a.y8_row, a.scales_row})
-      validate_stride(v, "norm strides");
-    if (a.y8) {
-      if (a.type8 != NEMO_TYPE_I8 && a.type8 != NEMO_TYPE_F8_E4M3)
-        fail(NEMO_ERR_UNSUPPORTED, "the 8-bit output is I8 or F8_E4M3");
-      if (a.group != 0 && a.group != 32 && a.group != 64 && a.group != 128)
-        fail(NEMO_ERR_INVALID, "group must be 0, 32, 64 or 128");
-      if (a.group && a.hidden % a.group) fail(NEMO_ERR_INVALID, "group must divide hidden");
-      if (!a.scales) fail(NEMO_ERR_INVALID, "8-bit output needs scales");
-    }
-    if (a.rows == 0) return;
-    if (!a.x || (!a.sum && !a.y && !a.y8)) fail(NEMO_ERR_INVALID, "null argument");
+    validate_norm(*args);
+    if (args->rows == 0) return;
     set_device(ctx);
-    hip_check(launch_norm8(a, (hipStream_t)stream), "rmsnorm");
+    hip_check(launch_norm8(*args, (hipStream_t)stream), "rmsnorm");
+  });
+}
+
+nemo_status nemo_model_set_attention(nemo_model* model, const nemo_model_attention* attention) {
+  return guarded([&] {
+    if (!model || !attention) fail(NEMO_ERR_INVALID, "null argument");
+    if (model->finalized) fail(NEMO_ERR_INVALID, "model is finalized");
+    nemo_model_attention w = *attention;
+    w.rope.head_dim = model->dims.head_dim;
+    validate_rope(w.rope);
+    if (w.global_every < 0) fail(NEMO_ERR_INVALID, "global_every must be 0 or more");
+    validate_attention({model->dims.q_heads, model->dims.kv_heads, model->dims.head_dim, kF16, w.left, w.right, w.sinks,
+                        0.f});
+    set_device(model->ctx);
+    model->angles = rope_angles(w.rope, model->turns);
+    model->attention = w;
+    model->windowed = true;
+  });
+}
+
+nemo_status nemo_plan_token_states8(nemo_plan* plan, int32_t type8, int32_t group, void* d_y8, float* d_scales,
+                                    int64_t capacity, int64_t* rows, void* stream) {
+  return guarded([&] {
+    if (!plan || !d_y8 || !d_scales || !rows) fail(NEMO_ERR_INVALID, "null argument");
+    std::lock_guard<std::mutex> lock(plan->mu);
+    const nemo_model* m = plan->model;
+    if (m->dims.merge_after_layer == m->dims.layers)
+      fail(NEMO_ERR_UNSUPPORTED, "the model merges after its last layer: it has no merged token states");
+    const Ragged& last = plan->last_rows;
+    const int64_t n = last.start[last.count];
+    if (n == 0) fail(NEMO_ERR_INVALID, "plan has not run");
+    if (capacity < n)
+      fail(NEMO_ERR_INVALID, "room for " + std::to_string(capacity) + " token states; the run has " + std::to_string(n));
+    nemo_norm_args a{};
+    a.type = kF16;
+    a.hidden = m->dims.hidden;
+    a.rows = n;
+    a.x = plan->x_red.get();
+    a.weight = m->output_norm;
+    a.y8 = d_y8;
+    a.scales = d_scales;
+    a.x_row = a.y8_row = a.hidden;
+    a.type8 = type8;
+    a.group = group;
+    a.epsilon = m->dims.rms_epsilon;
+    validate_norm(a);
+    a.scales_row = group ? a.hidden / group : 1;
+    set_device(m->ctx);
+    hipStream_t s = stream ? (hipStream_t)stream : plan->stream;
+    PlanEnqueue enqueue(plan, s);
+    hip_check(launch_norm8(a, s), "token states");
+    *rows = n;
   });
 }

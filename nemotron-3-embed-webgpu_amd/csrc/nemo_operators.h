@@ -30,6 +30,9 @@ hipError_t launch_norm8(const nemo_norm_args& args, hipStream_t stream);
 constexpr int kUnbounded = 1 << 30;
 // Bytes of workspace with which the keys of a batch's queries are split.
 size_t window_workspace(const nemo_attention_config& c, int count, int64_t q_rows, int64_t max_kv);
+// The index arrays of requests that follow each other, and each row's position.
+hipError_t launch_ragged_index(const Ragged& rows, int64_t* positions, int32_t* q_start, int64_t* kv_start,
+                               int32_t* kv_len, hipStream_t stream);
 hipError_t launch_window_attention(const nemo_attention_config& c, const nemo_attention_batch& b, hipStream_t stream);
 
 }  // namespace nemo

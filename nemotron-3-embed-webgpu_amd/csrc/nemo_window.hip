@@ -821,6 +821,23 @@ __global__ __launch_bounds__(256) void window_join_kernel(WindowArgs a, Partials
   out[threadIdx.x] = (T)(l == 0.f ? 0.f : sum / l);
 }
 
+__global__ __launch_bounds__(256) void ragged_index_kernel(Ragged rows, int64_t* __restrict__ positions,
+                                                           int32_t* __restrict__ q_start,
+                                                           int64_t* __restrict__ kv_start,
+                                                           int32_t* __restrict__ kv_len) {
+  const int t = blockIdx.x * 256 + threadIdx.x, total = rows.start[rows.count];
+  if (t < total) {
+    int b = 0;
+    while (t >= rows.start[b + 1]) ++b;
+    positions[t] = t - rows.start[b];
+  }
+  if (t <= rows.count) q_start[t] = rows.start[t];
+  if (t < rows.count) {
+    kv_start[t] = rows.start[t];
+    kv_len[t] = rows.start[t + 1] - rows.start[t];
+  }
+}
+
 // Which kernel a batch takes and how its keys are split, by its sizes alone.
 // `tiles` of 32 rows, of which window_few_kernel has `places` on the chip at a
 // time, and the keys that a query sees. Few rows: while the tiles fit (32
@@ -854,6 +871,13 @@ Plan window_plan(const nemo_attention_config& c, int count, int64_t q_rows, int6
 size_t window_workspace(const nemo_attention_config& c, int count, int64_t q_rows, int64_t max_kv) {
   const int splits = window_plan(c, count, q_rows, max_kv).splits;
   return splits == 1 ? 0 : (size_t)splits * q_rows * c.q_heads * (c.head_dim * 4 + 8);
+}
+
+hipError_t launch_ragged_index(const Ragged& rows, int64_t* positions, int32_t* q_start, int64_t* kv_start,
+                               int32_t* kv_len, hipStream_t stream) {
+  const int n = std::max(rows.start[rows.count], rows.count + 1);
+  ragged_index_kernel<<<(n + 255) / 256, 256, 0, stream>>>(rows, positions, q_start, kv_start, kv_len);
+  return hipGetLastError();
 }
 
 hipError_t launch_window_attention(const nemo_attention_config& c, const nemo_attention_batch& b, hipStream_t stream) {

@@ -33,7 +33,8 @@ EXPORTED = [
     "nemo_weight_dequantize", "nemo_dequantize",
     "nemo_requantize_q40", "nemo_probe_stream",
     "nemo_rope_config_default", "nemo_rope_create", "nemo_rope_destroy", "nemo_rope_apply",
-    "nemo_window_attention_workspace", "nemo_window_attention", "nemo_rmsnorm",
+    "nemo_window_attention_workspace", "nemo_window_attention", "nemo_rmsnorm", "nemo_model_set_attention",
+    "nemo_plan_token_states8",
 ]
 
 
@@ -93,6 +94,14 @@ class AttentionBatch(ctypes.Structure):
         ("k_head", ctypes.c_int64), ("v_row", ctypes.c_int64), ("v_head", ctypes.c_int64),
         ("out_row", ctypes.c_int64), ("out_head", ctypes.c_int64), ("workspace", ctypes.c_void_p),
         ("workspace_bytes", ctypes.c_size_t),
+    ]
+
+
+class ModelAttention(ctypes.Structure):
+    """nemo_model_attention (include/nemo.h)."""
+    _fields_ = [
+        ("left", ctypes.c_int32), ("right", ctypes.c_int32), ("sinks", ctypes.c_int32),
+        ("global_every", ctypes.c_int32), ("rope", RopeConfig),
     ]
 
 
@@ -163,6 +172,8 @@ def load() -> ctypes.CDLL:
                                                   ctypes.c_int64, ctypes.POINTER(sz)]),
         "nemo_window_attention": (i32, [vp, ctypes.POINTER(AttentionConfig), ctypes.POINTER(AttentionBatch), vp]),
         "nemo_rmsnorm": (i32, [vp, ctypes.POINTER(NormArgs), vp]),
+        "nemo_model_set_attention": (i32, [vp, ctypes.POINTER(ModelAttention)]),
+        "nemo_plan_token_states8": (i32, [vp, i32, i32, vp, vp, ctypes.c_int64, i64p, vp]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(L, name)

@@ -14,7 +14,7 @@ import ctypes
 
 from . import _lib
 from ._lib import (ROPE_BANDS, ROPE_HALF, ROPE_INTERLEAVED, ROPE_LINEAR, ROPE_NONE, ROPE_YARN, TYPE_BF16, TYPE_F16,
-                   TYPE_F32, TYPE_I8, AttentionBatch, AttentionConfig, NormArgs, RopeConfig, RopeHeads, check)
+                   TYPE_F32, TYPE_I8, AttentionBatch, AttentionConfig, ModelAttention, NormArgs, RopeConfig, RopeHeads, check)
 from .runtime import HipContext
 
 TYPE_E4M3 = _lib.TYPE_F8_E4M3
@@ -93,6 +93,14 @@ def attention_batch(count: int, q_rows: int, kv_rows: int, max_kv: int, d_q_star
                           d_workspace if workspace_bytes else 0, workspace_bytes)
 
 
+def model_attention(left: int = -1, right: int = -1, sinks: int = 0, global_every: int = 0,
+                    **rope_fields) -> ModelAttention:
+    """The ``attention`` of a NemotronHipModel: windows and sinks of its
+    layers, every ``global_every``-th of which sees all keys, and its rotary
+    positions (fields of nemo_rope_config; head_dim is the model's)."""
+    return ModelAttention(left, right, sinks, global_every, rope_config(128, **rope_fields))
+
+
 class WindowAttention:
     """Attention of one configuration (nemo_window_attention)."""
 
@@ -139,7 +147,7 @@ class RmsNorm:
 
 __all__ = [
     "ROPE_BANDS", "ROPE_HALF", "ROPE_INTERLEAVED", "ROPE_LINEAR", "ROPE_NONE", "ROPE_YARN", "TYPE_BF16", "TYPE_E4M3",
-    "TYPE_F16", "TYPE_F32", "TYPE_I8", "AttentionBatch", "AttentionConfig", "NormArgs", "RmsNorm", "Rope",
-    "RopeConfig", "RopeHeads", "WindowAttention", "attention_batch", "attention_config", "norm_args", "rope_config",
-    "rope_heads",
+    "TYPE_F16", "TYPE_F32", "TYPE_I8", "AttentionBatch", "AttentionConfig", "ModelAttention", "NormArgs", "RmsNorm", "Rope",
+    "RopeConfig", "RopeHeads", "WindowAttention", "attention_batch", "attention_config", "model_attention",
+    "norm_args", "rope_config", "rope_heads",
 ]

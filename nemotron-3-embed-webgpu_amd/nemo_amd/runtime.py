@@ -214,6 +214,21 @@ class NemotronHipPlan:
             self._leave()
         return buf.view(np.float32 if name == "embeddings" else np.float16)
 
+    def token_states8(self, d_y8: int, d_scales: int, capacity: int, type8: int = _lib.TYPE_I8, group: int = 0,
+                      stream: int = 0) -> int:
+        """Enqueue the last run's token states in 8 bits with scales (device
+        buffers of ``capacity`` rows); returns their number: request after
+        request, contextual_merged_length(length) rows each."""
+        rows = ctypes.c_int64(0)
+        self._enter()
+        try:
+            check(_lib.load().nemo_plan_token_states8(self._ptr, type8, group, ctypes.c_void_p(d_y8),
+                                                      ctypes.c_void_p(d_scales), capacity, ctypes.byref(rows),
+                                                      ctypes.c_void_p(stream or None)))
+        finally:
+            self._leave()
+        return rows.value
+
     def destroy(self) -> None:
         """destroy() (src/webgpu/model.ts:141-144): later calls fail with
         'plan was destroyed'; the device memory is released now, or when
@@ -245,7 +260,9 @@ class NemotronHipModel:
     parsed ``GGUFModel`` (src/gguf/types.ts:37-44; dims default to its
     metadata), a mapping name -> (ggml_type, dims, bytes), or None together
     with ``synthetic_seed`` for seeded synthetic weights (``overrides``, a
-    mapping of the same form, then replaces some of them).
+    mapping of the same form, then replaces some of them). ``attention``
+    (operators.model_attention) gives the layers windows, sinks and other
+    rotary positions than the reference's.
     """
 
     # No per-binding storage limit on HIP: the engine's storage cap does not
@@ -253,7 +270,8 @@ class NemotronHipModel:
     maxStorageBufferBindingSize = None
 
     def __init__(self, source=None, dims: Dims | None = None, device: int = 0, synthetic_seed: int | None = None,
-                 embedding_type: int = TYPE_F16, overrides: dict | None = None):
+                 embedding_type: int = TYPE_F16, overrides: dict | None = None,
+                 attention: "_lib.ModelAttention | None" = None):
         self.ctx = HipContext.shared(device)
         is_gguf = hasattr(source, "dataOffset") and hasattr(source, "metadata") and hasattr(source, "version")
         if dims is None and is_gguf:
@@ -283,6 +301,8 @@ class NemotronHipModel:
         else:
             for name, (ggml_type, dims_, data) in source.items():
                 self.set_tensor(name, ggml_type, dims_, data)
+        if attention is not None:
+            check(L.nemo_model_set_attention(self._ptr, ctypes.byref(attention)))
         check(L.nemo_model_finalize(self._ptr))
 
     @property
