@@ -84,25 +84,38 @@ struct OneRow {
   float m = -INFINITY, l = 0.f, o[HD / 64] = {};
   __device__ __forceinline__ void keys(const T* q, const T* k, int64_t k_row, const T* v, int64_t v_row, int j0,
                                        int j1, float scale2) {
+    typedef T vec __attribute__((ext_vector_type(8)));
     const int lane = threadIdx.x & 63;
     for (int jb = j0; jb < j1; jb += 64) {
-      const int j = jb + lane;
+      const int j = min(jb + lane, j1 - 1);
       float s = 0.f;
-      if (j < j1)
-        for (int d = 0; d < HD; ++d) s = fmaf((float)q[d], (float)k[j * k_row + d], s);
-      s = j < j1 ? s * scale2 : -INFINITY;
+      for (int d = 0; d < HD; d += 8) {
+        const vec a = *(const vec*)(q + d), b = *(const vec*)(k + j * k_row + d);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s = fmaf((float)a[e], (float)b[e], s);
+      }
+      s = jb + lane < j1 ? s * scale2 : -INFINITY;
       float most = s;
       for (int x = 32; x > 0; x >>= 1) most = fmaxf(most, __shfl_xor(most, x, 64));
       const float mn = fmaxf(m, most), ref = mn == -INFINITY ? 0.f : mn;
-      const float alpha = exp2f(m - ref), p = j < j1 ? exp2f(s - ref) : 0.f;
+      const float alpha = exp2f(m - ref), p = jb + lane < j1 ? exp2f(s - ref) : 0.f;
       float sum = p;
       for (int x = 32; x > 0; x >>= 1) sum += __shfl_xor(sum, x, 64);
       l = l * alpha + sum;
       m = mn;
       for (int i = 0; i < HD / 64; ++i) o[i] *= alpha;
-      for (int t = 0; t < min(64, j1 - jb); ++t) {
-        const float pt = __shfl(p, t, 64);
-        for (int i = 0; i < HD / 64; ++i) o[i] = fmaf(pt, (float)v[(jb + t) * v_row + lane + 64 * i], o[i]);
+      for (int t0 = 0; t0 < min(64, j1 - jb); t0 += 8) {
+        float r[8][HD / 64];
+#pragma unroll
+        for (int t = 0; t < 8; ++t)
+#pragma unroll
+          for (int i = 0; i < HD / 64; ++i) r[t][i] = (float)v[min(jb + t0 + t, j1 - 1) * v_row + lane + 64 * i];
+#pragma unroll
+        for (int t = 0; t < 8; ++t) {
+          const float pt = __shfl(p, t0 + t, 64);
+#pragma unroll
+          for (int i = 0; i < HD / 64; ++i) o[i] = jb + t0 + t < j1 ? fmaf(pt, r[t][i], o[i]) : o[i];
+        }
       }
     }
   }
@@ -304,7 +317,9 @@ struct Rows {
 #pragma unroll
       for (int r = 1; r < 16; ++r) top = fmaxf(top, s[r]);
       top *= scale2;
-      const float raised = fmaxf(m, fmaxf(top, __shfl_xor(top, 32, 64)));
+      const int high = !(add <= 0x1p15f), other = __shfl_xor(high, 32, 64);
+      const bool raise = high | other;  // only the rows that ask: none depends on another
+      const float raised = raise ? fmaxf(m, fmaxf(top, __shfl_xor(top, 32, 64))) : m;
       const float alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - raised);
       l *= alpha;
 #pragma unroll
@@ -464,6 +479,28 @@ __device__ __forceinline__ void image_rows(int lane, Do&& each) {
   for (int i = 0; i < kKeys / kPer; ++i) each(i, kPer * i + lane / kChunks, lane % kChunks);
 }
 
+// Whether, of the slots [t0, t1), one that not all rows of windows first ..
+// last see has a value that is not finite: only then can their sums have met
+// one that they do not see. By a wave.
+template <typename T, int HD>
+__device__ __forceinline__ bool hidden_spoil(const WindowArgs& a, const Heads<T>& h, const KeyList& list,
+                                             const Seen& first, const Seen& last, int t0, int t1) {
+  typedef T vec __attribute__((ext_vector_type(8)));
+  constexpr int kChunks = HD / 8, kPer = 64 / kChunks;
+  const int lane = threadIdx.x & 63;
+  float z = 0.f;
+  auto scan = [&](int from, int to) {
+    for (int t = max(from, t0) + lane / kChunks; t < min(to, t1); t += kPer) {
+      const vec v = *(const vec*)(h.v + list.key(t) * a.b.v_row + 8 * (lane % kChunks));
+#pragma unroll
+      for (int e = 0; e < 8; ++e) z = fmaf((float)v[e], 0.f, z);
+    }
+  };
+  scan(list.pad ? list.pad : a.sinks, last.lo);
+  scan(max(first.hi, list.pad), list.n);
+  return __builtin_amdgcn_ballot_w64(z != 0.f) != 0;
+}
+
 // A row over the slots [t0, t1) that it sees, key by key.
 template <typename T, int HD>
 __device__ __forceinline__ OneRow<T, HD> one_row(const WindowArgs& a, const Heads<T>& h, const KeyList& list,
@@ -491,6 +528,7 @@ template <typename T, int HD>
 __global__ __launch_bounds__(256, HD == 128 ? 2 : 3) void window_tile_kernel(WindowArgs a) {
   constexpr int IMG = 2 * kKeys * HD;  // bytes of an image of 32 keys
   __shared__ __attribute__((aligned(16))) uint8_t lds[2][2][2 * IMG];  // [K, V][round & 1]
+  __shared__ __attribute__((aligned(16))) uint8_t first_k[IMG];        // K of the first block
   const nemo_attention_batch& b = a.b;
   const int kvh = blockIdx.x % a.kv_heads, tile_no = blockIdx.x / a.kv_heads;  // an XCD's L2 keeps to one KV head of 8
   const Request<kTileRows> r(a, tile_no);
@@ -508,7 +546,8 @@ __global__ __launch_bounds__(256, HD == 128 ? 2 : 3) void window_tile_kernel(Win
   const int rounds = (list.n + 63) >> 6;
 
   // A wave copies 16 rows of K and of V a round: half of one of the two images
-  // of each. V's first image of round `at` is the block before the round's.
+  // of each. V's first image of round `at` is the block before the round's, of
+  // round 0 zeros.
   const int64_t k_stride = 2 * b.k_row, v_stride = 2 * b.v_row;
   const Stager<HD, 16, false> ks(16 * (wave & 1), k_stride);
   const Stager<HD, 16, true> vs(16 * (wave & 1), v_stride);
@@ -533,27 +572,23 @@ __global__ __launch_bounds__(256, HD == 128 ? 2 : 3) void window_tile_kernel(Win
   };
   uint8_t* const rows_image = lds[wave >> 1][1] + (wave & 1) * IMG;  // of this wave's queries, later outputs
   if (rounds) {
-    // K of the first block, where V's block before the first would be (p is 0 for that)
     const Stager<HD, 8, false> k0(8 * wave, k_stride);
     k0.copy(k0.range((const uint8_t*)heads.k + list.key(0) * k_stride, k_stride, list.rows(0)),
-            lds[1][0] + 8 * wave * 2 * HD);
+            first_k + 8 * wave * 2 * HD);
     image_rows<HD>(lane, [&](int i, int r, int chunk) {
       const int at = min(w0 + r, rows - 1);
       copy_address(heads.query(at, a.query(at)) + 8 * (chunk ^ k_swizzle<HD>(r)), rows_image + 1024 * i);
     });
-    if (wave >> 1) vs.copy(v_range(0), v_image(0));
+    vs.copy(v_range(0), v_image(0));
     ks.copy(k_range(0), k_image(0));
-    if (wave >> 1)
-      asm volatile("s_waitcnt vmcnt(%0)" ::"n"(IMG / 1024) : "memory");
-    else
-      asm volatile("s_waitcnt vmcnt(%0)" ::"n"(IMG / 2048) : "memory");
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(IMG / 1024) : "memory");
     __builtin_amdgcn_s_barrier();
     acc.load(rows_image, lane);
-    s = acc.scores(lds[1][0], lane);
+    s = acc.scores(first_k, lane);
     hidden(0);
   }
   typename Mma<T>::frag p[2] = {};
-  const bool tail = 64 * rounds - 32 < list.n;  // the last round's second block has slots
+  const bool tail = rounds && 64 * rounds - 32 < list.n;  // the last round's second block has slots
   auto landed = [&] {
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();  // the round has landed, and every wave has left the other buffers
@@ -586,8 +621,9 @@ __global__ __launch_bounds__(256, HD == 128 ? 2 : 3) void window_tile_kernel(Win
   // A value that some rows of the wave do not see meets their probability 0;
   // where it is not finite, their sums are not, and they are taken again. (One
   // query's rows see the same keys.)
-  const uint64_t bad = a.query(min(w0, w1)) == a.query(w1) ? 0 : __builtin_amdgcn_ballot_w64(acc.spoilt());
-  const uint32_t again = (uint32_t)(bad | bad >> 32);
+  const uint64_t bad = a.query(w0) == a.query(w1) ? 0 : __builtin_amdgcn_ballot_w64(acc.spoilt());
+  uint32_t again = (uint32_t)(bad | bad >> 32);
+  if (again && !hidden_spoil<T, HD>(a, heads, list, first, last, 0, list.n)) again = 0;
   // Outputs go through LDS: whole rows to memory, 16 bytes a lane.
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
   __builtin_amdgcn_s_barrier();
@@ -743,7 +779,8 @@ __global__ __launch_bounds__(64 * kFewWaves) void window_few_kernel(WindowArgs a
     const int i = a.query(at);
     return part.rows * split + out_row + (int64_t)i * a.kv_heads * a.group + (at - i * a.group);
   };
-  const uint32_t again = spoilt;
+  uint32_t again = spoilt;
+  if (again && !hidden_spoil<T, HD>(a, heads, list, first, last, 32 * block0, 32 * block1)) again = 0;
   if (valid && !(again >> mrow & 1)) {
     if (part.ml) {
       const int64_t at = partial(row0 + mrow);

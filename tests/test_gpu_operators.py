@@ -400,6 +400,26 @@ def test_attention_hidden_values_reach_no_result(torch_cuda, H, K, dtype, D):
     close(out[~touched], want[~touched], tol[~touched])
 
 
+@pytest.mark.parametrize("H,K", FEW_MANY)
+@pytest.mark.parametrize("key", [3, 200])
+def test_attention_spoilt_queries_and_keys(torch_cuda, H, K, key):
+    """A NaN in a query spoils that query, one in a key the queries that see
+    it, and both leave the others as they are."""
+    n = 280
+    b = Batch(BF16, H, K, 64, 30, 5, 1, [n], [n], poison=False)
+    b.run()
+    clean = b.out.clone()
+    b.q[100] = math.nan
+    b.k[key] = math.nan
+    b.dq, b.dk = torch.cat([b.q, b.q[:3]]).cuda(), b.k.cuda()
+    b.out.fill_(7.0)
+    b.run()
+    bad = ref.visible(n, n, 30, 5, 1)[:, key].clone()
+    bad[100] = True
+    out = b.out[:n]
+    assert torch.isnan(out[bad]).all() and torch.equal(out[~bad], clean[:n][~bad])
+
+
 def test_attention_cut_index_arrays(torch_cuda):
     """Entries outside the buffers are cut to them."""
     b = Batch(F16, 4, 2, 64, 50, 0, 0, [10, 6], [80, 60], poison=False)
