@@ -47,7 +47,8 @@ struct Seen {
 // floor(q_start[i] group / ROWS) + i, which leaves it at least as many numbers
 // as it has tiles. The request of tile number t is the last whose first is not
 // above t; none (i = -1) before the first request. Each lane looks at one
-// request and has its whole entry at hand when it is the one.
+// request and has its whole entry at hand when it is the one. (Of entries that
+// do not ascend it may be one whose first tile is behind t.)
 template <int ROWS>
 struct Request {
   int i, tile, q0, queries, keys;
@@ -177,7 +178,8 @@ __device__ __forceinline__ int v_swizzle(int row) {
 // (zeros past its end) or an address. The compiler, which knows of the builtin for this that
 // it writes LDS, waits for every copy in flight before each transposed read;
 // written as here it has no register to be waited for, and the loops wait
-// for their images themselves.
+// for their images themselves. (m0 is reserved: the compiler sets it where it
+// uses it itself.)
 __device__ __forceinline__ uint32_t lds_address(const uint8_t* to) { return (uint32_t)(uintptr_t)(lds_void*)to; }
 __device__ __forceinline__ void copy_range(u32x4 range, uint32_t offset, const uint8_t* to) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
@@ -190,6 +192,13 @@ __device__ __forceinline__ void copy_address(const void* from, const uint8_t* to
                :
                : "s"(lds_address(to)), "v"(from)
                : "memory");
+}
+// A barrier that waits for none of the wave's work in flight; no access of
+// memory is moved over it.
+__device__ __forceinline__ void meet() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
 }
 
 // Copies of ROWS key rows into an image by one wave, 1 KB an instruction:
@@ -534,7 +543,7 @@ __global__ __launch_bounds__(256, HD == 128 ? 2 : 3) void window_tile_kernel(Win
   const Request<kTileRows> r(a, tile_no);
   if (r.i < 0) return;
   const int rows = r.queries * a.group, row0 = (tile_no - r.tile) * kTileRows;
-  if (row0 >= rows) return;
+  if ((unsigned)row0 >= (unsigned)rows) return;
   const Heads<T> heads(a, r.q0, r.kv0, kvh);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), hl = lane >> 5;
   const int behind = r.keys - r.queries;  // position of query 0
@@ -582,7 +591,7 @@ __global__ __launch_bounds__(256, HD == 128 ? 2 : 3) void window_tile_kernel(Win
     vs.copy(v_range(0), v_image(0));
     ks.copy(k_range(0), k_image(0));
     asm volatile("s_waitcnt vmcnt(%0)" ::"n"(IMG / 1024) : "memory");
-    __builtin_amdgcn_s_barrier();
+    meet();
     acc.load(rows_image, lane);
     s = acc.scores(first_k, lane);
     hidden(0);
@@ -591,7 +600,7 @@ __global__ __launch_bounds__(256, HD == 128 ? 2 : 3) void window_tile_kernel(Win
   const bool tail = rounds && 64 * rounds - 32 < list.n;  // the last round's second block has slots
   auto landed = [&] {
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-    __builtin_amdgcn_s_barrier();  // the round has landed, and every wave has left the other buffers
+    meet();  // the round has landed, and every wave has left the other buffers
   };
   auto steps = [&](int at, const uint8_t* v, const uint8_t* k, auto&& copies) {
     acc.step(s, p, v, k, lane, a.scale2, [&](int c) { copies(c); });
@@ -626,7 +635,7 @@ __global__ __launch_bounds__(256, HD == 128 ? 2 : 3) void window_tile_kernel(Win
   if (again && !hidden_spoil<T, HD>(a, heads, list, first, last, 0, list.n)) again = 0;
   // Outputs go through LDS: whole rows to memory, 16 bytes a lane.
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-  __builtin_amdgcn_s_barrier();
+  meet();
   acc.store((T*)(rows_image + (lane & 31) * 2 * HD), lane & 31, hl);
   asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
   image_rows<HD>(lane, [&](int i, int r, int chunk) {
@@ -672,7 +681,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void window_few_kernel(WindowArgs a
   const Request<32> r(a, tile_no);
   if (r.i < 0) return;
   const int rows = r.queries * a.group, row0 = (tile_no - r.tile) * 32;
-  if (row0 >= rows) return;
+  if ((unsigned)row0 >= (unsigned)rows) return;
   const Heads<T> heads(a, r.q0, r.kv0, kvh);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), hl = lane >> 5;
   const int behind = r.keys - r.queries, row1 = min(row0 + 31, rows - 1);
@@ -824,7 +833,7 @@ __global__ __launch_bounds__(256) void window_join_kernel(WindowArgs a, Partials
   const Request<1> r(a, tile_no);
   if (r.i < 0) return;
   const int row = tile_no - r.tile, lane = threadIdx.x & 63;
-  if (row >= r.queries * a.group) return;
+  if ((unsigned)row >= (unsigned)(r.queries * a.group)) return;
   const int i = a.query(row), h = kvh * a.group + (row - i * a.group);
   const int64_t at = (int64_t)(r.q0 + i) * a.kv_heads * a.group + h;
   // every wave: lane z's split

@@ -435,6 +435,20 @@ def test_attention_cut_index_arrays(torch_cuda):
     assert not b.out.any()  # no keys: every row, the last three too, is 0
 
 
+@pytest.mark.parametrize("H,K,keys", [(4, 2, 300), (64, 32, 300), (4, 2, 3000)])
+@pytest.mark.parametrize("q_start", [[0, 297, 5, 300], [290, 295, 0, 299], [300, 0, 300, 0], [0, -7, 200, 100]])
+def test_attention_of_requests_out_of_order(torch_cuda, H, K, keys, q_start):
+    """q_start that does not ascend says nothing about the results, but only
+    rows of the buffers are read and written."""
+    b = Batch(F16, H, K, 64, -1, 0, 0, [5, 5, 5], [keys] * 3, poison=False)
+    n = 300
+    q, out = (torch.full((3 * n, H, 64), 7.0, dtype=F16, device="cuda") for _ in range(2))
+    b.dq, b.out = q[n:2 * n], out[n:2 * n]
+    b.q_start = torch.tensor(q_start, dtype=torch.int32).cuda()
+    b.run()
+    assert (out[:n] == 7.0).all() and (out[2 * n:] == 7.0).all()
+
+
 def test_attention_far_offsets(torch_cuda):
     """A cache whose last request starts past 2^32 bytes and 2^31 elements."""
     K, D = 8, 128
