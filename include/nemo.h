@@ -254,7 +254,8 @@ nemo_status nemo_probe_stream(const void* d_src, size_t bytes, int32_t loads_per
  * any layout, for callers that build a layer from nemo_weight_matmul and
  * these. All are enqueued on `stream` (NULL: the default stream) and return;
  * nothing is allocated, so they can be captured into a HIP graph after one
- * eager call of the same kind. Strides count elements. */
+ * eager call of the same kind. Strides count elements; addresses are multiples
+ * of their values' size; rows and heads that are written do not overlap. */
 
 #define NEMO_TYPE_I8 24        /* GGML's code */
 #define NEMO_TYPE_BF16 30      /* GGML's code */
@@ -347,7 +348,8 @@ typedef struct nemo_attention_config {
  * read on the device when the work runs (a captured graph may be replayed
  * with other lengths); entries outside the buffers are cut to q_rows and
  * kv_rows. Key and value rows are at least head_dim apart. Rows of `out` that
- * belong to no request are left as they were. */
+ * belong to no request are left as they were. `out` and the workspace overlap no
+ * other buffer. */
 typedef struct nemo_attention_batch {
   int32_t count;             /* requests */
   int64_t q_rows, kv_rows;   /* rows of q and out, of k and v */
@@ -375,7 +377,9 @@ nemo_status nemo_window_attention(nemo_ctx* ctx, const nemo_attention_config* co
  * in 32 bits from the unrounded h; sum = h and y in `type`; and
  *   scales = max |y| / 127 (I8) or / 448 (F8_E4M3), y8 = round(y / scale)
  * of the unrounded y over a whole row or over each `group` columns (scale 0,
- * and y8 0, where y is 0; NaN where y holds a NaN; to even on ties). */
+ * and y8 0, where y is 0; NaN where y holds a NaN; to even on ties). Where
+ * sum or y is x or delta it has the same row stride; other overlap of an input
+ * and an output is not allowed. */
 typedef struct nemo_norm_args {
   int32_t type;              /* of x, delta, sum, y: F32, F16 or BF16 */
   int32_t hidden;            /* >= 1 */

@@ -1599,9 +1599,16 @@ static void validate_stride(int64_t v, const char* what) {
   if (v < 0 || v > kMaxStride) fail(NEMO_ERR_INVALID, std::string(what) + " must be in [0, 2^23]");
 }
 
-static void validate_rope_heads(const nemo_rope_heads& s) {
+// Addresses of values of `bytes` bytes.
+static void validate_aligned(std::initializer_list<const void*> addresses, size_t bytes) {
+  for (const void* p : addresses)
+    if ((uintptr_t)p % bytes) fail(NEMO_ERR_INVALID, "address is not a multiple of its values' size");
+}
+
+static void validate_rope_heads(const nemo_rope_heads& s, int32_t type) {
   if (s.heads < 0 || s.heads > 65536) fail(NEMO_ERR_INVALID, "rope heads must be in [0, 65536]");
   if (s.heads && (!s.x || !s.y)) fail(NEMO_ERR_INVALID, "null argument");
+  if (s.heads) validate_aligned({s.x, s.y}, type == kF32 ? 4 : 2);
   for (int64_t v : {s.x_row, s.x_head, s.y_row, s.y_head}) validate_stride(v, "rope strides");
 }
 
@@ -1612,8 +1619,9 @@ nemo_status nemo_rope_apply(nemo_rope* rope, int32_t type, const nemo_rope_heads
     if (type != kF32 && type != kF16 && type != NEMO_TYPE_BF16)
       fail(NEMO_ERR_UNSUPPORTED, "rope takes F32, F16 or BF16");
     if (rows < 0 || rows > kMaxRows) fail(NEMO_ERR_INVALID, "rows must be in [0, 2^23]");
-    validate_rope_heads(*q);
-    if (k) validate_rope_heads(*k);
+    validate_rope_heads(*q, type);
+    if (k) validate_rope_heads(*k, type);
+    validate_aligned({d_positions}, 8);
     set_device(rope->ctx);
     hip_check(launch_rope_apply(rope->angles, type, *q, k, rows, d_positions, base, (hipStream_t)stream), "rope");
   });
@@ -1666,6 +1674,8 @@ nemo_status nemo_window_attention(nemo_ctx* ctx, const nemo_attention_config* co
       fail(NEMO_ERR_INVALID, "rows of k and v must not overlap");
     for (const void* p : {b.q, b.k, b.v, (const void*)b.out, (const void*)b.workspace})
       if ((uintptr_t)p & 15) fail(NEMO_ERR_INVALID, "attention buffers must be 16-byte aligned");
+    validate_aligned({b.q_start, b.kv_len}, 4);
+    validate_aligned({b.kv_start}, 8);
     const size_t need = b.workspace ? window_workspace(*config, b.count, b.q_rows, b.max_kv) : 0;
     if (b.workspace && b.workspace_bytes < need)
       fail(NEMO_ERR_INVALID, "workspace has " + std::to_string(b.workspace_bytes) + " bytes; this batch needs " +
@@ -1692,6 +1702,8 @@ static void validate_norm(const nemo_norm_args& a) {
     if (!a.scales) fail(NEMO_ERR_INVALID, "8-bit output needs scales");
   }
   if (a.rows && (!a.x || (!a.sum && !a.y && !a.y8))) fail(NEMO_ERR_INVALID, "null argument");
+  validate_aligned({a.x, a.delta, a.sum, a.y}, a.type == kF32 ? 4 : 2);
+  validate_aligned({a.weight, a.y8 ? a.scales : nullptr}, 4);
 }
 
 nemo_status nemo_rmsnorm(nemo_ctx* ctx, const nemo_norm_args* args, void* stream) {

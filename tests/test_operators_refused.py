@@ -46,6 +46,10 @@ def test_rope_calls():
     refused(apply, AT, 1, good, None, (1 << 23) + 1, 0, 0, None, match="rows")
     refused(apply, AT, 1, ops.rope_heads(0, AT, 4, 64), None, 1, 0, 0, None, match="null")
     refused(apply, AT, 1, good, ops.rope_heads(AT, 0, 4, 64), 1, 0, 0, None, match="null")
+    refused(apply, AT, 1, ops.rope_heads(AT, AT + 1, 4, 64), None, 1, 0, 0, None, match="multiple")
+    refused(apply, AT, 0, ops.rope_heads(AT + 2, AT, 4, 64), None, 1, 0, 0, None, match="multiple")
+    refused(apply, AT, 1, good, ops.rope_heads(AT + 1, AT, 4, 64), 1, 0, 0, None, match="multiple")
+    refused(apply, AT, 1, good, None, 1, AT + 4, 0, None, match="multiple")
     refused(apply, AT, 1, ops.rope_heads(AT, AT, -1, 64), None, 1, 0, 0, None, match="heads")
     refused(apply, AT, 1, ops.rope_heads(AT, AT, 4, 64, x_row=-8), None, 1, 0, 0, None, match="strides")
     refused(apply, AT, 1, good, ops.rope_heads(AT, AT, 4, 64, y_head=1 << 24), 1, 0, 0, None, match="strides")
@@ -87,9 +91,10 @@ def batch(**kw):
     (dict(max_kv=-1), "max_kv"), (dict(q=None), "null"), (dict(out=None), "null"), (dict(k=None), "null"),
     (dict(v=None), "null"), (dict(q_start=None), "null"), (dict(kv_start=None), "null"), (dict(kv_len=None), "null"),
     (dict(q=AT + 2), "aligned"), (dict(k=AT + 8), "aligned"), (dict(out=AT + 4), "aligned"),
+    (dict(q_start=AT + 2), "multiple"), (dict(kv_len=AT + 1), "multiple"), (dict(kv_start=AT + 4), "multiple"),
     (dict(workspace=AT + 1), "aligned"), (dict(q_row=-8), "strides"), (dict(k_row=1 << 24), "strides"),
     (dict(kv_rows=2, k_row=56), "overlap"), (dict(kv_rows=2, v_row=0), "overlap"),
-(dict(v_head=60), "multiples of 8"), (dict(out_row=4), "multiples of 8"),
+    (dict(v_head=60), "multiples of 8"), (dict(out_row=4), "multiples of 8"),
 ])
 def test_attention_batches(fields, match):
     refused(_lib.load().nemo_window_attention, AT, config(), batch(**fields), None, match=match)
@@ -121,6 +126,8 @@ def norm(**kw):
     (dict(rows=(1 << 23) + 1), 1, "rows"), (dict(epsilon=-1.0), 1, "epsilon"), (dict(epsilon=math.nan), 1, "epsilon"),
     (dict(type8=12), 5, "I8 or F8_E4M3"), (dict(group=16), 1, "group"), (dict(group=-32), 1, "group"),
     (dict(hidden=130, group=64), 1, "divide"), (dict(scales=None), 1, "scales"), (dict(x=None), 1, "null"),
+    (dict(x=AT + 1), 1, "multiple"), (dict(delta=AT + 1), 1, "multiple"), (dict(y=AT + 3), 1, "multiple"),
+    (dict(type=0, x=AT + 2), 1, "multiple"), (dict(weight=AT + 2), 1, "multiple"), (dict(scales=AT + 1), 1, "multiple"),
     (dict(y8=None), 1, "null"), (dict(x_row=-1), 1, "strides"), (dict(y8_row=1 << 24), 1, "strides"),
 ])
 def test_norms(fields, status, match):
