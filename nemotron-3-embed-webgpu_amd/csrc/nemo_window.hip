@@ -527,8 +527,14 @@ __device__ __forceinline__ OneRow<T, HD> one_row(const WindowArgs& a, const Head
 // ---------------------------------------------------------------------------
 // Many rows: a workgroup of 4 waves takes 128 rows, 32 a wave, and stages 64
 // keys a round for all of them. A block's scores are taken one block ahead and
-// its product with V one behind, so the K rows of a round begin 64 slots after
-// its V rows, which begin at the last block of the round before.
+// its product with V one behind, so the K rows of a round begin a block after
+// the round's own, its V rows a block before.
+//
+// Where such tiles are too few for the chip, 8 waves take 64 rows: PARTS = 4
+// pairs of waves attend a quarter of the keys each, 32 a round, and add up in
+// LDS (requests of 512, 77, 1 and 300 tokens, 16 heads of 128 over up to 1040
+// keys: 18.7 us; 24 with 128 rows or by window_few_kernel, 20 with two parts of
+// two waves, of which a SIMD then has one).
 //
 // Bound by issue: 32768 tokens of 32 heads of 128 (8 KV heads, window 1024),
 // 543 GFLOP, take 597 us, MFMA 48 % and vector units 45 % of the cycles, which
@@ -540,43 +546,46 @@ __device__ __forceinline__ OneRow<T, HD> one_row(const WindowArgs& a, const Head
 // tokens, heads of 64, 5 rounds each, are bound by latency: 16.8 us.
 // ---------------------------------------------------------------------------
 
-constexpr int kTileRows = 128;
-
-template <typename T, int HD>
-__global__ __launch_bounds__(256, HD == 128 ? 2 : 3) void window_tile_kernel(WindowArgs a) {
+template <typename T, int HD, int PARTS>
+__global__ __launch_bounds__(PARTS == 1 ? 256 : 512, PARTS == 1 && HD == 64 ? 3 : 2) void window_tile_kernel(WindowArgs a) {
   constexpr int IMG = 2 * kKeys * HD;  // bytes of an image of 32 keys
-  __shared__ __attribute__((aligned(16))) uint8_t lds[2][2][2 * IMG];  // [K, V][round & 1]
-  __shared__ __attribute__((aligned(16))) uint8_t first_k[IMG];        // K of the first block
+  constexpr int GROUPS = PARTS == 1 ? 4 : 2, ROWS = 32 * GROUPS;   // of 32 rows, a wave of each part
+  constexpr int BLOCKS = PARTS == 1 ? 2 : 1, ROUND = 32 * BLOCKS;  // of 32 keys; keys of a part's round
+  constexpr int COPY = ROUND / GROUPS;                             // of which a wave copies
+  __shared__ __attribute__((aligned(16))) uint8_t lds[PARTS][2][2][BLOCKS * IMG];  // [part][K, V][round & 1]
+  __shared__ __attribute__((aligned(16))) uint8_t extra[PARTS == 1 ? IMG : 16];
   const nemo_attention_batch& b = a.b;
   const int kvh = blockIdx.x % a.kv_heads, tile_no = blockIdx.x / a.kv_heads;  // an XCD's L2 keeps to one KV head of 8
-  const Request<kTileRows> r(a, tile_no);
+  const Request<ROWS> r(a, tile_no);
   if (r.i < 0) return;
-  const int rows = r.queries * a.group, row0 = (tile_no - r.tile) * kTileRows;
+  const int rows = r.queries * a.group, row0 = (tile_no - r.tile) * ROWS;
   if ((unsigned)row0 >= (unsigned)rows) return;
   const Heads<T> heads(a, r.q0, r.kv0, kvh);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), hl = lane >> 5;
   const int behind = r.keys - r.queries;  // position of query 0
-  const KeyList list(a, behind + a.query(row0), behind + a.query(min(row0 + kTileRows - 1, rows - 1)), r.keys);
-  const int w0 = row0 + 32 * wave, w1 = min(w0 + 31, rows - 1);
+  const KeyList list(a, behind + a.query(row0), behind + a.query(min(row0 + ROWS - 1, rows - 1)), r.keys);
+  const int group = wave % GROUPS, part = wave / GROUPS;
+  const int w0 = row0 + 32 * group, w1 = min(w0 + 31, rows - 1);
   const int row = min(w0 + (lane & 31), rows - 1);  // (a wave past the rows takes the last one's)
   auto window = [&](int at) { return list.window(a, behind + a.query(at), r.keys); };
   const Seen mine = window(row), first = window(min(w0, rows - 1)), last = window(w1);
-  const int rounds = (list.n + 63) >> 6;
+  const int rounds = (list.n + ROUND * PARTS - 1) / (ROUND * PARTS), base = ROUND * rounds * part;
 
-  // A wave copies 16 rows of K and of V a round: half of one of the two images
-  // of each. V's first image of round `at` is the block before the round's, of
+  // A wave copies COPY rows of K and of V a round, of one of the two images of
+  // each. V's first image of round `at` is the block before the round's, of
   // round 0 zeros.
   const int64_t k_stride = 2 * b.k_row, v_stride = 2 * b.v_row;
-  const Stager<HD, 16, false> ks(16 * (wave & 1), k_stride);
-  const Stager<HD, 16, true> vs(16 * (wave & 1), v_stride);
-  auto v_image = [&](int odd) { return lds[1][odd] + 16 * wave * 2 * HD; };
-  auto k_image = [&](int odd) { return lds[0][odd] + 16 * wave * 2 * HD; };
+  const int second = COPY * group / 32;
+  const Stager<HD, COPY, false> ks(COPY * group % 32, k_stride);
+  const Stager<HD, COPY, true> vs(COPY * group % 32, v_stride);
+  auto v_image = [&](int odd) { return lds[part][1][odd] + COPY * group * 2 * HD; };
+  auto k_image = [&](int odd) { return lds[part][0][odd] + COPY * group * 2 * HD; };
   auto v_range = [&](int at) {
-    const int t0 = 64 * at - 32 + 32 * (wave >> 1);
-    return vs.range((const uint8_t*)heads.v + list.key(t0) * v_stride, v_stride, list.rows(t0));
+    const int t0 = base + ROUND * at - 32 + 32 * second;
+    return vs.range((const uint8_t*)heads.v + list.key(t0) * v_stride, v_stride, t0 < base ? 0 : list.rows(t0));
   };
   auto k_range = [&](int at) {
-    const int t0 = 64 * at + 32 + 32 * (wave >> 1);
+    const int t0 = base + ROUND * at + 32 + 32 * second;
     return ks.range((const uint8_t*)heads.k + list.key(t0) * k_stride, k_stride, list.rows(t0));
   };
   Rows<T, HD> acc;
@@ -588,12 +597,15 @@ __global__ __launch_bounds__(256, HD == 128 ? 2 : 3) void window_tile_kernel(Win
       hide(s, t0, hl, mine.lo, mine.hi, a.sinks);
     }
   };
-  uint8_t* const rows_image = lds[wave >> 1][1] + (wave & 1) * IMG;  // of this wave's queries, later outputs
+  // K of the first block; the group's queries, of which each part copies some
+  uint8_t* const first_k = PARTS == 1 ? extra : lds[part][0][1];
+  uint8_t* const rows_image = PARTS == 1 ? lds[0][group >> 1][1] + (group & 1) * IMG : lds[group][1][1];
   if (rounds) {
-    const Stager<HD, 8, false> k0(8 * wave, k_stride);
-    k0.copy(k0.range((const uint8_t*)heads.k + list.key(0) * k_stride, k_stride, list.rows(0)),
-            first_k + 8 * wave * 2 * HD);
+    const Stager<HD, 32 / GROUPS, false> k0(32 / GROUPS * group, k_stride);
+    k0.copy(k0.range((const uint8_t*)heads.k + list.key(base) * k_stride, k_stride, list.rows(base)),
+            first_k + 32 / GROUPS * group * 2 * HD);
     image_rows<HD>(lane, [&](int i, int r, int chunk) {
+      if (i % PARTS != part) return;
       const int at = min(w0 + r, rows - 1);
       copy_address(heads.query(at, a.query(at)) + 8 * (chunk ^ k_swizzle<HD>(r)), rows_image + 1024 * i);
     });
@@ -603,19 +615,20 @@ __global__ __launch_bounds__(256, HD == 128 ? 2 : 3) void window_tile_kernel(Win
     meet();
     acc.load(rows_image, lane);
     s = acc.scores(first_k, lane);
-    hidden(0);
+    hidden(base);
   }
   typename Mma<T>::frag p[2] = {};
-  const bool tail = rounds && 64 * rounds - 32 < list.n;  // the last round's second block has slots
+  const bool tail = rounds && base + ROUND * rounds - 32 < list.n;  // the last round's last block has slots
   auto landed = [&] {
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
     meet();  // the round has landed, and every wave has left the other buffers
   };
-  auto steps = [&](int at, const uint8_t* v, const uint8_t* k, auto&& copies) {
-    acc.step(s, p, v, k, lane, a.scale2, [&](int c) { copies(c); });
-    hidden(64 * at + 32);
-    acc.step(s, p, v + IMG, k + IMG, lane, a.scale2, [&](int c) { copies(HD / 16 + c); });
-    hidden(64 * at + 64);
+  auto steps = [&](int at, const uint8_t* v_at, const uint8_t* k_at, auto&& copies) {
+#pragma unroll
+    for (int k = 0; k < BLOCKS; ++k) {
+      acc.step(s, p, v_at + k * IMG, k_at + k * IMG, lane, a.scale2, [&](int c) { copies(HD / 16 * k + c); });
+      hidden(base + ROUND * at + 32 + 32 * k);
+    }
   };
   // (No round behind the last is staged but as zeros, which nobody reads.)
   for (int at = 0; at < rounds; at += 2) {
@@ -624,18 +637,61 @@ __global__ __launch_bounds__(256, HD == 128 ? 2 : 3) void window_tile_kernel(Win
       if (at + u >= rounds) break;
       landed();
       const u32x4 v = v_range(at + u + 1), k = k_range(at + u + 1);
-      steps(at + u, lds[1][u], lds[0][u], [&](int c) {
+      steps(at + u, lds[part][1][u], lds[part][0][u], [&](int c) {
         constexpr int N = HD / 32;  // copies of each
         if (c < N) vs.copy(v, c, v_image(1 - u));
         else if (c < 2 * N) ks.copy(k, c - N, k_image(1 - u));
       });
     }
   }
-  if (tail) {
-    landed();
-    acc.values(lds[1][rounds & 1], lane, p);
-  }
+  if (rounds && ROUND * rounds - 32 < list.n) landed();  // (for the first part, so for all)
+  if (tail) acc.values(lds[part][1][rounds & 1], lane, p);
   acc.l += __shfl_xor(acc.l, 32, 64);
+  if constexpr (PARTS > 1) {
+    // The other parts' sums go to the first's waves, each register as its 64 lanes.
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    meet();
+    auto sums = [&](int from) { return (float4v*)((uint8_t*)lds + (GROUPS * (from - 1) + group) * 2 * IMG) + lane; };
+    auto ml = [&](int from) {
+      return (float2*)((uint8_t*)lds + GROUPS * (PARTS - 1) * 2 * IMG) + 64 * (GROUPS * (from - 1) + group) + lane;
+    };
+    if (part) {
+      *ml(part) = make_float2(acc.m, acc.l);
+#pragma unroll
+      for (int db = 0; db < HD / 32; ++db)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          sums(part)[64 * (4 * db + j)] =
+              float4v{acc.o[db][4 * j], acc.o[db][4 * j + 1], acc.o[db][4 * j + 2], acc.o[db][4 * j + 3]};
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    meet();
+    if (part) return;
+    // (a part that saw nothing has the maximum -infinity and zeros)
+    auto weight = [](float m, float most) { return m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - most); };
+    float most = acc.m;
+#pragma unroll
+    for (int k = 1; k < PARTS; ++k) most = fmaxf(most, ml(k)->x);
+    const float f = weight(acc.m, most);
+    acc.l *= f;
+#pragma unroll
+    for (int db = 0; db < HD / 32; ++db)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc.o[db][r] *= f;
+#pragma unroll
+    for (int k = 1; k < PARTS; ++k) {
+      const float w = weight(ml(k)->x, most);
+      acc.l = fmaf(w, ml(k)->y, acc.l);
+#pragma unroll
+      for (int db = 0; db < HD / 32; ++db)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float4v v = sums(k)[64 * (4 * db + j)];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc.o[db][4 * j + e] = fmaf(w, v[e], acc.o[db][4 * j + e]);
+        }
+    }
+  }
   // A value that some rows of the wave do not see meets their probability 0;
   // where it is not finite, their sums are not, and they are taken again. (One
   // query's rows see the same keys.)
@@ -643,12 +699,15 @@ __global__ __launch_bounds__(256, HD == 128 ? 2 : 3) void window_tile_kernel(Win
   uint32_t again = (uint32_t)(bad | bad >> 32);
   if (again && !hidden_spoil<T, HD>(a, heads, list, first, last, 0, list.n)) again = 0;
   // Outputs go through LDS: whole rows to memory, 16 bytes a lane.
-  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-  meet();
-  acc.store((T*)(rows_image + (lane & 31) * 2 * HD), lane & 31, hl);
+  if constexpr (PARTS == 1) {
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    meet();
+  }
+  uint8_t* const out_image = PARTS == 1 ? rows_image : (uint8_t*)lds + (4 * PARTS * BLOCKS - GROUPS + group) * IMG;
+  acc.store((T*)(out_image + (lane & 31) * 2 * HD), lane & 31, hl);
   asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
   image_rows<HD>(lane, [&](int i, int r, int chunk) {
-    const u32x4 v = *(const u32x4*)(rows_image + r * 2 * HD + 16 * (chunk ^ k_swizzle<HD>(r)));
+    const u32x4 v = *(const u32x4*)(out_image + r * 2 * HD + 16 * (chunk ^ k_swizzle<HD>(r)));
     if (w0 + r < rows && !(again >> r & 1)) *(u32x4*)(heads.output(w0 + r, a.query(w0 + r)) + 8 * chunk) = v;
   });
   for (uint32_t todo = again; todo; todo &= todo - 1) {
@@ -900,30 +959,49 @@ __global__ __launch_bounds__(256) void ragged_index_kernel(Ragged rows, int64_t*
 
 // Which kernel a batch takes and how its keys are split, by its sizes alone.
 // `tiles` of 32 rows, of which window_few_kernel has `places` on the chip at a
-// time, and the keys that a query sees. Few rows: while the tiles fit (32
-// heads of 64, 8 KV heads, microseconds few : tile kernel: 500 tokens +-128 9.2
-// : 9.0, 1000 15.4 : 9.6; 512 behind 3000, window 512, 10.9 : 11.9), or nearly
-// and with many keys each (32 heads of 128: 512 tokens behind 8192 keys 106 :
-// 140, 4 x 128 of a 1024-key window 24.9 : 24.4, 64 single tokens of up to 4096
-// 174 : 185). A split costs a second launch, 3.5 us, and is taken from 1280 keys
-// (single token, 32 heads of 64, unsplit : split: 1100 keys 8.3 : 9.4, 1800 10.5
-// : 9.4, 8000 33.6 : 11.0), into pieces of 256 keys and more for more rows, whose
-// sums are written and read again (8 tokens over 8192 keys of 128: pieces of 256
+// time, and the keys that a query sees; microseconds few : tile : tile of 4
+// parts, 32 heads, 8 KV heads.
+//  Tiles that fit: few (64: 500 tokens +-128 9.2 : 9.0, 512 of a 512-key window
+//  10.6 : 12.0; 128: 250 tokens of a 512-key window 10.1 : 15.4 : 13.2, 256
+//  behind 8192 keys 52 : 134 : 74).
+//  More than twice as many: tile (64: 2000 tokens +-128 28 : 13.8; 128: 520
+//  tokens, 1024 keys 33 : 23.6 : 32.4).
+//  Between, heads of 128 whose tiles of 64 rows fit: 4 parts from 384 keys (500
+//  tokens of 132 keys 14.8 : 9.7 : 10.8, 260 15.9 : 11.6 : 12.2, 516 18.6 : 15.6
+//  : 13.6, 1028 23.4 : 23.6 : 17.7; 4 x 128, 1028 keys 24.4 : 24.5 : 20.2).
+//  Between, requests of at most one tile, whose keys come from memory: few
+//  from 1.5 places on (single tokens, heads of 128, 2052 keys: 36 of them 76 :
+//  68, 44 81 : 76, 52 84 : 84, 64 97 : 103; heads of 64: 72 71 : 72, 88 77 : 80,
+//  104 97 : 110).
+//  Between, larger requests, heads of 64: few up to 1.5 places from 2048 keys
+//  (1028 keys: 600 tokens 18.5 : 18.5; 2052: 600 27.5 : 31.5, 800 33.2 : 31.4;
+//  8600: 600 80 : 110); else tile.
+// A split costs a second launch, 3.5 us, and is taken from 1280 keys (single
+// token, heads of 64, unsplit : split: 1100 keys 8.3 : 9.4, 1800 10.5 : 9.4,
+// 8000 33.6 : 11.0), into pieces of 256 keys and more for more rows, whose sums
+// are written and read again (8 tokens over 8192 keys of 128: pieces of 256
 // 20.6, of 512 15.7).
 struct Plan {
-  bool few;
+  enum { kFew, kTile, kParts } kernel;
   int splits;
 };
 Plan window_plan(const nemo_attention_config& c, int count, int64_t q_rows, int64_t max_kv) {
-  if (count == 0 || q_rows == 0) return {false, 1};
+  if (count == 0 || q_rows == 0) return {Plan::kTile, 1};
   const int64_t rows = q_rows * (c.q_heads / c.kv_heads);
-  const int64_t tiles = std::max<int64_t>(rows / 32, count) * c.kv_heads, places = c.head_dim == 64 ? 512 : 256;
+  auto tiles_of = [&](int n) { return std::max<int64_t>(rows / n, count) * c.kv_heads; };
+  const int64_t tiles = tiles_of(32), places = c.head_dim == 64 ? 512 : 256;
   int64_t keys = max_kv;
   if (c.left >= 0 && c.right >= 0) keys = std::min(keys, (int64_t)c.left + c.right + 1 + c.sinks);
-  if (tiles > places && (tiles > 2 * places || keys < 1024)) return {false, 1};
+  if (tiles > places) {
+    if (tiles > 2 * places) return {Plan::kTile, 1};
+    if (c.head_dim == 128 && tiles_of(64) <= places && keys >= 384) return {Plan::kParts, 1};
+    const bool few = rows / count <= 32 ? 2 * tiles >= 3 * places && keys >= 512
+                                        : 2 * tiles <= 3 * places && keys >= 2048 && c.head_dim == 64;
+    return {few ? Plan::kFew : Plan::kTile, 1};
+  }
   const int64_t piece = 256 + 8 * std::min<int64_t>(32, rows / count);
   const int64_t splits = keys < 1280 ? 1 : std::min<int64_t>({places / tiles, keys / piece, 64});
-  return {true, (int)std::max<int64_t>(1, splits)};
+  return {Plan::kFew, (int)std::max<int64_t>(1, splits)};
 }
 
 }  // namespace
@@ -962,9 +1040,15 @@ hipError_t launch_window_attention(const nemo_attention_config& c, const nemo_at
   auto launch = [&](auto type, auto hd) {
     constexpr int HD = decltype(hd)::value;
     typedef decltype(type) T;
-    if (!plan.few) {
-      window_tile_kernel<T, HD><<<tiles(kTileRows), 256, 0, stream>>>(a);
+    if (plan.kernel == Plan::kTile) {
+      window_tile_kernel<T, HD, 1><<<tiles(128), 256, 0, stream>>>(a);
       return;
+    }
+    if constexpr (HD == 128) {
+      if (plan.kernel == Plan::kParts) {
+        window_tile_kernel<T, HD, 4><<<tiles(64), 512, 0, stream>>>(a);
+        return;
+      }
     }
     window_few_kernel<T, HD><<<dim3(tiles(32), splits), 64 * kFewWaves, 0, stream>>>(a, part);
     if (splits > 1) window_join_kernel<T, HD><<<tiles(1), 256, 0, stream>>>(a, part);

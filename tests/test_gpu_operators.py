@@ -420,6 +420,52 @@ def test_attention_spoilt_queries_and_keys(torch_cuda, H, K, key):
     assert torch.isnan(out[bad]).all() and torch.equal(out[~bad], clean[:n][~bad])
 
 
+# 32 query and 8 KV heads of 128, 260 to 500 queries of 384 keys and more: tiles whose keys are dealt to four parts
+PARTS = dict(H=32, K=8, D=128)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("left,right,sinks", [(-1, -1, 0), (-1, 0, 0), (400, 0, 4), (383, 64, 0), (500, 17, 200), (-1, 5, 0),
+                                              (5, -1, 3), (1000, 1000, 1), (0, 0, 1000)])
+def test_attention_in_parts(torch_cuda, dtype, left, right, sinks):
+    """Requests of fewer keys than parts have, without tokens, without keys."""
+    Batch(dtype, *PARTS.values(), left, right, sinks, [1, 200, 0, 33, 57, 64]).run(max_kv=4000).check()
+    Batch(dtype, *PARTS.values(), left, right, sinks, [5, 0, 100, 3, 240, 17], [900, 30, 700, 0, 25, 17]).run().check()
+    Batch(dtype, *PARTS.values(), left, right, sinks, [300], [1333]).run().check()
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_attention_in_parts_scores_that_rise_and_fall(torch_cuda, dtype):
+    b = Batch(dtype, *PARTS.values(), 450, 20, 3, [300], [700], poison=False)
+    size = torch.cat([torch.linspace(0.01, 40, 250), torch.linspace(40, 0.01, 200), torch.linspace(0.01, 60, 250)])
+    b.k = (b.k[:700] * size[:, None, None]).to(dtype)
+    b.v = b.v[:700]
+    b.dk, b.dv = b.k.cuda(), b.v.cuda()
+    b.run().check()
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_attention_in_parts_spoilt_values(torch_cuda, dtype):
+    """Infinite values, NaN queries and keys reach the queries that see them alone."""
+    left, right, sinks, n, m = 500, 0, 2, 300, 900
+    b = Batch(dtype, *PARTS.values(), left, right, sinks, [n], [m], poison=False)
+    bad = [130, 899]
+    for j, value in zip(bad, (math.inf, math.nan)):
+        b.v[j] = value
+    b.k[700] = math.nan
+    b.q[30] = math.nan
+    b.dq, b.dk, b.dv = torch.cat([b.q, b.q[:3]]).cuda(), b.k.cuda(), b.v.cuda()
+    b.out.fill_(7.0)
+    b.run()
+    touched = ref.visible(n, m, left, right, sinks)[:, bad + [700]].any(1)
+    touched[30] = True
+    out = b.out[:n]
+    assert not torch.isfinite(out[touched].float()).any()
+    want, tol = ref.attention(torch.nan_to_num(b.q), *(torch.nan_to_num(t[:m], nan=0.0, posinf=0.0, neginf=0.0)
+                                                       for t in (b.k, b.v)), left, right, sinks, 128 ** -0.5)
+    close(out[~touched], want[~touched], tol[~touched])
+
+
 def test_attention_cut_index_arrays(torch_cuda):
     """Entries outside the buffers are cut to them."""
     b = Batch(F16, 4, 2, 64, 50, 0, 0, [10, 6], [80, 60], poison=False)
