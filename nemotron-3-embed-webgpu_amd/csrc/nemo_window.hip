@@ -393,8 +393,8 @@ struct Rows {
     };
     constexpr int AHEAD = DC / 2;  // fragments are read that many MFMAs before they are used
     auto fragment = [&](int c) {
+      vf[c] = value(v_image, lane, c / DB, c % DB);  // first: the wait for the keys' is theirs too
       kf[c] = key(k_image, lane, c);
-      vf[c] = value(v_image, lane, c / DB, c % DB);
     };
 #pragma unroll
     for (int c = 0; c < AHEAD; ++c) fragment(c);
@@ -536,13 +536,18 @@ __device__ __forceinline__ OneRow<T, HD> one_row(const WindowArgs& a, const Head
 // keys: 18.7 us; 24 with 128 rows or by window_few_kernel, 20 with two parts of
 // two waves, of which a SIMD then has one).
 //
-// Bound by issue: 32768 tokens of 32 heads of 128 (8 KV heads, window 1024),
-// 543 GFLOP, take 597 us, MFMA 48 % and vector units 45 % of the cycles, which
-// a SIMD's two waves hardly overlap (64 multiply-adds beside 8 MFMA take their
-// sum), at a clock that falls to 1.9 GHz. The steps on the way: scores and
-// product of one block in turn 676 us, one block ahead and behind 670 (fewer
-// cycles, lower clock), queries and outputs through LDS and the hidden slots
-// by a mask of bits 629, copies in assembly 618. 16 ragged requests, 2860
+// Bound by the steps' instructions and by power: 32768 tokens of 32 heads of
+// 128 (8 KV heads, window 1024), 543 GFLOP, take 580 to 600 us, 1.14 M cycles
+// at a clock that falls to 1.9 GHz and below, of which the MFMAs are 50 %. A
+// step of a SIMD's two waves takes 1.29 k cycles by itself, 1.02 k of them
+// MFMAs, with the rounds' barriers and copies 1.55 k, and a workgroup's
+// beginning and end are a fifth of its time. Without copies it is 11 % less,
+// without LDS reads 3, without exponentials nothing; fragments read over the
+// barrier, a fifth fewer scalar instructions and workgroups that start apart
+// gave 0 to 3 % of cycles and no time. The steps on the way: scores and product
+// of one block in turn 676 us, one block ahead and behind 670, queries and
+// outputs through LDS and the hidden slots by a mask of bits 629, copies in
+// assembly 618, values' fragments before the keys' 600. 16 ragged requests, 2860
 // tokens, heads of 64, 5 rounds each, are bound by latency: 16.8 us.
 // ---------------------------------------------------------------------------
 
