@@ -46,35 +46,39 @@ struct Seen {
 // numbered through a batch without a table: request i's first number is
 // floor(q_start[i] group / ROWS) + i, which leaves it at least as many numbers
 // as it has tiles. The request of tile number t is the last whose first is not
-// above t; none (i = -1) before the first request. Each lane looks at one
-// request and has its whole entry at hand when it is the one. (Of entries that
-// do not ascend it may be one whose first tile is behind t.)
+// above t; none (i = -1) before the first request. A wave looks at 64 requests
+// at a time, evenly over those that it may be, until they are 64 or fewer; a
+// lane then has the request's whole entry at hand. (Of entries that do not
+// ascend it may be one whose first tile is behind t.)
 template <int ROWS>
 struct Request {
   int i, tile, q0, queries, keys;
   int64_t kv0;
   __device__ __forceinline__ Request(const WindowArgs& a, int t) {
     const nemo_attention_batch& b = a.b;
-    i = -1;
-    for (int i0 = 0; i0 < b.count; i0 += 64) {
-      const int at = min(i0 + (int)(threadIdx.x & 63), b.count - 1);
-      const int begin = min(max(b.q_start[at], 0), (int)b.q_rows);
-      const int end = min(b.q_start[at + 1], (int)b.q_rows);
-      const int64_t kv = min(max(b.kv_start[at], (int64_t)0), b.kv_rows);
-      const int len = (int)min((int64_t)max(b.kv_len[at], 0), b.kv_rows - kv);
-      const int first = (int)((int64_t)begin * a.group / ROWS) + at;
-      const int n = (int)__popcll(__builtin_amdgcn_ballot_w64(i0 + (int)(threadIdx.x & 63) < b.count && first <= t));
-      if (n) {
-        i = i0 + n - 1;
-        tile = __builtin_amdgcn_readlane(first, n - 1);
-        q0 = __builtin_amdgcn_readlane(begin, n - 1);
-        queries = max(__builtin_amdgcn_readlane(end, n - 1) - q0, 0);
-        keys = __builtin_amdgcn_readlane(len, n - 1);
-        kv0 = (int64_t)(uint32_t)__builtin_amdgcn_readlane((int)kv, n - 1) |
-              (int64_t)__builtin_amdgcn_readlane((int)(kv >> 32), n - 1) << 32;
-      }
-      if (n < 64) break;
+    const int lane = threadIdx.x & 63;
+    auto row = [&](int at) { return min(max(b.q_start[at], 0), (int)b.q_rows); };
+    auto number = [&](int begin, int at) { return (int)((int64_t)begin * a.group / ROWS) + at; };
+    int from = 0, left = b.count;
+    while (left > 64) {
+      const int step = (left + 63) >> 6, at = from + min(lane * step, left - 1);
+      const int n = (int)__popcll(__builtin_amdgcn_ballot_w64(lane * step < left && number(row(at), at) <= t));
+      from += max(n - 1, 0) * step;
+      left = min(step, b.count - from);
     }
+    const int at = min(from + lane, b.count - 1), begin = row(at), end = min(b.q_start[at + 1], (int)b.q_rows);
+    const int64_t kv = min(max(b.kv_start[at], (int64_t)0), b.kv_rows);
+    const int len = (int)min((int64_t)max(b.kv_len[at], 0), b.kv_rows - kv), first = number(begin, at);
+    const int n = (int)__popcll(__builtin_amdgcn_ballot_w64(lane < left && first <= t));
+    i = from + n - 1;
+    if (!n) i = -1;
+    const int of = max(n - 1, 0);
+    tile = __builtin_amdgcn_readlane(first, of);
+    q0 = __builtin_amdgcn_readlane(begin, of);
+    queries = max(__builtin_amdgcn_readlane(end, of) - q0, 0);
+    keys = __builtin_amdgcn_readlane(len, of);
+    kv0 = (int64_t)(uint32_t)__builtin_amdgcn_readlane((int)kv, of) |
+          (int64_t)__builtin_amdgcn_readlane((int)(kv >> 32), of) << 32;
   }
 };
 

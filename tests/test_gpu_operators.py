@@ -318,6 +318,12 @@ def test_attention_many_requests(torch_cuda, dtype, D):
     Batch(dtype, 8, 8, D, 50, 0, 2, [min(1, n) for n in lens], [n * 11 for n in lens]).run().check()
 
 
+@pytest.mark.parametrize("count", [64, 65, 128, 500, 4097, 4200])
+def test_attention_numbers_of_requests(torch_cuda, count):
+    """Around the numbers at which the search for a tile's request takes another round."""
+    Batch(F16, 2, 1, 64, 9, 0, 1, [(5 * i * i + i) % 4 for i in range(count)]).run().check()
+
+
 @pytest.mark.parametrize("dtype,D", [(F16, 64), (BF16, 128)])
 @pytest.mark.parametrize("H,K", [(1, 1), (3, 1), (5, 1), (8, 1), (16, 2), (40, 1), (6, 6), (24, 8)])
 def test_attention_head_groups(torch_cuda, dtype, D, H, K):
