@@ -377,9 +377,9 @@ nemo_status nemo_window_attention(nemo_ctx* ctx, const nemo_attention_config* co
  * in 32 bits from the unrounded h; sum = h and y in `type`; and
  *   scales = max |y| / 127 (I8) or / 448 (F8_E4M3), y8 = round(y / scale)
  * of the unrounded y over a whole row or over each `group` columns (scale 0,
- * and y8 0, where y is 0; NaN where y holds a NaN; to even on ties). Where
- * sum or y is x or delta it has the same row stride; other overlap of an input
- * and an output is not allowed. */
+ * and y8 0, where y is 0; NaN where y holds a NaN; to even on ties, the
+ * quotient as 64 bits give it). Where sum or y is x or delta it has the same
+ * row stride; other overlap of an input and an output is not allowed. */
 typedef struct nemo_norm_args {
   int32_t type;              /* of x, delta, sum, y: F32, F16 or BF16 */
   int32_t hidden;            /* >= 1 */

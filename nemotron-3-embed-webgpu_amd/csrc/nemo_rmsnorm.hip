@@ -2,12 +2,16 @@
 // delta, y = h / sqrt(mean(h^2) + eps) * w, y8 = round(y / s) with s = max |y|
 // / 127 (bytes) or / 448 (8-bit floats) over a row or a group of columns.
 //
-// The row's factor cancels in y / s = h w top / max |h w|, whose four roundings
-// in 32 bits leave it within 2^-22 of itself. Next to a border between two codes
-// that decides wrongly a few times in a million values, so each is coded from
-// both ends of 2^-21 around it, and a wave in which two codes differ (about one
-// in a hundred) takes its values again in 64 bits. In 64 bits throughout, 16384
-// x 8192 bf16 to 8-bit floats with scales of 128 columns took 226 us.
+// The row's factor cancels in y / s = h w top / max |h w|, whose seven roundings
+// in 32 bits (h and its product with w, here and in the maximum, the quotient,
+// and two products with that) leave it within 7 2^-24 of itself. Next to a
+// border between two codes that decides wrongly a few times in a million
+// values, so each is coded from both ends of 2^-21 around it, and a wave in
+// which two codes differ (about one in a hundred) takes its values again in 64
+// bits, with what the sum x + delta of 32-bit values lost, and rounds once. (The
+// sum of 16-bit values is exact but for a delta some 2^-13 of its x and
+// smaller.) In 64 bits throughout, 16384 x 8192 bf16 to 8-bit floats with scales
+// of 128 columns took 226 us.
 //
 // Bound by memory: each value is read and written once, 16 bytes a lane. Those
 // 16384 rows, 944 MB, take 177 us (5.3 TB/s; a copy reaches 4.9 to 5.4).
@@ -47,6 +51,15 @@ __device__ __forceinline__ uint32_t code4(bool bytes, float a, float b, float c,
            ((uint32_t)(int)rintf(c) & 255u) << 16 | (uint32_t)(int)rintf(d) << 24;
   const int low = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
   return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, low, true);
+}
+
+// v with its last bit set where 32 bits do not hold it, rounded to zero before:
+// a code of that is v's own.
+__device__ __forceinline__ float odd(double v) {
+  const float f = (float)v;
+  uint32_t bits = __float_as_uint(f);
+  if ((double)f != v) bits = (bits - (fabs((double)f) > fabs(v) ? 1 : 0)) | 1;
+  return __uint_as_float(bits);
 }
 
 // The scale of values h w `factor` whose largest |h w| is `peak` (its bits), and
@@ -95,7 +108,8 @@ __global__ __launch_bounds__(WAVES > 4 ? 64 * WAVES : 256) void norm8_kernel(nem
   const int first = 8 * (64 * (wave % WAVES) + lane);
   const T* x = (const T*)a.x + row * a.x_row;
   const T* delta = (const T*)a.delta + row * a.delta_row;
-  float h[NV][8];
+  constexpr bool LOST = sizeof(T) == 4;
+  float h[NV][8], lost[LOST ? NV : 1][8] = {};  // h and what its rounding left out
   float sum = 0.f;
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
@@ -116,7 +130,14 @@ __global__ __launch_bounds__(WAVES > 4 ? 64 * WAVES : 256) void norm8_kernel(nem
       if (c < a.hidden) {
         const vec v = *(const vec*)(delta + c);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) h[i][e] += (float)v[e];
+        for (int e = 0; e < 8; ++e) {
+          const float from = h[i][e], add = (float)v[e];
+          h[i][e] = from + add;
+          if constexpr (LOST) {
+            const float added = h[i][e] - from;
+            lost[i][e] = (from - (h[i][e] - added)) + (add - added);
+          }
+        }
       }
     }
   }
@@ -124,6 +145,7 @@ __global__ __launch_bounds__(WAVES > 4 ? 64 * WAVES : 256) void norm8_kernel(nem
   for (int i = 0; i < NV; ++i)
 #pragma unroll
     for (int e = 0; e < 8; ++e) sum = fmaf(h[i][e], h[i][e], sum);
+  auto exact = [&](int i, int e) { return LOST ? (double)h[i][e] + (double)lost[LOST ? i : 0][e] : (double)h[i][e]; };
   sum = wave_sum(sum);
   if constexpr (WAVES > 1) {
     if (lane == 0) part[wave] = sum;
@@ -172,14 +194,14 @@ __global__ __launch_bounds__(WAVES > 4 ? 64 * WAVES : 256) void norm8_kernel(nem
     uint32_t most = lanes_max(own, 64);
     if constexpr (WAVES > 1) {
       if (lane == __builtin_ctzll(__builtin_amdgcn_ballot_w64(own == most))) {
-        uint64_t exact = 0;
+        uint64_t most64 = 0;
 #pragma unroll
         for (int i = 0; i < NV; ++i)
 #pragma unroll
           for (int e = 0; e < 8; ++e)
-            if (magnitude(h[i][e] * w[i][e]) == most) exact = magnitude((double)h[i][e] * (double)w[i][e]);
+            if (magnitude(h[i][e] * w[i][e]) == most) most64 = max(most64, magnitude(exact(i, e) * (double)w[i][e]));
         peaks[wave] = most;
-        peaks64[wave] = exact;
+        peaks64[wave] = most64;
       }
       __syncthreads();
 #pragma unroll
@@ -223,7 +245,7 @@ __global__ __launch_bounds__(WAVES > 4 ? 64 * WAVES : 256) void norm8_kernel(nem
   for (int i = 0; i < NV; ++i) {
     peak64[i] = 0;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) peak64[i] = max(peak64[i], magnitude((double)h[i][e] * (double)w[i][e]));
+    for (int e = 0; e < 8; ++e) peak64[i] = max(peak64[i], magnitude(exact(i, e) * (double)w[i][e]));
   }
   if (a.group) {
 #pragma unroll
@@ -248,7 +270,7 @@ __global__ __launch_bounds__(WAVES > 4 ? 64 * WAVES : 256) void norm8_kernel(nem
     const Quantizer64 q(peak64[i], inv, top);
     float v[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = (float)((double)h[i][e] * (double)w[i][e] * q.inv);
+    for (int e = 0; e < 8; ++e) v[e] = odd(exact(i, e) * (double)w[i][e] * q.inv);
     put(c, q.scale, u32x2{code4(bytes, v[0], v[1], v[2], v[3]), code4(bytes, v[4], v[5], v[6], v[7])});
   }
 }
@@ -264,7 +286,8 @@ __global__ __launch_bounds__(256) void norm8_any_kernel(nemo_norm_args a) {
   const int64_t row = blockIdx.x;
   const T* x = (const T*)a.x + row * a.x_row;
   const T* delta = a.delta ? (const T*)a.delta + row * a.delta_row : nullptr;
-  auto load = [&](int c) { return (float)x[c] + (delta ? (float)delta[c] : 0.f); };
+  auto exact = [&](int c) { return (double)(float)x[c] + (delta ? (double)(float)delta[c] : 0.0); };
+  auto load = [&](int c) { return (float)exact(c); };
   float sum = 0.f;
   for (int c = threadIdx.x; c < a.hidden; c += 256) {
     const float v = load(c);
@@ -278,7 +301,7 @@ __global__ __launch_bounds__(256) void norm8_any_kernel(nemo_norm_args a) {
   auto weight = [&](int c) { return a.weight ? a.weight[c] : 1.f; };
   uint64_t most = 0;
   if (a.y8 && a.group == 0) {
-    for (int c = threadIdx.x; c < a.hidden; c += 256) most = max(most, magnitude((double)load(c) * (double)weight(c)));
+    for (int c = threadIdx.x; c < a.hidden; c += 256) most = max(most, magnitude(exact(c) * (double)weight(c)));
     most = lanes_max(most, 64);
     if (lane == 0) peaks[wave] = most;
     __syncthreads();
@@ -288,15 +311,16 @@ __global__ __launch_bounds__(256) void norm8_any_kernel(nemo_norm_args a) {
   float* scales = a.y8 ? a.scales + row * a.scales_row : nullptr;
   const int width = a.group ? a.group : 128;  // columns of a wave's step, up to 2 a lane
   for (int at = width * wave; at < a.hidden; at += 4 * width) {
-    float h[2], w[2];
+    double h[2];
+    float w[2];
     uint64_t peak = 0;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const int c = at + lane + 64 * i;
       const bool in = lane + 64 * i < width && c < a.hidden;
-      h[i] = in ? load(c) : 0.f;
+      h[i] = in ? exact(c) : 0.0;
       w[i] = in ? weight(c) : 0.f;
-      peak = max(peak, magnitude((double)h[i] * (double)w[i]));
+      peak = max(peak, magnitude(h[i] * (double)w[i]));
     }
     peak = a.group ? lanes_max(peak, 64) : most;
     const Quantizer64 q(peak, inv, top);
@@ -305,10 +329,10 @@ __global__ __launch_bounds__(256) void norm8_any_kernel(nemo_norm_args a) {
     for (int i = 0; i < 2; ++i) {
       const int c = at + lane + 64 * i;
       if (lane + 64 * i >= width || c >= a.hidden) continue;
-      if (a.sum) ((T*)a.sum)[row * a.sum_row + c] = (T)h[i];
-      if (a.y) ((T*)a.y)[row * a.y_row + c] = (T)(h[i] * inv * w[i]);
+      if (a.sum) ((T*)a.sum)[row * a.sum_row + c] = (T)(float)h[i];
+      if (a.y) ((T*)a.y)[row * a.y_row + c] = (T)((float)h[i] * inv * w[i]);
       if (a.y8) {
-        const float v = (float)((double)h[i] * (double)w[i] * q.inv);
+        const float v = odd(h[i] * (double)w[i] * q.inv);
         ((uint8_t*)a.y8)[row * a.y8_row + c] = (uint8_t)code4(a.type8 == NEMO_TYPE_I8, v, 0.f, 0.f, 0.f);
       }
     }
@@ -332,8 +356,12 @@ hipError_t launch_norm_type(const nemo_norm_args& a, hipStream_t stream) {
     norm8_kernel<T, 4, 1><<<rows, 256, 0, stream>>>(a);
   else if (blocks <= 512)
     norm8_kernel<T, 4, 2><<<rows, 256, 0, stream>>>(a);
-  else if (blocks <= 1024)  // (16384 x 8192: 4 waves of 4 blocks 219 us, 8 of 2 179, 16 of one 189)
+  else if (blocks <= 1024 && sizeof(T) == 2)  // (16384 x 8192: 4 waves of 4 blocks 219 us, 8 of 2 177, 16 of one 188)
     norm8_kernel<T, 8, 2><<<rows, 512, 0, stream>>>(a);
+  else if (blocks <= 1024)  // (what its sums lost takes registers too: 4096 x 8192, 8 of 2 88 us, 16 of one 81)
+    norm8_kernel<T, 16, 1><<<rows, 1024, 0, stream>>>(a);
+  else if (blocks <= 2048)  // (4096 x 16384, 16 waves: f32, 4 blocks 256 us, 2 180; bf16 140, 98)
+    norm8_kernel<T, 16, 2><<<rows, 1024, 0, stream>>>(a);
   else
     norm8_kernel<T, 16, 4><<<rows, 1024, 0, stream>>>(a);
   return hipGetLastError();

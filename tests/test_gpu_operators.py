@@ -186,6 +186,37 @@ def test_norm(torch_cuda, dtype, type8, rows, hidden, group, shift):
     check8(y8, scales, want, rel, type8, group)
 
 
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
+@pytest.mark.parametrize("type8", [ops.TYPE_I8, ops.TYPE_E4M3])
+@pytest.mark.parametrize("rows,hidden,group", [(600, 512, 0), (300, 4096, 64), (150, 8192, 0), (40, 16384, 128), (300, 1000, 0),
+                                               (20, 12296, 0), (20, 20008, 0)])
+def test_norm_codes_are_those_of_64_bits(torch_cuda, dtype, type8, rows, hidden, group):
+    """A code is round(h w top / max |h w|) in 64 bits, the sum x + delta
+    included: values are left out whose quotient is within 2^-40 of a border
+    between two codes, and 16-bit ones whose sum 32 bits do not hold (of which
+    the rest of a group depends on at most the largest)."""
+    x, delta, w = rand(61, rows, hidden, dtype=dtype), rand(62, rows, hidden, dtype=dtype), 1 + 0.1 * rand(63, hidden)
+    dx, dd, dw = x.cuda(), delta.cuda(), w.cuda()
+    y8 = torch.empty(rows, hidden, dtype=torch.int8 if type8 == ops.TYPE_I8 else torch.float8_e4m3fn, device="cuda")
+    scales = torch.empty(rows, hidden // group if group else 1, device="cuda")
+    ops.RmsNorm().run(ops.norm_args(CODE[dtype], rows, hidden, dx.data_ptr(), dw.data_ptr(), 1e-5, dd.data_ptr(),
+                                    d_y8=y8.data_ptr(), type8=type8, d_scales=scales.data_ptr(), group=group), stream())
+    torch.cuda.synchronize()
+    h = x.double() + delta.double()
+    held = torch.ones_like(h, dtype=torch.bool) if dtype == F32 else h == h.float().double()
+    v = (h * w.double()).view(rows, -1, group or hidden)
+    held = held.view(v.shape)
+    held &= held.gather(-1, v.abs().argmax(-1, keepdim=True))
+    u = v * (127.0 if type8 == ops.TYPE_I8 else 448.0) / v.abs().amax(-1, keepdim=True)
+    unit = torch.ones_like(u) if type8 == ops.TYPE_I8 else torch.exp2(
+        torch.floor(torch.log2(u.abs().clamp(min=2.0 ** -6))) - 3)  # the codes' distance
+    steps = u / unit
+    clear = ((steps.abs() % 1 - 0.5).abs() > 2.0 ** -40) & held
+    got = y8.cpu().float().double().view(u.shape)
+    assert clear.double().mean() > 0.99
+    assert torch.equal(got[clear], (torch.round(steps) * unit)[clear])
+
+
 def test_norm_in_place_and_parts(torch_cuda):
     """The sum replaces the residual and y the branch; each output alone gives
     the same bits; padded rows keep their padding."""
