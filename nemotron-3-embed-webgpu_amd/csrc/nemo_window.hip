@@ -973,15 +973,17 @@ __global__ __launch_bounds__(256) void ragged_index_kernel(Ragged rows, int64_t*
 //  Tiles that fit: few (64: 500 tokens +-128 9.2 : 9.0, 512 of a 512-key window
 //  10.6 : 12.0; 128: 250 tokens of a 512-key window 10.1 : 15.4 : 13.2, 256
 //  behind 8192 keys 52 : 134 : 74).
+//  More, requests of at most 8 rows, whose keys come from memory: few from 512
+//  keys and 1.5 to 8 times the places (single tokens, heads of 128, 2052 keys:
+//  36 of them 76 : 68, 44 81 : 76, 52 84 : 84, 96 141 : 164, 256 370 : 386, 512
+//  735 : 749; 132 keys: 96 23 : 19.6; heads of 64: 104 97 : 110, 320 260 : 280,
+//  1024 830 : 783), else tile, as for more rows (64 x 4 tokens, heads of 128 117
+//  : 99; 64 x 8 131 : 101).
 //  More than twice as many: tile (64: 2000 tokens +-128 28 : 13.8; 128: 520
 //  tokens, 1024 keys 33 : 23.6 : 32.4).
 //  Between, heads of 128 whose tiles of 64 rows fit: 4 parts from 384 keys (500
 //  tokens of 132 keys 14.8 : 9.7 : 10.8, 260 15.9 : 11.6 : 12.2, 516 18.6 : 15.6
 //  : 13.6, 1028 23.4 : 23.6 : 17.7; 4 x 128, 1028 keys 24.4 : 24.5 : 20.2).
-//  Between, requests of at most one tile, whose keys come from memory: few
-//  from 1.5 places on (single tokens, heads of 128, 2052 keys: 36 of them 76 :
-//  68, 44 81 : 76, 52 84 : 84, 64 97 : 103; heads of 64: 72 71 : 72, 88 77 : 80,
-//  104 97 : 110).
 //  Between, larger requests, heads of 64: few up to 1.5 places from 2048 keys
 //  (1028 keys: 600 tokens 18.5 : 18.5; 2052: 600 27.5 : 31.5, 800 33.2 : 31.4;
 //  8600: 600 80 : 110); else tile.
@@ -1002,11 +1004,11 @@ Plan window_plan(const nemo_attention_config& c, int count, int64_t q_rows, int6
   int64_t keys = max_kv;
   if (c.left >= 0 && c.right >= 0) keys = std::min(keys, (int64_t)c.left + c.right + 1 + c.sinks);
   if (tiles > places) {
+    if (rows / count <= 8)
+      return {keys >= 512 && 2 * tiles >= 3 * places && tiles <= 8 * places ? Plan::kFew : Plan::kTile, 1};
     if (tiles > 2 * places) return {Plan::kTile, 1};
     if (c.head_dim == 128 && tiles_of(64) <= places && keys >= 384) return {Plan::kParts, 1};
-    const bool few = rows / count <= 32 ? 2 * tiles >= 3 * places && keys >= 512
-                                        : 2 * tiles <= 3 * places && keys >= 2048 && c.head_dim == 64;
-    return {few ? Plan::kFew : Plan::kTile, 1};
+    return {c.head_dim == 64 && 2 * tiles <= 3 * places && keys >= 2048 ? Plan::kFew : Plan::kTile, 1};
   }
   const int64_t piece = 256 + 8 * std::min<int64_t>(32, rows / count);
   const int64_t splits = keys < 1280 ? 1 : std::min<int64_t>({places / tiles, keys / piece, 64});

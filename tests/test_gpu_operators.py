@@ -518,14 +518,14 @@ def test_attention_cut_index_arrays(torch_cuda):
     assert not b.out.any()  # no keys: every row, the last three too, is 0
 
 
-@pytest.mark.parametrize("H,K,keys", [(4, 2, 300), (64, 32, 300), (4, 2, 3000)])
+@pytest.mark.parametrize("H,K,D,keys", [(4, 2, 64, 300), (64, 32, 64, 300), (4, 2, 64, 3000), (32, 8, 128, 400)])
 @pytest.mark.parametrize("q_start", [[0, 297, 5, 300], [290, 295, 0, 299], [300, 0, 300, 0], [0, -7, 200, 100]])
-def test_attention_of_requests_out_of_order(torch_cuda, H, K, keys, q_start):
+def test_attention_of_requests_out_of_order(torch_cuda, H, K, D, keys, q_start):
     """q_start that does not ascend says nothing about the results, but only
     rows of the buffers are read and written."""
-    b = Batch(F16, H, K, 64, -1, 0, 0, [5, 5, 5], [keys] * 3, poison=False)
+    b = Batch(F16, H, K, D, -1, 0, 0, [5, 5, 5], [keys] * 3, poison=False)
     n = 300
-    q, out = (torch.full((3 * n, H, 64), 7.0, dtype=F16, device="cuda") for _ in range(2))
+    q, out = (torch.full((3 * n, H, D), 7.0, dtype=F16, device="cuda") for _ in range(2))
     b.dq, b.out = q[n:2 * n], out[n:2 * n]
     b.q_start = torch.tensor(q_start, dtype=torch.int32).cuda()
     b.run()
@@ -585,6 +585,37 @@ def test_attention_streams_and_graph(torch_cuda):
         b.attention.run(args, stream())
         torch.cuda.synchronize()
         assert torch.equal(replayed, b.out)
+
+
+def test_attention_on_two_streams_at_once(torch_cuda):
+    """One object, two batches with a workspace each, in flight together; both
+    captured into one graph on its one stream may share one."""
+    a = Batch(F16, 8, 2, 64, 4000, 0, 4, [1] * 3, [6000, 3, 5000], seed=71, poison=False)
+    b = Batch(F16, 8, 2, 64, 4000, 0, 4, [2] * 3, [5500, 40, 4000], seed=75, poison=False)
+    one, two = a.args(), b.args()
+    assert one.workspace_bytes and two.workspace_bytes
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        a.attention.run(one, streams[0].cuda_stream)
+        a.attention.run(two, streams[1].cuda_stream)
+    torch.cuda.synchronize()
+    a.check()
+    b.check()
+    first = one if one.workspace_bytes >= two.workspace_bytes else two
+    one.workspace = two.workspace = first.workspace
+    one.workspace_bytes = two.workspace_bytes = first.workspace_bytes
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        for args in (one, two):
+            a.attention.run(args, torch.cuda.current_stream().cuda_stream)
+    for _ in range(3):
+        a.out.fill_(7.0)
+        b.out.fill_(7.0)
+        g.replay()
+        torch.cuda.synchronize()
+        a.check()
+        b.check()
 
 
 def test_attention_same_bits(torch_cuda):
