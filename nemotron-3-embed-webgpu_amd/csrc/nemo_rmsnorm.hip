@@ -53,6 +53,11 @@ __device__ __forceinline__ uint32_t code4(bool bytes, float a, float b, float c,
   return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, low, true);
 }
 
+__device__ __forceinline__ uint8_t code1(bool bytes, float v) {
+  if (bytes) return (uint8_t)(int)rintf(v);
+  return (uint8_t)__builtin_amdgcn_cvt_pk_fp8_f32(v, v, 0, false);
+}
+
 // v with its last bit set where 32 bits do not hold it, rounded to zero before:
 // a code of that is v's own.
 __device__ __forceinline__ float odd(double v) {
@@ -275,9 +280,60 @@ __global__ __launch_bounds__(WAVES > 4 ? 64 * WAVES : 256) void norm8_kernel(nem
   }
 }
 
-// Any sizes, strides and alignments: a workgroup reads its row once for the
-// norm, once more for a whole row's scale, and once to write (a lane what it
-// has just read).
+// Any alignment and stride: a lane holds 8 values of a row of up to 512, one
+// wave a row, value i of column 64 i + lane. All in 64 bits (4096 x 147 f32 to
+// 8-bit floats 6.9 us, by the kernel below 10).
+template <typename T>
+__global__ __launch_bounds__(256) void norm8_values_kernel(nemo_norm_args a) {
+  constexpr int NV = 8;
+  const int lane = threadIdx.x & 63;
+  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (row >= a.rows) return;
+  const T* x = (const T*)a.x + row * a.x_row;
+  const T* delta = (const T*)a.delta + row * a.delta_row;
+  double h[NV];
+  float w[NV], sum = 0.f;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int c = 64 * i + lane;
+    h[i] = c < a.hidden ? (double)(float)x[c] + (a.delta ? (double)(float)delta[c] : 0.0) : 0.0;
+    w[i] = a.weight && c < a.hidden ? a.weight[c] : 1.f;
+    sum = fmaf((float)h[i], (float)h[i], sum);
+  }
+  sum = wave_sum(sum);
+  const float inv = 1.0f / sqrtf(sum / (float)a.hidden + a.epsilon);
+  uint64_t peak[NV], most = 0;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int c = 64 * i + lane;
+    peak[i] = magnitude(h[i] * (double)w[i]);
+    most = max(most, peak[i]);
+    if (c >= a.hidden) continue;
+    if (a.sum) ((T*)a.sum)[row * a.sum_row + c] = (T)(float)h[i];
+    if (a.y) ((T*)a.y)[row * a.y_row + c] = (T)((float)h[i] * inv * w[i]);
+  }
+  if (!a.y8) return;
+  most = lanes_max(most, 64);
+  const bool bytes = a.type8 == NEMO_TYPE_I8;
+#pragma unroll
+  for (int i = 0; i < NV; i += 2) {
+    if (a.group == 128) peak[i] = peak[i + 1] = max(peak[i], peak[i + 1]);
+#pragma unroll
+    for (int k = i; k < i + 2; ++k) {
+      const int c = 64 * k + lane;
+      const uint64_t top = a.group ? lanes_max(peak[k], min(a.group, 64)) : most;
+      if (c >= a.hidden) continue;
+      const Quantizer64 q(top, inv, bytes ? 127.0 : 448.0);
+      if (a.group ? c % a.group == 0 : c == 0) a.scales[row * a.scales_row + (a.group ? c / a.group : 0)] = q.scale;
+      ((uint8_t*)a.y8)[row * a.y8_row + c] = code1(bytes, odd(h[k] * (double)w[k] * q.inv));
+    }
+  }
+}
+
+// Longer rows of any alignment and stride: a workgroup reads its row once for
+// the norm, once more for a whole row's scale, and once to write (a lane what it
+// has just read). Codes are decided as above. Bound by its loads and stores of
+// single values, some ten each (4096 x 3145 f32 to 8-bit floats 67 us, 2.5 TB/s).
 template <typename T>
 __global__ __launch_bounds__(256) void norm8_any_kernel(nemo_norm_args a) {
   __shared__ float part[4];
@@ -286,11 +342,9 @@ __global__ __launch_bounds__(256) void norm8_any_kernel(nemo_norm_args a) {
   const int64_t row = blockIdx.x;
   const T* x = (const T*)a.x + row * a.x_row;
   const T* delta = a.delta ? (const T*)a.delta + row * a.delta_row : nullptr;
-  auto exact = [&](int c) { return (double)(float)x[c] + (delta ? (double)(float)delta[c] : 0.0); };
-  auto load = [&](int c) { return (float)exact(c); };
   float sum = 0.f;
   for (int c = threadIdx.x; c < a.hidden; c += 256) {
-    const float v = load(c);
+    const float v = (float)x[c] + (delta ? (float)delta[c] : 0.f);
     sum = fmaf(v, v, sum);
   }
   sum = wave_sum(sum);
@@ -298,44 +352,65 @@ __global__ __launch_bounds__(256) void norm8_any_kernel(nemo_norm_args a) {
   __syncthreads();
   sum = part[0] + part[1] + part[2] + part[3];
   const float inv = 1.0f / sqrtf(sum / (float)a.hidden + a.epsilon);
-  auto weight = [&](int c) { return a.weight ? a.weight[c] : 1.f; };
+  auto exact = [](float from, float add, float w) { return ((double)from + (double)add) * (double)w; };
   uint64_t most = 0;
   if (a.y8 && a.group == 0) {
-    for (int c = threadIdx.x; c < a.hidden; c += 256) most = max(most, magnitude(exact(c) * (double)weight(c)));
+    float near = -1.f;  // the largest magnitude so far less what 32 bits may be off by
+    for (int c = threadIdx.x; c < a.hidden; c += 256) {
+      const float from = (float)x[c], add = delta ? (float)delta[c] : 0.f, w = a.weight ? a.weight[c] : 1.f;
+      const float v = fabsf((from + add) * w);
+      if (v < near) continue;
+      near = fmaxf(near, v * (1 - 0x1p-20f) - 0x1p-140f);
+      most = max(most, magnitude(exact(from, add, w)));
+    }
     most = lanes_max(most, 64);
     if (lane == 0) peaks[wave] = most;
     __syncthreads();
     for (int w = 0; w < 4; ++w) most = max(most, peaks[w]);
   }
-  const double top = a.type8 == NEMO_TYPE_I8 ? 127.0 : 448.0;
+  const bool bytes = a.type8 == NEMO_TYPE_I8;
+  const float top = bytes ? 127.f : 448.f;
   float* scales = a.y8 ? a.scales + row * a.scales_row : nullptr;
+  uint8_t* y8 = (uint8_t*)a.y8 + row * a.y8_row;
   const int width = a.group ? a.group : 128;  // columns of a wave's step, up to 2 a lane
   for (int at = width * wave; at < a.hidden; at += 4 * width) {
-    double h[2];
-    float w[2];
-    uint64_t peak = 0;
+    float from[2], add[2], h[2], w[2];
+    uint32_t peak = 0;
+    bool in[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const int c = at + lane + 64 * i;
-      const bool in = lane + 64 * i < width && c < a.hidden;
-      h[i] = in ? exact(c) : 0.0;
-      w[i] = in ? weight(c) : 0.f;
-      peak = max(peak, magnitude(h[i] * (double)w[i]));
+      in[i] = lane + 64 * i < width && c < a.hidden;
+      from[i] = in[i] ? (float)x[c] : 0.f;
+      add[i] = in[i] && delta ? (float)delta[c] : 0.f;
+      w[i] = in[i] && a.weight ? a.weight[c] : 1.f;
+      h[i] = from[i] + add[i];
+      peak = max(peak, magnitude(h[i] * w[i]));
+      if (in[i] && a.sum) ((T*)a.sum)[row * a.sum_row + c] = (T)h[i];
+      if (in[i] && a.y) ((T*)a.y)[row * a.y_row + c] = (T)(h[i] * inv * w[i]);
     }
-    peak = a.group ? lanes_max(peak, 64) : most;
-    const Quantizer64 q(peak, inv, top);
-    if (a.y8 && lane == 0 && (a.group || at == 0)) scales[a.group ? at / a.group : 0] = q.scale;
+    if (!a.y8) continue;
+    const double most_value = __builtin_bit_cast(double, most);
+    const Quantizer q(a.group ? lanes_max(peak, 64) : magnitude((float)most_value), inv, top);
+    uint8_t code[2];
+    float scale = q.scale;
+    bool unsure = q.unsure;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const int c = at + lane + 64 * i;
-      if (lane + 64 * i >= width || c >= a.hidden) continue;
-      if (a.sum) ((T*)a.sum)[row * a.sum_row + c] = (T)(float)h[i];
-      if (a.y) ((T*)a.y)[row * a.y_row + c] = (T)((float)h[i] * inv * w[i]);
-      if (a.y8) {
-        const float v = odd(h[i] * (double)w[i] * q.inv);
-        ((uint8_t*)a.y8)[row * a.y8_row + c] = (uint8_t)code4(a.type8 == NEMO_TYPE_I8, v, 0.f, 0.f, 0.f);
-      }
+      code[i] = code1(bytes, h[i] * w[i] * q.low);
+      unsure |= code[i] != code1(bytes, h[i] * w[i] * q.high);
     }
+    if (__builtin_amdgcn_ballot_w64(unsure)) {
+      const uint64_t own = max(magnitude(exact(from[0], add[0], w[0])), magnitude(exact(from[1], add[1], w[1])));
+      const Quantizer64 q64(a.group ? lanes_max(own, 64) : most, inv, top);
+      scale = q64.scale;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) code[i] = code1(bytes, odd(exact(from[i], add[i], w[i]) * q64.inv));
+    }
+    if (lane == 0 && (a.group || at == 0)) scales[a.group ? at / a.group : 0] = scale;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      if (in[i]) y8[at + lane + 64 * i] = code[i];
   }
 }
 
@@ -348,7 +423,9 @@ hipError_t launch_norm_type(const nemo_norm_args& a, hipStream_t stream) {
                        fits(a.sum, a.sum_row) && fits(a.y, a.y_row) && ((uintptr_t)a.weight & 15) == 0 &&
                        (!a.y8 || (((uintptr_t)a.y8 & 7) == 0 && a.y8_row % 8 == 0)) && blocks <= 64 * 16 * 4;
   const unsigned rows = (unsigned)a.rows;
-  if (!vectors)
+  if (!vectors && a.hidden <= 512)
+    norm8_values_kernel<T><<<(rows + 3) / 4, 256, 0, stream>>>(a);
+  else if (!vectors)
     norm8_any_kernel<T><<<rows, 256, 0, stream>>>(a);
   else if (blocks <= 64)
     norm8_kernel<T, 1, 1><<<(rows + 3) / 4, 256, 0, stream>>>(a);

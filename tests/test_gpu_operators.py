@@ -189,7 +189,8 @@ def test_norm(torch_cuda, dtype, type8, rows, hidden, group, shift):
 @pytest.mark.parametrize("dtype", [F16, BF16, F32])
 @pytest.mark.parametrize("type8", [ops.TYPE_I8, ops.TYPE_E4M3])
 @pytest.mark.parametrize("rows,hidden,group", [(600, 512, 0), (300, 4096, 64), (150, 8192, 0), (40, 16384, 128), (300, 1000, 0),
-                                               (20, 12296, 0), (20, 20008, 0)])
+                                               (20, 12296, 0), (20, 20008, 0), (90, 131, 0), (70, 1001, 0), (60, 3145, 0),
+                                               (30, 7003, 0), (9, 16383, 0), (5, 16385, 0)])
 def test_norm_codes_are_those_of_64_bits(torch_cuda, dtype, type8, rows, hidden, group):
     """A code is round(h w top / max |h w|) in 64 bits, the sum x + delta
     included: values are left out whose quotient is within 2^-40 of a border
@@ -215,6 +216,32 @@ def test_norm_codes_are_those_of_64_bits(torch_cuda, dtype, type8, rows, hidden,
     got = y8.cpu().float().double().view(u.shape)
     assert clear.double().mean() > 0.99
     assert torch.equal(got[clear], (torch.round(steps) * unit)[clear])
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("hidden,group", [(384, 32), (512, 128), (1920, 64), (3968, 128), (4160, 64), (16256, 128), (16512, 32)])
+def test_norm_of_unaligned_rows_in_place(torch_cuda, dtype, hidden, group):
+    """Rows that begin anywhere, with space between them; the sum replaces the residual."""
+    rows = 6
+    x, delta, w = rand(65, rows, hidden, dtype=dtype), rand(66, rows, hidden, dtype=dtype), 1 + 0.1 * rand(67, hidden)
+    stride = hidden + 3
+    dx = torch.zeros(rows * stride + 1, dtype=dtype).cuda()[1:].view(rows, stride)
+    dd = torch.zeros_like(dx)
+    dx[:, :hidden], dd[:, :hidden] = x.cuda(), delta.cuda()
+    dw = torch.zeros(hidden + 1).cuda()[1:]
+    dw.copy_(w)
+    y8 = torch.zeros(rows, stride, dtype=torch.int8, device="cuda")
+    scales = torch.zeros(rows, hidden // group, device="cuda")
+    y = torch.full((rows, stride), 7.0, dtype=dtype, device="cuda")
+    ops.RmsNorm().run(ops.norm_args(CODE[dtype], rows, hidden, dx.data_ptr(), dw.data_ptr(), 1e-5, dd.data_ptr(), dx.data_ptr(),
+                                    y.data_ptr(), y8.data_ptr(), ops.TYPE_I8, scales.data_ptr(), group, x_row=stride,
+                                    delta_row=stride, sum_row=stride, y_row=stride, y8_row=stride), stream())
+    torch.cuda.synchronize()
+    h, want, rel = ref.norm(x, delta, w, 1e-5)
+    close(dx[:, :hidden], h, (ref.HALF[dtype] + 2.0 ** -24) * h.abs() + ref.TINY[dtype], "sum")
+    close(y[:, :hidden], want, (ref.HALF[dtype] + rel) * want.abs() + ref.TINY[dtype], "y")
+    check8(y8[:, :hidden], scales, want, rel, ops.TYPE_I8, group)
+    assert not dx[:, hidden:].any() and (y[:, hidden:] == 7.0).all() and not y8[:, hidden:].any()
 
 
 def test_norm_in_place_and_parts(torch_cuda):
