@@ -21,7 +21,7 @@ struct RopeArgs {
   const int64_t* positions;
   int64_t base, rows;
   float magnitude;
-  int head_dim, pairs;
+  int head_dim, pairs, rest;  // rest: values behind the pairs that are copied, none where heads are turned in place
   bool half;
 };
 
@@ -51,7 +51,7 @@ __device__ __forceinline__ double rope_position(const RopeArgs& a, int64_t t) {
 // value of one head.
 template <typename T>
 __global__ __launch_bounds__(256) void rope_any_kernel(RopeArgs a) {
-  const int rest = a.head_dim - 2 * a.pairs, units = a.pairs + rest;
+  const int units = a.pairs + a.rest;
   const int64_t heads = a.q.heads + a.k.heads, total = a.rows * heads * units;
   for (int64_t n = blockIdx.x * 256ll + threadIdx.x; n < total; n += gridDim.x * 256ll) {
     const int u = (int)(n % units);
@@ -71,14 +71,13 @@ __global__ __launch_bounds__(256) void rope_any_kernel(RopeArgs a) {
   }
 }
 
-// 16-byte vectors of E values. A head is `units` units: interleaved, one
+// Vectors of E values, up to 16 bytes. A head is `units` units: interleaved, one
 // vector each; half, first the vectors of the pairs' first values, each with
 // that of their second ones, then the vectors that are copied. A thread
 // computes the angles of its unit once and turns it in every `slots`-th head
 // of its token.
-template <typename T>
+template <typename T, int E>
 __global__ __launch_bounds__(256) void rope_vector_kernel(RopeArgs a, int units, int slots, int tokens) {
-  constexpr int E = 16 / sizeof(T);
   typedef T vec __attribute__((ext_vector_type(E)));
   const int per = units * slots, u = threadIdx.x % units;
   const int64_t t = (int64_t)blockIdx.x * tokens + threadIdx.x / per;
@@ -116,42 +115,49 @@ __global__ __launch_bounds__(256) void rope_vector_kernel(RopeArgs a, int units,
     }
     return;
   }
-  float2 cs[E / 2];
+  if constexpr (E > 1) {
+    float2 cs[E / 2];
 #pragma unroll
-  for (int e = 0; e < E / 2; ++e) cs[e] = rope_angle(a, E / 2 * u + e, p);
-  for (int h = slot; h < heads; h += slots) {
-    const T* x;
-    T* y;
-    rope_head(a, t, h, x, y);
-    const vec v = *(const vec*)(x + E * u);
-    vec r;
+    for (int e = 0; e < E / 2; ++e) cs[e] = rope_angle(a, E / 2 * u + e, p);
+    for (int h = slot; h < heads; h += slots) {
+      const T* x;
+      T* y;
+      rope_head(a, t, h, x, y);
+      const vec v = *(const vec*)(x + E * u);
+      vec r;
 #pragma unroll
-    for (int e = 0; e < E / 2; ++e) {
-      r[2 * e] = (T)((float)v[2 * e] * cs[e].x - (float)v[2 * e + 1] * cs[e].y);
-      r[2 * e + 1] = (T)((float)v[2 * e] * cs[e].y + (float)v[2 * e + 1] * cs[e].x);
+      for (int e = 0; e < E / 2; ++e) {
+        r[2 * e] = (T)((float)v[2 * e] * cs[e].x - (float)v[2 * e + 1] * cs[e].y);
+        r[2 * e + 1] = (T)((float)v[2 * e] * cs[e].y + (float)v[2 * e + 1] * cs[e].x);
+      }
+      *(vec*)(y + E * u) = r;
     }
-    *(vec*)(y + E * u) = r;
   }
 }
 
-bool aligned_heads(const nemo_rope_heads& s, int E) {
-  return (((uintptr_t)s.x | (uintptr_t)s.y) & 15) == 0 &&
+bool aligned_heads(const nemo_rope_heads& s, int E, int bytes) {
+  return (((uintptr_t)s.x | (uintptr_t)s.y) & (bytes - 1)) == 0 &&
          s.x_row % E == 0 && s.x_head % E == 0 && s.y_row % E == 0 && s.y_head % E == 0;
 }
 
-template <typename T>
+// By vectors of E values, or narrower ones that the sizes, strides and
+// addresses allow (8192 tokens of 32 bf16 heads of 128, 40 of them turned by
+// halves, vectors of 4: 49 us, single values by rope_any_kernel 122; 102 turned,
+// vectors of 1 80 : 103).
+template <typename T, int E = 16 / sizeof(T)>
 hipError_t launch_rope_type(const RopeArgs& a, hipStream_t stream) {
-  constexpr int E = 16 / sizeof(T);
-  const int heads = a.q.heads + a.k.heads, rotary = 2 * a.pairs;
-  const bool vectors = a.head_dim % E == 0 && rotary % E == 0 && (!a.half || a.pairs % E == 0) &&
-                       aligned_heads(a.q, E) && (!a.k.heads || aligned_heads(a.k, E));
-  const int units = (a.half ? a.pairs : rotary) / E + (a.head_dim - rotary) / E;
+  const int heads = a.q.heads + a.k.heads, rotary = 2 * a.pairs, bytes = E * sizeof(T);
+  const bool vectors = a.head_dim % E == 0 && rotary % E == 0 && (a.half ? a.pairs % E == 0 : E > 1) &&
+                       aligned_heads(a.q, E, bytes) && (!a.k.heads || aligned_heads(a.k, E, bytes));
+  const int units = (a.half ? a.pairs : rotary) / E + a.rest / E;
   if (vectors && units <= 256) {
     const int slots = std::max(1, std::min({heads, 256 / units, a.rows >= 512 ? (heads + 3) / 4 : heads}));
     const int tokens = 256 / (units * slots);
-    rope_vector_kernel<T><<<(unsigned)((a.rows + tokens - 1) / tokens), 256, 0, stream>>>(a, units, slots, tokens);
+    rope_vector_kernel<T, E><<<(unsigned)((a.rows + tokens - 1) / tokens), 256, 0, stream>>>(a, units, slots, tokens);
+  } else if constexpr (E > 1) {
+    return launch_rope_type<T, E / 2>(a, stream);
   } else {
-    const int64_t total = a.rows * heads * (a.pairs + a.head_dim - rotary);
+    const int64_t total = a.rows * heads * (a.pairs + a.rest);
     rope_any_kernel<T><<<(unsigned)std::min<int64_t>((total + 255) / 256, 1 << 16), 256, 0, stream>>>(a);
   }
   return hipGetLastError();
@@ -162,7 +168,11 @@ hipError_t launch_rope_type(const RopeArgs& a, hipStream_t stream) {
 hipError_t launch_rope_apply(const RopeAngles& angles, int type, const nemo_rope_heads& q, const nemo_rope_heads* k,
                              int64_t rows, const int64_t* positions, int64_t base, hipStream_t stream) {
   RopeArgs a{q, k ? *k : nemo_rope_heads{}, angles.turns, positions, base, rows, angles.magnitude, angles.head_dim,
-             angles.rotary / 2, angles.half};
+             angles.rotary / 2, 0, angles.half};
+  auto copied = [](const nemo_rope_heads& s) {
+    return s.heads && !(s.x == s.y && s.x_row == s.y_row && s.x_head == s.y_head);
+  };
+  if (copied(a.q) || copied(a.k)) a.rest = angles.head_dim - angles.rotary;
   if (rows == 0 || a.q.heads + a.k.heads == 0) return hipSuccess;
   switch (type) {
     case NEMO_TYPE_F32: return launch_rope_type<float>(a, stream);

@@ -101,6 +101,48 @@ def test_rope_in_place_in_projection_rows(torch_cuda, half, shift):
     assert torch.equal(after[:, (H + K) * d:], before[:, (H + K) * d:]) and torch.equal(after[-1], before[-1])
 
 
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("half", [False, True])
+@pytest.mark.parametrize("rows", [3, 600])
+@pytest.mark.parametrize("d,rotary,shift,pad", [(128, 102, 0, 0), (128, 40, 0, 0), (128, 72, 4, 8), (64, 64, 2, 2), (64, 36, 1, 1),
+                                                (160, 80, 0, 4), (300, 300, 0, 0), (6, 2, 0, 0)])
+def test_rope_by_narrower_vectors(torch_cuda, dtype, half, rows, d, rotary, shift, pad):
+    """Sizes, addresses and strides that leave vectors of 8, 4, 2 and 1 values;
+    space between the rows stays."""
+    heads, width = 5, 5 * d + pad
+    rope, freq, mag = make_rope(d, rotary, half, "linear")
+    x = rand(8, rows * width + 16, dtype=dtype).cuda()
+    y = torch.full_like(x, 7.0)
+    size = x.element_size() * shift
+    rope.apply(CODE[dtype], ops.rope_heads(x.data_ptr() + size, y.data_ptr() + size, heads, d, x_row=width), None, rows, base=77,
+               stream=stream())
+    torch.cuda.synchronize()
+    turned, out = (t[shift:shift + rows * width].view(rows, width).cpu() for t in (x, y))
+    close(out[:, :heads * d].reshape(rows, heads, d),
+          *ref.rope(turned[:, :heads * d].reshape(rows, heads, d), torch.arange(rows) + 77, freq, half, mag))
+    assert (out[:, heads * d:] == 7.0).all() and (y[:shift] == 7.0).all() and (y[shift + rows * width:] == 7.0).all()
+
+
+@pytest.mark.parametrize("half", [False, True])
+@pytest.mark.parametrize("rotary", [40, 102, 32])
+def test_rope_part_of_a_head_in_place(torch_cuda, half, rotary):
+    """The rest of a head stays bit for bit, NaN with it; queries in place
+    beside keys that go elsewhere."""
+    rope, freq, mag = make_rope(128, rotary, half, "none")
+    q, k = rand(9, 300, 4, 128, dtype=F16), rand(10, 300, 2, 128, dtype=F16)
+    q[:, :, rotary:] = math.nan
+    for elsewhere in (False, True):
+        dq, dk = q.cuda(), k.cuda()
+        ok = torch.zeros_like(dk) if elsewhere else dk
+        rope.apply(ops.TYPE_F16, ops.rope_heads(dq.data_ptr(), dq.data_ptr(), 4, 128),
+                   ops.rope_heads(dk.data_ptr(), ok.data_ptr(), 2, 128), 300, stream=stream())
+        torch.cuda.synchronize()
+        want, tol = ref.rope(torch.nan_to_num(q), torch.arange(300), freq, half, mag)
+        close(dq[..., :rotary], want[..., :rotary], tol[..., :rotary] if torch.is_tensor(tol) else tol)
+        assert torch.isnan(dq[..., rotary:]).all()
+        close(ok, *ref.rope(k, torch.arange(300), freq, half, mag))
+
+
 def test_rope_turns_back(torch_cuda):
     """By a position and by its negative gives the values back, but for two
     roundings of pairs (a, b): each of a + b's magnitude."""
