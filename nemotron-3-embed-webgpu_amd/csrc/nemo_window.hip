@@ -701,10 +701,12 @@ __global__ __launch_bounds__(PARTS == 1 ? 256 : 512, PARTS == 1 && HD == 64 ? 3 
         }
     }
   }
-  // A value that some rows of the wave do not see meets their probability 0;
-  // where it is not finite, their sums are not, and they are taken again. (One
-  // query's rows see the same keys.)
-  const uint64_t bad = a.query(w0) == a.query(w1) ? 0 : __builtin_amdgcn_ballot_w64(acc.spoilt());
+  // The list is that of all rows of the tile, and a value that some of them do
+  // not see meets their probability 0; where it is not finite, their sums are
+  // not, and they are taken again. (The rows of a tile of one query see every
+  // key of the list. Those of a wave of one query need not.)
+  const bool one_query = a.query(row0) == a.query(min(row0 + ROWS - 1, rows - 1));
+  const uint64_t bad = one_query ? 0 : __builtin_amdgcn_ballot_w64(acc.spoilt());
   uint32_t again = (uint32_t)(bad | bad >> 32);
   if (again && !hidden_spoil<T, HD>(a, heads, list, first, last, 0, list.n)) again = 0;
   // Outputs go through LDS: whole rows to memory, 16 bytes a lane.
