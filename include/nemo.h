@@ -347,9 +347,9 @@ typedef struct nemo_attention_config {
 /* Buffers are 16-byte aligned, strides multiples of 8. The index arrays are
  * read on the device when the work runs (a captured graph may be replayed
  * with other lengths); entries outside the buffers are cut to q_rows and
- * kv_rows. Key and value rows are at least head_dim apart. Rows of `out` that
- * belong to no request are left as they were. `out` and the workspace overlap no
- * other buffer. */
+ * kv_rows. Key and value rows are at least head_dim apart; the row strides of
+ * a k and v of one row are not used. Rows of `out` that belong to no request are
+ * left as they were. `out` and the workspace overlap no other buffer. */
 typedef struct nemo_attention_batch {
   int32_t count;             /* requests */
   int64_t q_rows, kv_rows;   /* rows of q and out, of k and v */

@@ -1034,6 +1034,8 @@ hipError_t launch_ragged_index(const Ragged& rows, int64_t* positions, int32_t* 
 hipError_t launch_window_attention(const nemo_attention_config& c, const nemo_attention_batch& b, hipStream_t stream) {
   if (b.count == 0 || b.q_rows == 0) return hipSuccess;
   WindowArgs a{b, c.kv_heads, c.q_heads / c.kv_heads, 0, 0, 0, 0.f, 0, 0};
+  // Copies' ranges end one stride behind a row's start; that of a single row may be anything.
+  if (b.kv_rows == 1) a.b.k_row = a.b.v_row = c.head_dim;
   while (1 << a.shift < a.group) ++a.shift;
   a.magic = (uint32_t)((((uint64_t)1 << a.shift) - a.group) * ((uint64_t)1 << 32) / a.group + 1);
   auto bound = [](int v) { return v < 0 ? kUnbounded : std::min(v, kUnbounded); };

@@ -45,3 +45,21 @@ def test_attention_hidden_values_of_a_tile(torch_cuda, H, K, D, n, left, right, 
     want, tol = ref.attention(b.q, b.k[:m], torch.nan_to_num(b.v[:m], nan=0.0, posinf=0.0, neginf=0.0), left, right, sinks,
                               D ** -0.5)
     T.close(out[~touched], want[~touched], tol[~touched])
+
+
+@pytest.mark.parametrize("dtype,D", [(F16, 64), (F16, 128), (BF16, 128)])
+@pytest.mark.parametrize("row", [0, 64])
+@pytest.mark.parametrize("H,K,q_lens", [(4, 2, [1]), (4, 2, [3, 1, 20]), (32, 8, [600, 1]), (32, 8, [260, 30])])
+def test_attention_of_one_key_row(torch_cuda, H, K, q_lens, row, dtype, D):
+    """A cache of a single row, which every request has, whatever the distance
+    to a next row is said to be: the result is its value."""
+    b = T.Batch(dtype, H, K, D, -1, -1, 0, q_lens, [1] * len(q_lens), poison=False)
+    b.dk, b.dv = b.dk[:1], b.dv[:1]
+    b.starts = [0] * len(q_lens)
+    b.kv_start.zero_()
+    args = b.args(max_kv=400)  # (a hint that reaches every kernel)
+    assert args.kv_rows == 1
+    args.k_row = args.v_row = row
+    b.attention.run(args, T.stream())
+    torch.cuda.synchronize()
+    b.check()
