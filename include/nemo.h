@@ -419,9 +419,9 @@ nemo_status nemo_model_set_attention(nemo_model* model, const nemo_model_attenti
  * a token: the final RMSNorm of each request's merged rows, unpooled, as
  * nemo_rmsnorm writes it (y8 [rows][hidden], scales [rows] or [rows][hidden /
  * group]), request after request, max(1, ceil(0.64 length)) rows each. `rows`
- * receives their number; more than `capacity`, and a plan that has not run or
- * whose model merges after its last layer, are refused. Enqueued on `stream`
- * (NULL: the plan's own) after the run. */
+ * receives their number; more than `capacity`, and a plan that has not run,
+ * whose last run failed, or whose model merges after its last layer, are
+ * refused. Enqueued on `stream` (NULL: the plan's own) after the run. */
 nemo_status nemo_plan_token_states8(nemo_plan* plan, int32_t type8, int32_t group, void* d_y8, float* d_scales,
                                     int64_t capacity, int64_t* rows, void* stream);
 

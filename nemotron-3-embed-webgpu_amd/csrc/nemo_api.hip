@@ -331,6 +331,10 @@ struct nemo_plan {
   // Rows of the last layer run (the attention's RoPE positions) and, made
   // on request, its rotated query and key heads.
   Ragged last_rows{};
+  // Merged rows of the last pass, for its token states: none from its start
+  // until it is enqueued to its end (last_rows are the unmerged ones until the
+  // merge, and a pass that fails leaves some of its states).
+  Ragged state_rows{};
   DevPtr q, k;
   // Rotated attended keys and transposed values of a pass's long requests
   // (attention's preparation pass), room for attn_keys_cap keys per kv head.
@@ -1022,6 +1026,7 @@ static void enqueue_graph(nemo_plan* p, const uint32_t* d_ids, const Ragged& src
                           hipStream_t s, Mark&& mark) {
   nemo_model* m = p->model;
   const nemo_dims& d = m->dims;
+  p->state_rows = Ragged{};
   const int H = d.hidden, QKV = (d.q_heads + 2 * d.kv_heads) * d.head_dim, QW = d.q_heads * d.head_dim;
   const int F = d.intermediate;
   uint16_t* x_full = (uint16_t*)p->x_full.get();
@@ -1209,6 +1214,7 @@ static void enqueue_graph(nemo_plan* p, const uint32_t* d_ids, const Ragged& src
   mark(10, true);
   hip_check(launch_mean_pool(norm_red, dst, H, d_out, s), "mean pool");
   mark(10, false);
+  p->state_rows = dst;
 }
 
 static void check_ids_host(nemo_plan* p, const uint32_t* ids, size_t n_ids, const Ragged& src) {
@@ -1741,9 +1747,9 @@ nemo_status nemo_plan_token_states8(nemo_plan* plan, int32_t type8, int32_t grou
     const nemo_model* m = plan->model;
     if (m->dims.merge_after_layer == m->dims.layers)
       fail(NEMO_ERR_UNSUPPORTED, "the model merges after its last layer: it has no merged token states");
-    const Ragged& last = plan->last_rows;
+    const Ragged& last = plan->state_rows;
     const int64_t n = last.start[last.count];
-    if (n == 0) fail(NEMO_ERR_INVALID, "plan has not run");
+    if (n == 0) fail(NEMO_ERR_INVALID, "plan has not run, or its last run failed");
     if (capacity < n)
       fail(NEMO_ERR_INVALID, "room for " + std::to_string(capacity) + " token states; the run has " + std::to_string(n));
     nemo_norm_args a{};
