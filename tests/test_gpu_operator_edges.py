@@ -63,3 +63,70 @@ def test_attention_of_one_key_row(torch_cuda, H, K, q_lens, row, dtype, D):
     b.attention.run(args, T.stream())
     torch.cuda.synchronize()
     b.check()
+
+
+def tied_row(dtype, type8, hidden, seed, with_delta):
+    """x, delta and w of a row whose two largest products, in columns of two
+    lanes of a wave, round to the same 32 bits and whose second is the larger
+    one; the other columns' quotients lie between the borders of two codes that
+    the two would give. Returns x, delta, w, products (64 bits)."""
+    g = torch.Generator().manual_seed(seed)
+
+    def products(targets):
+        """h, delta and w whose products are the targets' nearest of some hundred."""
+        t = targets.double()[:, None].expand(-1, 400)
+        if with_delta:  # what 32 bits lose of the sum
+            h = t.float()
+            d, w = (t - h.double()).float(), torch.ones_like(h)
+            return h, d, w, h.double() + d.double()
+        h = (1 + torch.rand(t.shape, generator=g)).to(dtype)
+        w = (t / h.double()).float()
+        return h, torch.zeros_like(h), w, h.double() * w.double()
+
+    top = 127.0 if type8 == ops.TYPE_I8 else 448.0
+    P = 400.0 * (1 + 2.0 ** -10)
+    h, d, w, p = products(torch.tensor([P, P * (1 + 2.0 ** -26)], dtype=torch.float64))
+    if with_delta:
+        first, second = (h[0, 0], d[0, 0], w[0, 0], p[0, 0]), (h[1, 0], d[1, 0], w[1, 0], p[1, 0])
+    else:
+        h, d, w, p = (t.flatten() for t in (h, d, w, p))
+        same = (p.float() == torch.tensor(P).float()).nonzero().flatten()
+        lo, hi = same[p[same].argmin()], same[p[same].argmax()]
+        first, second = (tuple(t[i] for t in (h, d, w, p)) for i in (lo, hi))
+    low, high = float(first[3]), float(second[3])
+    assert low < high and torch.tensor(low).float() == torch.tensor(high).float()
+    if type8 == ops.TYPE_I8:
+        border = torch.arange(30, 126) + 0.5
+    else:  # the middles between 8-bit floats
+        border = torch.cat([(torch.arange(8, 16) + 0.5) * 2.0 ** e for e in range(-2, 5)])
+    border = border.double()[torch.arange(hidden) % len(border)]
+    a, b = low * border / top, high * border / top
+    h, d, w, p = products((a + b) / 2)
+    inside = (p > a[:, None]) & (p < b[:, None])
+    pick = (p - ((a + b) / 2)[:, None]).abs().masked_fill(~inside, math.inf).argmin(1, keepdim=True)
+    x, delta, weight, v, between = (t.gather(1, pick).flatten() for t in (h, d, w, p, inside))
+    for column, (ph, pd, pw, pp) in ((1, first), (hidden // 4 // 8 * 8 % 512 + 9, second)):
+        x[column], delta[column], weight[column], v[column], between[column] = ph, pd, pw, pp, False
+    return x, delta, weight, v, between, high
+
+
+@pytest.mark.parametrize("dtype,with_delta", [(F16, False), (F32, False), (F32, True)])
+@pytest.mark.parametrize("type8", [ops.TYPE_I8, ops.TYPE_E4M3])
+@pytest.mark.parametrize("hidden", [512, 1024, 4096, 8192, 16384, 32768, 1001])
+def test_norm_codes_of_peaks_that_tie(torch_cuda, hidden, type8, dtype, with_delta):
+    """A row's scale is that of its exactly largest product, where several
+    round to the same 32 bits."""
+    x, delta, w, v, between, peak = tied_row(dtype, type8, hidden, 81, with_delta)
+    x, delta = x.to(dtype), delta.to(dtype)
+    dx, dd, dw = x.cuda(), delta.cuda(), w.cuda()
+    y8 = torch.empty(hidden, dtype=torch.int8 if type8 == ops.TYPE_I8 else torch.float8_e4m3fn, device="cuda")
+    scale = torch.empty(1, device="cuda")
+    ops.RmsNorm().run(ops.norm_args(T.CODE[dtype], 1, hidden, dx.data_ptr(), dw.data_ptr(), 1e-5,
+                                    dd.data_ptr() if with_delta else 0, d_y8=y8.data_ptr(), type8=type8,
+                                    d_scales=scale.data_ptr()), T.stream())
+    torch.cuda.synchronize()
+    u = v * (127.0 if type8 == ops.TYPE_I8 else 448.0) / peak
+    unit = torch.ones_like(u) if type8 == ops.TYPE_I8 else torch.exp2(torch.floor(torch.log2(u.abs())) - 3)
+    clear = ((u / unit) % 1 - 0.5).abs() > 2.0 ** -40
+    assert (between & clear).sum() > hidden / 8
+    assert torch.equal(y8.cpu().double()[clear], (torch.round(u / unit) * unit)[clear])
