@@ -254,8 +254,9 @@ nemo_status nemo_probe_stream(const void* d_src, size_t bytes, int32_t loads_per
  * any layout, for callers that build a layer from nemo_weight_matmul and
  * these. All are enqueued on `stream` (NULL: the default stream) and return;
  * nothing is allocated, so they can be captured into a HIP graph after one
- * eager call of the same kind. Strides count elements; addresses are multiples
- * of their values' size; rows and heads that are written do not overlap. */
+ * eager call of the same kind. Strides count elements and are in [0, 2^23];
+ * addresses are multiples of their values' size; rows and heads that are
+ * written do not overlap. */
 
 #define NEMO_TYPE_I8 24        /* GGML's code */
 #define NEMO_TYPE_BF16 30      /* GGML's code */
@@ -315,11 +316,11 @@ typedef struct nemo_rope_heads {
   int32_t heads;
 } nemo_rope_heads;
 
-/* Turn the heads of `rows` tokens, `type` F32, F16 or BF16 (arithmetic in 32
- * bits, one rounding), of q and, unless it is NULL, of k in the same launch.
- * Row t has position base + d_positions[t] (device; NULL: base + t). Angles
- * are position * f_i in 64 bits, reduced there: their error is about 2^-53 of
- * the angle. Negative positions turn back. */
+/* Turn the heads of `rows` tokens (at most 2^23), `type` F32, F16 or BF16
+ * (arithmetic in 32 bits, one rounding), of q and, unless it is NULL, of k in
+ * the same launch. Row t has position base + d_positions[t] (device; NULL: base
+ * + t). Angles are position * f_i in 64 bits, reduced there: their error is
+ * about 2^-53 of the angle. Negative positions turn back. */
 nemo_status nemo_rope_apply(nemo_rope* rope, int32_t type, const nemo_rope_heads* q, const nemo_rope_heads* k,
                             int64_t rows, const int64_t* d_positions, int64_t base, void* stream);
 
@@ -351,8 +352,8 @@ typedef struct nemo_attention_config {
  * a k and v of one row are not used. Rows of `out` that belong to no request are
  * left as they were. `out` and the workspace overlap no other buffer. */
 typedef struct nemo_attention_batch {
-  int32_t count;             /* requests */
-  int64_t q_rows, kv_rows;   /* rows of q and out, of k and v */
+  int32_t count;             /* requests: 0..2^20, times kv_heads at most 2^22 */
+  int64_t q_rows, kv_rows;   /* rows of q and out, times q_heads at most 2^26; of k and v, at most 2^30 */
   int64_t max_kv;            /* the longest kv_len, or more: a hint for the split of the keys over the chip */
   const int32_t* q_start;    /* device [count + 1], ascending */
   const int64_t* kv_start;   /* device [count] */
@@ -382,8 +383,8 @@ nemo_status nemo_window_attention(nemo_ctx* ctx, const nemo_attention_config* co
  * row stride; other overlap of an input and an output is not allowed. */
 typedef struct nemo_norm_args {
   int32_t type;              /* of x, delta, sum, y: F32, F16 or BF16 */
-  int32_t hidden;            /* >= 1 */
-  int64_t rows;
+  int32_t hidden;            /* 1..2^30 */
+  int64_t rows;              /* 0..2^23 */
   const void* x;
   const void* delta;         /* NULL: h = x */
   const float* weight;       /* [hidden]; NULL: 1 */

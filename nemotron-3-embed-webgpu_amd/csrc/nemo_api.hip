@@ -1597,9 +1597,12 @@ nemo_status nemo_rope_destroy(nemo_rope* rope) {
   });
 }
 
-// Largest stride, in elements, and largest numbers of rows: they keep every
-// offset within 63 bits, a tile's within 31, and grids within 2^32 threads.
+// Largest stride, in elements, largest numbers of rows, and of columns: they
+// keep every offset within 63 bits, a tile's and a row's columns within 31, and
+// the grids of rotations (256 threads a row at most) and of attention below
+// 2^32 threads. (The norm's launches take a part of the rows each.)
 constexpr int64_t kMaxStride = 1 << 23, kMaxRows = 1 << 23, kMaxKeys = 1 << 30, kMaxQueries = 1 << 26;
+constexpr int32_t kMaxHidden = 1 << 30;
 
 static void validate_stride(int64_t v, const char* what) {
   if (v < 0 || v > kMaxStride) fail(NEMO_ERR_INVALID, std::string(what) + " must be in [0, 2^23]");
@@ -1694,7 +1697,7 @@ nemo_status nemo_window_attention(nemo_ctx* ctx, const nemo_attention_config* co
 static void validate_norm(const nemo_norm_args& a) {
   if (a.type != kF32 && a.type != kF16 && a.type != NEMO_TYPE_BF16)
     fail(NEMO_ERR_UNSUPPORTED, "the norm takes F32, F16 or BF16");
-  if (a.hidden < 1) fail(NEMO_ERR_INVALID, "hidden must be positive");
+  if (a.hidden < 1 || a.hidden > kMaxHidden) fail(NEMO_ERR_INVALID, "hidden must be in [1, 2^30]");
   if (a.rows < 0 || a.rows > kMaxRows) fail(NEMO_ERR_INVALID, "rows must be in [0, 2^23]");
   if (!(a.epsilon >= 0) || !isfinite(a.epsilon)) fail(NEMO_ERR_INVALID, "epsilon must be finite and 0 or more");
   for (int64_t v : {a.x_row, a.delta_row, a.sum_row, a.y_row, a.y8_row, a.scales_row})

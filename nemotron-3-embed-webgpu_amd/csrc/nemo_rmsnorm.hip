@@ -457,13 +457,28 @@ hipError_t launch_norm_type(const nemo_norm_args& a, hipStream_t stream) {
 }  // namespace
 
 hipError_t launch_norm8(const nemo_norm_args& args, hipStream_t stream) {
-  if (args.rows == 0) return hipSuccess;
-  switch (args.type) {
-    case NEMO_TYPE_F32: return launch_norm_type<float>(args, stream);
-    case NEMO_TYPE_F16: return launch_norm_type<half_t>(args, stream);
-    case NEMO_TYPE_BF16: return launch_norm_type<bf16_t>(args, stream);
-    default: return hipErrorInvalidValue;
+  // Rows of a launch: with up to 1024 threads a row, fewer threads than the 2^32 that a grid may not reach.
+  constexpr int64_t kLaunchRows = 1 << 21;
+  const int64_t size = args.type == NEMO_TYPE_F32 ? 4 : 2;
+  for (int64_t row = 0; row < args.rows; row += kLaunchRows) {
+    nemo_norm_args a = args;
+    auto skip = [row](auto* p, int64_t bytes) { return p ? (decltype(p))((uintptr_t)p + row * bytes) : p; };
+    a.rows = std::min(kLaunchRows, args.rows - row);
+    a.x = skip(a.x, a.x_row * size);
+    a.delta = skip(a.delta, a.delta_row * size);
+    a.sum = skip(a.sum, a.sum_row * size);
+    a.y = skip(a.y, a.y_row * size);
+    a.y8 = skip(a.y8, a.y8_row);
+    a.scales = skip(a.scales, a.scales_row * 4);
+    hipError_t e = hipErrorInvalidValue;
+    switch (a.type) {
+      case NEMO_TYPE_F32: e = launch_norm_type<float>(a, stream); break;
+      case NEMO_TYPE_F16: e = launch_norm_type<half_t>(a, stream); break;
+      case NEMO_TYPE_BF16: e = launch_norm_type<bf16_t>(a, stream); break;
+    }
+    if (e != hipSuccess) return e;
   }
+  return hipSuccess;
 }
 
 }  // namespace nemo

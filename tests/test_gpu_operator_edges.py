@@ -130,3 +130,24 @@ def test_norm_codes_of_peaks_that_tie(torch_cuda, hidden, type8, dtype, with_del
     clear = ((u / unit) % 1 - 0.5).abs() > 2.0 ** -40
     assert (between & clear).sum() > hidden / 8
     assert torch.equal(y8.cpu().double()[clear], (torch.round(u / unit) * unit)[clear])
+
+
+@pytest.mark.parametrize("hidden", [8, 9])
+def test_norm_of_more_rows_than_a_launch_takes(torch_cuda, hidden):
+    """Rows past 2^21 are another launch's; the sum replaces the residual, and
+    outputs' rows have space between them."""
+    rows = (1 << 21) + 7
+    x, delta, w = T.rand(91, rows, hidden, dtype=F16), T.rand(92, rows, hidden, dtype=F16), 1 + 0.1 * T.rand(93, hidden)
+    dx, dd, dw = x.cuda(), delta.cuda(), w.cuda()
+    y = torch.full((rows, hidden + 8), 7.0, dtype=F16, device="cuda")
+    y8 = torch.zeros(rows, hidden + 8, dtype=torch.int8, device="cuda")
+    scales = torch.full((rows, 2), 7.0, device="cuda")
+    ops.RmsNorm().run(ops.norm_args(ops.TYPE_F16, rows, hidden, dx.data_ptr(), dw.data_ptr(), 1e-5, dd.data_ptr(),
+                                    dx.data_ptr(), y.data_ptr(), y8.data_ptr(), ops.TYPE_I8, scales.data_ptr(),
+                                    y_row=hidden + 8, y8_row=hidden + 8, scales_row=2), T.stream())
+    torch.cuda.synchronize()
+    h, want, rel = ref.norm(x, delta, w, 1e-5)
+    T.close(dx, h, (ref.HALF[F16] + 2.0 ** -24) * h.abs() + ref.TINY[F16], "sum")
+    T.close(y[:, :hidden], want, (ref.HALF[F16] + rel) * want.abs() + ref.TINY[F16], "y")
+    T.check8(y8[:, :hidden].contiguous(), scales[:, :1], want, rel, ops.TYPE_I8, 0)
+    assert (y[:, hidden:] == 7.0).all() and not y8[:, hidden:].any() and (scales[:, 1] == 7.0).all()

@@ -88,3 +88,78 @@ plan.run_sync(ids, [3, 1])
 assert states() == rt.contextual_merged_length(3) + rt.contextual_merged_length(1)
 print("ok")
 """)
+
+
+@pytest.mark.parametrize("type_,hidden", [("TYPE_BF16", 2048), ("TYPE_BF16", 8192), ("TYPE_F32", 8192),
+                                          ("TYPE_F16", 16384), ("TYPE_F32", 32768), ("TYPE_F16", 40001),
+                                          ("TYPE_F16", 96)])
+@pytest.mark.parametrize("rows", [1, (1 << 21) + 5, (1 << 23) - 1, 1 << 23])
+def test_norm_grids_hold_their_rows(on_host, type_, hidden, rows):
+    """The most rows that the norm takes, in grids below 2^32 threads, each
+    row once: the launches' parts begin where the ones before end."""
+    on_host(f"""
+rows, hidden, type_ = {rows}, {hidden}, ops.{type_}
+size = 4 if type_ == ops.TYPE_F32 else 2
+at = {{"x": 1 << 40, "delta": 2 << 40, "sum": 3 << 40, "y": 4 << 40, "y8": 5 << 40, "scales": 6 << 40}}
+args = ops.norm_args(type_, rows, hidden, at["x"], 7 << 40, 1e-5, at["delta"], at["sum"], at["y"], at["y8"],
+                     ops.TYPE_I8, at["scales"])
+parts = []
+CALL = ctypes.CFUNCTYPE(None, ctypes.c_uint32, ctypes.c_uint32, ctypes.POINTER(_lib.NormArgs))
+
+@CALL
+def launched(grid, block, first):
+    a = first.contents
+    assert grid * block < 1 << 32 and 64 * a.rows <= grid * block, (grid, block, a.rows)
+    parts.append((a.rows, a.x, a.delta, a.sum, a.y, a.y8, a.scales, a.weight))
+
+ctypes.c_void_p.in_dll(host, "host_on_launch").value = ctypes.cast(launched, ctypes.c_void_p).value
+ops.RmsNorm().run(args)
+done = 0
+for n, x, delta, sum_, y, y8, scales, weight in parts:
+    assert [x, delta, sum_, y] == [at[k] + done * hidden * size for k in ("x", "delta", "sum", "y")]
+    assert (y8, scales, weight) == (at["y8"] + done * hidden, at["scales"] + 4 * done, 7 << 40)
+    done += n
+assert done == rows and most_threads.value < 1 << 32, (done, most_threads.value)
+print("ok")
+""")
+
+
+def test_attention_and_rope_grids(on_host):
+    """The largest calls that are taken, by every kernel: grids below 2^32 threads."""
+    on_host("""
+A = 1 << 40
+for heads, kv, dim in ((1, 1, 64), (32, 8, 128), (1024, 1, 64), (1024, 1024, 128), (4, 4, 128)):
+    for count in (1, (1 << 22) // kv if kv >= 4 else 1 << 20):
+        for max_kv in (1, 1000, 1 << 30):
+            rows = (1 << 26) // heads
+            a = ops.WindowAttention(ops.attention_config(heads, kv, dim))
+            side = (A, heads * dim, dim)
+            need = a.workspace_bytes(count, rows, max_kv)
+            a.run(ops.attention_batch(count, rows, 1 << 30, max_kv, A, A, A, side, side, side, side, A, need))
+            assert most_threads.value < 1 << 32, (heads, kv, dim, count, max_kv, most_threads.value)
+rope = ops.Rope(ops.rope_config(1024))
+for type_ in (ops.TYPE_F32, ops.TYPE_F16):
+    for heads in (1, 7, 65536):
+        for shift in (0, 4):
+            s = ops.rope_heads(A + shift, A + shift, heads, 1024, x_row=1 << 23, x_head=1024)
+            rope.apply(type_, s, s, 1 << 23)
+            assert most_threads.value < 1 << 32, (type_, heads, shift, most_threads.value)
+print("ok")
+""")
+
+
+def test_norm_of_too_many_columns_is_refused(on_host):
+    on_host("""
+A = 1 << 40
+for hidden in ((1 << 30) + 1, (1 << 31) - 1):
+    args = ops.norm_args(ops.TYPE_F16, 1, 8, A, d_y=A)
+    args.hidden = hidden
+    try:
+        ops.RmsNorm().run(args)
+    except rt.NemoError as e:
+        assert "hidden must be" in str(e), e
+    else:
+        raise AssertionError(hidden)
+assert launches.value == 0
+print("ok")
+""")
