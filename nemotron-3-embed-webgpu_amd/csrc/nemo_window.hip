@@ -13,6 +13,7 @@
 // score registers have. K and V go row-major into LDS by DMA; K fragments are
 // 16-byte reads, V^T fragments transposed reads (ds_read_b64_tr_b16).
 #include <algorithm>
+#include <type_traits>
 
 #include "nemo_operators.h"
 
@@ -296,14 +297,23 @@ struct Rows {
     for (int c = 0; c < DC; ++c) s = Mma<T>::mma(key(image, lane, c), q[c], s);
     return s;
   }
-  // Probabilities 2^(s - m) are taken against a reference m that is the row's
-  // largest score so far only when it was last raised: it is raised when the
-  // sum of a lane's 16 says that one may have passed 2^15 (or is not a
-  // number, as for a row that has seen nothing, whose m is -infinity), and
-  // they are taken again. So the common block needs no maximum, no exchange
-  // between lanes and no rescaling, and one wave vote. Numerator and
-  // denominator share the reference, so the result is the softmax; the sum is
-  // that of the rounded probabilities.
+  // Probabilities 2^(s - m) are taken against a reference m that lay BELOW under
+  // the row's largest score when it was last raised: it is raised when the sum
+  // of a lane's 16 passes MOST (or is not a number, as for a row that has seen
+  // nothing, whose m is -infinity), and they are taken again. So the common
+  // block needs no maximum, no exchange between lanes and no rescaling, and one
+  // wave vote. Numerator and denominator share the reference, so the result is
+  // the softmax; the sum is that of the rounded probabilities.
+  //
+  // Half precision rounds what is below 2^-14 by up to 2^-25 whatever it is:
+  // with a largest probability of 2^8 and more that is 2^-33 of it, and a long
+  // cache of even scores that lie 17 under a sink's keeps its share of the
+  // result (with a largest one of 1, e^-17 became 2^-24, 44 % more). Its MOST
+  // is what no sum of finite ones reaches, so the raise comes when one
+  // overflows: at 2^15, as for bf16, the headroom lost cost the 16 ragged
+  // requests 0.6 us; now they take what they took without BELOW.
+  static constexpr bool HALF = std::is_same<T, half_t>::value;
+  static constexpr float BELOW = HALF ? 8.f : 0.f, MOST = HALF ? 0x1p20f : 0x1p15f;
   static __device__ __forceinline__ float sum(const frag (&p)[2]) {
     float v = 0.f;
 #pragma unroll
@@ -324,15 +334,15 @@ struct Rows {
   // reference where it has to be.
   __device__ __forceinline__ void settle(const float16v& s, float scale2, frag (&p)[2]) {
     float add = sum(p);
-    if (__builtin_amdgcn_ballot_w64(!(add <= 0x1p15f))) {
+    if (__builtin_amdgcn_ballot_w64(!(add <= MOST))) {
       asm volatile("");  // keeps the rare path a branch
       float top = s[0];
 #pragma unroll
       for (int r = 1; r < 16; ++r) top = fmaxf(top, s[r]);
       top *= scale2;
-      const int high = !(add <= 0x1p15f), other = __shfl_xor(high, 32, 64);
+      const int high = !(add <= MOST), other = __shfl_xor(high, 32, 64);
       const bool raise = high | other;  // only the rows that ask: none depends on another
-      const float raised = raise ? fmaxf(m, fmaxf(top, __shfl_xor(top, 32, 64))) : m;
+      const float raised = raise ? fmaxf(m, fmaxf(top, __shfl_xor(top, 32, 64)) - BELOW) : m;
       const float alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - raised);
       l *= alpha;
 #pragma unroll

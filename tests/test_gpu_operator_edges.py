@@ -151,3 +151,31 @@ def test_norm_of_more_rows_than_a_launch_takes(torch_cuda, hidden):
     T.close(y[:, :hidden], want, (ref.HALF[F16] + rel) * want.abs() + ref.TINY[F16], "y")
     T.check8(y8[:, :hidden].contiguous(), scales[:, :1], want, rel, ops.TYPE_I8, 0)
     assert (y[:, hidden:] == 7.0).all() and not y8[:, hidden:].any() and (scales[:, 1] == 7.0).all()
+
+
+@pytest.mark.parametrize("H,K,D,n,m", [(8, 1, 64, 1, 60000), (8, 1, 128, 1, 60000), (8, 2, 128, 40, 5000),
+                                       (64, 32, 64, 300, 3000), (32, 8, 128, 300, 3000)])
+def test_attention_in_half_precision_behind_a_strong_sink(torch_cuda, H, K, D, n, m):
+    """The first key's score lies 17 above a long cache of even ones, each of
+    which has e^-17 of its probability, and all of the result: the first
+    value is 0.
+
+    operator_refs.attention's bound with one term smaller: probabilities are
+    taken against a reference at least 8 powers of two below the row's largest
+    score, so their sum is 2^8 or more and those that are rounded by up to
+    2^-25 whatever they are add 2^-33 (sum |v| + n |out|)."""
+    b = T.Batch(F16, H, K, D, -1, 0, 1, [n], [m], poison=False)
+    u = T.rand(51, D)
+    b.q = (u + 0.01 * b.q.float()).half()
+    b.k = (0.01 * b.k.float()).half()
+    b.k[0] = (17 * D ** 0.5 / (u * u).sum() * u).half()
+    b.v = (1 + 0.1 * b.v.float()).half()
+    b.v[0] = 0
+    b.dq, b.dk, b.dv = torch.cat([b.q, torch.zeros(3, H, D, dtype=F16)]).cuda(), b.k.cuda(), b.v.cuda()
+    b.run()
+    want, tol = ref.attention(b.q, b.k[:m], b.v[:m], -1, 0, 1, D ** -0.5)
+    seen = ref.visible(n, m, -1, 0, 1).double()
+    for h in range(H):
+        small = ref.TINY[F16] * (seen @ b.v[:m, h * K // H].double().abs() + seen.sum(1, keepdim=True) * want[:, h].abs())
+        tol[:, h] -= (1 - 2.0 ** -8) * small
+    T.close(b.out[:n], want, tol)
