@@ -1736,7 +1736,9 @@ nemo_status nemo_model_set_attention(nemo_model* model, const nemo_model_attenti
     validate_attention({model->dims.q_heads, model->dims.kv_heads, model->dims.head_dim, kF16, w.left, w.right, w.sinks,
                         0.f});
     set_device(model->ctx);
-    model->angles = rope_angles(w.rope, model->turns);
+    DevPtr turns;  // the model keeps the ones that it has until these are there
+    model->angles = rope_angles(w.rope, turns);
+    model->turns = std::move(turns);
     model->attention = w;
     model->windowed = true;
   });

@@ -11,6 +11,8 @@ typedef struct { uint32_t x, y, z; } dim3_t;
 
 /* Launches so far, and the largest number of threads of one of them. */
 uint64_t host_launches, host_most_threads;
+/* The last address that was handed out, and the last that was taken back. */
+void *host_last_malloc, *host_last_free;
 /* Called for each launch, if set: its grid and block, and the first argument. */
 void (*host_on_launch)(uint32_t grid, uint32_t block, void* first);
 
@@ -33,8 +35,8 @@ int hipLaunchKernel(const void* f, dim3_t grid, dim3_t block, void** args, size_
   return 0;
 }
 
-int hipMalloc(void** p, size_t n) { return (*p = calloc(1, n)) ? 0 : 2; }
-int hipFree(void* p) { return free(p), 0; }
+int hipMalloc(void** p, size_t n) { return (host_last_malloc = *p = calloc(1, n)) ? 0 : 2; }
+int hipFree(void* p) { return free(host_last_free = p), 0; }
 int hipHostMalloc(void** p, size_t n, unsigned flags) { return (void)flags, hipMalloc(p, n); }
 int hipHostFree(void* p) { return free(p), 0; }
 int hipMemcpy(void* to, const void* from, size_t n, int kind) { return (void)kind, memcpy(to, from, n), 0; }

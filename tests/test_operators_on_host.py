@@ -163,3 +163,32 @@ for hidden in ((1 << 30) + 1, (1 << 31) - 1):
 assert launches.value == 0
 print("ok")
 """)
+
+
+def test_a_failed_change_of_attention_keeps_the_one_before(on_host):
+    """A second nemo_model_set_attention that fails, wherever it does, frees
+    what it allocated itself and not the frequencies that the model has."""
+    on_host("""
+dims = rt.make_dims(hidden=256, q_heads=4, kv_heads=2, head_dim=64, intermediate=256, layers=2, vocab=300,
+                    merge_after_layer=1)
+context, model = rt.HipContext.shared(0), ctypes.c_void_p()
+_lib.check(L.nemo_model_create(context.ptr, ctypes.byref(dims), ctypes.byref(model)))
+last = {k: ctypes.c_void_p.in_dll(host, "host_last_" + k) for k in ("malloc", "free")}
+
+def change(theta):
+    return L.nemo_model_set_attention(model, ctypes.byref(ops.model_attention(8, 8, theta=theta)))
+
+assert change(1e4) == 0
+kept = last["malloc"].value
+failed = 0
+while True:
+    L.nemo_debug_fail_after(1 + failed)
+    status = change(1e5)
+    L.nemo_debug_fail_after(0)
+    if status == 0:
+        break
+    failed += 1
+    assert last["free"].value != kept, failed
+assert failed >= 2 and last["free"].value == kept
+print("ok")
+""")
