@@ -14,7 +14,10 @@
 // of 128 columns took 226 us.
 //
 // Bound by memory: each value is read and written once, 16 bytes a lane. Those
-// 16384 rows, 944 MB, take 177 us (5.3 TB/s; a copy reaches 4.9 to 5.4).
+// 16384 rows, 944 MB, take 177 us call after call (5.3 TB/s; a copy reaches 4.9
+// to 5.4), 182 at the least and 195 mostly where a trace sets the calls apart;
+// 2399 x 2048 f16 to bytes and f16 11.6 and 12.7 there, 44 MB that 5.4 TB/s
+// would take in 8.2.
 #include <algorithm>
 
 #include "nemo_operators.h"

@@ -551,18 +551,19 @@ __device__ __forceinline__ OneRow<T, HD> one_row(const WindowArgs& a, const Head
 // two waves, of which a SIMD then has one).
 //
 // Bound by the steps' instructions and by power: 32768 tokens of 32 heads of
-// 128 (8 KV heads, window 1024), 543 GFLOP, take 580 to 600 us, 1.14 M cycles
-// at a clock that falls to 1.9 GHz and below, of which the MFMAs are 50 %. A
-// step of a SIMD's two waves takes 1.29 k cycles by itself, 1.02 k of them
-// MFMAs, with the rounds' barriers and copies 1.55 k, and a workgroup's
-// beginning and end are a fifth of its time. Without copies it is 11 % less,
-// without LDS reads 3, without exponentials nothing; fragments read over the
-// barrier, a fifth fewer scalar instructions and workgroups that start apart
-// gave 0 to 3 % of cycles and no time. The steps on the way: scores and product
-// of one block in turn 676 us, one block ahead and behind 670, queries and
-// outputs through LDS and the hidden slots by a mask of bits 629, copies in
-// assembly 618, values' fragments before the keys' 600. 16 ragged requests, 2860
-// tokens, heads of 64, 5 rounds each, are bound by latency: 16.8 us.
+// 128 (8 KV heads, window 1024), 543 GFLOP, take 608 us call after call (584 at
+// the least), 1.16 M cycles at a clock that falls to 1.9 GHz and below, of which
+// the MFMAs are 49 %. A step of a SIMD's two waves takes 1.29 k cycles by
+// itself, 1.02 k of them MFMAs, with the rounds' barriers and copies 1.55 k, and
+// a workgroup's beginning and end are a fifth of its time. Without copies it is
+// 11 % less, without LDS reads 3, without exponentials nothing; fragments read
+// over the barrier, a fifth fewer scalar instructions and workgroups that start
+// apart gave 0 to 3 % of cycles and no time. The steps on the way: scores and
+// product of one block in turn 676 us, one block ahead and behind 670, queries
+// and outputs through LDS and the hidden slots by a mask of bits 629, copies in
+// assembly 618, values' fragments before the keys' 600 to 608. 16 ragged
+// requests, 2860 tokens, heads of 64, 5 rounds each, are bound by latency: 16.7
+// us.
 // ---------------------------------------------------------------------------
 
 template <typename T, int HD, int PARTS>
@@ -745,7 +746,7 @@ __global__ __launch_bounds__(PARTS == 1 ? 256 : 512, PARTS == 1 && HD == 64 ? 3 
 // to that many workgroups as well, whose sums a second kernel joins.
 //
 // Bound by memory where the caches are long: 64 tokens over 983 MB of keys and
-// values 177 us (5.6 TB/s), one over 131072 keys 98 us and its join 4.2; by
+// values 173 us (5.7 TB/s), one over 131072 keys 95 us and its join 4.6; by
 // latency below: one token over 1028 keys of 64 8.6 us, of which the lookup,
 // first loads and sums are about three quarters. With 4 waves it took 11.7.
 // ---------------------------------------------------------------------------
