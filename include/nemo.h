@@ -426,6 +426,138 @@ nemo_status nemo_model_set_attention(nemo_model* model, const nemo_model_attenti
 nemo_status nemo_plan_token_states8(nemo_plan* plan, int32_t type8, int32_t group, void* d_y8, float* d_scales,
                                     int64_t capacity, int64_t* rows, void* stream);
 
+/* ---- low-bit operators of an attention block -------------------------------
+ * What stands between nemo_rmsnorm's 8-bit rows and the output projection in
+ * a block that is served in few bits: products of 8-bit rows, norms of heads
+ * before their rotation, a cache of 4-bit floats in pages, and attention over
+ * it. The reference has no counterparts. They follow the conventions of the
+ * operators above: enqueued on `stream`, nothing allocated, strides in elements
+ * and in [0, 2^23]. */
+
+/* RMSNorm of each query and key head, then its rotation, in one pass:
+ *   h = x / sqrt(mean over the head of x^2 + epsilon) * weight,  y = h turned
+ * by nemo_rope_apply's angles (values that it copies are normed only), in 32
+ * bits with one rounding at the end. Head h's weight begins at
+ * weight + h weight_head; 0: one weight for all heads. */
+typedef struct nemo_head_norm {
+  const float* q_weight;       /* [head_dim] each; NULL: 1 */
+  const float* k_weight;
+  int64_t q_weight_head, k_weight_head;
+  float epsilon;               /* >= 0 */
+} nemo_head_norm;
+nemo_status nemo_rope_norm_apply(nemo_rope* rope, int32_t type, const nemo_rope_heads* q, const nemo_rope_heads* k,
+                                 const nemo_head_norm* norm, int64_t rows, const int64_t* d_positions, int64_t base,
+                                 void* stream);
+
+/* Products of 8-bit rows, as nemo_rmsnorm writes them with group 0, and 8-bit
+ * weights with a scale for each output channel:
+ *   y[i][j] = type(x_scale[i] w_scale[j] (sum over k of x[i][k] w[j][k]) + bias[j])
+ * The sum is exact (32-bit integers); it is rounded to 32 bits, scaled by
+ * x_scale, then by w_scale, and the bias is added, in 32 bits. k 0 leaves the
+ * bias. x and w are 16-byte aligned, their row strides multiples of 16 and at
+ * least k (for more than one row); bytes of a row behind k may hold anything.
+ * y overlaps no other buffer. */
+typedef struct nemo_matmul8_args {
+  int32_t type;                /* of y: F32, F16 or BF16 */
+  int32_t n, k;                /* 0..2^23 output channels; 0..131071 */
+  int64_t m;                   /* 0..2^23 rows */
+  const int8_t* x;             /* [m][k] */
+  const float* x_scale;        /* [m], x_scale_row apart */
+  const int8_t* w;             /* [n][k] */
+  const float* w_scale;        /* [n] */
+  const float* bias;           /* [n]; NULL: none */
+  void* y;                     /* [m][n] */
+  int64_t x_row, x_scale_row, w_row, y_row; /* y_row at least n for more than one row */
+} nemo_matmul8_args;
+nemo_status nemo_matmul8(nemo_ctx* ctx, const nemo_matmul8_args* args, void* stream);
+
+/* A cache of keys and values in 4-bit floats. Each 32 values of a head share a
+ * power of two: value = code 2^(byte - 127), the codes E2M1 floats (0, 0.5, 1,
+ * 1.5, 2, 3, 4, 6; bit 3 the sign), as CDNA4 converts them to 16 bits in one
+ * instruction and without a rounding; byte 255 makes its 32 values NaN.
+ *
+ * Tokens lie in pages of `page` tokens of one request, P = page, D = head_dim.
+ * A page holds its KV heads one after the other, each as
+ *   K codes   [P][D / 2]             two codes a byte, the first in the low bits
+ *   V codes   [P / 4][16][4][D / 32] 4 tokens' pieces of D / 16 values side by side
+ *   K scales  [P / 8][D / 32][8]
+ *   V scales  [P / 8][D / 32][8]
+ * P (D + D / 16) bytes. Pages may be shared by requests that only read them. */
+typedef struct nemo_cache4_config {
+  int32_t kv_heads;            /* 1..1024 */
+  int32_t head_dim;            /* 64 or 128 */
+  int32_t page;                /* 32, 64, 128, 256, 512 or 1024 tokens */
+} nemo_cache4_config;
+
+/* Bytes of a page: kv_heads page (head_dim + head_dim / 16). */
+nemo_status nemo_cache4_page_bytes(const nemo_cache4_config* config, size_t* bytes);
+
+/* Where the tokens of `count` requests are: token t of request b is token
+ * t % page of page table[b table_row + t / page]. The arrays are read on the device when
+ * the work runs. Pages outside [0, pages), and tokens past table_row pages,
+ * are not there: they are not written, read as zeros, and no query sees them. */
+typedef struct nemo_cache4_pages {
+  int32_t count;               /* requests: 0..2^20, times kv_heads at most 2^22 */
+  int32_t pages;               /* pages that `data` holds */
+  void* data;                  /* device, 16-byte aligned */
+  const int32_t* table;        /* device [count][table_row] */
+  int64_t table_row;           /* pages of a request's row of the table: 0..2^23 */
+  const int32_t* kv_len;       /* device [count]: tokens of each request, those of this call's rows among them */
+} nemo_cache4_pages;
+
+/* Key and value rows of requests' last tokens: rows q_start[b] .. q_start[b + 1]
+ * - 1 are request b's; of its n rows, row i is token kv_len - n + i (rows
+ * before token 0 have none). Head h of row t starts at k + t k_row + h k_head. */
+typedef struct nemo_cache4_rows {
+  int32_t type;                /* F32, F16 or BF16 */
+  int64_t rows;                /* rows of k and v: 0..2^23 */
+  const int32_t* q_start;      /* device [count + 1], ascending; entries are cut to `rows` */
+  const int64_t* positions;    /* device [rows]: what the rotation of a row goes by; NULL: its token's number */
+  void *k, *v;
+  int64_t k_row, k_head, v_row, v_head;
+} nemo_cache4_rows;
+
+/* Append rows to a cache: keys are turned by `rope` (NULL: as they are; its
+ * head_dim is the cache's), keys and values rounded to 4 bits: the smallest
+ * power of two 2^s with max |x| <= 7 2^s, s in [-126, 125], and the nearest
+ * code, to an even one on ties, up to 6. All of it is computed in 64 bits, so
+ * a code is that of the exact value. 32 values with a NaN or an infinity
+ * become NaN. k and v are only read. Rows of a call that share a page write
+ * bytes of their own. */
+nemo_status nemo_cache4_append(nemo_ctx* ctx, const nemo_cache4_config* config, const nemo_cache4_pages* pages,
+                               const nemo_cache4_rows* rows, nemo_rope* rope, void* stream);
+/* The other way: the rows' values from the cache, in `type`; `positions` is
+ * not used. Rows that belong to no request or token are left as they were. */
+nemo_status nemo_cache4_read(nemo_ctx* ctx, const nemo_cache4_config* config, const nemo_cache4_pages* pages,
+                             const nemo_cache4_rows* rows, void* stream);
+
+/* nemo_window_attention over a cache in pages: request b's queries are rows
+ * q_start[b] .. q_start[b + 1] - 1 of q and out, its keys the kv_len[b] tokens of
+ * the cache, and what a query sees goes by nemo_attention_config, whose kv_heads
+ * and head_dim are the cache's. Keys and values are read as `type`, exactly
+ * (F16 from 2^-14 to 65504; what lies above is infinite). Softmax sums and
+ * outputs are in 32 bits, the probabilities rounded to `type` for the product
+ * with v. Keys and values that a query does not see reach its result in no
+ * form, NaN neither. A request's rows are left as they were where it has none. */
+typedef struct nemo_cache4_queries {
+  int64_t q_rows;              /* rows of q and out, times q_heads at most 2^26 */
+  int64_t max_kv;              /* the longest kv_len, or more: a hint for the split of the keys over the chip */
+  const int32_t* q_start;      /* device [count + 1], ascending; entries are cut to q_rows */
+  const void* q;               /* 16-byte aligned, strides multiples of 8, as out */
+  void* out;
+  int64_t q_row, q_head, out_row, out_head;
+  void* workspace;             /* device, 16-byte aligned; NULL: the keys of a query are not split */
+  size_t workspace_bytes;      /* at least nemo_cache4_attention_workspace's when workspace is given */
+} nemo_cache4_queries;
+
+/* Bytes of workspace for such a call (0: none is used), with the conditions of
+ * nemo_window_attention_workspace. */
+nemo_status nemo_cache4_attention_workspace(const nemo_attention_config* attention, int32_t count, int64_t q_rows,
+                                            int64_t max_kv, size_t* bytes);
+nemo_status nemo_cache4_attention(nemo_ctx* ctx, const nemo_cache4_config* config,
+                                  const nemo_attention_config* attention, const nemo_cache4_pages* pages,
+                                  const nemo_cache4_queries* queries, void* stream);
+
 /* ---- offline requantization (src/gguf/quantization.ts:77-131) ------------ */
 
 /* requantizeMatrixToQ40 (src/gguf/quantization.ts:101-131) on the GPU: the

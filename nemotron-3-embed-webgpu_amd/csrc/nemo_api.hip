@@ -1725,6 +1725,169 @@ nemo_status nemo_rmsnorm(nemo_ctx* ctx, const nemo_norm_args* args, void* stream
   });
 }
 
+// ---------------------------------------------------------------------------
+// Low-bit operators of an attention block
+// ---------------------------------------------------------------------------
+
+static void validate_type(int32_t type, const char* what) {
+  if (type != kF32 && type != kF16 && type != NEMO_TYPE_BF16)
+    fail(NEMO_ERR_UNSUPPORTED, std::string(what) + " F32, F16 or BF16");
+}
+
+nemo_status nemo_rope_norm_apply(nemo_rope* rope, int32_t type, const nemo_rope_heads* q, const nemo_rope_heads* k,
+                                 const nemo_head_norm* norm, int64_t rows, const int64_t* d_positions, int64_t base,
+                                 void* stream) {
+  return guarded([&] {
+    if (!rope || !q || !norm) fail(NEMO_ERR_INVALID, "null argument");
+    validate_type(type, "the norm of heads takes");
+    if (rows < 0 || rows > kMaxRows) fail(NEMO_ERR_INVALID, "rows must be in [0, 2^23]");
+    validate_rope_heads(*q, type);
+    if (k) validate_rope_heads(*k, type);
+    if (!(norm->epsilon >= 0) || !isfinite(norm->epsilon))
+      fail(NEMO_ERR_INVALID, "epsilon must be finite and 0 or more");
+    for (int64_t v : {norm->q_weight_head, norm->k_weight_head}) validate_stride(v, "weight strides");
+    validate_aligned({norm->q_weight, norm->k_weight}, 4);
+    validate_aligned({d_positions}, 8);
+    set_device(rope->ctx);
+    hip_check(launch_rope_norm(rope->angles, type, *q, k, *norm, rows, d_positions, base, (hipStream_t)stream),
+              "norm of heads");
+  });
+}
+
+// Largest sum of k products of bytes: 2^14 k below 2^31.
+constexpr int32_t kMaxMatmul8K = (1 << 17) - 1;
+
+nemo_status nemo_matmul8(nemo_ctx* ctx, const nemo_matmul8_args* args, void* stream) {
+  return guarded([&] {
+    if (!ctx || !args) fail(NEMO_ERR_INVALID, "null argument");
+    const nemo_matmul8_args& a = *args;
+    validate_type(a.type, "the 8-bit product is");
+    if (a.m < 0 || a.m > kMaxRows) fail(NEMO_ERR_INVALID, "m must be in [0, 2^23]");
+    if (a.n < 0 || a.n > kMaxRows) fail(NEMO_ERR_INVALID, "n must be in [0, 2^23]");
+    if (a.m * a.n > (int64_t)1 << 38) fail(NEMO_ERR_INVALID, "m times n must be at most 2^38");
+    if (a.k < 0 || a.k > kMaxMatmul8K) fail(NEMO_ERR_INVALID, "k must be in [0, 131071]");
+    for (int64_t v : {a.x_row, a.x_scale_row, a.w_row, a.y_row}) validate_stride(v, "matmul8 strides");
+    if (a.m == 0 || a.n == 0) return;
+    if (!a.x_scale || !a.w_scale || !a.y || (a.k && (!a.x || !a.w))) fail(NEMO_ERR_INVALID, "null argument");
+    if (a.x_row % 16 || a.w_row % 16) fail(NEMO_ERR_INVALID, "row strides of x and w must be multiples of 16");
+    if ((a.m > 1 && a.x_row < a.k) || (a.n > 1 && a.w_row < a.k))
+      fail(NEMO_ERR_INVALID, "rows of x and w must not overlap");
+    if (a.m > 1 && a.y_row < a.n) fail(NEMO_ERR_INVALID, "rows of y must not overlap");
+    if (((uintptr_t)a.x | (uintptr_t)a.w) & 15) fail(NEMO_ERR_INVALID, "x and w must be 16-byte aligned");
+    validate_aligned({a.y}, a.type == kF32 ? 4 : 2);
+    validate_aligned({a.x_scale, a.w_scale, a.bias}, 4);
+    set_device(ctx);
+    hip_check(launch_matmul8(a, (hipStream_t)stream), "8-bit product");
+  });
+}
+
+static void validate_cache4(const nemo_cache4_config& c) {
+  if (c.kv_heads < 1 || c.kv_heads > 1024) fail(NEMO_ERR_INVALID, "kv_heads must be in [1, 1024]");
+  if (c.head_dim != 64 && c.head_dim != 128) fail(NEMO_ERR_UNSUPPORTED, "head_dim must be 64 or 128");
+  if (c.page < 32 || c.page > 1024 || (c.page & (c.page - 1)))
+    fail(NEMO_ERR_INVALID, "page must be 32, 64, 128, 256, 512 or 1024");
+}
+
+static void validate_cache4_pages(const nemo_cache4_config& c, const nemo_cache4_pages& p) {
+  if (p.count < 0 || p.count > (1 << 20) || (int64_t)p.count * c.kv_heads > (1 << 22))
+    fail(NEMO_ERR_INVALID, "count must be in [0, 2^20], count times kv_heads at most 2^22");
+  if (p.pages < 0) fail(NEMO_ERR_INVALID, "pages must be 0 or more");
+  validate_stride(p.table_row, "table_row");
+  if (p.count == 0) return;
+  if (!p.kv_len || (p.table_row && !p.table) || (p.pages && !p.data)) fail(NEMO_ERR_INVALID, "null argument");
+  validate_aligned({p.kv_len, p.table}, 4);
+  if ((uintptr_t)p.data & 15) fail(NEMO_ERR_INVALID, "pages must be 16-byte aligned");
+}
+
+// Whether there is work.
+static bool validate_cache4_rows(const nemo_cache4_pages& p, const nemo_cache4_rows& r) {
+  validate_type(r.type, "rows of a cache are");
+  if (r.rows < 0 || r.rows > kMaxRows) fail(NEMO_ERR_INVALID, "rows must be in [0, 2^23]");
+  for (int64_t v : {r.k_row, r.k_head, r.v_row, r.v_head}) validate_stride(v, "cache row strides");
+  if (p.count == 0 || r.rows == 0) return false;
+  if (!r.q_start || !r.k || !r.v) fail(NEMO_ERR_INVALID, "null argument");
+  validate_aligned({r.k, r.v}, r.type == kF32 ? 4 : 2);
+  validate_aligned({r.q_start}, 4);
+  validate_aligned({r.positions}, 8);
+  return true;
+}
+
+nemo_status nemo_cache4_page_bytes(const nemo_cache4_config* config, size_t* bytes) {
+  return guarded([&] {
+    if (!config || !bytes) fail(NEMO_ERR_INVALID, "null argument");
+    validate_cache4(*config);
+    *bytes = (size_t)config->kv_heads * config->page * (config->head_dim + config->head_dim / 16);
+  });
+}
+
+nemo_status nemo_cache4_append(nemo_ctx* ctx, const nemo_cache4_config* config, const nemo_cache4_pages* pages,
+                               const nemo_cache4_rows* rows, nemo_rope* rope, void* stream) {
+  return guarded([&] {
+    if (!ctx || !config || !pages || !rows) fail(NEMO_ERR_INVALID, "null argument");
+    validate_cache4(*config);
+    validate_cache4_pages(*config, *pages);
+    if (rope && rope->angles.head_dim != config->head_dim)
+      fail(NEMO_ERR_INVALID, "the rope's head_dim is not the cache's");
+    if (rope && rope->ctx->device != ctx->device) fail(NEMO_ERR_INVALID, "the rope is another device's");
+    if (!validate_cache4_rows(*pages, *rows)) return;
+    set_device(ctx);
+    hip_check(launch_cache4_append(*config, *pages, *rows, rope ? &rope->angles : nullptr, (hipStream_t)stream),
+              "append to cache");
+  });
+}
+
+nemo_status nemo_cache4_read(nemo_ctx* ctx, const nemo_cache4_config* config, const nemo_cache4_pages* pages,
+                             const nemo_cache4_rows* rows, void* stream) {
+  return guarded([&] {
+    if (!ctx || !config || !pages || !rows) fail(NEMO_ERR_INVALID, "null argument");
+    validate_cache4(*config);
+    validate_cache4_pages(*config, *pages);
+    if (!validate_cache4_rows(*pages, *rows)) return;
+    set_device(ctx);
+    hip_check(launch_cache4_read(*config, *pages, *rows, (hipStream_t)stream), "read from cache");
+  });
+}
+
+nemo_status nemo_cache4_attention_workspace(const nemo_attention_config* attention, int32_t count, int64_t q_rows,
+                                            int64_t max_kv, size_t* bytes) {
+  return guarded([&] {
+    if (!attention || !bytes) fail(NEMO_ERR_INVALID, "null argument");
+    validate_attention(*attention);
+    validate_attention_sizes(*attention, count, q_rows, max_kv);
+    *bytes = cache4_workspace(*attention, count, q_rows, max_kv);
+  });
+}
+
+nemo_status nemo_cache4_attention(nemo_ctx* ctx, const nemo_cache4_config* config,
+                                  const nemo_attention_config* attention, const nemo_cache4_pages* pages,
+                                  const nemo_cache4_queries* queries, void* stream) {
+  return guarded([&] {
+    if (!ctx || !config || !attention || !pages || !queries) fail(NEMO_ERR_INVALID, "null argument");
+    const nemo_cache4_queries& b = *queries;
+    validate_cache4(*config);
+    validate_attention(*attention);
+    if (attention->kv_heads != config->kv_heads || attention->head_dim != config->head_dim)
+      fail(NEMO_ERR_INVALID, "kv_heads and head_dim must be the cache's");
+    validate_cache4_pages(*config, *pages);
+    validate_attention_sizes(*attention, pages->count, b.q_rows, b.max_kv);
+    for (int64_t v : {b.q_row, b.q_head, b.out_row, b.out_head}) {
+      validate_stride(v, "attention strides");
+      if (v % 8) fail(NEMO_ERR_INVALID, "attention strides must be multiples of 8");
+    }
+    if (pages->count == 0 || b.q_rows == 0) return;
+    if (!b.q_start || !b.q || !b.out) fail(NEMO_ERR_INVALID, "null argument");
+    for (const void* p : {b.q, (const void*)b.out, (const void*)b.workspace})
+      if ((uintptr_t)p & 15) fail(NEMO_ERR_INVALID, "attention buffers must be 16-byte aligned");
+    validate_aligned({b.q_start}, 4);
+    const size_t need = b.workspace ? cache4_workspace(*attention, pages->count, b.q_rows, b.max_kv) : 0;
+    if (b.workspace && b.workspace_bytes < need)
+      fail(NEMO_ERR_INVALID, "workspace has " + std::to_string(b.workspace_bytes) + " bytes; this batch needs " +
+                                 std::to_string(need));
+    set_device(ctx);
+    hip_check(launch_cache4_attention(*config, *attention, *pages, b, (hipStream_t)stream), "cache attention");
+  });
+}
+
 nemo_status nemo_model_set_attention(nemo_model* model, const nemo_model_attention* attention) {
   return guarded([&] {
     if (!model || !attention) fail(NEMO_ERR_INVALID, "null argument");

@@ -1,0 +1,581 @@
+// Attention over a paged cache of 4-bit floats for gfx950 (include/nemo.h
+// nemo_cache4_attention): softmax(scale q.k) v over the keys j <= p + right that
+// have j >= p - left or j < sinks.
+//
+// Rows are (query, head of the group) pairs of one request and KV head, query
+// by query; a wave takes 16 QT of them and 32 keys a step. Codes go from memory
+// to registers and become 16-bit floats there, two by an instruction and
+// exactly: no LDS, no scale left to be applied.
+//
+// Scores are taken transposed, S^T = K Q^T (two tiles of 16 keys x 16 rows by
+// v_mfma_f32_16x16x32), so a lane holds one row, and which keys a tile has is
+// free: lane group h = lane / 16 gets the scores of keys 8 h .. 8 h + 7, in order,
+// as its registers of both tiles. That is the second operand of O^T = V^T P^T
+// (16 columns x 16 rows over 32 keys). K's operand is a key's D / 4 values from
+// D / 4 h on, 16 bytes for heads of 128; V's operand is one column of 8 keys: a
+// lane decodes D / 16 columns of its 8 keys, which lie side by side in the cache,
+// and exchanges halves of neighbouring keys' registers.
+#include <algorithm>
+#include <type_traits>
+
+#include "nemo_cache4.h"
+
+namespace nemo {
+
+namespace {
+
+struct AttendArgs {
+  nemo_cache4_queries b;
+  Cache4 c;
+  int group, left, right, sinks;
+  float scale2;  // of the scores, in units of log2
+  // row / group for rows below 2^31: (row + the high half of row * magic) >> shift
+  uint32_t magic;
+  int shift;
+  __device__ __forceinline__ int query(int row) const {
+    return (int)((__umulhi((uint32_t)row, magic) + (uint32_t)row) >> shift);
+  }
+};
+
+// The window of a query at p over a request's n keys: [lo, hi).
+struct Seen {
+  int lo, hi;
+  __device__ __forceinline__ Seen(int from, int to) : lo(from), hi(to) {}
+  __device__ __forceinline__ Seen(const AttendArgs& a, int p, int n) {
+    hi = max(0, min(n, a.right >= kUnbounded ? n : p + a.right + 1));
+    lo = a.left >= kUnbounded ? 0 : min(hi, max(0, p - a.left));
+  }
+};
+
+// The request of tile number t, and the number of its first tile; tiles of ROWS
+// (query, head of the group) rows are numbered through a batch without a
+// table: request i's first number is floor(q_start[i] group / ROWS) + i, which
+// leaves it at least as many numbers as it has tiles. None (i = -1) before the
+// first request. A wave looks at 64 requests at a time, evenly over those that
+// it may be.
+struct Request {
+  int i, tile, q0, queries, keys;
+  __device__ __forceinline__ Request(const AttendArgs& a, int t, int ROWS) {
+    const int lane = threadIdx.x & 63;
+    auto row = [&](int at) { return min(max(a.b.q_start[at], 0), (int)a.b.q_rows); };
+    auto number = [&](int begin, int at) { return (int)((int64_t)begin * a.group / ROWS) + at; };
+    int from = 0, left = a.c.count;
+    while (left > 64) {
+      const int step = (left + 63) >> 6, at = from + min(lane * step, left - 1);
+      const int n = (int)__popcll(__builtin_amdgcn_ballot_w64(lane * step < left && number(row(at), at) <= t));
+      from += max(n - 1, 0) * step;
+      left = min(step, a.c.count - from);
+    }
+    const int at = min(from + lane, a.c.count - 1), begin = row(at), end = row(at + 1);
+    const int len = (int)min((int64_t)max(a.c.kv_len[at], 0), min(a.c.table_row << a.c.shift, (int64_t)1 << 30));
+    const int first = number(begin, at);
+    const int n = (int)__popcll(__builtin_amdgcn_ballot_w64(lane < left && first <= t));
+    i = from + n - 1;
+    if (!n) i = -1;
+    const int of = max(n - 1, 0);
+    tile = __builtin_amdgcn_readlane(first, of);
+    q0 = __builtin_amdgcn_readlane(begin, of);
+    queries = max(__builtin_amdgcn_readlane(end, of) - q0, 0);
+    keys = __builtin_amdgcn_readlane(len, of);
+  }
+};
+
+// The blocks of 32 keys that the rows of queries at p0 .. p1 see: those of the
+// sinks before the window, then the window's.
+struct Blocks {
+  int sinks, skip, n;
+  __device__ __forceinline__ Blocks(const AttendArgs& a, const Seen& first, const Seen& last) {
+    const int lo = first.lo >> 5, hi = (last.hi + 31) >> 5;
+    sinks = min((min(a.sinks, last.hi) + 31) >> 5, lo);
+    skip = lo - sinks;
+    n = max(hi - skip, 0);
+  }
+  __device__ __forceinline__ int block(int t) const { return t < sinks ? t : t + skip; }
+};
+
+template <typename T>
+struct Mma;
+template <>
+struct Mma<half_t> {
+  typedef half8v frag;
+  typedef half2v pair;
+  static constexpr int kFinite = 140;  // largest scale byte with finite values
+  static __device__ __forceinline__ float add(pair p, float sum) {
+    return __builtin_amdgcn_fdot2(p, pair{(half_t)1.f, (half_t)1.f}, sum, false);
+  }
+  static __device__ __forceinline__ float4v mma(frag a, frag b, float4v c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+  }
+  template <int B>
+  static __device__ __forceinline__ uint32_t decode(uint32_t codes, float scale) {
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, scale, B));
+  }
+};
+template <>
+struct Mma<bf16_t> {
+  typedef bf16_t frag __attribute__((ext_vector_type(8)));
+  typedef bf16_t pair __attribute__((ext_vector_type(2)));
+  static constexpr int kFinite = 252;
+  static __device__ __forceinline__ float add(pair p, float sum) {
+    return __builtin_amdgcn_fdot2_f32_bf16(p, pair{(bf16_t)1.f, (bf16_t)1.f}, sum, false);
+  }
+  static __device__ __forceinline__ float4v mma(frag a, frag b, float4v c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+  }
+  template <int B>
+  static __device__ __forceinline__ uint32_t decode(uint32_t codes, float scale) {
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, B));
+  }
+};
+
+// The power of two of byte i of eight scale bytes. (A conversion reads the
+// exponent's bits alone, so those of other bytes beside it may stay.)
+__device__ __forceinline__ float power(u32x2 bytes, int i) {
+  const uint32_t w = bytes[i >> 2];
+  const int s = 23 - 8 * (i & 3);
+  return __uint_as_float(s >= 0 ? w << s : w >> -s);
+}
+
+// What a lane has of a block of 32 keys. K tile u's row l % 16 = 4 b + j is key
+// 8 b + 4 u + j, so a lane's scores of both tiles are of keys that follow each other.
+template <int D>
+struct Raw {
+  static constexpr int W = D / 32;  // registers of 8 codes: a key's quarter of K, 4 keys' pieces of V times two
+  typedef uint32_t vec __attribute__((ext_vector_type(W)));
+  vec k[2], v[2];
+  u32x2 k_scales, v_scales;
+  // The page's KV head begins at `head`; key t of it is the block's first.
+  __device__ __forceinline__ void load(const uint8_t* head, int shift, int t, int lane) {
+    typedef Cache4Head<D> Head;
+    const int row = lane & 15, h = lane >> 4, key = 8 * (row >> 2) + (row & 3);
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      k[u] = *(const vec*)(head + Head::k_codes(t + key + 4 * u) + h * (D / 8));
+      v[u] = *(const vec*)(head + Head::v_codes(shift, t + 8 * h + 4 * u, row));
+    }
+    k_scales = *(const u32x2*)(head + Head::scale(shift, false, t + 8 * (row >> 2), h * (D / 32) / 4));
+    v_scales = *(const u32x2*)(head + Head::scale(shift, true, t + 8 * h, row * (D / 32) / 16));
+  }
+};
+
+// A wave's 16 QT rows: row 16 i + l % 16 in lane l for each i, whose group h = l / 16
+// holds output columns D / 16 (4 h + e) + t in register e of o[i][t], and the sum
+// of its own keys' probabilities.
+template <typename T, int D, int QT>
+struct Rows {
+  static constexpr int W = D / 32, C = D / 16;
+  typedef Mma<T> M;
+  typedef typename M::frag frag;
+  typedef typename M::pair pair;
+  frag q[QT][W];
+  float4v o[QT][C];
+  float m[QT], l[QT];  // reference and sum of the probabilities
+
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int i = 0; i < QT; ++i) {
+      m[i] = -INFINITY;
+      l[i] = 0.f;
+#pragma unroll
+      for (int t = 0; t < C; ++t) o[i][t] = float4v{0.f, 0.f, 0.f, 0.f};
+    }
+  }
+  // Probabilities are taken against a reference that is raised when the sum of a
+  // lane's 8 passes MOST, as in window attention: f16's largest is 2^BELOW and
+  // more, so that what lies far below it keeps its share among f16's smallest
+  // values.
+  static constexpr bool HALF = std::is_same<T, half_t>::value;
+  static constexpr float BELOW = HALF ? 8.f : 0.f, MOST = HALF ? 0x1p20f : 0x1p15f;
+  static __device__ __forceinline__ float exponentials(const float (&s)[8], float scale2, float m, frag& p) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) p[i] = (T)__builtin_amdgcn_exp2f(fmaf(s[i], scale2, -m));
+    float v = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) v = M::add(pair{p[i], p[i + 1]}, v);
+    return v;
+  }
+  __device__ __forceinline__ void settle(int i, const float (&s)[8], float scale2, frag& p) {
+    float add = exponentials(s, scale2, m[i], p);
+    if (__builtin_amdgcn_ballot_w64(!(add <= MOST))) {
+      asm volatile("");  // keeps the rare path a branch
+      float top = s[0];
+#pragma unroll
+      for (int r = 1; r < 8; ++r) top = fmaxf(top, s[r]);
+      top *= scale2;
+      int raise = !(add <= MOST);
+#pragma unroll
+      for (int x = 16; x < 64; x *= 2) {
+        raise |= __shfl_xor(raise, x, 64);  // only the rows that ask: none depends on another
+        top = fmaxf(top, __shfl_xor(top, x, 64));
+      }
+      const float raised = raise ? fmaxf(m[i], top - BELOW) : m[i];
+      const float alpha = m[i] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[i] - raised);
+      l[i] *= alpha;
+#pragma unroll
+      for (int t = 0; t < C; ++t) o[i][t] *= alpha;
+      m[i] = raised;
+      add = exponentials(s, scale2, raised == -INFINITY ? 0.f : raised, p);
+    }
+    l[i] += add;
+  }
+  // Whether a value of the lane's rows is not finite.
+  __device__ __forceinline__ bool spoilt() const {
+    float z = 0.f;
+#pragma unroll
+    for (int i = 0; i < QT; ++i) {
+      z = fmaf(l[i], 0.f, z);
+#pragma unroll
+      for (int t = 0; t < C; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) z = fmaf(o[i][t][e], 0.f, z);
+    }
+    return z != 0.f;
+  }
+};
+
+// Which of the 8 keys from j on a row sees, as bits.
+__device__ __forceinline__ uint32_t seen8(int j, const Seen& s, int sinks) {
+  auto below = [&](int t) { return (1u << max(0, min(t - j, 8))) - 1; };
+  return below(s.hi) & (~below(s.lo) | below(sinks));
+}
+
+// One block of 32 keys from key j0 on. `hide`: not every row sees all of them;
+// `seen`: what its lane's rows see. `careful`: values that are not finite are met
+// one by one, those of keys that a row does not see left out.
+template <typename T, int D, int QT>
+__device__ __forceinline__ void attend(Rows<T, D, QT>& a, const Raw<D>& raw, float scale2, bool hide, bool careful,
+                                       const uint32_t (&seen)[QT], uint32_t any) {
+  constexpr int W = D / 32;
+  typedef Mma<T> M;
+  typedef typename M::frag frag;
+  const int lane = threadIdx.x & 63;
+  float4v s[QT][2];
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    const float power = __uint_as_float((raw.k_scales[u] >> (8 * (lane & 3))) << 23);
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      const uint32_t c = raw.k[u][w];
+      const u32x4 f = {M::template decode<0>(c, power), M::template decode<1>(c, power),
+                       M::template decode<2>(c, power), M::template decode<3>(c, power)};
+#pragma unroll
+      for (int i = 0; i < QT; ++i)
+        s[i][u] = M::mma(__builtin_bit_cast(frag, f), a.q[i][w], w ? s[i][u] : float4v{0.f, 0.f, 0.f, 0.f});
+    }
+  }
+  frag p[QT];
+  u32x2 scales = raw.v_scales;
+  if (hide) {
+    // values of keys that no row sees are taken times 2^-127
+    uint32_t keep[2];
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      keep[x] = 0;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) keep[x] |= any >> (4 * x + e) & 1 ? 255u << (8 * e) : 0;
+      scales[x] &= keep[x];
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < QT; ++i) {
+    float v[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = s[i][e >> 2][e & 3];
+    if (hide) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = seen[i] >> e & 1 ? v[e] : -INFINITY;
+    }
+    a.settle(i, v, scale2, p[i]);
+  }
+  if (careful) {
+    // values that are not finite: their place holds 2^-127, and the rows that see
+    // one become NaN in its 32 columns
+    frag bad;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const uint32_t byte = scales[e >> 2] >> (8 * (e & 3)) & 255;
+      bad[e] = (T)(byte > M::kFinite ? 1.f : 0.f);
+      if (byte > M::kFinite) scales[e >> 2] &= ~(255u << (8 * (e & 3)));
+    }
+#pragma unroll
+    for (int i = 0; i < QT; ++i) {
+      frag sees;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) sees[e] = (T)(!hide || (seen[i] >> e & 1) ? 1.f : 0.f);
+      const float4v n = M::mma(bad, sees, float4v{0.f, 0.f, 0.f, 0.f});
+#pragma unroll
+      for (int t = 0; t < D / 16; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (n[e] > 0.f) a.o[i][t][e] = __uint_as_float(0x7fc00000u);
+    }
+  }
+  // V: columns 2 b, 2 b + 1 of the lane's piece, for each of its 8 keys in one register
+  float power[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) power[e] = nemo::power(scales, e);
+  auto columns = [&](auto at) {
+    constexpr int B = decltype(at)::value;
+    uint32_t r[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      if constexpr (D == 128) r[e] = M::template decode<B>(raw.v[e >> 2][e & 3], power[e]);
+      else r[e] = e & 1 ? M::template decode<B + 2>(raw.v[e >> 2][e >> 1 & 1], power[e])
+                        : M::template decode<B>(raw.v[e >> 2][e >> 1 & 1], power[e]);
+    }
+    u32x4 low, high;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      low[e] = __builtin_amdgcn_perm(r[2 * e + 1], r[2 * e], 0x05040100u);
+      high[e] = __builtin_amdgcn_perm(r[2 * e + 1], r[2 * e], 0x07060302u);
+    }
+#pragma unroll
+    for (int i = 0; i < QT; ++i) {
+      a.o[i][2 * B] = M::mma(__builtin_bit_cast(frag, low), p[i], a.o[i][2 * B]);
+      a.o[i][2 * B + 1] = M::mma(__builtin_bit_cast(frag, high), p[i], a.o[i][2 * B + 1]);
+    }
+  };
+  columns(std::integral_constant<int, 0>{});
+  columns(std::integral_constant<int, 1>{});
+  if constexpr (D == 128) {
+    columns(std::integral_constant<int, 2>{});
+    columns(std::integral_constant<int, 3>{});
+  }
+}
+
+// Sums of a split: the row's reference and sum, and its output values.
+struct Partials {
+  float2* ml;  // [split][row], null: not split
+  float* o;    // [split][row][D]
+  int64_t rows;
+  int splits;
+};
+
+// A workgroup takes 16 QT rows; its waves every WAVES-th block of keys, whose
+// sums they add in LDS. With `splits` above 1 the blocks are dealt out to that
+// many workgroups as well, whose sums a second kernel joins.
+template <typename T, int D, int QT, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void cache4_attention_kernel(AttendArgs a, Partials part) {
+  constexpr int C = D / 16, W = D / 32;
+  typedef typename Mma<T>::frag frag;
+  __shared__ __attribute__((aligned(16))) float sums[WAVES][16][D];  // of 16 rows at a time
+  __shared__ float2 ml[WAVES][16];
+  const int kvh = blockIdx.x % a.c.kv_heads, tile_no = blockIdx.x / a.c.kv_heads, split = blockIdx.y;
+  const Request r(a, tile_no, 16 * QT);
+  if (r.i < 0) return;
+  const int rows = r.queries * a.group, row0 = (tile_no - r.tile) * 16 * QT;
+  if ((unsigned)row0 >= (unsigned)rows) return;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 4;
+  const int behind = r.keys - r.queries;  // position of query 0
+  auto window = [&](int row) { return Seen(a, behind + a.query(row), r.keys); };
+  const Seen first = window(row0), last = window(min(row0 + 16 * QT, rows) - 1);
+  const Blocks blocks(a, first, last);
+  const int block0 = (int)((int64_t)blocks.n * split / part.splits);
+  const int block1 = (int)((int64_t)blocks.n * (split + 1) / part.splits);
+  const int head_of = kvh * a.group;  // query head of row 0 of a query
+  Rows<T, D, QT> acc;
+  int lo[QT], hi[QT];
+#pragma unroll
+  for (int i = 0; i < QT; ++i) {
+    const int row = min(row0 + 16 * i + (lane & 15), rows - 1), query = a.query(row);
+    const Seen s(a, behind + query, r.keys);
+    lo[i] = s.lo;
+    hi[i] = s.hi;
+    const T* q = (const T*)a.b.q + (int64_t)(r.q0 + query) * a.b.q_row +
+                 (int64_t)(head_of + row - query * a.group) * a.b.q_head + h * (D / 4);
+#pragma unroll
+    for (int w = 0; w < W; ++w) acc.q[i][w] = *(const frag*)(q + 8 * w);
+  }
+  const int32_t* table = a.c.table + r.i * a.c.table_row;
+  const int per = a.c.shift - 5;  // log2 of a page's blocks
+  // Page of the wave's block t, none (-1) past the last and where it is not there.
+  auto page_of = [&](int t) {
+    if (t >= block1) return -1;
+    const int page = __builtin_amdgcn_readfirstlane(table[blocks.block(t) >> per]);
+    return (unsigned)page < (unsigned)a.c.pages ? page : -1;
+  };
+  auto load = [&](Raw<D>& raw, int page, int t) {
+    if (page < 0) return;
+    raw.load(a.c.data + a.c.head<D>(page, kvh), a.c.shift, (blocks.block(t) & ((1 << per) - 1)) << 5, lane);
+  };
+  for (int careful = 0;; ++careful) {
+    acc.clear();
+    Raw<D> raw, next;
+    int t = block0 + wave, page = page_of(t), next_page = page_of(t + WAVES);
+    load(raw, page, t);
+    for (; t < block1; t += WAVES) {
+      load(next, next_page, t + WAVES);
+      const int after = page_of(t + 2 * WAVES);
+      if (page >= 0) {
+        const int j0 = blocks.block(t) << 5;
+        const bool hide = j0 + 32 > first.hi || (j0 < last.lo && j0 + 32 > a.sinks);
+        uint32_t seen[QT] = {}, any = 255;
+        if (hide) {
+          any = seen8(j0 + 8 * h, Seen(first.lo, last.hi), a.sinks);
+#pragma unroll
+          for (int i = 0; i < QT; ++i) seen[i] = seen8(j0 + 8 * h, Seen(lo[i], hi[i]), a.sinks);
+        }
+        attend<T, D, QT>(acc, raw, a.scale2, hide, careful, seen, any);
+      }
+      raw = next;
+      page = next_page;
+      next_page = after;
+    }
+    if (careful || !__builtin_amdgcn_ballot_w64(acc.spoilt())) break;
+  }
+  // The waves' sums, 16 rows at a time.
+  constexpr int THREADS = 64 * WAVES, PER = 16 * D / THREADS;  // columns of a thread
+  static_assert(PER >= 4 && D % PER == 0, "whole vectors of one row");
+#pragma unroll
+  for (int i = 0; i < QT; ++i) {
+    acc.l[i] += __shfl_xor(acc.l[i], 16, 64);
+    acc.l[i] += __shfl_xor(acc.l[i], 32, 64);
+    if (i) __syncthreads();
+    if (h == 0) ml[wave][lane & 15] = make_float2(acc.m[i], acc.l[i]);
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+#pragma unroll
+      for (int t = 0; t < C; t += 4)
+        *(float4v*)&sums[wave][lane & 15][(C * (4 * h + e) + t) ^ (4 * (lane & 7))] =
+            float4v{acc.o[i][t][e], acc.o[i][t + 1][e], acc.o[i][t + 2][e], acc.o[i][t + 3][e]};
+    __syncthreads();
+    const int row = threadIdx.x * PER / D, c0 = threadIdx.x * PER % D, at = row0 + 16 * i + row;
+    if (at >= rows) continue;
+    float m = -INFINITY, l = 0.f, v[PER] = {};
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) m = fmaxf(m, ml[w][row].x);
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) {
+      const float2 s = ml[w][row];
+      if (s.x == -INFINITY && s.y == 0.f) continue;  // saw nothing
+      const float f = s.x == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(s.x - m);
+      l = fmaf(f, s.y, l);
+#pragma unroll
+      for (int c = 0; c < PER; c += 4) {
+        const float4v o = *(const float4v*)&sums[w][row][(c0 + c) ^ (4 * (row & 7))];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[c + e] = fmaf(f, o[e], v[c + e]);
+      }
+    }
+    const int query = a.query(at), head = head_of + at - query * a.group;
+    if (part.ml) {
+      const int64_t to = part.rows * split + (int64_t)(r.q0 + query) * a.c.kv_heads * a.group + head;
+      if (c0 == 0) part.ml[to] = make_float2(m, l);
+#pragma unroll
+      for (int c = 0; c < PER; c += 4)
+        *(float4v*)(part.o + to * D + c0 + c) = float4v{v[c], v[c + 1], v[c + 2], v[c + 3]};
+    } else {
+      typedef T vec __attribute__((ext_vector_type(4)));
+      const float inv = l == 0.f ? 0.f : 1.0f / l;
+      T* out = (T*)a.b.out + (int64_t)(r.q0 + query) * a.b.out_row + (int64_t)head * a.b.out_head + c0;
+#pragma unroll
+      for (int c = 0; c < PER; c += 4)
+        *(vec*)(out + c) = vec{(T)(v[c] * inv), (T)(v[c + 1] * inv), (T)(v[c + 2] * inv), (T)(v[c + 3] * inv)};
+    }
+  }
+}
+
+// Joins the splits, at most 64: a workgroup a row. Thread (g, c) adds columns 4
+// c.. of splits g, g + G, ..., and the G sums are added in order.
+template <typename T, int D>
+__global__ __launch_bounds__(256) void cache4_join_kernel(AttendArgs a, Partials part) {
+  constexpr int C = D / 4, G = 256 / C;
+  __shared__ float weight[64];
+  __shared__ float4v sums[G][C];
+  const int kvh = blockIdx.x % a.c.kv_heads, tile_no = blockIdx.x / a.c.kv_heads;
+  const Request r(a, tile_no, 1);
+  if (r.i < 0) return;
+  const int row = tile_no - r.tile, lane = threadIdx.x & 63;
+  if ((unsigned)row >= (unsigned)(r.queries * a.group)) return;
+  const int i = a.query(row), head = kvh * a.group + (row - i * a.group);
+  const int64_t at = (int64_t)(r.q0 + i) * a.c.kv_heads * a.group + head;
+  // every wave: lane z's split
+  const float2 ml = lane < part.splits ? part.ml[part.rows * lane + at] : make_float2(-INFINITY, 0.f);
+  float m = ml.x;
+#pragma unroll
+  for (int x = 32; x > 0; x >>= 1) m = fmaxf(m, __shfl_xor(m, x, 64));
+  const bool empty = ml.x == -INFINITY && ml.y == 0.f;  // saw nothing
+  const float f = empty ? 0.f : ml.x == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(ml.x - m);
+  float l = empty ? 0.f : f * ml.y;
+#pragma unroll
+  for (int x = 32; x > 0; x >>= 1) l += __shfl_xor(l, x, 64);
+  if (threadIdx.x < 64) weight[lane] = empty ? -1.f : f;
+  __syncthreads();
+  const int c = threadIdx.x % C, g = threadIdx.x / C;
+  float4v v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int z = g; z < part.splits; z += G) {
+    const float4v o = *(const float4v*)(part.o + (part.rows * z + at) * D + 4 * c);
+    const float w = weight[z];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = w == -1.f ? v[e] : fmaf(w, o[e], v[e]);
+  }
+  sums[g][c] = v;
+  __syncthreads();
+  if (threadIdx.x >= D) return;
+  float sum = 0.f;
+#pragma unroll
+  for (int k = 0; k < G; ++k) sum += sums[k][threadIdx.x / 4][threadIdx.x % 4];
+  T* out = (T*)a.b.out + (int64_t)(r.q0 + i) * a.b.out_row + (int64_t)head * a.b.out_head;
+  out[threadIdx.x] = (T)(l == 0.f ? 0.f : sum / l);
+}
+
+// Rows of a tile and how the keys are split, by a batch's sizes alone.
+struct Plan {
+  int tiles16, splits;  // rows of a tile / 16
+};
+Plan plan_of(const nemo_attention_config& c, int count, int64_t q_rows, int64_t max_kv) {
+  if (count == 0 || q_rows == 0) return {1, 1};
+  const int64_t rows = q_rows * (c.q_heads / c.kv_heads);
+  const int tiles16 = rows / count <= 16 ? 1 : 4;
+  const int64_t tiles = std::max<int64_t>(rows / (16 * tiles16), count) * c.kv_heads;
+  int64_t keys = max_kv;
+  if (c.left >= 0 && c.right >= 0) keys = std::min(keys, (int64_t)c.left + c.right + 1 + c.sinks);
+  const int64_t splits = std::min<int64_t>({512 / tiles, keys / 1024, 64});
+  return {tiles16, (int)std::max<int64_t>(1, splits)};
+}
+
+}  // namespace
+
+size_t cache4_workspace(const nemo_attention_config& c, int count, int64_t q_rows, int64_t max_kv) {
+  const int splits = plan_of(c, count, q_rows, max_kv).splits;
+  return splits == 1 ? 0 : (size_t)splits * q_rows * c.q_heads * (c.head_dim * 4 + 8);
+}
+
+hipError_t launch_cache4_attention(const nemo_cache4_config& cache, const nemo_attention_config& c,
+                                   const nemo_cache4_pages& p, const nemo_cache4_queries& b, hipStream_t stream) {
+  if (p.count == 0 || b.q_rows == 0) return hipSuccess;
+  AttendArgs a{b, Cache4(cache, p), c.q_heads / c.kv_heads, 0, 0, 0, 0.f, 0, 0};
+  while (1 << a.shift < a.group) ++a.shift;
+  a.magic = (uint32_t)((((uint64_t)1 << a.shift) - a.group) * ((uint64_t)1 << 32) / a.group + 1);
+  auto bound = [](int v) { return v < 0 ? kUnbounded : std::min(v, kUnbounded); };
+  a.left = bound(c.left);
+  a.right = bound(c.right);
+  a.sinks = std::min(c.sinks, kUnbounded);
+  a.scale2 = (c.scale > 0.f ? c.scale : 1.0f / sqrtf((float)c.head_dim)) * 1.4426950408889634f;
+  const Plan plan = plan_of(c, p.count, b.q_rows, b.max_kv);
+  const int splits = b.workspace ? plan.splits : 1;
+  const int64_t rows = b.q_rows * c.q_heads;
+  Partials part{nullptr, nullptr, rows, splits};
+  if (splits > 1) {
+    part.o = (float*)b.workspace;
+    part.ml = (float2*)(part.o + splits * rows * c.head_dim);
+  }
+  auto tiles = [&](int r) { return (unsigned)(b.q_rows * a.group / r + p.count) * c.kv_heads; };
+  auto launch = [&](auto type, auto d) {
+    constexpr int D = decltype(d)::value;
+    typedef decltype(type) T;
+    if (plan.tiles16 == 1) cache4_attention_kernel<T, D, 1, 4><<<dim3(tiles(16), splits), 256, 0, stream>>>(a, part);
+    else cache4_attention_kernel<T, D, 4, 4><<<dim3(tiles(64), splits), 256, 0, stream>>>(a, part);
+    if (splits > 1) cache4_join_kernel<T, D><<<tiles(1), 256, 0, stream>>>(a, part);
+  };
+  auto typed = [&](auto type) {
+    if (c.head_dim == 64) launch(type, std::integral_constant<int, 64>{});
+    else launch(type, std::integral_constant<int, 128>{});
+  };
+  if (c.type == NEMO_TYPE_F16) typed(half_t{});
+  else typed(bf16_t{});
+  return hipGetLastError();
+}
+
+}  // namespace nemo

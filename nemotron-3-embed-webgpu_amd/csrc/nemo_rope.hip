@@ -8,6 +8,7 @@
 // 2^20, 671 MB, take 118 us (5.7 TB/s; a copy reaches 4.9 to 5.4), 5001 tokens
 // of 15 f32 heads of 96 12.8 (medians 121 and 13.7), one token 2.3.
 #include <algorithm>
+#include <type_traits>
 
 #include "nemo_operators.h"
 
@@ -163,7 +164,176 @@ hipError_t launch_rope_type(const RopeArgs& a, hipStream_t stream) {
   return hipGetLastError();
 }
 
+// ---------------------------------------------------------------------------
+// The norm of each head on the way: h = x / sqrt(mean x^2 + eps) w, then turned.
+// A head is `lanes` lanes of a wave, each with NI items of it: by halves the
+// vectors of a pair's first and second values (two vectors side by side behind
+// the pairs), interleaved one vector. The lanes add up their squares, so a
+// head is read once, and a thread's angles and weights serve every `slots`-th
+// head of its token.
+// ---------------------------------------------------------------------------
+
+// E values, as one vector where the addresses allow it.
+template <typename T, int E, bool VECTORS>
+__device__ __forceinline__ void load_values(const T* p, float (&v)[E]) {
+  if constexpr (VECTORS && E > 1) {
+    typedef T vec __attribute__((ext_vector_type(E)));
+    const vec t = *(const vec*)p;
+#pragma unroll
+    for (int e = 0; e < E; ++e) v[e] = (float)t[e];
+  } else {
+#pragma unroll
+    for (int e = 0; e < E; ++e) v[e] = (float)p[e];
+  }
+}
+template <typename T, int E, bool VECTORS>
+__device__ __forceinline__ void store_values(T* p, const float (&v)[E]) {
+  if constexpr (VECTORS && E > 1) {
+    typedef T vec __attribute__((ext_vector_type(E)));
+    vec t;
+#pragma unroll
+    for (int e = 0; e < E; ++e) t[e] = (T)v[e];
+    *(vec*)p = t;
+  } else {
+#pragma unroll
+    for (int e = 0; e < E; ++e) p[e] = (T)v[e];
+  }
+}
+
+template <typename T, int E, bool HALF, bool VECTORS, int NI>
+__global__ __launch_bounds__(256) void rope_norm_kernel(RopeArgs a, nemo_head_norm n, int lanes, int slots,
+                                                        int tokens) {
+  constexpr int V = HALF ? 2 : 1, C = HALF ? E : E / 2;  // vectors and pairs of an item
+  const int per = lanes * slots, l = threadIdx.x % lanes, slot = threadIdx.x % per / lanes;
+  const int64_t t = (int64_t)blockIdx.x * tokens + threadIdx.x / per;
+  if ((int)threadIdx.x >= tokens * per || t >= a.rows) return;  // (a head's lanes together)
+  const int heads = a.q.heads + a.k.heads, items = a.head_dim / (V * E);
+  const double p = rope_position(a, t);
+  int at[NI][V];
+  bool real[NI], turned[NI];
+  float2 cs[NI][C];
+#pragma unroll
+  for (int i = 0; i < NI; ++i) {
+    const int item = l + lanes * i;
+    real[i] = item < items;
+    turned[i] = real[i] && (HALF ? item < a.pairs / E : item < 2 * a.pairs / E);
+    at[i][0] = HALF && !turned[i] ? 2 * E * item : E * item;  // (2 pairs + 2 E (item - pairs / E))
+    if constexpr (HALF) at[i][1] = turned[i] ? a.pairs + E * item : at[i][0] + E;
+#pragma unroll
+    for (int c = 0; c < C; ++c) cs[i][c] = turned[i] ? rope_angle(a, C * item + c, p) : make_float2(1.f, 0.f);
+  }
+  float w[NI][V][E];
+  int weights = -1;  // whose weights w holds
+  for (int h = slot; h < heads; h += slots) {
+    const T* x;
+    T* y;
+    rope_head(a, t, h, x, y);
+    const bool key = h >= a.q.heads;
+    const int64_t stride = key ? n.k_weight_head : n.q_weight_head;
+    if (weights != (int)key || stride) {
+      weights = key;
+      const float* from = key ? n.k_weight : n.q_weight;
+      if (from) from += stride * (key ? h - a.q.heads : h);
+#pragma unroll
+      for (int i = 0; i < NI; ++i)
+#pragma unroll
+        for (int v = 0; v < V; ++v)
+#pragma unroll
+          for (int e = 0; e < E; ++e) w[i][v][e] = from && real[i] ? from[at[i][v] + e] : 1.f;
+    }
+    float r[NI][V][E], sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < NI; ++i)
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        if (real[i]) {
+          load_values<T, E, VECTORS>(x + at[i][v], r[i][v]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < E; ++e) r[i][v][e] = 0.f;
+        }
+#pragma unroll
+        for (int e = 0; e < E; ++e) sum = fmaf(r[i][v][e], r[i][v][e], sum);
+      }
+    for (int o = lanes >> 1; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
+    const float f = 1.0f / sqrtf(sum / a.head_dim + n.epsilon);
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+      if (!real[i]) continue;
+#pragma unroll
+      for (int v = 0; v < V; ++v)
+#pragma unroll
+        for (int e = 0; e < E; ++e) r[i][v][e] *= f * w[i][v][e];
+      if (turned[i]) {
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+          float& u = HALF ? r[i][0][c] : r[i][0][2 * c];
+          float& z = HALF ? r[i][V - 1][c] : r[i][0][2 * c + 1];
+          const float first = u * cs[i][c].x - z * cs[i][c].y;
+          z = u * cs[i][c].y + z * cs[i][c].x;
+          u = first;
+        }
+      }
+#pragma unroll
+      for (int v = 0; v < V; ++v) store_values<T, E, VECTORS>(y + at[i][v], r[i][v]);
+    }
+  }
+}
+
+// By the widest vectors that sizes, strides and addresses allow.
+template <typename T, int E = 16 / sizeof(T)>
+hipError_t launch_rope_norm_type(const RopeArgs& a, const nemo_head_norm& n, hipStream_t stream) {
+  const int heads = a.q.heads + a.k.heads, rest = a.head_dim - 2 * a.pairs, bytes = E * sizeof(T);
+  const bool fits = a.half ? a.pairs % E == 0 && rest % (2 * E) == 0
+                           : E > 1 && 2 * a.pairs % E == 0 && a.head_dim % E == 0;
+  const bool vectors = aligned_heads(a.q, E, bytes) && (!a.k.heads || aligned_heads(a.k, E, bytes));
+  auto launch = [&](auto half, auto v, auto ni, int items) {
+    int lanes = 1;
+    while (lanes < items && lanes < 64) lanes *= 2;
+    const int slots = std::max(1, std::min({heads, 256 / lanes, a.rows >= 512 ? (heads + 3) / 4 : heads}));
+    const int tokens = 256 / (lanes * slots);
+    rope_norm_kernel<T, E, decltype(half)::value, decltype(v)::value, decltype(ni)::value>
+        <<<(unsigned)((a.rows + tokens - 1) / tokens), 256, 0, stream>>>(a, n, lanes, slots, tokens);
+    return hipGetLastError();
+  };
+  auto sized = [&](auto half, auto v) {
+    const int items = a.head_dim / (decltype(half)::value ? 2 * E : E);
+    if (items <= 64) return launch(half, v, std::integral_constant<int, 1>{}, items);
+    if (items <= 128) return launch(half, v, std::integral_constant<int, 2>{}, items);
+    if constexpr (E <= 4) {
+      if (items <= 256) return launch(half, v, std::integral_constant<int, 4>{}, items);
+      if constexpr (E <= 2) return launch(half, v, std::integral_constant<int, 8>{}, items);
+    }
+    return hipErrorInvalidValue;  // (1024 values are 128 items of 8, 256 of 4, 512 of 2)
+  };
+  if (fits && vectors) {
+    if constexpr (E > 1) {
+      if (!a.half) return sized(std::false_type{}, std::true_type{});
+    }
+    if (a.half) return sized(std::true_type{}, std::true_type{});
+  }
+  if constexpr (E == 2) {  // single values
+    if (!a.half) return sized(std::false_type{}, std::false_type{});
+  }
+  if constexpr (E > 1) return launch_rope_norm_type<T, E / 2>(a, n, stream);
+  return hipErrorInvalidValue;
+}
+
 }  // namespace
+
+hipError_t launch_rope_norm(const RopeAngles& angles, int type, const nemo_rope_heads& q, const nemo_rope_heads* k,
+                            const nemo_head_norm& norm, int64_t rows, const int64_t* positions, int64_t base,
+                            hipStream_t stream) {
+  const RopeArgs a{q, k ? *k : nemo_rope_heads{}, angles.turns, positions, base, rows, angles.magnitude,
+                   angles.head_dim, angles.rotary / 2, 0, angles.half};
+  if (rows == 0 || a.q.heads + a.k.heads == 0) return hipSuccess;
+  switch (type) {
+    case NEMO_TYPE_F32: return launch_rope_norm_type<float>(a, norm, stream);
+    case NEMO_TYPE_F16: return launch_rope_norm_type<half_t>(a, norm, stream);
+    case NEMO_TYPE_BF16: return launch_rope_norm_type<bf16_t>(a, norm, stream);
+    default: return hipErrorInvalidValue;
+  }
+}
 
 hipError_t launch_rope_apply(const RopeAngles& angles, int type, const nemo_rope_heads& q, const nemo_rope_heads* k,
                              int64_t rows, const int64_t* positions, int64_t base, hipStream_t stream) {

@@ -15,6 +15,7 @@
 #include <algorithm>
 #include <type_traits>
 
+#include "nemo_lds_copy.h"
 #include "nemo_operators.h"
 
 namespace nemo {
@@ -138,7 +139,6 @@ typedef short short4v __attribute__((ext_vector_type(4)));
 typedef short short8v __attribute__((ext_vector_type(8)));
 typedef bf16_t bf16x8 __attribute__((ext_vector_type(8)));
 typedef float float8v __attribute__((ext_vector_type(8)));
-typedef __attribute__((address_space(3))) void lds_void;
 typedef __attribute__((address_space(3))) short4v lds_short4v;
 
 template <typename T>
@@ -177,33 +177,6 @@ __device__ __forceinline__ int k_swizzle(int row) {
 template <int HD>
 __device__ __forceinline__ int v_swizzle(int row) {
   return HD == 128 ? 4 * (row & 3) : 4 * ((row >> 1) & 1);
-}
-
-// Copies of 16 bytes a lane into LDS at `to` + 16 lane, from a buffer's range
-// (zeros past its end) or an address. The compiler, which knows of the builtin for this that
-// it writes LDS, waits for every copy in flight before each transposed read;
-// written as here it has no register to be waited for, and the loops wait
-// for their images themselves. (m0 is reserved: the compiler sets it where it
-// uses it itself.)
-__device__ __forceinline__ uint32_t lds_address(const uint8_t* to) { return (uint32_t)(uintptr_t)(lds_void*)to; }
-__device__ __forceinline__ void copy_range(u32x4 range, uint32_t offset, const uint8_t* to) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
-               :
-               : "s"(lds_address(to)), "v"(offset), "s"(range)
-               : "memory");
-}
-__device__ __forceinline__ void copy_address(const void* from, const uint8_t* to) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
-               :
-               : "s"(lds_address(to)), "v"(from)
-               : "memory");
-}
-// A barrier that waits for none of the wave's work in flight; no access of
-// memory is moved over it.
-__device__ __forceinline__ void meet() {
-  asm volatile("" ::: "memory");
-  __builtin_amdgcn_s_barrier();
-  asm volatile("" ::: "memory");
 }
 
 // Copies of ROWS key rows into an image by one wave, 1 KB an instruction:

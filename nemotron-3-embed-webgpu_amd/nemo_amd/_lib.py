@@ -35,6 +35,8 @@ EXPORTED = [
     "nemo_rope_config_default", "nemo_rope_create", "nemo_rope_destroy", "nemo_rope_apply",
     "nemo_window_attention_workspace", "nemo_window_attention", "nemo_rmsnorm", "nemo_model_set_attention",
     "nemo_plan_token_states8",
+    "nemo_rope_norm_apply", "nemo_matmul8", "nemo_cache4_page_bytes", "nemo_cache4_append", "nemo_cache4_read",
+    "nemo_cache4_attention_workspace", "nemo_cache4_attention",
 ]
 
 
@@ -117,6 +119,55 @@ class NormArgs(ctypes.Structure):
     ]
 
 
+class HeadNorm(ctypes.Structure):
+    """nemo_head_norm (include/nemo.h)."""
+    _fields_ = [
+        ("q_weight", ctypes.c_void_p), ("k_weight", ctypes.c_void_p), ("q_weight_head", ctypes.c_int64),
+        ("k_weight_head", ctypes.c_int64), ("epsilon", ctypes.c_float),
+    ]
+
+
+class Matmul8Args(ctypes.Structure):
+    """nemo_matmul8_args (include/nemo.h)."""
+    _fields_ = [
+        ("type", ctypes.c_int32), ("n", ctypes.c_int32), ("k", ctypes.c_int32), ("m", ctypes.c_int64),
+        ("x", ctypes.c_void_p), ("x_scale", ctypes.c_void_p), ("w", ctypes.c_void_p), ("w_scale", ctypes.c_void_p),
+        ("bias", ctypes.c_void_p), ("y", ctypes.c_void_p), ("x_row", ctypes.c_int64), ("x_scale_row", ctypes.c_int64),
+        ("w_row", ctypes.c_int64), ("y_row", ctypes.c_int64),
+    ]
+
+
+class Cache4Config(ctypes.Structure):
+    """nemo_cache4_config (include/nemo.h)."""
+    _fields_ = [("kv_heads", ctypes.c_int32), ("head_dim", ctypes.c_int32), ("page", ctypes.c_int32)]
+
+
+class Cache4Pages(ctypes.Structure):
+    """nemo_cache4_pages (include/nemo.h)."""
+    _fields_ = [
+        ("count", ctypes.c_int32), ("pages", ctypes.c_int32), ("data", ctypes.c_void_p), ("table", ctypes.c_void_p),
+        ("table_row", ctypes.c_int64), ("kv_len", ctypes.c_void_p),
+    ]
+
+
+class Cache4Rows(ctypes.Structure):
+    """nemo_cache4_rows (include/nemo.h)."""
+    _fields_ = [
+        ("type", ctypes.c_int32), ("rows", ctypes.c_int64), ("q_start", ctypes.c_void_p),
+        ("positions", ctypes.c_void_p), ("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("k_row", ctypes.c_int64),
+        ("k_head", ctypes.c_int64), ("v_row", ctypes.c_int64), ("v_head", ctypes.c_int64),
+    ]
+
+
+class Cache4Queries(ctypes.Structure):
+    """nemo_cache4_queries (include/nemo.h)."""
+    _fields_ = [
+        ("q_rows", ctypes.c_int64), ("max_kv", ctypes.c_int64), ("q_start", ctypes.c_void_p), ("q", ctypes.c_void_p),
+        ("out", ctypes.c_void_p), ("q_row", ctypes.c_int64), ("q_head", ctypes.c_int64), ("out_row", ctypes.c_int64),
+        ("out_head", ctypes.c_int64), ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t),
+    ]
+
+
 _lib = None
 
 
@@ -174,6 +225,18 @@ def load() -> ctypes.CDLL:
         "nemo_rmsnorm": (i32, [vp, ctypes.POINTER(NormArgs), vp]),
         "nemo_model_set_attention": (i32, [vp, ctypes.POINTER(ModelAttention)]),
         "nemo_plan_token_states8": (i32, [vp, i32, i32, vp, vp, ctypes.c_int64, i64p, vp]),
+        "nemo_rope_norm_apply": (i32, [vp, i32, ctypes.POINTER(RopeHeads), ctypes.POINTER(RopeHeads),
+                                       ctypes.POINTER(HeadNorm), ctypes.c_int64, vp, ctypes.c_int64, vp]),
+        "nemo_matmul8": (i32, [vp, ctypes.POINTER(Matmul8Args), vp]),
+        "nemo_cache4_page_bytes": (i32, [ctypes.POINTER(Cache4Config), ctypes.POINTER(sz)]),
+        "nemo_cache4_append": (i32, [vp, ctypes.POINTER(Cache4Config), ctypes.POINTER(Cache4Pages),
+                                     ctypes.POINTER(Cache4Rows), vp, vp]),
+        "nemo_cache4_read": (i32, [vp, ctypes.POINTER(Cache4Config), ctypes.POINTER(Cache4Pages),
+                                   ctypes.POINTER(Cache4Rows), vp]),
+        "nemo_cache4_attention_workspace": (i32, [ctypes.POINTER(AttentionConfig), i32, ctypes.c_int64,
+                                                  ctypes.c_int64, ctypes.POINTER(sz)]),
+        "nemo_cache4_attention": (i32, [vp, ctypes.POINTER(Cache4Config), ctypes.POINTER(AttentionConfig),
+                                        ctypes.POINTER(Cache4Pages), ctypes.POINTER(Cache4Queries), vp]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(L, name)

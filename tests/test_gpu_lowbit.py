@@ -1,0 +1,769 @@
+"""The low-bit operators of an attention block (nemo_amd.operators) against
+their definitions in 64 bits: norms of heads with their rotation, products of
+8-bit rows, a paged cache of 4-bit floats and attention over it."""
+import math
+
+import pytest
+import torch
+
+import lowbit_refs as lref
+import operator_refs as ref
+from nemo_amd import operators as ops
+
+pytestmark = pytest.mark.gpu
+
+CODE = {torch.float16: ops.TYPE_F16, torch.bfloat16: ops.TYPE_BF16, torch.float32: ops.TYPE_F32}
+F16, BF16, F32 = torch.float16, torch.bfloat16, torch.float32
+
+
+def rand(seed, *shape, dtype=F32):
+    g = torch.Generator().manual_seed(seed)
+    return torch.randn(*shape, generator=g).to(dtype)
+
+
+def stream():
+    return torch.cuda.current_stream().cuda_stream
+
+
+def close(got, want, tol, what=""):
+    off = (got.double().cpu() - want).abs() - tol
+    if not off.numel():
+        return
+    assert not torch.isnan(off).any(), f"{what}: NaN"
+    assert off.max() <= 0, f"{what}: {int((off > 0).sum())} of {off.numel()} outside, by up to {float(off.max())}"
+
+
+def side(t):
+    return t.data_ptr(), t.stride(0), t.stride(1)
+
+
+# ---- norms of heads with their rotation -------------------------------------------
+
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
+@pytest.mark.parametrize("half", [False, True])
+@pytest.mark.parametrize("rows,heads,kv,d,rotary", [
+    (1, 32, 8, 128, 0),
+    (515, 40, 0, 64, 64),       # no keys
+    (37, 6, 2, 96, 40),         # part of the head; half of 20 values is no whole vector of 16-bit ones
+    (700, 5, 5, 80, 32),
+    (601, 3, 1, 256, 96),
+    (9, 3, 1, 10, 6),           # no vector fits
+    (5, 1, 1, 2, 2),            # one pair
+    (66, 3, 2, 1024, 1000),     # the widest heads
+    (3, 2, 1, 1022, 1022),
+    (4, 2, 1, 514, 6),
+])
+def test_norm_of_heads(torch_cuda, dtype, half, rows, heads, kv, d, rotary):
+    rope = ops.Rope(ops.rope_config(d, rotary_dim=rotary, theta=1e4, magnitude=1.25,
+                                    layout=ops.ROPE_HALF if half else ops.ROPE_INTERLEAVED))
+    freq = ref.rope_frequencies(rotary or d, 1e4)
+    q, k = rand(1, rows, heads, d, dtype=dtype), rand(2, rows, kv, d, dtype=dtype)
+    qw, kw = 1 + rand(3, d) / 4, 1 + rand(4, kv, d) / 4  # keys: a weight a head
+    pos = torch.randint(-50, 1 << 22, (rows,), generator=torch.Generator().manual_seed(3))
+    dq, dk, dqw, dkw, dpos = (t.cuda() for t in (q, k, qw, kw, pos))
+    oq, ok = torch.full_like(dq, math.nan), torch.full_like(dk, math.nan)
+    rope.norm_apply(CODE[dtype], ops.rope_heads(dq.data_ptr(), oq.data_ptr(), heads, d),
+                    ops.rope_heads(dk.data_ptr(), ok.data_ptr(), kv, d) if kv else None,
+                    ops.head_norm(dqw.data_ptr(), dkw.data_ptr(), 1e-3, k_weight_head=d), rows, dpos.data_ptr(),
+                    stream=stream())
+    torch.cuda.synchronize()
+    for got, x, w in ((oq, q, qw), (ok, k, kw)):
+        y, tol = lref.head_norm(x, w, 1e-3, pos, freq, half, 1.25)
+        close(got, y, tol + ref.HALF[dtype] * y.abs() + ref.TINY[dtype])
+
+
+@pytest.mark.parametrize("half", [False, True])
+@pytest.mark.parametrize("shift,pad", [(0, 0), (1, 0), (2, 6), (4, 4)])
+def test_norm_of_heads_in_place(torch_cuda, half, shift, pad):
+    """Query and key heads where they stand in rows of a projection; value
+    heads, other rows and the space between stay. Shifted rows fit narrower
+    vectors, by one element none."""
+    d, H, K, rows = 64, 6, 2, 41
+    width = (H + 2 * K) * d + pad
+    rope = ops.Rope(ops.rope_config(d, theta=1e4, layout=ops.ROPE_HALF if half else ops.ROPE_INTERLEAVED))
+    freq = ref.rope_frequencies(d, 1e4)
+    flat = rand(5, rows * width + 8, dtype=F16)
+    dev = flat.cuda()
+    x = dev.data_ptr() + 2 * shift
+    rope.norm_apply(ops.TYPE_F16, ops.rope_heads(x, x, H, d, x_row=width),
+                    ops.rope_heads(x + 2 * H * d, x + 2 * H * d, K, d, x_row=width), ops.head_norm(), rows - 1,
+                    base=1000, stream=stream())
+    torch.cuda.synchronize()
+    got = dev.cpu()
+    before, after = (t[shift:shift + rows * width].view(rows, width) for t in (flat, got))
+    heads = (H + K) * d
+    y, tol = lref.head_norm(before[:-1, :heads].reshape(rows - 1, H + K, d), None, 1e-5, torch.arange(rows - 1) + 1000,
+                            freq, half, 1.0)
+    close(after[:-1, :heads].reshape(rows - 1, H + K, d), y, tol + ref.HALF[F16] * y.abs() + ref.TINY[F16])
+    assert torch.equal(after[:, heads:], before[:, heads:]) and torch.equal(after[-1], before[-1])
+    assert torch.equal(got[:shift], flat[:shift]) and torch.equal(got[shift + rows * width:], flat[shift + rows * width:])
+
+
+def test_norm_of_zeros_nan_and_nothing(torch_cuda):
+    """A head of zeros stays zeros with an epsilon; a NaN spoils its own head
+    only; no rows and no heads are no work."""
+    rope = ops.Rope(ops.rope_config(64))
+    x = rand(6, 5, 4, 64, dtype=BF16)
+    x[1, 2] = 0
+    x[3, 0, 17] = math.nan
+    dx = x.cuda()
+    dy = torch.zeros_like(dx)
+    heads = ops.rope_heads(dx.data_ptr(), dy.data_ptr(), 4, 64)
+    rope.norm_apply(ops.TYPE_BF16, heads, None, ops.head_norm(), 0, stream=stream())
+    rope.norm_apply(ops.TYPE_BF16, ops.rope_heads(0, 0, 0, 64), None, ops.head_norm(), 5, stream=stream())
+    torch.cuda.synchronize()
+    assert not dy.any()
+    rope.norm_apply(ops.TYPE_BF16, heads, None, ops.head_norm(), 5, stream=stream())
+    torch.cuda.synchronize()
+    got = dy.cpu()
+    assert not got[1, 2].any() and torch.isnan(got[3, 0]).all()
+    keep = torch.ones(5, 4, dtype=torch.bool)
+    keep[3, 0] = False
+    assert torch.isfinite(got[keep]).all()
+
+
+# ---- products of 8-bit rows --------------------------------------------------------
+
+def rows8(seed, rows, k, low=-127):
+    g = torch.Generator().manual_seed(seed)
+    pad = (k + 15) // 16 * 16
+    return torch.randint(low, 128, (rows, pad), generator=g, dtype=torch.int8), torch.rand(rows, generator=g) / 100 + 1e-4
+
+
+def matmul(dtype, m, n, k, bias=False, y_pad=0, shift=0, low=-127):
+    x, xs = rows8(m + k, m, k, low)
+    w, ws = rows8(n + 7 * k, n, k, low)
+    b = rand(9, n) * 10 if bias else None
+    dx, dxs, dw, dws = (t.cuda() for t in (x, xs, w, ws))
+    db = b.cuda() if bias else None
+    out = torch.full((m * (n + y_pad) + shift + 8,), 7.0, dtype=dtype, device="cuda")
+    ops.Matmul8().run(ops.matmul8_args(CODE[dtype], m, n, k, dx.data_ptr(), dxs.data_ptr(), dw.data_ptr(), dws.data_ptr(),
+                                       out.data_ptr() + shift * out.element_size(), db.data_ptr() if bias else 0,
+                                       y_row=n + y_pad), stream=stream())
+    torch.cuda.synchronize()
+    flat = out.cpu()
+    y = flat[shift:shift + m * (n + y_pad)].view(m, n + y_pad)
+    close(y[:, :n], *lref.matmul8(x[:, :k], xs, w[:, :k], ws, b, dtype))
+    assert (y[:, n:] == 7.0).all() and (flat[:shift] == 7.0).all() and (flat[shift + m * (n + y_pad):] == 7.0).all()
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
+@pytest.mark.parametrize("m", [1, 5, 16, 17, 33, 64, 65, 77, 129, 300])
+@pytest.mark.parametrize("n,k,bias", [(128, 256, False), (200, 1000, True), (17, 48, False), (333, 1, True),
+                                      (130, 127, False)])
+def test_matmul8(torch_cuda, dtype, m, n, k, bias):
+    matmul(dtype, m, n, k, bias)
+
+
+@pytest.mark.parametrize("m,n,k", [(1, 1, 1), (1, 4096, 2048), (3, 1, 6144), (64, 48, 131071), (2, 3, 0), (70, 5, 0),
+                                   (200, 40, 20011)])
+def test_matmul8_sizes(torch_cuda, m, n, k):
+    """Single values, the longest rows (with the largest products: sums up to
+    2^31), and none."""
+    matmul(F32, m, n, k, True, low=-128)
+
+
+@pytest.mark.parametrize("m,n,k", [(4096, 4096, 300), (4099, 4101, 128), (2100, 8190, 640)])
+def test_matmul8_large_tiles(torch_cuda, m, n, k):
+    matmul(F16, m, n, k)
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("y_pad,shift", [(0, 1), (3, 0), (4, 2), (5, 3)])
+@pytest.mark.parametrize("m", [3, 100])
+def test_matmul8_output_layouts(torch_cuda, dtype, y_pad, shift, m):
+    """Rows and addresses that fit no vector; what is beside them stays."""
+    matmul(dtype, m, 68, 64, True, y_pad, shift)
+
+
+@pytest.mark.parametrize("m", [3, 70, 600])
+def test_matmul8_of_a_norm(torch_cuda, m):
+    """Rows and scales as nemo_rmsnorm writes them beside each other in wider
+    buffers; the row's end behind k holds what was there."""
+    hidden, n = 328, 96
+    x = rand(20, m, hidden, dtype=F16)
+    dx = x.cuda()
+    y8 = torch.full((m, 352), 99, dtype=torch.int8, device="cuda")
+    scales = torch.zeros(m, 3, dtype=torch.float32, device="cuda")
+    ops.RmsNorm().run(ops.norm_args(ops.TYPE_F16, m, hidden, dx.data_ptr(), d_y8=y8.data_ptr(), y8_row=352,
+                                    d_scales=scales.data_ptr(), scales_row=3), stream=stream())
+    w, ws = rows8(21, n, hidden)
+    dw, dws = w.cuda(), ws.cuda()
+    y = torch.empty(m, n, dtype=F16, device="cuda")
+    ops.Matmul8().run(ops.matmul8_args(ops.TYPE_F16, m, n, hidden, y8.data_ptr(), scales.data_ptr(), dw.data_ptr(),
+                                       dws.data_ptr(), y.data_ptr(), x_row=352, x_scale_row=3), stream=stream())
+    torch.cuda.synchronize()
+    assert (y8[:, hidden:] == 99).all()
+    close(y, *lref.matmul8(y8[:, :hidden].cpu(), scales[:, 0].cpu(), w[:, :hidden], ws, None, F16))
+
+
+def test_matmul8_at_the_end_of_a_buffer(torch_cuda):
+    """The last row ends with its k bytes: the rest of its 16 is not there."""
+    for m, n in ((2, 3), (80, 90)):
+        k = 37
+        x, xs = rows8(30, m, k)
+        w, ws = rows8(31, n, k)
+        flat = [torch.cat([t[:-1].flatten(), t[-1, :k]]).cuda() for t in (x, w)]
+        dxs, dws = xs.cuda(), ws.cuda()
+        y = torch.empty(m, n, device="cuda")
+        ops.Matmul8().run(ops.matmul8_args(ops.TYPE_F32, m, n, k, flat[0].data_ptr(), dxs.data_ptr(),
+                                           flat[1].data_ptr(), dws.data_ptr(), y.data_ptr()), stream=stream())
+        torch.cuda.synchronize()
+        close(y, *lref.matmul8(x[:, :k], xs, w[:, :k], ws, None, F32))
+
+
+# ---- the cache -----------------------------------------------------------------------
+
+def ints(*values, dtype=torch.int32):
+    return torch.tensor(values, dtype=dtype).cuda()
+
+
+class Pages:
+    """A cache of zeros on the device with its pages in random order."""
+
+    def __init__(self, heads, dim, page, kv_lens, room=0, fill=0):
+        self.heads, self.dim, self.page, self.kv_lens = heads, dim, page, list(kv_lens)
+        self.cache = ops.Cache4(ops.cache4_config(heads, dim, page))
+        per = [(n + page - 1) // page for n in kv_lens]
+        self.count = sum(per) + 2
+        order = torch.randperm(self.count, generator=torch.Generator().manual_seed(sum(kv_lens)))
+        self.table = torch.full((len(per), max(per + [1]) + room), -1, dtype=torch.int32)
+        at = 0
+        for b, n in enumerate(per):
+            self.table[b, :n] = order[at:at + n]
+            at += n
+        self.data = torch.full((self.count, self.cache.page_bytes), fill, dtype=torch.uint8, device="cuda")
+        self.upload()
+
+    def upload(self):
+        self.d_table, self.d_len = self.table.cuda(), ints(*self.kv_lens)
+        self.pages = ops.cache4_pages(len(self.kv_lens), self.count, self.data.data_ptr(), self.d_table.data_ptr(),
+                                      self.table.shape[1], self.d_len.data_ptr())
+
+    def put(self, b, kc, ks, vc, vs):
+        """Request b's tokens from codes and scales."""
+        n = (kc.shape[0] + self.page - 1) // self.page * self.page
+        whole = [torch.cat([t, torch.zeros(n - t.shape[0], *t.shape[1:], dtype=torch.uint8)]) for t in (kc, ks, vc, vs)]
+        self.data[self.table[b, :n // self.page].long().cuda()] = lref.pack_pages(*whole, self.page).cuda()
+
+
+def row_tokens(q_lens, kv_lens):
+    return torch.cat([torch.arange(m - n, m) for n, m in zip(q_lens, kv_lens)])
+
+
+def starts(q_lens):
+    return ints(*([0] + torch.tensor(q_lens).cumsum(0).tolist()))
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
+@pytest.mark.parametrize("heads,dim,page,q_lens,kv_lens", [
+    (1, 64, 32, [1], [1]),
+    (2, 128, 32, [5, 0, 1, 40], [5, 7, 64, 77]),
+    (3, 64, 64, [130, 3], [130, 70]),
+    (8, 128, 128, [1] * 70, [i * 3 + 1 for i in range(70)]),  # more requests than a wave has lanes
+    (5, 128, 256, [31], [300]),
+])
+def test_append_writes_the_documented_bytes(torch_cuda, dtype, heads, dim, page, q_lens, kv_lens):
+    """Without a rotation: each code is the nearest of the exact value, each
+    byte in its place, no other byte changed; read gives the values back."""
+    rows = sum(q_lens)
+    kv = (rand(1, rows, 2 * heads, dim) * torch.exp2(rand(2, rows, 2 * heads, 1) * 2)).to(dtype)
+    kv[rows // 2, 0, :32] = 0  # a block of zeros
+    pages = Pages(heads, dim, page, kv_lens, fill=0xa5)
+    before = pages.data.cpu()
+    dkv, start = kv.cuda(), starts(q_lens)
+    k, v = dkv[:, :heads], dkv[:, heads:]
+    pages.cache.append(pages.pages, ops.cache4_rows(CODE[dtype], rows, start.data_ptr(), side(k), side(v)), stream=stream())
+    out = torch.full((rows, 2 * heads, dim), math.nan, device="cuda")
+    pages.cache.read(pages.pages, ops.cache4_rows(ops.TYPE_F32, rows, start.data_ptr(), side(out[:, :heads]),
+                                                  side(out[:, heads:])), stream=stream())
+    torch.cuda.synchronize()
+    codes, scales, _ = lref.encode4(kv.double())
+    want = lref.decode4(codes, scales)
+    assert torch.equal(out.cpu().double(), want)
+    # the bytes: a cache of 0xa5 whose appended tokens hold the codes
+    token, b = row_tokens(q_lens, kv_lens), torch.repeat_interleave(torch.arange(len(q_lens)), torch.tensor(q_lens))
+    expect = before.clone()
+    for at in range(0, rows, max(1, rows // 40)):
+        i = int(token[at]) % page
+        p = int(pages.table[b[at], int(token[at]) // page])
+        kc, ks, vc, vs = (torch.zeros(page, heads, n, dtype=torch.uint8) for n in (dim, dim // 32, dim, dim // 32))
+        kc[i], ks[i], vc[i], vs[i] = codes[at, :heads], scales[at, :heads], codes[at, heads:], scales[at, heads:]
+        bytes_ = lref.pack_pages(kc, ks, vc, vs, page)[0]
+        mark = [torch.zeros_like(t) for t in (kc, ks, vc, vs)]
+        for t, full in zip(mark, (15, 255, 15, 255)):
+            t[i] = full
+        mask = lref.pack_pages(*mark, page)[0] != 0
+        got = pages.data[p].cpu()
+        assert torch.equal(got[mask], bytes_[mask])
+        expect[p][mask] = got[mask]
+    unused = [p for p in range(pages.count) if p not in set(pages.table.flatten().tolist())]
+    assert torch.equal(pages.data.cpu()[unused], before[unused])
+    if rows <= 40:
+        assert torch.equal(pages.data.cpu(), expect)
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("half", [False, True])
+@pytest.mark.parametrize("rotary", [0, 40, 2])
+@pytest.mark.parametrize("given", [False, True])
+def test_append_turns_keys(torch_cuda, dtype, dim, half, rotary, given):
+    """Codes are those of the rotation in 64 bits; only where that lies within
+    2^-32 of a border of two codes may it be the other one."""
+    heads, q_lens, kv_lens = 2, [70, 1, 33], [70, 5001, 90]
+    rows = sum(q_lens)
+    rope = ops.Rope(ops.rope_config(dim, rotary_dim=rotary, theta=1e5, scaling=ops.ROPE_YARN, factor=4.0,
+                                    layout=ops.ROPE_HALF if half else ops.ROPE_INTERLEAVED, magnitude=0.75))
+    freq = ref.rope_frequencies(rotary or dim, 1e5, "yarn", factor=4.0)
+    k, v = rand(3, rows, heads, dim, dtype=dtype), rand(4, rows, heads, dim, dtype=dtype)
+    pos = torch.randint(-9, 1 << 20, (rows,), generator=torch.Generator().manual_seed(8)) if given else row_tokens(q_lens, kv_lens)
+    pages = Pages(heads, dim, 64, kv_lens)
+    dk, dv, dpos, start = k.cuda(), v.cuda(), pos.cuda(), starts(q_lens)
+    pages.cache.append(pages.pages, ops.cache4_rows(CODE[dtype], rows, start.data_ptr(), side(dk), side(dv),
+                                                    dpos.data_ptr() if given else 0), rope, stream=stream())
+    out = torch.empty(2, rows, heads, dim, device="cuda")
+    pages.cache.read(pages.pages, ops.cache4_rows(ops.TYPE_F32, rows, start.data_ptr(), side(out[0]), side(out[1])),
+                     stream=stream())
+    torch.cuda.synchronize()
+    assert torch.equal(dk.cpu(), k)
+    turned = lref.turn(k.double(), pos, freq, half, 0.75)
+    for got, x in ((out[0], turned), (out[1], v.double())):
+        codes, scales, margin = lref.encode4(x)
+        differ = got.cpu().double() != lref.decode4(codes, scales)
+        assert not (differ & (margin > 2.0 ** -32)).any()
+
+
+def test_append_of_values_at_the_ends(torch_cuda):
+    """Ties, the largest and the smallest values, infinities and NaN."""
+    x = torch.zeros(4, 1, 64)
+    x[0, 0, :14] = torch.tensor([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0, -0.25, -0.75, -1.25, -1.75, -2.5, -5.0, 7.0])
+    x[0, 0, 32:34] = torch.tensor([7.0000005, 6.5])  # just above 7: the next power of two
+    x[1, 0, :32] = torch.tensor([3.4028234663852886e38, -3.0e38] * 16)
+    x[1, 0, 32:] = torch.tensor([1e-45, -3e-40] * 16)
+    x[2, 0, 3], x[2, 0, 40] = math.inf, math.nan
+    x[2, 0, 4], x[2, 0, 41] = 1.0, 1.0
+    x[3, 0, :32] = 2.0 ** -127
+    pages = Pages(1, 64, 32, [4])
+    dx, start = x.cuda(), starts([4])
+    pages.cache.append(pages.pages, ops.cache4_rows(ops.TYPE_F32, 4, start.data_ptr(), side(dx), side(dx)), stream=stream())
+    out = torch.zeros(2, 4, 1, 64, device="cuda")
+    pages.cache.read(pages.pages, ops.cache4_rows(ops.TYPE_F32, 4, start.data_ptr(), side(out[0]), side(out[1])), stream=stream())
+    torch.cuda.synchronize()
+    codes, scales, _ = lref.encode4(x.double())
+    want = lref.decode4(codes, scales)
+    for got in out.cpu():
+        assert torch.isnan(got[2]).all()
+        for i in (0, 1, 3):
+            assert torch.equal(got[i].double(), want[i].float().double()), i
+    assert want[0, 0, :14].tolist() == [0, 1, 1, 2, 2, 4, 4, -0.0, -1, -1, -2, -2, -4, 6] and want[0, 0, 32:34].tolist() == [8, 6]
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_read_of_every_code_and_scale(torch_cuda, dtype, dim):
+    """All bytes that a cache may hold, appended or not."""
+    codes = torch.arange(256 * dim).view(256, 1, dim).remainder(16).to(torch.uint8)
+    codes[1::2] = codes[1::2].flip(-1)
+    scales = torch.arange(256, dtype=torch.uint8).view(256, 1, 1).expand(256, 1, dim // 32).contiguous()
+    pages = Pages(1, dim, 32, [256])
+    pages.put(0, codes, scales, codes.flip(-1), scales)
+    out = torch.zeros(2, 256, 1, dim + 3, dtype=dtype, device="cuda")  # rows that no vector fits
+    start = starts([256])
+    pages.cache.read(pages.pages, ops.cache4_rows(CODE[dtype], 256, start.data_ptr(), side(out[0]), side(out[1])), stream=stream())
+    torch.cuda.synchronize()
+    for got, c in ((out[0], codes), (out[1], codes.flip(-1))):
+        want = lref.decode4(c, scales).to(dtype)
+        assert torch.equal(torch.isnan(got[..., :dim].cpu()), torch.isnan(want))
+        assert torch.equal(torch.nan_to_num(got[..., :dim].cpu()), torch.nan_to_num(want))
+        assert not got[..., dim:].any()
+
+
+def test_rows_and_pages_that_are_not_there(torch_cuda):
+    """Rows outside the requests, before token 0, in pages outside the buffer
+    or past the table's row: not written, read as zeros or not at all."""
+    heads, dim, page = 2, 64, 32
+    pages = Pages(heads, dim, page, [70, 40, 33])
+    pages.table[0, 1] = pages.count  # tokens 32 .. 63 of request 0
+    pages.table[1, 0] = -5
+    pages.kv_lens = [70, 40, 100]  # request 2: more than its row of the table (3 pages) holds
+    pages.upload()
+    # rows 0, 1: no request's; request 0: 70 rows, 1: 50 rows for 40 tokens, 2: 10 rows, of which 4 past the table; 3 more
+    start, rows = ints(2, 72, 122, 132), 135
+    k, v = rand(1, rows, heads, dim, dtype=F16).cuda(), rand(2, rows, heads, dim, dtype=F16).cuda()
+    pages.table[2, 2] = next(p for p in range(pages.count) if p not in set(pages.table.flatten().tolist()))
+    pages.upload()
+    before = pages.data.clone()
+    pages.cache.append(pages.pages, ops.cache4_rows(ops.TYPE_F16, rows, start.data_ptr(), side(k), side(v)), stream=stream())
+    out = torch.full((2, rows, heads, dim), 7.0, device="cuda")
+    pages.cache.read(pages.pages, ops.cache4_rows(ops.TYPE_F32, rows, start.data_ptr(), side(out[0]), side(out[1])), stream=stream())
+    torch.cuda.synchronize()
+    for got, x in ((out[0].cpu(), k), (out[1].cpu(), v)):
+        codes, scales, _ = lref.encode4(x.cpu().double())
+        want = lref.decode4(codes, scales).float()
+        want[:2] = 7.0
+        want[2 + 32:2 + 64] = 0  # page outside
+        want[72:82] = 7.0  # before token 0
+        want[82:114] = 0  # page -5
+        want[128:132] = 0  # past the table
+        want[132:] = 7.0
+        assert torch.equal(got, want)
+    used = set(pages.table.flatten().tolist())
+    unused = [p for p in range(pages.count) if p not in used]
+    assert torch.equal(pages.data[unused], before[unused])
+
+
+def test_append_strides(torch_cuda):
+    """Rows whose heads lie apart, between other values, and head-major, at
+    addresses that fit no vector."""
+    heads, dim, rows = 3, 128, 21
+    for dtype in (F16, F32):
+        flat = rand(5, heads * rows * (dim + 5) * 2 + 1, dtype=dtype).cuda()[1:]
+        k = torch.as_strided(flat, (rows, heads, dim), (dim + 5, rows * (dim + 5), 1))
+        v = torch.as_strided(flat, (rows, heads, dim), (heads * (dim + 5), dim + 5, 1), heads * rows * (dim + 5) + 1)
+        pages = Pages(heads, dim, 32, [rows])
+        start = starts([rows])
+        pages.cache.append(pages.pages, ops.cache4_rows(CODE[dtype], rows, start.data_ptr(), side(k), side(v)), stream=stream())
+        out = torch.zeros(2, rows, heads, dim, device="cuda")
+        pages.cache.read(pages.pages, ops.cache4_rows(ops.TYPE_F32, rows, start.data_ptr(), side(out[0]), side(out[1])),
+                         stream=stream())
+        torch.cuda.synchronize()
+        for got, x in ((out[0], k), (out[1], v)):
+            codes, scales, _ = lref.encode4(x.cpu().double())
+            assert torch.equal(got.cpu().double(), lref.decode4(codes, scales))
+
+
+# ---- attention over the cache --------------------------------------------------------
+
+def random_cache(seed, kv_lens, heads, dim, page, spread=2):
+    """Codes and powers of two around 1 for each request."""
+    g = torch.Generator().manual_seed(seed)
+    pages, held = Pages(heads, dim, page, kv_lens, fill=0xff), []  # where no token is, all is NaN
+    for b, n in enumerate(kv_lens):
+        kc, vc = (torch.randint(0, 16, (n, heads, dim), generator=g).to(torch.uint8) for _ in range(2))
+        ks, vs = (torch.randint(126 - spread, 126 + spread, (n, heads, dim // 32), generator=g).to(torch.uint8) for _ in range(2))
+        if n:
+            whole = (n + page - 1) // page * page
+            full = []
+            for t, fill in ((kc, 15), (ks, 255), (vc, 15), (vs, 255)):
+                full.append(torch.cat([t, torch.full((whole - n, *t.shape[1:]), fill, dtype=torch.uint8)]))
+            pages.data[pages.table[b, :whole // page].long().cuda()] = lref.pack_pages(*full, page).cuda()
+        held.append((lref.decode4(kc, ks), lref.decode4(vc, vs)))
+    return pages, held
+
+
+def attend(pages, q, q_lens, left=-1, right=0, sinks=0, scale=0.0, workspace=True, max_kv=None, out=None, start=None):
+    H = q.shape[1]
+    config = ops.attention_config(H, pages.heads, pages.dim, CODE[q.dtype], left=left, right=right, sinks=sinks, scale=scale)
+    dq = q.cuda()
+    out = torch.full_like(dq, math.nan) if out is None else out
+    start = starts(q_lens) if start is None else start
+    most = max(pages.kv_lens + [0]) if max_kv is None else max_kv
+    need = pages.cache.workspace_bytes(config, len(pages.kv_lens), q.shape[0], most) if workspace else 0
+    space = torch.full((max(need, 16),), 0xff, dtype=torch.uint8, device="cuda")
+    pages.cache.attention(config, pages.pages, ops.cache4_queries(
+        q.shape[0], most, start.data_ptr(), side(dq), side(out), space.data_ptr(), need), stream=stream())
+    torch.cuda.synchronize()
+    return out, need
+
+
+def check(out, held, q, q_lens, left=-1, right=0, sinks=0, scale=0.0):
+    row = 0
+    for (k, v), n in zip(held, q_lens):
+        want, tol = ref.attention(q[row:row + n], k, v, left, right, sinks, scale or k.shape[-1] ** -0.5)
+        close(out[row:row + n], want, tol, f"rows {row} to {row + n}")
+        row += n
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("heads,kv,page,q_lens,kv_lens,left,right,sinks", [
+    (1, 1, 32, [1], [1], -1, 0, 0),
+    (4, 1, 32, [1], [33], -1, 0, 0),
+    (8, 2, 64, [1, 1, 1], [5, 64, 200], -1, 0, 0),
+    (6, 2, 32, [1, 1], [300, 77], 40, 0, 3),       # groups of three; window and sinks inside blocks
+    (32, 1, 32, [1], [100], -1, 0, 0),             # one KV head for all: more rows than a tile of single tokens
+    (8, 2, 128, [3, 0, 5], [140, 20, 5], -1, 0, 0),
+    (3, 3, 32, [70], [70], -1, 0, 0),              # a prompt, every row another window
+    (5, 1, 64, [40, 17], [200, 17], 30, 0, 5),
+    (4, 2, 32, [33], [90], 10, 4, 40),             # sinks that overlap windows, keys behind a query
+    (2, 1, 32, [50], [20], 8, 0, 2),               # more queries than keys: rows that see nothing
+    (4, 4, 32, [2], [0], -1, -1, 0),               # no keys at all
+    (2, 1, 64, [90], [64], -1, -1, 0),             # every key
+    (7, 1, 32, [66], [130], 0, 0, 0),              # a window of one key
+])
+def test_attention(torch_cuda, dtype, dim, heads, kv, page, q_lens, kv_lens, left, right, sinks):
+    pages, held = random_cache(sum(kv_lens), kv_lens, kv, dim, page)
+    q = rand(7, sum(q_lens), heads, dim, dtype=dtype)
+    out, _ = attend(pages, q, q_lens, left, right, sinks)
+    check(out, held, q, q_lens, left, right, sinks)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("workspace", [False, True])
+@pytest.mark.parametrize("q_lens,kv_lens", [([1], [4500]), ([2, 1], [3001, 2999]), ([30], [5000])])
+def test_attention_over_long_caches(torch_cuda, dtype, dim, workspace, q_lens, kv_lens):
+    """Keys dealt out to workgroups, whose sums are joined; the workspace
+    holds NaN before."""
+    pages, held = random_cache(3, kv_lens, 2, dim, 64)
+    q = rand(8, sum(q_lens), 6, dim, dtype=dtype)
+    out, need = attend(pages, q, q_lens, workspace=workspace)
+    assert not workspace or need > 0
+    check(out, held, q, q_lens)
+
+
+@pytest.mark.parametrize("max_kv", [0, 1, 1 << 40])
+def test_max_kv_is_a_hint(torch_cuda, max_kv):
+    pages, held = random_cache(4, [700, 5], 1, 64, 32)
+    q = rand(9, 3, 2, 64, dtype=F16)
+    out, _ = attend(pages, q, [1, 2], max_kv=max_kv)
+    check(out, held, q, [1, 2])
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("where", ["keys", "values", "both"])
+@pytest.mark.parametrize("q_lens,left,right", [([1], 50, 0), ([80], 50, 0), ([80], 3, 2)])
+def test_nan_that_a_query_does_not_see(torch_cuda, dtype, where, q_lens, left, right):
+    """Blocks of NaN in some tokens: rows that see one are NaN (a key's whole
+    row, a value's 32 columns), all others what they are without."""
+    n, heads, dim = 160, 2, 128
+    pages, held = random_cache(5, [n], heads, dim, 32)
+    g = torch.Generator().manual_seed(6)
+    codes = [torch.randint(0, 16, (n, heads, dim), generator=g).to(torch.uint8) for _ in range(2)]
+    scales = [torch.randint(124, 129, (n, heads, 4), generator=g).to(torch.uint8) for _ in range(2)]
+    clean = [lref.decode4(c, s) for c, s in zip(codes, scales)]
+    spots = [(3, 0, 1), (40, 1, 0), (95, 0, 3), (130, 1, 2)]
+    for t, h, b in spots:
+        if where != "values":
+            scales[0][t, h, b] = 255
+        if where != "keys":
+            scales[1][t, h, b] = 255
+    pages.put(0, codes[0], scales[0], codes[1], scales[1])
+    q = rand(10, sum(q_lens), 6, dim, dtype=dtype)
+    out, _ = attend(pages, q, q_lens, left, right, 1)
+    out = out.cpu()
+    see = ref.visible(sum(q_lens), n, left, right, 1)
+    want, tol = ref.attention(q, clean[0], clean[1], left, right, 1, dim ** -0.5)
+    bad = torch.zeros(out.shape, dtype=torch.bool)
+    for t, h, b in spots:
+        rows = see[:, t]
+        if where != "values":
+            bad[rows, 3 * h:3 * h + 3] = True
+        if where != "keys":
+            bad[rows, 3 * h:3 * h + 3, 32 * b:32 * b + 32] = True
+    assert torch.isnan(out[bad]).all()
+    assert bad.any() or sum(q_lens) == 1
+    close(torch.where(bad, want.to(dtype), out), want, tol)
+
+
+def test_attention_leaves_other_rows(torch_cuda):
+    """Rows of out before, between and behind the requests' stay, heads may lie
+    apart, requests share pages, and entries out of order stay in the buffers."""
+    kv, heads, dim = 2, 4, 64
+    pages, held = random_cache(12, [100, 60], kv, dim, 32)
+    pages.table[1] = pages.table[0]  # the second request reads the first one's tokens
+    pages.upload()
+    q = rand(11, 12, heads, dim, dtype=F16)
+    out = torch.full((12, heads, dim + 8), 7.0, dtype=F16, device="cuda")
+    start = ints(2, 5, 9)
+    attend(pages, q, None, out=out[..., :dim], start=start)
+    got = out.cpu()
+    assert (got[:2] == 7.0).all() and (got[9:] == 7.0).all() and (got[..., dim:] == 7.0).all()
+    k, v = held[0]
+    check(got[2:5, :, :dim], [(k, v)], q[2:5], [3])
+    check(got[5:9, :, :dim], [(k[:60], v[:60])], q[5:9], [4])
+    for bad in (ints(5, 2, 9), ints(-4, 6, 1 << 30), ints(40, 50, 60), ints(9, 9, 0)):
+        attend(pages, q, None, out=out[..., :dim], start=bad)
+    assert (out[..., dim:] == 7.0).all()
+
+
+def test_pages_that_are_not_there_hold_no_keys(torch_cuda):
+    kv, heads, dim = 1, 4, 128
+    pages, held = random_cache(13, [200, 64], kv, dim, 32)
+    pages.table[0, 2], pages.table[0, 4] = pages.count + 7, -1
+    pages.table[1, 0] = pages.table[1, 1] = 1 << 30  # none of its keys are there
+    pages.kv_lens = [1 << 29, 64]  # past the table: only its keys are there
+    pages.upload()
+    room = pages.table.shape[1] * 32
+    q = rand(12, 3, heads, dim, dtype=BF16)
+    # request 0 has `room` keys, of which some pages are missing
+    out, _ = attend(pages, q, [2, 1], right=-1)
+    k, v = held[0]
+    there = torch.ones(room, dtype=torch.bool)
+    there[64:96] = there[128:160] = False
+    there[200:] = False
+    # (keys behind 200 are NaN in their page: they are seen, so both rows are NaN)
+    assert torch.isnan(out[:2]).all() and not out[2].any()
+    pages.kv_lens = [200, 64]
+    pages.upload()
+    out, _ = attend(pages, q, [2, 1], right=-1)
+    check(out[:2], [(k[there[:200]], v[there[:200]])], q[:2], [2], right=-1)
+    assert not out[2].any()
+
+
+def test_a_strong_key_and_a_long_even_cache(torch_cuda):
+    """f16's probabilities far below the largest keep their share: one key some
+    17 above 4000 even ones."""
+    n, dim = 4000, 64
+    kc, vc = torch.zeros(n, 1, dim, dtype=torch.uint8), torch.full((n, 1, dim), 2, dtype=torch.uint8)
+    kc[0], vc[0] = 2, 10  # ones; minus one as the value
+    scales = torch.full((n, 1, 2), 127, dtype=torch.uint8)
+    pages = Pages(1, dim, 64, [n])
+    pages.put(0, kc, scales, vc, scales)
+    held = [(lref.decode4(kc, scales), lref.decode4(vc, scales))]
+    for dtype in (F16, BF16):
+        q = torch.full((1, 1, dim), 17.0 / 8, dtype=dtype)
+        out, _ = attend(pages, q, [1])
+        check(out, held, q, [1])
+
+
+@pytest.mark.parametrize("scale", [0.01, 3.0])
+def test_attention_scale(torch_cuda, scale):
+    pages, held = random_cache(14, [150], 2, 128, 64)
+    q = rand(13, 20, 4, 128, dtype=F16)
+    out, _ = attend(pages, q, [20], scale=scale)
+    check(out, held, q, [20], scale=scale)
+
+
+def test_values_of_all_sizes(torch_cuda):
+    """Powers of two over the type's range, in one cache."""
+    for dtype, spread in ((F16, 12), (BF16, 40)):
+        pages, held = random_cache(15, [300], 1, 64, 32, spread)
+        held = [(k, v) for k, v in held]
+        q = (rand(14, 2, 2, 64) * 2.0 ** -spread).to(dtype)
+        out, _ = attend(pages, q, [2])
+        check(out, held, q, [2])
+
+
+# ---- as they are used together ---------------------------------------------------------
+
+def test_an_attention_block_in_few_bits(torch_cuda):
+    """Hidden rows of three requests through norm, 8-bit projection, norms of
+    heads and rotation, cache and attention: a prompt first, then two tokens one by
+    one from a captured graph, each replay checked against the definitions on
+    the values that the step before it left."""
+    hidden, H, K, D, page, dtype = 256, 8, 2, 64, 32, F16
+    lens = [40, 7, 65]
+    width = (H + 2 * K) * D
+    w, ws = rows8(40, width, hidden)
+    dw, dws = w.cuda(), ws.cuda()
+    qw, kw = (1 + rand(41, D) / 8), (1 + rand(42, D) / 8)
+    dqw, dkw = qw.cuda(), kw.cuda()
+    rope = ops.Rope(ops.rope_config(D, theta=1e4))
+    freq = ref.rope_frequencies(D, 1e4)
+    pages = Pages(K, D, page, [n + 2 for n in lens], room=1)
+    config = ops.attention_config(H, K, D, CODE[dtype], right=0)
+    norm, matmul8 = ops.RmsNorm(), ops.Matmul8()
+
+    class Step:
+        def __init__(self, q_lens):
+            rows = sum(q_lens)
+            self.q_lens, self.rows = q_lens, rows
+            self.x = torch.zeros(rows, hidden, dtype=dtype, device="cuda")
+            self.y8 = torch.zeros(rows, hidden, dtype=torch.int8, device="cuda")
+            self.scales = torch.zeros(rows, device="cuda")
+            self.qkv = torch.zeros(rows, H + 2 * K, D, dtype=dtype, device="cuda")
+            self.out = torch.zeros(rows, H, D, dtype=dtype, device="cuda")
+            self.pos = torch.zeros(rows, dtype=torch.int64, device="cuda")
+            self.start = starts(q_lens)
+
+        def run(self):
+            s, code, size = stream(), CODE[dtype], 2
+            norm.run(ops.norm_args(code, self.rows, hidden, self.x.data_ptr(), d_y8=self.y8.data_ptr(),
+                                   d_scales=self.scales.data_ptr()), stream=s)
+            matmul8.run(ops.matmul8_args(code, self.rows, width, hidden, self.y8.data_ptr(), self.scales.data_ptr(),
+                                         dw.data_ptr(), dws.data_ptr(), self.qkv.data_ptr()), stream=s)
+            q, k = self.qkv.data_ptr(), self.qkv.data_ptr() + size * H * D
+            rope.norm_apply(code, ops.rope_heads(q, q, H, D, x_row=width), ops.rope_heads(k, k, K, D, x_row=width),
+                            ops.head_norm(dqw.data_ptr(), dkw.data_ptr()), self.rows, self.pos.data_ptr(), stream=s)
+            heads = [(self.qkv.data_ptr() + size * at * D, width, D) for at in (H, H + K)]
+            pages.cache.append(pages.pages, ops.cache4_rows(code, self.rows, self.start.data_ptr(), *heads), stream=s)
+            pages.cache.attention(config, pages.pages, ops.cache4_queries(
+                self.rows, max(lens) + 2, self.start.data_ptr(), (q, width, D), side(self.out)), stream=s)
+
+        def check(self, cached, seed):
+            """From each operator's own input as the device has it."""
+            x = rand(seed, self.rows, hidden, dtype=dtype)
+            y = lref.matmul8(self.y8.cpu(), self.scales.cpu(), w[:, :hidden], ws, None, dtype)[0].view(self.rows, -1, D)
+            _, plain, rel = ref.norm(x, None, None, 1e-5)
+            close(self.y8.cpu().double() * self.scales.cpu().double()[:, None], plain,
+                  self.scales.cpu().double()[:, None] * (0.5 + 2.0 ** -20) + (rel + 2.0 ** -21) * plain.abs())
+            qkv = self.qkv.cpu()
+            close(qkv[:, H + K:], y[:, H + K:], ref.HALF[dtype] * y[:, H + K:].abs() * 1.01 + ref.TINY[dtype])
+            for sl, weight in ((slice(0, H), qw), (slice(H, H + K), kw)):
+                # the product's rounding to f16 goes into the norm: 2^-11 of each value, of
+                # which the root of the mean square has as much again
+                want, tol = lref.head_norm(y[:, sl], weight, 1e-5, self.pos.cpu(), freq, False, 1.0)
+                pair = torch.stack([want[..., 0::2], want[..., 1::2]], -1).norm(dim=-1).repeat_interleave(2, -1)
+                close(qkv[:, sl], want, tol + 2.0 ** -11 * want.abs() + 2 * 2.0 ** -11 * 1.01 * 2 ** 0.5 * pair + ref.TINY[dtype])
+            row = 0
+            for b, n in enumerate(self.q_lens):
+                new = qkv[row:row + n].double()
+                for i, sl in enumerate((slice(H, H + K), slice(H + K, None))):
+                    codes, scales, _ = lref.encode4(new[:, sl])
+                    cached[b][i] = torch.cat([cached[b][i], lref.decode4(codes, scales)])
+                want, tol = ref.attention(qkv[row:row + n, :H], *cached[b], -1, 0, 0, D ** -0.5)
+                close(self.out[row:row + n], want, tol)
+                row += n
+
+    cached = [[torch.zeros(0, K, D, dtype=torch.float64) for _ in range(2)] for _ in lens]
+    prompt = Step(lens)
+    prompt.x.copy_(rand(50, sum(lens), hidden, dtype=dtype))
+    prompt.pos.copy_(row_tokens(lens, lens))
+    pages.d_len.copy_(ints(*lens))
+    prompt.run()
+    torch.cuda.synchronize()
+    prompt.check(cached, 50)
+    step = Step([1, 1, 1])
+    graph = torch.cuda.CUDAGraph()
+    pages.d_len.copy_(ints(*[n + 1 for n in lens]))
+    step.run()  # (its tokens are written over by the first replay)
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        step.run()
+    for i in range(2):
+        now = [n + i + 1 for n in lens]
+        step.x.copy_(rand(60 + i, 3, hidden, dtype=dtype))
+        step.pos.copy_(torch.tensor(now) - 1)
+        pages.d_len.copy_(ints(*now))
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        step.check(cached, 60 + i)
+
+
+def test_calls_on_two_streams(torch_cuda):
+    """Two caches and products at once on streams of their own equal the calls
+    one after the other."""
+    a, held_a = random_cache(21, [900], 2, 64, 32)
+    b, held_b = random_cache(22, [1100], 2, 64, 32)
+    q = rand(23, 4, 4, 64, dtype=F16)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    outs = []
+    dq = q.cuda()
+    config = ops.attention_config(4, 2, 64, ops.TYPE_F16, right=0)
+    start = starts([4])
+    torch.cuda.synchronize()
+    for s, pages in zip(streams, (a, b)):
+        with torch.cuda.stream(s):
+            need = pages.cache.workspace_bytes(config, 1, 4, 1100)
+            space = torch.empty(max(need, 16), dtype=torch.uint8, device="cuda")
+            out = torch.empty_like(dq)
+            for _ in range(5):
+                pages.cache.attention(config, pages.pages, ops.cache4_queries(
+                    4, 1100, start.data_ptr(), side(dq), side(out), space.data_ptr(), need), stream=s.cuda_stream)
+            outs.append((out, space))
+    torch.cuda.synchronize()
+    check(outs[0][0], held_a, q, [4])
+    check(outs[1][0], held_b, q, [4])
+
+
+def test_results_do_not_change_from_call_to_call(torch_cuda):
+    """The same call again gives the same bits."""
+    pages, _ = random_cache(31, [3000, 200], 2, 128, 64)
+    q = rand(32, 40, 8, 128, dtype=BF16)
+    first, _ = attend(pages, q, [20, 20])
+    for _ in range(3):
+        again, _ = attend(pages, q, [20, 20])
+        assert torch.equal(first, again)
