@@ -2,15 +2,23 @@
 // it again, for gfx950 (include/nemo.h nemo_cache4_append, nemo_cache4_read).
 //
 // 32 values x of a head share the power of two 2^s, the smallest with max |x|
-// <= 7 2^s, and become the nearest E2M1 float of x / 2^s. Next to a border
-// between two codes the 32-bit roundings of a rotation decide wrongly a few
-// times in a million values, so angles, rotation and the division by 2^s (exact)
-// are in 64 bits, and the one rounding is that to the code.
+// <= 7 2^s, and become the nearest E2M1 float of x / 2^s, which is exact in 32
+// bits. A rotation is not: an angle's remainder and its sine in 32 bits, the
+// factor and two products leave it some 10 2^-24 of |a| + |b| off, and next to a
+// border between codes it is decided wrongly a few times in a million values.
+// So both ends of 2^-20 around it are coded, and where two codes or powers differ
+// (about one in fifty) the wave takes the rotation again in 64 bits.
+//
+// Bound by memory and by its instructions in equal parts: 31846 tokens of 8 KV
+// heads of 128 f16, 165 MB of rows and codes, 54 us (3.1 TB/s) to append and 31
+// (5.3 TB/s) to read. In 64 bits throughout they took 103 and, with codes taken
+// apart bit by bit, 40.
 //
 // A wave takes a token. Lane l computes the angle of pair l, which the 16 lanes
 // of a head pick up from LDS: lane l's head is l / 16 (of four at a time), its
 // values D / 16 (l % 16) .., one 4-byte piece of codes for heads of 128.
 #include <algorithm>
+#include <type_traits>
 
 #include "nemo_cache4.h"
 
@@ -22,6 +30,7 @@ struct RowsArgs {
   nemo_cache4_rows r;
   Cache4 c;
   RopeAngles angles;  // turns null: keys as they are
+  bool wide;          // a lane's D / 16 values may be read and written as one vector
 };
 
 // A row's token of its request, none (-1) for rows before the first request and
@@ -53,12 +62,22 @@ struct Token {
   }
 };
 
-// The largest magnitude's bits of 32 values, of which a lane has those of `m`.
+// The largest bits of LANES lanes side by side.
 template <int LANES>
-__device__ __forceinline__ uint64_t block_max(uint64_t m) {
+__device__ __forceinline__ uint32_t lanes_max(uint32_t v) {
+  auto moved = [](uint32_t x, auto to) {
+    return (uint32_t)__builtin_amdgcn_mov_dpp((int)x, decltype(to)::value, 15, 15, false);
+  };
+  v = max(v, moved(v, std::integral_constant<int, 0xb1>{}));                           // neighbours
+  v = max(v, moved(v, std::integral_constant<int, 0x4e>{}));                           // pairs of a quad
+  if constexpr (LANES > 4) v = max(v, moved(v, std::integral_constant<int, 0x141>{}));  // quads of 8
+  return v;
+}
+template <int LANES>
+__device__ __forceinline__ uint64_t lanes_max(uint64_t v) {
 #pragma unroll
-  for (int o = 1; o < LANES; o *= 2) m = max(m, (uint64_t)__shfl_xor((unsigned long long)m, o, 64));
-  return m;
+  for (int o = 1; o < LANES; o *= 2) v = max(v, (uint64_t)__shfl_xor((unsigned long long)v, o, 64));
+  return v;
 }
 
 // v in 32 bits, with its last bit set where they do not hold it, rounded to zero
@@ -70,121 +89,261 @@ __device__ __forceinline__ float odd(double v) {
   return __uint_as_float(bits);
 }
 
-// Codes of N values, two a byte, and the scale byte of the 32 that a lane's are
-// part of.
+// Codes of N values, two a byte.
 template <int N>
-__device__ __forceinline__ uint32_t encode(const double (&x)[N], int* scale) {
-  uint64_t m = 0;
-#pragma unroll
-  for (int i = 0; i < N; ++i) m = max(m, __builtin_bit_cast(uint64_t, x[i]) & 0x7fffffffffffffffull);
-  m = block_max<32 / N>(m);
-  const int e = (int)(m >> 52);
-  if (e == 0x7ff) {  // an infinity or a NaN
-    *scale = 255;
-    return 0;
+__device__ __forceinline__ uint32_t codes_of(const float (&u)[N]) {
+  uint32_t c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(0u, u[0], u[1], 1.0f, 0);
+  c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, u[2], u[3], 1.0f, 1);
+  if constexpr (N == 8) {
+    c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, u[4], u[5], 1.0f, 2);
+    c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, u[6], u[7], 1.0f, 3);
   }
-  // m = 2^(e - 1023) (1 + f): at most 7 2^s = 1.75 2^(s + 2)
-  const int s = min(max(e - 1023 - 2 + ((m & 0xfffffffffffffull) > 0xc000000000000ull), -126), 125);
-  *scale = s + 127;
-  const double inv = __builtin_bit_cast(double, (uint64_t)(1023 - s) << 52);
-  uint32_t codes = 0;
-#pragma unroll
-  for (int i = 0; i < N; i += 2) {
-    const float a = odd(x[i] * inv), b = odd(x[i + 1] * inv);
-    switch (i / 2) {
-      case 0: codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, a, b, 1.0f, 0); break;
-      case 1: codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, a, b, 1.0f, 1); break;
-      case 2: codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, a, b, 1.0f, 2); break;
-      default: codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, a, b, 1.0f, 3); break;
-    }
-  }
-  return codes;
+  return c;
 }
 
-template <typename T, int D>
+// s of 32 values whose largest has exponent e, biased by `bias`, and a fraction of
+// 1.75 or less or more: 2^(e - bias) (1 + f) is at most 7 2^s = 1.75 2^(s + 2).
+__device__ __forceinline__ int power_of(int e, int bias, bool more) { return min(max(e - bias - 2 + more, -126), 125); }
+__device__ __forceinline__ float inverse(int s) { return __uint_as_float((uint32_t)(127 - s) << 23); }
+
+template <typename T, int N>
+__device__ __forceinline__ void load_piece(const T* x, bool wide, T (&v)[N]) {
+  typedef T vec __attribute__((ext_vector_type(N)));
+  if (wide) {
+    const vec t = *(const vec*)x;
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = t[i];
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = x[i];
+  }
+}
+
+// How keys are turned: not; neighbouring pairs; halves of which a lane has values
+// of one, their partners one vector; halves in any other way.
+enum Turn { kPlain, kPairs, kHalves, kHalvesAny };
+
+template <typename T, int D, Turn TURN>
 __global__ __launch_bounds__(256) void cache4_append_kernel(RowsArgs a) {
   typedef Cache4Head<D> Head;
-  constexpr int N = D / 16;
-  __shared__ double2 angles[4][64];  // cosine and sine
+  constexpr int N = D / 16, LANES = 32 / N;
+  __shared__ float2 angles[4][64];  // cosine and sine
+  __shared__ double2 angles64[4][64];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t t = (int64_t)blockIdx.x * 4 + wave;
   if (t >= a.r.rows) return;  // (no barrier follows: a wave has its own angles)
-  const Token token(a.c, a.r.q_start, a.r.rows, t);
-  if (token.at < 0 || token.page < 0) return;
-  const int in = token.at & ((1 << a.c.shift) - 1), n = lane & 15, pairs = a.angles.rotary / 2;
-  const bool turn = a.angles.turns != nullptr, half = a.angles.half;
-  if (turn) {
-    if (lane < pairs) {
-      double p = (double)(a.r.positions ? a.r.positions[t] : (int64_t)token.at) * a.angles.turns[lane];
-      p -= rint(p);
-      double s, c;
-      sincospi(2.0 * p, &s, &c);
-      angles[wave][lane] = make_double2(c * a.angles.magnitude, s * a.angles.magnitude);
-    }
-    __builtin_amdgcn_wave_barrier();
-  }
-  for (int h = lane >> 4; h < 2 * a.c.kv_heads; h += 4) {
-    const bool value = h >= a.c.kv_heads;
-    const int kvh = value ? h - a.c.kv_heads : h;
-    const T* x = value ? (const T*)a.r.v + t * a.r.v_row + kvh * a.r.v_head
-                       : (const T*)a.r.k + t * a.r.k_row + kvh * a.r.k_head;
-    double v[N];
-#pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = (double)(float)x[N * n + i];
-    if (!value && turn) {
+  const int n = lane & 15, pairs = TURN == kPlain ? 0 : a.angles.rotary / 2, heads = a.c.kv_heads;
+  // Of a turned value: whether it is its pair's second, and where the first is.
+  auto second = [&](int d) { return TURN == kPairs ? d & 1 : (TURN == kHalves ? N * n : d) >= pairs; };
+  auto pair_of = [&](int d) { return TURN == kPairs ? d >> 1 : second(d) ? d - pairs : d; };
+  struct Piece {
+    T x[N], other[N];
+  };
+  auto load_key = [&](Piece& p, int h) {
+    if (h >= heads) return;
+    const T* x = (const T*)a.r.k + t * a.r.k_row + h * a.r.k_head;
+    load_piece<T, N>(x + N * n, a.wide, p.x);
+    if constexpr (TURN == kHalves) {
+      if (N * n < 2 * pairs) load_piece<T, N>(x + (N * n >= pairs ? N * n - pairs : N * n + pairs), true, p.other);
+    } else if constexpr (TURN == kHalvesAny) {
 #pragma unroll
       for (int i = 0; i < N; ++i) {
         const int d = N * n + i;
-        if (d >= 2 * pairs) continue;
-        const bool second = half ? d >= pairs : d & 1;
-        const int pair = half ? (second ? d - pairs : d) : d >> 1;
-        const double other = (double)(float)x[half ? (second ? d - pairs : d + pairs) : d ^ 1];
-        const double2 cs = angles[wave][pair];
-        v[i] = second ? other * cs.y + v[i] * cs.x : v[i] * cs.x - other * cs.y;
+        if (d < 2 * pairs) p.other[i] = x[d >= pairs ? d - pairs : d + pairs];
       }
     }
-    int scale;
-    const uint32_t codes = encode(v, &scale);
-    uint8_t* const to = a.c.data + a.c.head<D>(token.page, kvh);
-    uint8_t* const at = to + (value ? Head::v_codes(a.c.shift, in, n) : Head::k_codes(in) + n * Head::kScales);
+  };
+  auto load_value = [&](Piece& p, int h) {
+    if (h < heads) load_piece<T, N>((const T*)a.r.v + t * a.r.v_row + h * a.r.v_head + N * n, a.wide, p.x);
+  };
+  Piece key, value, next;
+  load_key(key, lane >> 4);
+  load_value(value, lane >> 4);
+  const Token token(a.c, a.r.q_start, a.r.rows, t);
+  if (token.at < 0 || token.page < 0) return;
+  const int in = token.at & ((1 << a.c.shift) - 1);
+  double turns = 0;  // whole turns of pair `lane`, less the whole ones
+  if constexpr (TURN != kPlain) {
+    if (lane < pairs) {
+      turns = (double)(a.r.positions ? a.r.positions[t] : (int64_t)token.at) * a.angles.turns[lane];
+      turns -= rint(turns);
+      float s, c;
+      sincospif(2.0f * (float)turns, &s, &c);
+      angles[wave][lane] = make_float2(c * a.angles.magnitude, s * a.angles.magnitude);
+    }
+    __builtin_amdgcn_wave_barrier();
+  }
+  uint8_t* to = a.c.data + a.c.head<D>(token.page, lane >> 4);
+  const int64_t step = a.c.head<D>(0, 4);
+  auto write = [&](bool is_value, uint32_t codes, int s, bool bad) {
+    uint8_t* const at = to + (is_value ? Head::v_codes(a.c.shift, in, n) : Head::k_codes(in) + n * Head::kScales);
+    if (bad) codes = 0;
     if constexpr (D == 128) *(uint32_t*)at = codes;
     else *(uint16_t*)at = (uint16_t)codes;
-    if (n % (32 / N) == 0) to[Head::scale(a.c.shift, value, in, n / (32 / N))] = (uint8_t)scale;
+    if (n % LANES == 0) to[Head::scale(a.c.shift, is_value, in, n / LANES)] = bad ? 255 : (uint8_t)(s + 127);
+  };
+  auto power32 = [](uint32_t bits) { return power_of((int)(bits >> 23), 127, (bits & 0x7fffff) > 0x600000); };
+  // Values that are in 32 bits what they are.
+  auto plain = [&](const Piece& piece, bool is_value, bool real) {
+    float u[N];
+    uint32_t peak = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      u[i] = real ? (float)piece.x[i] : 0.f;
+      peak = max(peak, __float_as_uint(u[i]) & 0x7fffffffu);
+    }
+    peak = lanes_max<LANES>(peak);
+    const int s = power32(peak);
+    const float inv = inverse(s);
+#pragma unroll
+    for (int i = 0; i < N; ++i) u[i] *= inv;
+    const uint32_t codes = codes_of<N>(u);
+    if (real) write(is_value, codes, s, peak >= 0x7f800000u);
+  };
+  bool exact = false;  // whether angles64 holds the token's
+  auto turned = [&](const Piece& piece, bool real) {
+    float u[N], most[N], peak = 0.f, error = 0.f, finite = 0.f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int d = N * n + i;
+      const float own = real ? (float)piece.x[i] : 0.f;
+      u[i] = own;
+      most[i] = 0.f;
+      if (d < 2 * pairs) {
+        const float other = real ? (float)(TURN == kPairs ? piece.x[i ^ 1] : piece.other[i]) : 0.f;
+        const float2 cs = angles[wave][pair_of(d)];
+        u[i] = fmaf(other, second(d) ? cs.y : -cs.y, own * cs.x);
+        most[i] = fabsf(own) + fabsf(other);
+      }
+      peak = fmaxf(peak, fabsf(u[i]));
+      error = fmaxf(error, most[i]);
+      finite = fmaf(u[i], 0.f, finite);
+    }
+    const float rel = fabsf(a.angles.magnitude) * 0x1p-20f;
+    peak = __uint_as_float(lanes_max<LANES>(__float_as_uint(peak)));
+    error = __uint_as_float(lanes_max<LANES>(__float_as_uint(error))) * rel;
+    int s = power32(__float_as_uint(peak));
+    const float inv = inverse(s), off = rel * inv;
+    float low[N], high[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const float v = u[i] * inv;
+      low[i] = fmaf(-most[i], off, v);
+      high[i] = fmaf(most[i], off, v);
+    }
+    uint32_t codes = codes_of<N>(low);
+    bool unsure = codes != codes_of<N>(high) || !(peak + error < INFINITY) || finite != 0.f ||
+                  power32(__float_as_uint(fmaxf(peak - error, 0.f))) != power32(__float_as_uint(peak + error));
+    bool bad = false;
+    if (__builtin_amdgcn_ballot_w64(unsure)) {
+      asm volatile("");  // keeps the rare path a branch
+      if (!exact) {
+        if (lane < pairs) {
+          double s64, c64;
+          sincospi(2.0 * turns, &s64, &c64);
+          angles64[wave][lane] = make_double2(c64 * a.angles.magnitude, s64 * a.angles.magnitude);
+        }
+        __builtin_amdgcn_wave_barrier();
+        exact = true;
+      }
+      double v[N];
+      uint64_t m = 0;
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const int d = N * n + i;
+        const double own = real ? (double)(float)piece.x[i] : 0.0;
+        v[i] = own;
+        if (d < 2 * pairs) {
+          const double other = real ? (double)(float)(TURN == kPairs ? piece.x[i ^ 1] : piece.other[i]) : 0.0;
+          const double2 cs = angles64[wave][pair_of(d)];
+          v[i] = fma(other, second(d) ? cs.y : -cs.y, own * cs.x);
+        }
+        m = max(m, __builtin_bit_cast(uint64_t, v[i]) & 0x7fffffffffffffffull);
+      }
+      m = lanes_max<LANES>(m);
+      bad = m >= 0x7ff0000000000000ull;
+      s = power_of((int)(m >> 52), 1023, (m & 0xfffffffffffffull) > 0xc000000000000ull);
+      const double inv64 = __builtin_bit_cast(double, (uint64_t)(1023 - s) << 52);
+#pragma unroll
+      for (int i = 0; i < N; ++i) u[i] = odd(v[i] * inv64);
+      codes = codes_of<N>(u);
+    }
+    if (real) write(false, codes, s, bad);
+  };
+  // (All lanes stay in the loops: a wave votes, and lanes exchange. Those past the last head write nothing.)
+  for (int h0 = 0, h = lane >> 4; h0 < heads; h0 += 4, h += 4) {
+    load_key(next, h + 4);
+    if constexpr (TURN == kPlain) plain(key, false, h < heads);
+    else turned(key, h < heads);
+    key = next;
+    load_value(next, h + 4);
+    plain(value, true, h < heads);
+    value = next;
+    to += step;
   }
 }
 
-// Values of a lane's piece: N codes of one scale.
+// Pairs of values by the conversions from 4 bits.
+template <typename T, int B>
+__device__ __forceinline__ void decode(uint32_t codes, float scale, T& a, T& b) {
+  if constexpr (std::is_same<T, float>::value) {
+    const float2v v = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, scale, B);
+    a = v[0], b = v[1];
+  } else if constexpr (std::is_same<T, half_t>::value) {
+    const half2v v = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, scale, B);
+    a = v[0], b = v[1];
+  } else {
+    const auto v = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, B);
+    a = v[0], b = v[1];
+  }
+}
+
 template <typename T, int D>
 __global__ __launch_bounds__(256) void cache4_read_kernel(RowsArgs a) {
   typedef Cache4Head<D> Head;
   constexpr int N = D / 16;
+  typedef T vec __attribute__((ext_vector_type(N)));
   const int lane = threadIdx.x & 63;
   const int64_t t = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (t >= a.r.rows) return;
   const Token token(a.c, a.r.q_start, a.r.rows, t);
   if (token.at < 0) return;
   const int in = token.at & ((1 << a.c.shift) - 1), n = lane & 15;
+#pragma unroll 2
   for (int h = lane >> 4; h < 2 * a.c.kv_heads; h += 4) {
     const bool value = h >= a.c.kv_heads;
     const int kvh = value ? h - a.c.kv_heads : h;
-    uint32_t codes = 0;
-    int scale = 127;
+    uint32_t codes = 0, scale = 127;
     if (token.page >= 0) {
       const uint8_t* const from = a.c.data + a.c.head<D>(token.page, kvh);
       const uint8_t* const at = from + (value ? Head::v_codes(a.c.shift, in, n) : Head::k_codes(in) + n * Head::kScales);
       codes = D == 128 ? *(const uint32_t*)at : *(const uint16_t*)at;
       scale = from[Head::scale(a.c.shift, value, in, n / (32 / N))];
     }
-    T* x = value ? (T*)a.r.v + t * a.r.v_row + kvh * a.r.v_head : (T*)a.r.k + t * a.r.k_row + kvh * a.r.k_head;
+    const float power = __uint_as_float(scale << 23);
+    T v[N];
+    decode<T, 0>(codes, power, v[0], v[1]);
+    decode<T, 1>(codes, power, v[2], v[3]);
+    if constexpr (N == 8) {
+      decode<T, 2>(codes, power, v[4], v[5]);
+      decode<T, 3>(codes, power, v[6], v[7]);
+    }
+    T* x = (value ? (T*)a.r.v + t * a.r.v_row + kvh * a.r.v_head : (T*)a.r.k + t * a.r.k_row + kvh * a.r.k_head) + N * n;
+    if (a.wide) {
+      vec w;
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int code = codes >> (4 * i) & 15, e = code >> 1 & 3, f = code & 1;
-      // 2^(e - 1) (1 + f / 2), or f / 2
-      const float m = e ? (float)(2 + f) * (float)(1 << e) * 0.25f : 0.5f * f;
-      const float p = scale == 255 ? __uint_as_float(0x7fc00000u) : ldexpf(m, scale - 127);
-      x[N * n + i] = (T)(code & 8 ? -p : p);
+      for (int i = 0; i < N; ++i) w[i] = v[i];
+      *(vec*)x = w;
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i) x[i] = v[i];
     }
   }
+}
+
+bool wide(const nemo_cache4_config& c, const nemo_cache4_rows& r) {
+  const int n = c.head_dim / 16, bytes = n * (r.type == NEMO_TYPE_F32 ? 4 : 2);
+  return (((uintptr_t)r.k | (uintptr_t)r.v) & (bytes - 1)) == 0 && (r.k_row | r.k_head | r.v_row | r.v_head) % n == 0;
 }
 
 template <typename Launch>
@@ -204,16 +363,22 @@ hipError_t by_type(int type, int head_dim, Launch&& launch) {
 hipError_t launch_cache4_append(const nemo_cache4_config& c, const nemo_cache4_pages& p, const nemo_cache4_rows& r,
                                 const RopeAngles* angles, hipStream_t stream) {
   if (p.count == 0 || r.rows == 0) return hipSuccess;
-  const RowsArgs a{r, Cache4(c, p), angles ? *angles : RopeAngles{}};
+  const RowsArgs a{r, Cache4(c, p), angles ? *angles : RopeAngles{}, wide(c, r)};
   return by_type(r.type, c.head_dim, [&](auto t, auto d) {
-    cache4_append_kernel<decltype(t), decltype(d)::value><<<(unsigned)((r.rows + 3) / 4), 256, 0, stream>>>(a);
+    const unsigned grid = (unsigned)((r.rows + 3) / 4);
+    typedef decltype(t) T;
+    constexpr int D = decltype(d)::value;
+    if (!angles) cache4_append_kernel<T, D, kPlain><<<grid, 256, 0, stream>>>(a);
+    else if (!angles->half) cache4_append_kernel<T, D, kPairs><<<grid, 256, 0, stream>>>(a);
+    else if (a.wide && angles->rotary / 2 % (D / 16) == 0) cache4_append_kernel<T, D, kHalves><<<grid, 256, 0, stream>>>(a);
+    else cache4_append_kernel<T, D, kHalvesAny><<<grid, 256, 0, stream>>>(a);
   });
 }
 
 hipError_t launch_cache4_read(const nemo_cache4_config& c, const nemo_cache4_pages& p, const nemo_cache4_rows& r,
                               hipStream_t stream) {
   if (p.count == 0 || r.rows == 0) return hipSuccess;
-  const RowsArgs a{r, Cache4(c, p), RopeAngles{}};
+  const RowsArgs a{r, Cache4(c, p), RopeAngles{}, wide(c, r)};
   return by_type(r.type, c.head_dim, [&](auto t, auto d) {
     cache4_read_kernel<decltype(t), decltype(d)::value><<<(unsigned)((r.rows + 3) / 4), 256, 0, stream>>>(a);
   });

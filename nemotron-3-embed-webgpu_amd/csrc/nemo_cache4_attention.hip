@@ -167,7 +167,16 @@ struct Rows {
   typedef Mma<T> M;
   typedef typename M::frag frag;
   typedef typename M::pair pair;
-  frag q[QT][W];
+  // Queries: in registers for one tile of rows, else an LDS image of rows, 16-byte
+  // chunk c of row r at c ^ (r % (D / 8)).
+  static constexpr bool IMAGE = QT > 1;
+  frag held[IMAGE ? 1 : W];
+  const uint8_t* image;
+  __device__ __forceinline__ frag query(int i, int w, int lane) const {
+    if constexpr (!IMAGE) return held[w];
+    const int row = lane & 15, chunk = W * (lane >> 4) + w;
+    return *(const frag*)(image + (16 * i + row) * 2 * D + 16 * (chunk ^ (row & (D / 8 - 1))));
+  }
   float4v o[QT][C];
   float m[QT], l[QT];  // reference and sum of the probabilities
 
@@ -240,27 +249,32 @@ __device__ __forceinline__ uint32_t seen8(int j, const Seen& s, int sinks) {
 }
 
 // One block of 32 keys from key j0 on. `hide`: not every row sees all of them;
-// `seen`: what its lane's rows see. `careful`: values that are not finite are met
+// `seen`: what its lane's rows see. CAREFUL: values that are not finite are met
 // one by one, those of keys that a row does not see left out.
-template <typename T, int D, int QT>
-__device__ __forceinline__ void attend(Rows<T, D, QT>& a, const Raw<D>& raw, float scale2, bool hide, bool careful,
+template <bool CAREFUL, typename T, int D, int QT>
+__device__ __forceinline__ void attend(Rows<T, D, QT>& a, const Raw<D>& raw, float scale2, bool hide,
                                        const uint32_t (&seen)[QT], uint32_t any) {
   constexpr int W = D / 32;
   typedef Mma<T> M;
   typedef typename M::frag frag;
   const int lane = threadIdx.x & 63;
   float4v s[QT][2];
+  const float powers[2] = {__uint_as_float((raw.k_scales[0] >> (8 * (lane & 3))) << 23),
+                           __uint_as_float((raw.k_scales[1] >> (8 * (lane & 3))) << 23)};
 #pragma unroll
-  for (int u = 0; u < 2; ++u) {
-    const float power = __uint_as_float((raw.k_scales[u] >> (8 * (lane & 3))) << 23);
+  for (int w = 0; w < W; ++w) {
+    frag q[QT];
 #pragma unroll
-    for (int w = 0; w < W; ++w) {
+    for (int i = 0; i < QT; ++i) q[i] = a.query(i, w, lane);
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
       const uint32_t c = raw.k[u][w];
+      const float power = powers[u];
       const u32x4 f = {M::template decode<0>(c, power), M::template decode<1>(c, power),
                        M::template decode<2>(c, power), M::template decode<3>(c, power)};
 #pragma unroll
       for (int i = 0; i < QT; ++i)
-        s[i][u] = M::mma(__builtin_bit_cast(frag, f), a.q[i][w], w ? s[i][u] : float4v{0.f, 0.f, 0.f, 0.f});
+        s[i][u] = M::mma(__builtin_bit_cast(frag, f), q[i], w ? s[i][u] : float4v{0.f, 0.f, 0.f, 0.f});
     }
   }
   frag p[QT];
@@ -287,7 +301,7 @@ __device__ __forceinline__ void attend(Rows<T, D, QT>& a, const Raw<D>& raw, flo
     }
     a.settle(i, v, scale2, p[i]);
   }
-  if (careful) {
+  if constexpr (CAREFUL) {
     // values that are not finite: their place holds 2^-127, and the rows that see
     // one become NaN in its 32 columns
     frag bad;
@@ -343,23 +357,26 @@ __device__ __forceinline__ void attend(Rows<T, D, QT>& a, const Raw<D>& raw, flo
   }
 }
 
-// Sums of a split: the row's reference and sum, and its output values.
+// Sums of a piece of a tile's keys: the rows' references and sums, and their
+// output values.
 struct Partials {
-  float2* ml;  // [split][row], null: not split
-  float* o;    // [split][row][D]
+  float2* ml;  // [piece][row], null: not split
+  float* o;    // [piece][row][D]
   int64_t rows;
-  int splits;
+  int splits, piece;  // most pieces of a tile, and the blocks of one, more where a tile has more
+  __device__ __forceinline__ int size(int blocks) const { return max(piece, (blocks + splits - 1) / splits); }
 };
 
 // A workgroup takes 16 QT rows; its waves every WAVES-th block of keys, whose
-// sums they add in LDS. With `splits` above 1 the blocks are dealt out to that
-// many workgroups as well, whose sums a second kernel joins.
+// sums they add in LDS. Where a tile has more blocks than a piece, each piece is a
+// workgroup, and a second kernel joins their sums.
 template <typename T, int D, int QT, int WAVES>
-__global__ __launch_bounds__(64 * WAVES) void cache4_attention_kernel(AttendArgs a, Partials part) {
+__global__ __launch_bounds__(64 * WAVES, QT == 1 ? 3 : 2) void cache4_attention_kernel(AttendArgs a, Partials part) {
   constexpr int C = D / 16, W = D / 32;
   typedef typename Mma<T>::frag frag;
   __shared__ __attribute__((aligned(16))) float sums[WAVES][16][D];  // of 16 rows at a time
   __shared__ float2 ml[WAVES][16];
+  __shared__ __attribute__((aligned(16))) uint8_t queries[Rows<T, D, QT>::IMAGE ? 16 * QT * 2 * D : 16];
   const int kvh = blockIdx.x % a.c.kv_heads, tile_no = blockIdx.x / a.c.kv_heads, split = blockIdx.y;
   const Request r(a, tile_no, 16 * QT);
   if (r.i < 0) return;
@@ -370,9 +387,13 @@ __global__ __launch_bounds__(64 * WAVES) void cache4_attention_kernel(AttendArgs
   auto window = [&](int row) { return Seen(a, behind + a.query(row), r.keys); };
   const Seen first = window(row0), last = window(min(row0 + 16 * QT, rows) - 1);
   const Blocks blocks(a, first, last);
-  const int block0 = (int)((int64_t)blocks.n * split / part.splits);
-  const int block1 = (int)((int64_t)blocks.n * (split + 1) / part.splits);
+  const int size = part.size(blocks.n), block0 = size * split, block1 = min(blocks.n, block0 + size);
+  if (block0 >= blocks.n && split) return;
+  const bool whole = blocks.n <= size;  // the tile's only piece
   const int head_of = kvh * a.group;  // query head of row 0 of a query
+  auto query_at = [&](int row, int query) {
+    return (const T*)a.b.q + (int64_t)(r.q0 + query) * a.b.q_row + (int64_t)(head_of + row - query * a.group) * a.b.q_head;
+  };
   Rows<T, D, QT> acc;
   int lo[QT], hi[QT];
 #pragma unroll
@@ -381,48 +402,69 @@ __global__ __launch_bounds__(64 * WAVES) void cache4_attention_kernel(AttendArgs
     const Seen s(a, behind + query, r.keys);
     lo[i] = s.lo;
     hi[i] = s.hi;
-    const T* q = (const T*)a.b.q + (int64_t)(r.q0 + query) * a.b.q_row +
-                 (int64_t)(head_of + row - query * a.group) * a.b.q_head + h * (D / 4);
+    if constexpr (!Rows<T, D, QT>::IMAGE) {
 #pragma unroll
-    for (int w = 0; w < W; ++w) acc.q[i][w] = *(const frag*)(q + 8 * w);
+      for (int w = 0; w < W; ++w) acc.held[w] = *(const frag*)(query_at(row, query) + h * (D / 4) + 8 * w);
+    }
+  }
+  if constexpr (Rows<T, D, QT>::IMAGE) {
+    for (int at = threadIdx.x; at < 16 * QT * (D / 8); at += 64 * WAVES) {
+      const int in = at / (D / 8), chunk = at % (D / 8), row = min(row0 + in, rows - 1);
+      *(u32x4*)(queries + in * 2 * D + 16 * (chunk ^ (in & (D / 8 - 1)))) =
+          *(const u32x4*)(query_at(row, a.query(row)) + 8 * chunk);
+    }
+    acc.image = queries;
+    __syncthreads();
   }
   const int32_t* table = a.c.table + r.i * a.c.table_row;
   const int per = a.c.shift - 5;  // log2 of a page's blocks
-  // Page of the wave's block t, none (-1) past the last and where it is not there.
-  auto page_of = [&](int t) {
-    if (t >= block1) return -1;
-    const int page = __builtin_amdgcn_readfirstlane(table[blocks.block(t) >> per]);
-    return (unsigned)page < (unsigned)a.c.pages ? page : -1;
-  };
-  auto load = [&](Raw<D>& raw, int page, int t) {
-    if (page < 0) return;
-    raw.load(a.c.data + a.c.head<D>(page, kvh), a.c.shift, (blocks.block(t) & ((1 << per) - 1)) << 5, lane);
-  };
-  for (int careful = 0;; ++careful) {
+  // The wave's blocks are block0 + wave + WAVES n, n < steps (none without pages); lane l
+  // has the page of the l-th of 64 steps, none (-1) where it is not there.
+  const int steps = a.c.pages ? (block1 - block0 - wave + WAVES - 1) / WAVES : 0;
+  auto attended = [&](auto careful) {
     acc.clear();
-    Raw<D> raw, next;
-    int t = block0 + wave, page = page_of(t), next_page = page_of(t + WAVES);
-    load(raw, page, t);
-    for (; t < block1; t += WAVES) {
-      load(next, next_page, t + WAVES);
-      const int after = page_of(t + 2 * WAVES);
-      if (page >= 0) {
-        const int j0 = blocks.block(t) << 5;
-        const bool hide = j0 + 32 > first.hi || (j0 < last.lo && j0 + 32 > a.sinks);
-        uint32_t seen[QT] = {}, any = 255;
-        if (hide) {
-          any = seen8(j0 + 8 * h, Seen(first.lo, last.hi), a.sinks);
-#pragma unroll
-          for (int i = 0; i < QT; ++i) seen[i] = seen8(j0 + 8 * h, Seen(lo[i], hi[i]), a.sinks);
-        }
-        attend<T, D, QT>(acc, raw, a.scale2, hide, careful, seen, any);
+    auto block_of = [&](int n) { return blocks.block(block0 + wave + WAVES * min(n, steps - 1)); };
+    int ids = 0;
+    // (Blocks past the last, and in pages that are not there, are loaded from places that are.)
+    auto load = [&](Raw<D>& raw, int n) {
+      if ((n & 63) == 0) {
+        const int page = table[block_of(n + lane) >> per];
+        ids = n + lane < steps && (unsigned)page < (unsigned)a.c.pages ? page : -1;
       }
-      raw = next;
-      page = next_page;
-      next_page = after;
+      const int page = __builtin_amdgcn_readlane(ids, n & 63);
+      raw.load(a.c.data + a.c.head<D>(max(page, 0), kvh), a.c.shift, (block_of(n) & ((1 << per) - 1)) << 5, lane);
+      return page >= 0;
+    };
+    auto step = [&](const Raw<D>& raw, int n) {
+      const int j0 = block_of(n) << 5;
+      const bool hide = j0 + 32 > first.hi || (j0 < last.lo && j0 + 32 > a.sinks);
+      uint32_t seen[QT] = {}, any = 255;
+      if (hide) {
+        any = seen8(j0 + 8 * h, Seen(first.lo, last.hi), a.sinks);
+#pragma unroll
+        for (int i = 0; i < QT; ++i) seen[i] = seen8(j0 + 8 * h, Seen(lo[i], hi[i]), a.sinks);
+      }
+      attend<decltype(careful)::value>(acc, raw, a.scale2, hide, seen, any);
+    };
+    if (steps <= 0) return;
+    // AHEAD steps are in flight behind the one that is worked on.
+    constexpr int AHEAD = QT == 1 ? 2 : 1;
+    Raw<D> raw[AHEAD + 1];
+    bool there[AHEAD + 1];
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) there[i] = load(raw[i], i);
+    for (int n = 0; n < steps; ++n) {
+      there[AHEAD] = load(raw[AHEAD], n + AHEAD);
+      if (there[0]) step(raw[0], n);
+#pragma unroll
+      for (int i = 0; i < AHEAD; ++i) {
+        raw[i] = raw[i + 1];
+        there[i] = there[i + 1];
+      }
     }
-    if (careful || !__builtin_amdgcn_ballot_w64(acc.spoilt())) break;
-  }
+  };
+  attended(std::false_type{});
+  if (__builtin_amdgcn_ballot_w64(acc.spoilt())) attended(std::true_type{});
   // The waves' sums, 16 rows at a time.
   constexpr int THREADS = 64 * WAVES, PER = 16 * D / THREADS;  // columns of a thread
   static_assert(PER >= 4 && D % PER == 0, "whole vectors of one row");
@@ -458,7 +500,7 @@ __global__ __launch_bounds__(64 * WAVES) void cache4_attention_kernel(AttendArgs
       }
     }
     const int query = a.query(at), head = head_of + at - query * a.group;
-    if (part.ml) {
+    if (!whole) {
       const int64_t to = part.rows * split + (int64_t)(r.q0 + query) * a.c.kv_heads * a.group + head;
       if (c0 == 0) part.ml[to] = make_float2(m, l);
 #pragma unroll
@@ -475,10 +517,10 @@ __global__ __launch_bounds__(64 * WAVES) void cache4_attention_kernel(AttendArgs
   }
 }
 
-// Joins the splits, at most 64: a workgroup a row. Thread (g, c) adds columns 4
-// c.. of splits g, g + G, ..., and the G sums are added in order.
+// Joins the pieces, at most 64: a workgroup a row, of tiles of `of` rows. Thread (g, c)
+// adds columns 4 c.. of pieces g, g + G, ..., and the G sums are added in order.
 template <typename T, int D>
-__global__ __launch_bounds__(256) void cache4_join_kernel(AttendArgs a, Partials part) {
+__global__ __launch_bounds__(256) void cache4_join_kernel(AttendArgs a, Partials part, int of) {
   constexpr int C = D / 4, G = 256 / C;
   __shared__ float weight[64];
   __shared__ float4v sums[G][C];
@@ -487,10 +529,15 @@ __global__ __launch_bounds__(256) void cache4_join_kernel(AttendArgs a, Partials
   if (r.i < 0) return;
   const int row = tile_no - r.tile, lane = threadIdx.x & 63;
   if ((unsigned)row >= (unsigned)(r.queries * a.group)) return;
+  const int row0 = row / of * of, behind = r.keys - r.queries;
+  const Blocks blocks(a, Seen(a, behind + a.query(row0), r.keys),
+                      Seen(a, behind + a.query(min(row0 + of, r.queries * a.group) - 1), r.keys));
+  const int size = part.size(blocks.n), pieces = (blocks.n + size - 1) / size;
+  if (pieces <= 1) return;  // the row is written
   const int i = a.query(row), head = kvh * a.group + (row - i * a.group);
   const int64_t at = (int64_t)(r.q0 + i) * a.c.kv_heads * a.group + head;
-  // every wave: lane z's split
-  const float2 ml = lane < part.splits ? part.ml[part.rows * lane + at] : make_float2(-INFINITY, 0.f);
+  // every wave: lane z's piece
+  const float2 ml = lane < pieces ? part.ml[part.rows * lane + at] : make_float2(-INFINITY, 0.f);
   float m = ml.x;
 #pragma unroll
   for (int x = 32; x > 0; x >>= 1) m = fmaxf(m, __shfl_xor(m, x, 64));
@@ -504,7 +551,7 @@ __global__ __launch_bounds__(256) void cache4_join_kernel(AttendArgs a, Partials
   const int c = threadIdx.x % C, g = threadIdx.x / C;
   float4v v = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
-  for (int z = g; z < part.splits; z += G) {
+  for (int z = g; z < pieces; z += G) {
     const float4v o = *(const float4v*)(part.o + (part.rows * z + at) * D + 4 * c);
     const float w = weight[z];
 #pragma unroll
@@ -522,17 +569,19 @@ __global__ __launch_bounds__(256) void cache4_join_kernel(AttendArgs a, Partials
 
 // Rows of a tile and how the keys are split, by a batch's sizes alone.
 struct Plan {
-  int tiles16, splits;  // rows of a tile / 16
+  int tiles16, splits, piece;  // rows of a tile / 16; most pieces of a tile, and the blocks of 32 keys of one
 };
 Plan plan_of(const nemo_attention_config& c, int count, int64_t q_rows, int64_t max_kv) {
-  if (count == 0 || q_rows == 0) return {1, 1};
+  if (count == 0 || q_rows == 0) return {1, 1, 1};
   const int64_t rows = q_rows * (c.q_heads / c.kv_heads);
   const int tiles16 = rows / count <= 16 ? 1 : 4;
   const int64_t tiles = std::max<int64_t>(rows / (16 * tiles16), count) * c.kv_heads;
   int64_t keys = max_kv;
   if (c.left >= 0 && c.right >= 0) keys = std::min(keys, (int64_t)c.left + c.right + 1 + c.sinks);
-  const int64_t splits = std::min<int64_t>({512 / tiles, keys / 1024, 64});
-  return {tiles16, (int)std::max<int64_t>(1, splits)};
+  const int64_t blocks = std::min<int64_t>(keys, 1 << 30) / 32 + 1;
+  const int64_t places = tiles16 == 1 ? 4096 : 512, least = tiles16 == 1 ? 64 : 32;
+  const int64_t piece = std::max<int64_t>({least, (blocks * tiles + places - 1) / places, (blocks + 63) / 64});
+  return {tiles16, (int)((blocks + piece - 1) / piece), (int)piece};
 }
 
 }  // namespace
@@ -556,7 +605,7 @@ hipError_t launch_cache4_attention(const nemo_cache4_config& cache, const nemo_a
   const Plan plan = plan_of(c, p.count, b.q_rows, b.max_kv);
   const int splits = b.workspace ? plan.splits : 1;
   const int64_t rows = b.q_rows * c.q_heads;
-  Partials part{nullptr, nullptr, rows, splits};
+  Partials part{nullptr, nullptr, rows, splits, plan.piece};
   if (splits > 1) {
     part.o = (float*)b.workspace;
     part.ml = (float2*)(part.o + splits * rows * c.head_dim);
@@ -567,7 +616,7 @@ hipError_t launch_cache4_attention(const nemo_cache4_config& cache, const nemo_a
     typedef decltype(type) T;
     if (plan.tiles16 == 1) cache4_attention_kernel<T, D, 1, 4><<<dim3(tiles(16), splits), 256, 0, stream>>>(a, part);
     else cache4_attention_kernel<T, D, 4, 4><<<dim3(tiles(64), splits), 256, 0, stream>>>(a, part);
-    if (splits > 1) cache4_join_kernel<T, D><<<tiles(1), 256, 0, stream>>>(a, part);
+    if (splits > 1) cache4_join_kernel<T, D><<<tiles(1), 256, 0, stream>>>(a, part, 16 * plan.tiles16);
   };
   auto typed = [&](auto type) {
     if (c.head_dim == 64) launch(type, std::integral_constant<int, 64>{});

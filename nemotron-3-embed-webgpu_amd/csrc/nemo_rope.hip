@@ -173,42 +173,53 @@ hipError_t launch_rope_type(const RopeArgs& a, hipStream_t stream) {
 // head of its token.
 // ---------------------------------------------------------------------------
 
-// E values, as one vector where the addresses allow it.
+// E values, read and written as one vector where the addresses allow it.
 template <typename T, int E, bool VECTORS>
-__device__ __forceinline__ void load_values(const T* p, float (&v)[E]) {
-  if constexpr (VECTORS && E > 1) {
-    typedef T vec __attribute__((ext_vector_type(E)));
-    const vec t = *(const vec*)p;
+struct Values {
+  typedef T vec __attribute__((ext_vector_type(E)));
+  vec v;
+  __device__ __forceinline__ void load(const T* p) {
+    if constexpr (VECTORS) {
+      v = *(const vec*)p;
+    } else {
 #pragma unroll
-    for (int e = 0; e < E; ++e) v[e] = (float)t[e];
-  } else {
-#pragma unroll
-    for (int e = 0; e < E; ++e) v[e] = (float)p[e];
+      for (int e = 0; e < E; ++e) v[e] = p[e];
+    }
   }
-}
-template <typename T, int E, bool VECTORS>
-__device__ __forceinline__ void store_values(T* p, const float (&v)[E]) {
-  if constexpr (VECTORS && E > 1) {
-    typedef T vec __attribute__((ext_vector_type(E)));
-    vec t;
+  __device__ __forceinline__ void store(T* p) const {
+    if constexpr (VECTORS) {
+      *(vec*)p = v;
+    } else {
 #pragma unroll
-    for (int e = 0; e < E; ++e) t[e] = (T)v[e];
-    *(vec*)p = t;
-  } else {
-#pragma unroll
-    for (int e = 0; e < E; ++e) p[e] = (T)v[e];
+      for (int e = 0; e < E; ++e) p[e] = v[e];
+    }
   }
+};
+
+// The sum over `lanes` (a power of two) lanes side by side.
+__device__ __forceinline__ float lanes_sum(float v, int lanes) {
+  auto moved = [](float x, auto to) {
+    return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), decltype(to)::value, 15, 15, false));
+  };
+  if (lanes > 1) v += moved(v, std::integral_constant<int, 0xb1>{});   // neighbours
+  if (lanes > 2) v += moved(v, std::integral_constant<int, 0x4e>{});   // pairs of a quad
+  if (lanes > 4) v += moved(v, std::integral_constant<int, 0x141>{});  // quads of 8, mirrored
+  if (lanes > 8) v += moved(v, std::integral_constant<int, 0x140>{});  // halves of 16, mirrored
+  if (lanes > 16) v += __shfl_xor(v, 16, 64);
+  if (lanes > 32) v += __shfl_xor(v, 32, 64);
+  return v;
 }
 
 template <typename T, int E, bool HALF, bool VECTORS, int NI>
 __global__ __launch_bounds__(256) void rope_norm_kernel(RopeArgs a, nemo_head_norm n, int lanes, int slots,
                                                         int tokens) {
   constexpr int V = HALF ? 2 : 1, C = HALF ? E : E / 2;  // vectors and pairs of an item
-  const int per = lanes * slots, l = threadIdx.x % lanes, slot = threadIdx.x % per / lanes;
+  const int per = lanes * slots, l = threadIdx.x % lanes;
   const int64_t t = (int64_t)blockIdx.x * tokens + threadIdx.x / per;
   if ((int)threadIdx.x >= tokens * per || t >= a.rows) return;  // (a head's lanes together)
-  const int heads = a.q.heads + a.k.heads, items = a.head_dim / (V * E);
-  const double p = rope_position(a, t);
+  const int slot = blockIdx.y * slots + threadIdx.x % per / lanes;
+  slots *= gridDim.y;
+  const int items = a.head_dim / (V * E);
   int at[NI][V];
   bool real[NI], turned[NI];
   float2 cs[NI][C];
@@ -219,65 +230,100 @@ __global__ __launch_bounds__(256) void rope_norm_kernel(RopeArgs a, nemo_head_no
     turned[i] = real[i] && (HALF ? item < a.pairs / E : item < 2 * a.pairs / E);
     at[i][0] = HALF && !turned[i] ? 2 * E * item : E * item;  // (2 pairs + 2 E (item - pairs / E))
     if constexpr (HALF) at[i][1] = turned[i] ? a.pairs + E * item : at[i][0] + E;
+    if (!real[i]) {
 #pragma unroll
-    for (int c = 0; c < C; ++c) cs[i][c] = turned[i] ? rope_angle(a, C * item + c, p) : make_float2(1.f, 0.f);
+      for (int v = 0; v < V; ++v) at[i][v] = 0;
+    }
   }
-  float w[NI][V][E];
-  int weights = -1;  // whose weights w holds
-  for (int h = slot; h < heads; h += slots) {
-    const T* x;
-    T* y;
-    rope_head(a, t, h, x, y);
-    const bool key = h >= a.q.heads;
-    const int64_t stride = key ? n.k_weight_head : n.q_weight_head;
-    if (weights != (int)key || stride) {
-      weights = key;
-      const float* from = key ? n.k_weight : n.q_weight;
-      if (from) from += stride * (key ? h - a.q.heads : h);
+  bool angles = false;
+  const float inv = 1.0f / a.head_dim;
+  typedef Values<T, E, VECTORS> vec;
+  // Every `slots`-th head of q or k from `first` on; the next one's values are on their way.
+  auto turn = [&](const nemo_rope_heads& s, const float* weight, int64_t weight_head, int first) {
+    if (first >= s.heads) return;
+    const T* x = (const T*)s.x + t * s.x_row + first * s.x_head;
+    T* y = (T*)s.y + t * s.y_row + first * s.y_head;
+    vec now[NI][V], next[NI][V];
+    auto load = [&](vec (&to)[NI][V]) {
+#pragma unroll
+      for (int i = 0; i < NI; ++i)
+#pragma unroll
+        for (int v = 0; v < V; ++v) to[i][v].load(x + at[i][v]);
+    };
+    load(now);
+    float w[NI][V][E];
+    auto weights = [&](int h) {
 #pragma unroll
       for (int i = 0; i < NI; ++i)
 #pragma unroll
         for (int v = 0; v < V; ++v)
 #pragma unroll
-          for (int e = 0; e < E; ++e) w[i][v][e] = from && real[i] ? from[at[i][v] + e] : 1.f;
+          for (int e = 0; e < E; ++e) w[i][v][e] = weight ? weight[h * weight_head + at[i][v] + e] : 1.f;
+    };
+    weights(first);
+    if (!angles) {
+      const double p = rope_position(a, t);
+#pragma unroll
+      for (int i = 0; i < NI; ++i)
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+          cs[i][c] = turned[i] ? rope_angle(a, C * (l + lanes * i) + c, p) : make_float2(1.f, 0.f);
+      angles = true;
     }
-    float r[NI][V][E], sum = 0.f;
-#pragma unroll
-    for (int i = 0; i < NI; ++i)
-#pragma unroll
-      for (int v = 0; v < V; ++v) {
-        if (real[i]) {
-          load_values<T, E, VECTORS>(x + at[i][v], r[i][v]);
-        } else {
-#pragma unroll
-          for (int e = 0; e < E; ++e) r[i][v][e] = 0.f;
-        }
-#pragma unroll
-        for (int e = 0; e < E; ++e) sum = fmaf(r[i][v][e], r[i][v][e], sum);
+    for (int h = first; h < s.heads; h += slots) {
+      if (h + slots < s.heads) {
+        x += slots * s.x_head;
+        load(next);
       }
-    for (int o = lanes >> 1; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
-    const float f = 1.0f / sqrtf(sum / a.head_dim + n.epsilon);
+      float r[NI][V][E], sum = 0.f;
 #pragma unroll
-    for (int i = 0; i < NI; ++i) {
-      if (!real[i]) continue;
+      for (int i = 0; i < NI; ++i)
 #pragma unroll
-      for (int v = 0; v < V; ++v)
+        for (int v = 0; v < V; ++v)
 #pragma unroll
-        for (int e = 0; e < E; ++e) r[i][v][e] *= f * w[i][v][e];
-      if (turned[i]) {
+          for (int e = 0; e < E; ++e) {
+            r[i][v][e] = real[i] ? (float)now[i][v].v[e] : 0.f;
+            sum = fmaf(r[i][v][e], r[i][v][e], sum);
+          }
+      const float mean = fmaf(lanes_sum(sum, lanes), inv, n.epsilon);
+      const float f = mean >= 0x1p-100f ? __builtin_amdgcn_rsqf(mean) : 1.0f / sqrtf(mean);  // (rsq of small ones is 0)
+      if (weight_head && h > first) weights(h);
 #pragma unroll
-        for (int c = 0; c < C; ++c) {
-          float& u = HALF ? r[i][0][c] : r[i][0][2 * c];
-          float& z = HALF ? r[i][V - 1][c] : r[i][0][2 * c + 1];
-          const float first = u * cs[i][c].x - z * cs[i][c].y;
-          z = u * cs[i][c].y + z * cs[i][c].x;
-          u = first;
+      for (int i = 0; i < NI; ++i) {
+#pragma unroll
+        for (int v = 0; v < V; ++v)
+#pragma unroll
+          for (int e = 0; e < E; ++e) r[i][v][e] *= f * w[i][v][e];
+        if (turned[i]) {
+#pragma unroll
+          for (int c = 0; c < C; ++c) {
+            float& u = HALF ? r[i][0][c] : r[i][0][2 * c];
+            float& z = HALF ? r[i][V - 1][c] : r[i][0][2 * c + 1];
+            const float turned_u = u * cs[i][c].x - z * cs[i][c].y;
+            z = u * cs[i][c].y + z * cs[i][c].x;
+            u = turned_u;
+          }
+        }
+        if (!real[i]) continue;
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          vec out;
+#pragma unroll
+          for (int e = 0; e < E; ++e) out.v[e] = (T)r[i][v][e];
+          out.store(y + at[i][v]);
         }
       }
+      y += slots * s.y_head;
 #pragma unroll
-      for (int v = 0; v < V; ++v) store_values<T, E, VECTORS>(y + at[i][v], r[i][v]);
+      for (int i = 0; i < NI; ++i)
+#pragma unroll
+        for (int v = 0; v < V; ++v) now[i][v] = next[i][v];
     }
-  }
+  };
+  turn(a.q, n.q_weight, n.q_weight_head, slot);
+  // head h of both is slot h % slots'
+  const int passed = a.q.heads % slots;
+  turn(a.k, n.k_weight, n.k_weight_head, slot >= passed ? slot - passed : slot - passed + slots);
 }
 
 // By the widest vectors that sizes, strides and addresses allow.
@@ -290,10 +336,12 @@ hipError_t launch_rope_norm_type(const RopeArgs& a, const nemo_head_norm& n, hip
   auto launch = [&](auto half, auto v, auto ni, int items) {
     int lanes = 1;
     while (lanes < items && lanes < 64) lanes *= 2;
-    const int slots = std::max(1, std::min({heads, 256 / lanes, a.rows >= 512 ? (heads + 3) / 4 : heads}));
-    const int tokens = 256 / (lanes * slots);
+    // As many heads a thread as leave the chip 8 waves a SIMD.
+    const int64_t want = (1 << 19) / (a.rows * lanes) + 1;
+    const int all = (int)std::min<int64_t>(heads, want), slots = std::min(all, 256 / lanes);
+    const int tokens = 256 / (lanes * slots), parts = (all + slots - 1) / slots;
     rope_norm_kernel<T, E, decltype(half)::value, decltype(v)::value, decltype(ni)::value>
-        <<<(unsigned)((a.rows + tokens - 1) / tokens), 256, 0, stream>>>(a, n, lanes, slots, tokens);
+        <<<dim3((unsigned)((a.rows + tokens - 1) / tokens), parts), 256, 0, stream>>>(a, n, lanes, slots, tokens);
     return hipGetLastError();
   };
   auto sized = [&](auto half, auto v) {

@@ -64,6 +64,7 @@ class Rope:
         check(_lib.load().nemo_rope_create(self.ctx.ptr, ctypes.byref(config), ctypes.byref(ptr)))
         self._ptr = ptr
         self._apply = _lib.load().nemo_rope_apply
+        self._norm_apply = _lib.load().nemo_rope_norm_apply
 
     def apply(self, type_: int, q: RopeHeads, k: RopeHeads | None, rows: int, d_positions: int = 0, base: int = 0,
               stream: int = 0) -> None:
@@ -75,7 +76,7 @@ class Rope:
                    d_positions: int = 0, base: int = 0, stream: int = 0) -> None:
         """RMSNorm of each head, then ``apply`` of it, in one pass
         (nemo_rope_norm_apply)."""
-        check(_lib.load().nemo_rope_norm_apply(self._ptr, type_, q, k, norm, rows, d_positions, base, stream))
+        check(self._norm_apply(self._ptr, type_, q, k, norm, rows, d_positions, base, stream))
 
     def destroy(self) -> None:
         ptr, self._ptr = self._ptr, None
@@ -223,14 +224,16 @@ class Cache4:
         n = ctypes.c_size_t(0)
         check(_lib.load().nemo_cache4_page_bytes(config, ctypes.byref(n)))
         self.page_bytes = n.value
+        self._append, self._read = _lib.load().nemo_cache4_append, _lib.load().nemo_cache4_read
+        self._attention = _lib.load().nemo_cache4_attention
 
     def append(self, pages: Cache4Pages, rows: Cache4Rows, rope: Rope | None = None, stream: int = 0) -> None:
         """Write the rows of requests' last tokens, keys turned by ``rope``."""
-        check(_lib.load().nemo_cache4_append(self.ctx.ptr, self.config, pages, rows, rope._ptr if rope else None, stream))
+        check(self._append(self.ctx.ptr, self.config, pages, rows, rope._ptr if rope else None, stream))
 
     def read(self, pages: Cache4Pages, rows: Cache4Rows, stream: int = 0) -> None:
         """The values of requests' last tokens into rows."""
-        check(_lib.load().nemo_cache4_read(self.ctx.ptr, self.config, pages, rows, stream))
+        check(self._read(self.ctx.ptr, self.config, pages, rows, stream))
 
     @staticmethod
     def workspace_bytes(attention: AttentionConfig, count: int, q_rows: int, max_kv: int) -> int:
@@ -240,7 +243,7 @@ class Cache4:
 
     def attention(self, attention: AttentionConfig, pages: Cache4Pages, queries: Cache4Queries, stream: int = 0) -> None:
         """Attention of the query rows over the cache."""
-        check(_lib.load().nemo_cache4_attention(self.ctx.ptr, self.config, attention, pages, queries, stream))
+        check(self._attention(self.ctx.ptr, self.config, attention, pages, queries, stream))
 
 
 __all__ = [
