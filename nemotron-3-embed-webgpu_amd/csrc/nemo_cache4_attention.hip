@@ -18,7 +18,9 @@
 #include <algorithm>
 #include <type_traits>
 
+#include "nemo_attention_tile.h"
 #include "nemo_cache4.h"
+#include "nemo_lds_copy.h"
 
 namespace nemo {
 
@@ -94,9 +96,9 @@ struct Blocks {
 };
 
 template <typename T>
-struct Mma;
+struct Mma16;
 template <>
-struct Mma<half_t> {
+struct Mma16<half_t> {
   typedef half8v frag;
   typedef half2v pair;
   static constexpr int kFinite = 140;  // largest scale byte with finite values
@@ -112,7 +114,7 @@ struct Mma<half_t> {
   }
 };
 template <>
-struct Mma<bf16_t> {
+struct Mma16<bf16_t> {
   typedef bf16_t frag __attribute__((ext_vector_type(8)));
   typedef bf16_t pair __attribute__((ext_vector_type(2)));
   static constexpr int kFinite = 252;
@@ -162,9 +164,9 @@ struct Raw {
 // holds output columns D / 16 (4 h + e) + t in register e of o[i][t], and the sum
 // of its own keys' probabilities.
 template <typename T, int D, int QT>
-struct Rows {
+struct Rows16 {
   static constexpr int W = D / 32, C = D / 16;
-  typedef Mma<T> M;
+  typedef Mma16<T> M;
   typedef typename M::frag frag;
   typedef typename M::pair pair;
   // Queries: in registers for one tile of rows, else an LDS image of rows, 16-byte
@@ -252,10 +254,10 @@ __device__ __forceinline__ uint32_t seen8(int j, const Seen& s, int sinks) {
 // `seen`: what its lane's rows see. CAREFUL: values that are not finite are met
 // one by one, those of keys that a row does not see left out.
 template <bool CAREFUL, typename T, int D, int QT>
-__device__ __forceinline__ void attend(Rows<T, D, QT>& a, const Raw<D>& raw, float scale2, bool hide,
+__device__ __forceinline__ void attend(Rows16<T, D, QT>& a, const Raw<D>& raw, float scale2, bool hide,
                                        const uint32_t (&seen)[QT], uint32_t any) {
   constexpr int W = D / 32;
-  typedef Mma<T> M;
+  typedef Mma16<T> M;
   typedef typename M::frag frag;
   const int lane = threadIdx.x & 63;
   float4v s[QT][2];
@@ -357,6 +359,60 @@ __device__ __forceinline__ void attend(Rows<T, D, QT>& a, const Raw<D>& raw, flo
   }
 }
 
+// The rows over every `stride`-th block from `from` to before `end`. first, last: the
+// windows of the rows' first and last query; lo, hi: those of the lane's rows.
+template <bool CAREFUL, typename T, int D, int QT>
+__device__ __forceinline__ void attend_blocks(const AttendArgs& a, Rows16<T, D, QT>& acc, const Request& r,
+                                              const Blocks& blocks, const Seen& first, const Seen& last,
+                                              const int (&lo)[QT], const int (&hi)[QT], int kvh, int from, int stride,
+                                              int end) {
+  acc.clear();
+  const int steps = (end - from + stride - 1) / stride;
+  if (end <= from) return;
+  const int lane = threadIdx.x & 63, h = lane >> 4;
+  const int32_t* table = a.c.table + r.i * a.c.table_row;
+  const int per = a.c.shift - 5;  // log2 of a page's blocks
+  // Lane l has the page of the l-th of 64 steps, none (-1) where it is not there.
+  auto block_of = [&](int n) { return blocks.block(from + stride * min(n, steps - 1)); };
+  int ids = 0;
+  // (Blocks past the last, and in pages that are not there, are loaded from places that are.)
+  auto load = [&](Raw<D>& raw, int n) {
+    if ((n & 63) == 0) {
+      const int page = table[block_of(n + lane) >> per];
+      ids = n + lane < steps && (unsigned)page < (unsigned)a.c.pages ? page : -1;
+    }
+    const int page = __builtin_amdgcn_readlane(ids, n & 63);
+    raw.load(a.c.data + a.c.head<D>(max(page, 0), kvh), a.c.shift, (block_of(n) & ((1 << per) - 1)) << 5, lane);
+    return page >= 0;
+  };
+  auto step = [&](const Raw<D>& raw, int n) {
+    const int j0 = block_of(n) << 5;
+    const bool hide = j0 + 32 > first.hi || (j0 < last.lo && j0 + 32 > a.sinks);
+    uint32_t seen[QT] = {}, any = 255;
+    if (hide) {
+      any = seen8(j0 + 8 * h, Seen(first.lo, last.hi), a.sinks);
+#pragma unroll
+      for (int i = 0; i < QT; ++i) seen[i] = seen8(j0 + 8 * h, Seen(lo[i], hi[i]), a.sinks);
+    }
+    attend<CAREFUL>(acc, raw, a.scale2, hide, seen, any);
+  };
+  // AHEAD steps are in flight behind the one that is worked on.
+  constexpr int AHEAD = QT == 1 && !CAREFUL ? 2 : 1;
+  Raw<D> raw[AHEAD + 1];
+  bool there[AHEAD + 1];
+#pragma unroll
+  for (int i = 0; i < AHEAD; ++i) there[i] = load(raw[i], i);
+  for (int n = 0; n < steps; ++n) {
+    there[AHEAD] = load(raw[AHEAD], n + AHEAD);
+    if (there[0]) step(raw[0], n);
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) {
+      raw[i] = raw[i + 1];
+      there[i] = there[i + 1];
+    }
+  }
+}
+
 // Sums of a piece of a tile's keys: the rows' references and sums, and their
 // output values.
 struct Partials {
@@ -365,18 +421,28 @@ struct Partials {
   int64_t rows;
   int splits, piece;  // most pieces of a tile, and the blocks of one, more where a tile has more
   __device__ __forceinline__ int size(int blocks) const { return max(piece, (blocks + splits - 1) / splits); }
+  // This workgroup's piece of a query's head.
+  __device__ __forceinline__ int64_t at(const AttendArgs& a, int query, int head) const {
+    return rows * blockIdx.y + (int64_t)query * a.c.kv_heads * a.group + head;
+  }
 };
 
-// A workgroup takes 16 QT rows; its waves every WAVES-th block of keys, whose
-// sums they add in LDS. Where a tile has more blocks than a piece, each piece is a
-// workgroup, and a second kernel joins their sums.
+// Few rows: a workgroup takes 16 QT of them; its waves every WAVES-th block of keys,
+// whose sums they add in LDS. Where a tile has more blocks than a piece, each piece
+// is a workgroup, and a second kernel joins their sums.
+//
+// Bound by memory over long caches: 64 tokens over 1.08 GB of 4-bit keys and values 218
+// us (4.9 TB/s; a copy reaches 4.9 to 5.2), one over 131072 keys 28 us (5.1 TB/s) and
+// its join 4 to 5; by latency below. With one step in flight, a wait for each
+// page's number and registers copied between the two files it was 408. The split
+// by pieces and not by shares of each request's keys gave 293 -> 227.
 template <typename T, int D, int QT, int WAVES>
 __global__ __launch_bounds__(64 * WAVES, QT == 1 ? 3 : 2) void cache4_attention_kernel(AttendArgs a, Partials part) {
   constexpr int C = D / 16, W = D / 32;
-  typedef typename Mma<T>::frag frag;
+  typedef typename Mma16<T>::frag frag;
   __shared__ __attribute__((aligned(16))) float sums[WAVES][16][D];  // of 16 rows at a time
   __shared__ float2 ml[WAVES][16];
-  __shared__ __attribute__((aligned(16))) uint8_t queries[Rows<T, D, QT>::IMAGE ? 16 * QT * 2 * D : 16];
+  __shared__ __attribute__((aligned(16))) uint8_t queries[Rows16<T, D, QT>::IMAGE ? 16 * QT * 2 * D : 16];
   const int kvh = blockIdx.x % a.c.kv_heads, tile_no = blockIdx.x / a.c.kv_heads, split = blockIdx.y;
   const Request r(a, tile_no, 16 * QT);
   if (r.i < 0) return;
@@ -394,7 +460,7 @@ __global__ __launch_bounds__(64 * WAVES, QT == 1 ? 3 : 2) void cache4_attention_
   auto query_at = [&](int row, int query) {
     return (const T*)a.b.q + (int64_t)(r.q0 + query) * a.b.q_row + (int64_t)(head_of + row - query * a.group) * a.b.q_head;
   };
-  Rows<T, D, QT> acc;
+  Rows16<T, D, QT> acc;
   int lo[QT], hi[QT];
 #pragma unroll
   for (int i = 0; i < QT; ++i) {
@@ -402,12 +468,12 @@ __global__ __launch_bounds__(64 * WAVES, QT == 1 ? 3 : 2) void cache4_attention_
     const Seen s(a, behind + query, r.keys);
     lo[i] = s.lo;
     hi[i] = s.hi;
-    if constexpr (!Rows<T, D, QT>::IMAGE) {
+    if constexpr (!Rows16<T, D, QT>::IMAGE) {
 #pragma unroll
       for (int w = 0; w < W; ++w) acc.held[w] = *(const frag*)(query_at(row, query) + h * (D / 4) + 8 * w);
     }
   }
-  if constexpr (Rows<T, D, QT>::IMAGE) {
+  if constexpr (Rows16<T, D, QT>::IMAGE) {
     for (int at = threadIdx.x; at < 16 * QT * (D / 8); at += 64 * WAVES) {
       const int in = at / (D / 8), chunk = at % (D / 8), row = min(row0 + in, rows - 1);
       *(u32x4*)(queries + in * 2 * D + 16 * (chunk ^ (in & (D / 8 - 1)))) =
@@ -416,55 +482,11 @@ __global__ __launch_bounds__(64 * WAVES, QT == 1 ? 3 : 2) void cache4_attention_
     acc.image = queries;
     __syncthreads();
   }
-  const int32_t* table = a.c.table + r.i * a.c.table_row;
-  const int per = a.c.shift - 5;  // log2 of a page's blocks
-  // The wave's blocks are block0 + wave + WAVES n, n < steps (none without pages); lane l
-  // has the page of the l-th of 64 steps, none (-1) where it is not there.
-  const int steps = a.c.pages ? (block1 - block0 - wave + WAVES - 1) / WAVES : 0;
-  auto attended = [&](auto careful) {
-    acc.clear();
-    auto block_of = [&](int n) { return blocks.block(block0 + wave + WAVES * min(n, steps - 1)); };
-    int ids = 0;
-    // (Blocks past the last, and in pages that are not there, are loaded from places that are.)
-    auto load = [&](Raw<D>& raw, int n) {
-      if ((n & 63) == 0) {
-        const int page = table[block_of(n + lane) >> per];
-        ids = n + lane < steps && (unsigned)page < (unsigned)a.c.pages ? page : -1;
-      }
-      const int page = __builtin_amdgcn_readlane(ids, n & 63);
-      raw.load(a.c.data + a.c.head<D>(max(page, 0), kvh), a.c.shift, (block_of(n) & ((1 << per) - 1)) << 5, lane);
-      return page >= 0;
-    };
-    auto step = [&](const Raw<D>& raw, int n) {
-      const int j0 = block_of(n) << 5;
-      const bool hide = j0 + 32 > first.hi || (j0 < last.lo && j0 + 32 > a.sinks);
-      uint32_t seen[QT] = {}, any = 255;
-      if (hide) {
-        any = seen8(j0 + 8 * h, Seen(first.lo, last.hi), a.sinks);
-#pragma unroll
-        for (int i = 0; i < QT; ++i) seen[i] = seen8(j0 + 8 * h, Seen(lo[i], hi[i]), a.sinks);
-      }
-      attend<decltype(careful)::value>(acc, raw, a.scale2, hide, seen, any);
-    };
-    if (steps <= 0) return;
-    // AHEAD steps are in flight behind the one that is worked on.
-    constexpr int AHEAD = QT == 1 ? 2 : 1;
-    Raw<D> raw[AHEAD + 1];
-    bool there[AHEAD + 1];
-#pragma unroll
-    for (int i = 0; i < AHEAD; ++i) there[i] = load(raw[i], i);
-    for (int n = 0; n < steps; ++n) {
-      there[AHEAD] = load(raw[AHEAD], n + AHEAD);
-      if (there[0]) step(raw[0], n);
-#pragma unroll
-      for (int i = 0; i < AHEAD; ++i) {
-        raw[i] = raw[i + 1];
-        there[i] = there[i + 1];
-      }
-    }
-  };
-  attended(std::false_type{});
-  if (__builtin_amdgcn_ballot_w64(acc.spoilt())) attended(std::true_type{});
+  // (without pages there are no keys)
+  const int from = block0 + wave, end = a.c.pages ? block1 : 0;
+  attend_blocks<false>(a, acc, r, blocks, first, last, lo, hi, kvh, from, WAVES, end);
+  if (__builtin_amdgcn_ballot_w64(acc.spoilt()))
+    attend_blocks<true>(a, acc, r, blocks, first, last, lo, hi, kvh, from, WAVES, end);
   // The waves' sums, 16 rows at a time.
   constexpr int THREADS = 64 * WAVES, PER = 16 * D / THREADS;  // columns of a thread
   static_assert(PER >= 4 && D % PER == 0, "whole vectors of one row");
@@ -501,7 +523,7 @@ __global__ __launch_bounds__(64 * WAVES, QT == 1 ? 3 : 2) void cache4_attention_
     }
     const int query = a.query(at), head = head_of + at - query * a.group;
     if (!whole) {
-      const int64_t to = part.rows * split + (int64_t)(r.q0 + query) * a.c.kv_heads * a.group + head;
+      const int64_t to = part.at(a, r.q0 + query, head);
       if (c0 == 0) part.ml[to] = make_float2(m, l);
 #pragma unroll
       for (int c = 0; c < PER; c += 4)
@@ -517,17 +539,20 @@ __global__ __launch_bounds__(64 * WAVES, QT == 1 ? 3 : 2) void cache4_attention_
   }
 }
 
-// Joins the pieces, at most 64: a workgroup a row, of tiles of `of` rows. Thread (g, c)
-// adds columns 4 c.. of pieces g, g + G, ..., and the G sums are added in order.
-template <typename T, int D>
-__global__ __launch_bounds__(256) void cache4_join_kernel(AttendArgs a, Partials part, int of) {
-  constexpr int C = D / 4, G = 256 / C;
-  __shared__ float weight[64];
-  __shared__ float4v sums[G][C];
-  const int kvh = blockIdx.x % a.c.kv_heads, tile_no = blockIdx.x / a.c.kv_heads;
+// Joins the pieces, at most 64, of tiles of `of` rows: WAVES waves of a workgroup take a
+// row. Lane l of wave w adds columns 4 (l % (D / 4)) .. of every G WAVES-th piece from
+// l / (D / 4) + G w on; the sums are added in order.
+template <typename T, int D, int WAVES>
+__global__ __launch_bounds__(256) void cache4_join_kernel(AttendArgs a, Partials part, int of, int items) {
+  constexpr int C = D / 4, G = 64 / C;
+  __shared__ float4v sums[WAVES][C];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int item = blockIdx.x * (4 / WAVES) + wave / WAVES, w = wave % WAVES;
+  if (item >= items) return;  // (one row a workgroup, or a wave each: no barrier is left behind)
+  const int kvh = item % a.c.kv_heads, tile_no = item / a.c.kv_heads;
   const Request r(a, tile_no, 1);
   if (r.i < 0) return;
-  const int row = tile_no - r.tile, lane = threadIdx.x & 63;
+  const int row = tile_no - r.tile;
   if ((unsigned)row >= (unsigned)(r.queries * a.group)) return;
   const int row0 = row / of * of, behind = r.keys - r.queries;
   const Blocks blocks(a, Seen(a, behind + a.query(row0), r.keys),
@@ -538,6 +563,15 @@ __global__ __launch_bounds__(256) void cache4_join_kernel(AttendArgs a, Partials
   const int64_t at = (int64_t)(r.q0 + i) * a.c.kv_heads * a.group + head;
   // every wave: lane z's piece
   const float2 ml = lane < pieces ? part.ml[part.rows * lane + at] : make_float2(-INFINITY, 0.f);
+  const int c = lane % C, g = lane / C;
+  constexpr int BATCH = 8;  // pieces whose values are on their way together
+  float4v o[BATCH];
+  auto load = [&](int z0) {
+#pragma unroll
+    for (int k = 0; k < BATCH; ++k)
+      o[k] = *(const float4v*)(part.o + (part.rows * min(z0 + k * G * WAVES + g, pieces - 1) + at) * D + 4 * c);
+  };
+  load(G * w);
   float m = ml.x;
 #pragma unroll
   for (int x = 32; x > 0; x >>= 1) m = fmaxf(m, __shfl_xor(m, x, 64));
@@ -546,42 +580,355 @@ __global__ __launch_bounds__(256) void cache4_join_kernel(AttendArgs a, Partials
   float l = empty ? 0.f : f * ml.y;
 #pragma unroll
   for (int x = 32; x > 0; x >>= 1) l += __shfl_xor(l, x, 64);
-  if (threadIdx.x < 64) weight[lane] = empty ? -1.f : f;
-  __syncthreads();
-  const int c = threadIdx.x % C, g = threadIdx.x / C;
+  const float weight = empty ? -1.f : f;
   float4v v = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-  for (int z = g; z < pieces; z += G) {
-    const float4v o = *(const float4v*)(part.o + (part.rows * z + at) * D + 4 * c);
-    const float w = weight[z];
+  for (int z0 = G * w; z0 < pieces; z0 += BATCH * G * WAVES) {
+    if (z0 > G * w) load(z0);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] = w == -1.f ? v[e] : fmaf(w, o[e], v[e]);
+    for (int k = 0; k < BATCH; ++k) {
+      const int z = z0 + k * G * WAVES + g;
+      const float of_z = __shfl(weight, z & 63, 64), by = z < pieces ? of_z : -1.f;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = by == -1.f ? v[e] : fmaf(by, o[k][e], v[e]);
+    }
   }
-  sums[g][c] = v;
-  __syncthreads();
-  if (threadIdx.x >= D) return;
-  float sum = 0.f;
 #pragma unroll
-  for (int k = 0; k < G; ++k) sum += sums[k][threadIdx.x / 4][threadIdx.x % 4];
+  for (int x = C; x < 64; x *= 2)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] += __shfl_xor(v[e], x, 64);
+  if constexpr (WAVES > 1) {
+    if (g == 0) sums[w][c] = v;
+    __syncthreads();
+    if (w) return;
+    v = sums[0][c];
+#pragma unroll
+    for (int k = 1; k < WAVES; ++k) v += sums[k][c];
+  }
+  if (g) return;
+  typedef T vec __attribute__((ext_vector_type(4)));
+  const float inv = l == 0.f ? 0.f : 1.0f / l;
   T* out = (T*)a.b.out + (int64_t)(r.q0 + i) * a.b.out_row + (int64_t)head * a.b.out_head;
-  out[threadIdx.x] = (T)(l == 0.f ? 0.f : sum / l);
+  *(vec*)(out + 4 * c) = vec{(T)(v[0] * inv), (T)(v[1] * inv), (T)(v[2] * inv), (T)(v[3] * inv)};
 }
 
-// Rows of a tile and how the keys are split, by a batch's sizes alone.
+// 16 rows from `begin` on over the blocks [block0, block1) of a tile's list, by one wave;
+// those whose bit of `mask` is set are written.
+template <typename T, int D>
+__device__ __forceinline__ void careful_rows(const AttendArgs& a, const Partials& part, const Request& r,
+                                             const Blocks& blocks, const Seen& first, const Seen& last, int kvh,
+                                             int begin, int rows, uint32_t mask, int block0, int block1, bool whole) {
+  constexpr int C = D / 16, W = D / 32;
+  typedef typename Mma16<T>::frag frag;
+  const int lane = threadIdx.x & 63, h = lane >> 4;
+  const int row = min(begin + (lane & 15), rows - 1), query = a.query(row), head = kvh * a.group + row - query * a.group;
+  const Seen mine(a, r.keys - r.queries + query, r.keys);
+  const int lo[1] = {mine.lo}, hi[1] = {mine.hi};
+  Rows16<T, D, 1> acc;
+  const T* q = (const T*)a.b.q + (int64_t)(r.q0 + query) * a.b.q_row + (int64_t)head * a.b.q_head + h * (D / 4);
+#pragma unroll
+  for (int w = 0; w < W; ++w) acc.held[w] = *(const frag*)(q + 8 * w);
+  attend_blocks<true>(a, acc, r, blocks, first, last, lo, hi, kvh, block0, 1, a.c.pages ? block1 : 0);
+  acc.l[0] += __shfl_xor(acc.l[0], 16, 64);
+  acc.l[0] += __shfl_xor(acc.l[0], 32, 64);
+  if (begin + (lane & 15) >= rows || !(mask >> (lane & 15) & 1)) return;
+  const float inv = !whole ? 1.f : acc.l[0] == 0.f ? 0.f : 1.0f / acc.l[0];
+  T* out = (T*)a.b.out + (int64_t)(r.q0 + query) * a.b.out_row + (int64_t)head * a.b.out_head;
+  const int64_t to = part.at(a, r.q0 + query, head);
+  if (!whole && h == 0) part.ml[to] = make_float2(acc.m[0], acc.l[0]);
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+#pragma unroll
+    for (int t = 0; t < C; ++t) {
+      const int column = C * (4 * h + e) + t;
+      if (whole) out[column] = (T)(acc.o[0][t][e] * inv);
+      else part.o[to * D + column] = acc.o[0][t][e];
+    }
+}
+
+// ---------------------------------------------------------------------------
+// Many rows: a workgroup of 4 waves takes 128, and 64 keys a round for all of
+// them, as window attention's tiles do: scores one block ahead and the product
+// with V one behind, on v_mfma_f32_32x32x16. Each wave decodes 16 keys of K and of
+// V of a round, among its products, into the images of the round behind it; their
+// codes are loaded a round before that.
+//
+// Bound by the steps' instructions, as that kernel: 2048 queries of 32 heads of 128
+// behind 16000 keys (8 KV heads) and three small requests, 575 GFLOP, take 547 us,
+// 1.05 PFLOP/s, of which the MFMAs are 44 % of the cycles. Waves that decode all keys for
+// 64 rows of their own, without LDS, took 775: decoding is then half of their
+// instructions.
+// ---------------------------------------------------------------------------
+
+// What a wave decodes: 16 tokens' codes. K: lane l has quarter l % 4 of key l / 4; V:
+// piece l % 16 of 4 tokens from 4 (l / 16) on.
+template <typename T, int D>
+struct Sixteen {
+  static constexpr int W = D / 32, ITEMS = W + 4;
+  typedef uint32_t vec __attribute__((ext_vector_type(W)));
+  typedef Mma16<T> M;
+  vec k, v;
+  uint32_t k_scale, v_scales;
+  // Tokens t .. t + 15 of a page whose KV head begins at `head`.
+  __device__ __forceinline__ void load_k(const uint8_t* head, int t, int shift, int lane) {
+    typedef Cache4Head<D> Head;
+    const int key = t + (lane >> 2), quarter = lane & 3;
+    k = *(const vec*)(head + Head::k_codes(key) + quarter * (D / 8));
+    k_scale = head[Head::scale(shift, false, key, quarter * (D / 32) / 4)];
+  }
+  __device__ __forceinline__ void load_v(const uint8_t* head, int t, int shift, int lane) {
+    typedef Cache4Head<D> Head;
+    const int first = t + 4 * (lane >> 4), piece = lane & 15;
+    v = *(const vec*)(head + Head::v_codes(shift, first, piece));
+    v_scales = *(const uint32_t*)(head + Head::scale(shift, true, first, piece * (D / 32) / 16));
+  }
+  // Zeros for the values whose bit of `keep` is not set.
+  __device__ __forceinline__ void drop(uint32_t keep) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if (keep >> e & 1) continue;
+      v_scales &= ~(255u << (8 * e));
+      if constexpr (D == 128) v[e] = 0;
+      else v[e >> 1] &= e & 1 ? 0xffffu : 0xffff0000u;
+    }
+  }
+  // Item i of ITEMS into images of which the tokens are rows `row0` ...
+  __device__ __forceinline__ void write(int i, uint8_t* k_image, uint8_t* v_image, int row0, int lane) const {
+    if (i < W) {
+      const float power = __uint_as_float(k_scale << 23);
+      const uint32_t c = k[i];
+      const u32x4 f = {M::template decode<0>(c, power), M::template decode<1>(c, power), M::template decode<2>(c, power),
+                       M::template decode<3>(c, power)};
+      const int row = row0 + (lane >> 2), chunk = W * (lane & 3) + i;
+      *(u32x4*)(k_image + row * 2 * D + 16 * (chunk ^ k_swizzle<D>(row))) = f;
+      return;
+    }
+    const int e = i - W, row = row0 + 4 * (lane >> 4) + e, piece = lane & 15;
+    const int s = 23 - 8 * e;
+    const float power = __uint_as_float(s >= 0 ? v_scales << s : v_scales >> -s);
+    if constexpr (D == 128) {
+      const uint32_t c = v[e];
+      const u32x4 f = {M::template decode<0>(c, power), M::template decode<1>(c, power), M::template decode<2>(c, power),
+                       M::template decode<3>(c, power)};
+      *(u32x4*)(v_image + row * 2 * D + 16 * (piece ^ v_swizzle<D>(row))) = f;
+    } else {
+      const uint32_t c = e & 1 ? v[e >> 1] >> 16 : v[e >> 1];
+      const u32x2 f = {M::template decode<0>(c, power), M::template decode<1>(c, power)};
+      *(u32x2*)(v_image + row * 2 * D + 16 * ((piece >> 1) ^ v_swizzle<D>(row)) + 8 * (piece & 1)) = f;
+    }
+  }
+};
+
+template <typename T, int D>
+__global__ __launch_bounds__(256, 2) void cache4_tile_kernel(AttendArgs a, Partials part) {
+  constexpr int IMG = 2 * kKeys * D, ROWS = 128;
+  __shared__ __attribute__((aligned(16))) uint8_t lds[2][2][2 * IMG];  // [K, V][round & 1]
+  __shared__ __attribute__((aligned(16))) uint8_t extra[IMG];          // K of the first block
+  const int kvh = blockIdx.x % a.c.kv_heads, tile_no = blockIdx.x / a.c.kv_heads;
+  const Request r(a, tile_no, ROWS);
+  if (r.i < 0) return;
+  const int rows = r.queries * a.group, row0 = (tile_no - r.tile) * ROWS;
+  if ((unsigned)row0 >= (unsigned)rows) return;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), hl = lane >> 5;
+  const int behind = r.keys - r.queries;  // position of query 0
+  auto window = [&](int row) { return Seen(a, behind + a.query(row), r.keys); };
+  const Seen all_first = window(row0), all_last = window(min(row0 + ROWS, rows) - 1);
+  const Blocks blocks(a, all_first, all_last);
+  const int size = part.size(blocks.n), block0 = size * blockIdx.y, block1 = min(blocks.n, block0 + size);
+  if (block0 >= blocks.n && blockIdx.y) return;
+  const bool whole = blocks.n <= size;               // the tile's only piece
+  const int count = a.c.pages ? block1 - block0 : 0;  // (without pages there are no keys)
+  // In slots of the piece's list of blocks a row sees t < hi with t >= lo or t < sinks. (A
+  // round may have a block behind the piece, which the next one has.)
+  const int before = 32 * block0, sinks = a.sinks - before;
+  auto listed = [&](int row) {
+    const Seen s = window(row);
+    return Seen(s.lo - 32 * blocks.skip - before, min(s.hi - 32 * blocks.skip - before, 32 * count));
+  };
+  const int w0 = row0 + 32 * wave, w1 = min(w0 + 31, rows - 1), row = min(w0 + (lane & 31), rows - 1);
+  const Seen mine = listed(row), first = listed(min(w0, rows - 1)), last = listed(w1);
+  const int rounds = (count + 1) >> 1, head_of = kvh * a.group;
+  auto query_at = [&](int at) {
+    const int i = a.query(at);
+    return (const T*)a.b.q + (int64_t)(r.q0 + i) * a.b.q_row + (int64_t)(head_of + at - i * a.group) * a.b.q_head;
+  };
+  auto output = [&](int at) {
+    const int i = a.query(at);
+    return (T*)a.b.out + (int64_t)(r.q0 + i) * a.b.out_row + (int64_t)(head_of + at - i * a.group) * a.b.out_head;
+  };
+  const int32_t* table = a.c.table + r.i * a.c.table_row;
+  const int per = a.c.shift - 5;  // log2 of a page's blocks
+  auto block_of = [&](int b) { return blocks.block(block0 + max(0, min(b, count - 1))); };
+  auto page_of = [&](int b) { return table[block_of(b) >> per]; };
+  // Pages that are not there are the slow path's.
+  bool missing = false;
+  if (count) {
+    for (int b = lane << per; b < count + (1 << per); b += 64 << per)
+      if ((unsigned)page_of(b) >= (unsigned)a.c.pages) missing = true;
+    if ((unsigned)page_of(blocks.sinks - block0) >= (unsigned)a.c.pages) missing = true;  // the window's first
+  }
+  missing = __builtin_amdgcn_ballot_w64(missing) != 0;
+  uint8_t* const rows_image = lds[wave >> 1][1] + (wave & 1) * IMG;
+  Rows<T, D> acc;
+  acc.clear();
+  if (!missing) {
+    // The wave decodes tokens 16 (wave % 2) .. of K's block 2 at + 1 + wave / 2 and V's
+    // 2 at - 1 + wave / 2 for round `at`.
+    const int second = wave >> 1, sixteen = 16 * (wave & 1);
+    Sixteen<T, D> codes;
+    auto head_at = [&](int page) { return a.c.data + a.c.head<D>(page, kvh); };
+    auto token = [&](int b) { return ((block_of(b) & ((1 << per) - 1)) << 5) + sixteen; };
+    // Values that no row sees are zeros.
+    auto seen = [&](int b) {
+      const bool listed = b >= 0 && b < count;
+      const int key = (block_of(b) << 5) + sixteen;
+      if (listed && (key >= all_first.lo || key + 16 <= a.sinks) && key + 16 <= all_last.hi) return;
+      asm volatile("");
+      uint32_t keep = 0;
+      if (listed)
+        keep = seen8(key + 4 * (lane >> 4), Seen(all_first.lo, all_last.hi), a.sinks);
+      codes.drop(keep);
+    };
+    int pages[2];  // of the V block that is loaded next, and of the K block
+    int coming;    // of the K block behind it, on its way
+    if (rounds) {
+      // K of the first block, by waves 0 and 1
+      const int p0 = __builtin_amdgcn_readfirstlane(page_of(0));
+      codes.load_k(head_at(p0), token(0), a.c.shift, lane);
+      if (!second) {
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) codes.write(i, extra, extra, sixteen, lane);
+      }
+      image_rows<D>(lane, [&](int i, int r, int chunk) {
+        *(u32x4*)(rows_image + 1024 * i + 16 * lane) =
+            *(const u32x4*)(query_at(min(w0 + r, rows - 1)) + 8 * (chunk ^ k_swizzle<D>(r)));
+      });
+      pages[0] = __builtin_amdgcn_readfirstlane(page_of(second - 1));
+      pages[1] = __builtin_amdgcn_readfirstlane(page_of(second + 1));
+      coming = page_of(second + 3);
+      codes.load_k(head_at(pages[1]), token(second + 1), a.c.shift, lane);
+      codes.load_v(head_at(pages[0]), token(second - 1), a.c.shift, lane);
+      seen(second - 1);
+#pragma unroll
+      for (int i = 0; i < Sixteen<T, D>::ITEMS; ++i)
+        codes.write(i, lds[0][0] + second * IMG, lds[1][0] + second * IMG, sixteen, lane);
+    }
+    auto landed = [&] {
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      meet();
+    };
+    // Codes of round `at`, whose V's pages are those of K's before.
+    auto load = [&](int at) {
+      pages[0] = pages[1];
+      pages[1] = __builtin_amdgcn_readfirstlane(coming);
+      coming = page_of(2 * at + 3 + second);
+      codes.load_k(head_at(pages[1]), token(2 * at + 1 + second), a.c.shift, lane);
+      codes.load_v(head_at(pages[0]), token(2 * at - 1 + second), a.c.shift, lane);
+    };
+    float16v s;
+    auto hidden = [&](int t0) {
+      if (t0 + 32 > first.hi || (t0 < last.lo && t0 + 32 > sinks)) {
+        asm volatile("");
+        hide(s, t0, hl, mine.lo, mine.hi, sinks);
+      }
+    };
+    typename Mma<T>::frag p[2] = {};
+    if (rounds) {
+      load(1);
+      landed();
+      acc.load(rows_image, lane);
+      s = acc.scores(extra, lane);
+      hidden(0);
+    }
+    for (int at = 0; at < rounds; ++at) {
+      landed();  // the round's images, and every wave has left the others
+      const int odd = at & 1;
+      constexpr int C = D / 16, CALLS = 2 * C, ITEMS = Sixteen<T, D>::ITEMS;
+      static_assert(ITEMS < CALLS, "a call for each item, and one for the loads");
+      seen(2 * at + 1 + second);
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        acc.step(s, p, lds[1][odd] + k * IMG, lds[0][odd] + k * IMG, lane, a.scale2, [&](int c) {
+          const int call = C * k + c;
+          if (call < ITEMS) codes.write(call, lds[0][1 - odd] + second * IMG, lds[1][1 - odd] + second * IMG, sixteen, lane);
+          else if (call == ITEMS) load(at + 2);
+        });
+        hidden(64 * at + 32 + 32 * k);
+      }
+    }
+    if (rounds && 2 * rounds == count) {
+      landed();
+      acc.values(lds[1][rounds & 1], lane, p);
+    }
+    acc.l += __shfl_xor(acc.l, 32, 64);
+  }
+  // Rows whose sums are not finite, which a value that they do not see may be
+  // the cause of, and rows over pages that are not there are taken again.
+  const uint64_t bad = missing ? ~0ull : __builtin_amdgcn_ballot_w64(acc.spoilt());
+  const uint32_t again = (uint32_t)(bad | bad >> 32);
+  if (whole) {
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    meet();
+    acc.store((T*)(rows_image + (lane & 31) * 2 * D), lane & 31, hl);
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    image_rows<D>(lane, [&](int i, int r, int chunk) {
+      const u32x4 v = *(const u32x4*)(rows_image + r * 2 * D + 16 * (chunk ^ k_swizzle<D>(r)));
+      if (w0 + r < rows && !(again >> r & 1)) *(u32x4*)(output(w0 + r) + 8 * chunk) = v;
+    });
+  } else if (w0 + (lane & 31) < rows && !(again >> (lane & 31) & 1)) {
+    const int i = a.query(row);
+    const int64_t to = part.at(a, r.q0 + i, head_of + row - i * a.group);
+    if (hl == 0) part.ml[to] = make_float2(acc.m, acc.l);
+#pragma unroll
+    for (int db = 0; db < D / 32; ++db)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        *(float4v*)(part.o + to * D + 32 * db + 8 * j + 4 * hl) =
+            float4v{acc.o[db][4 * j], acc.o[db][4 * j + 1], acc.o[db][4 * j + 2], acc.o[db][4 * j + 3]};
+  }
+  if (again) {
+    asm volatile("");
+    for (int i = 0; i < 2; ++i) {
+      const uint32_t mask = again >> (16 * i) & 0xffff;
+      const int begin = w0 + 16 * i;
+      if (mask && begin < rows)
+        careful_rows<T, D>(a, part, r, blocks, all_first, all_last, kvh, begin, rows, mask, block0, block1, whole);
+    }
+  }
+}
+
+// Rows of a tile and how the keys are split, by a batch's sizes alone (us, 32 heads of
+// 128, 8 KV heads; tiles of 16 : 32 : 128 rows).
+//  Requests of up to 32 rows: 16 (32 x 8 queries, 5000 keys 60 : 78 : 107, 8 over 60000 keys
+//  33 : 41 : 45; one of 4, 5000 keys 13.5 : 14.3 : 21).
+//  From 256 rows on, with 512 tiles of 128 or, all together, 32768 blocks of keys: 128 (16
+//  x 100 queries of 100 keys 26 : 25 : 16, 2048 of 2048 88 : 75 : 65, 128 over 60000 keys 260 :
+//  187 : 149).
+//  Between: 32 (32 x 32, 5000 keys 172 : 136 : 190; 512 of 512 15 : 12.5 : 18; 64 over 5000
+//  keys 27 : 24 : 28; 128 over 5000 34 : 31 : 35; 512 over 5000 83 : 66 : 68).
+// A split costs a second launch and is taken from 72 blocks on (one token: 5000 keys
+// 19.6 whole, 12 in pieces of 16 blocks; 1028 keys 8.5 and 11.3), into pieces that fill
+// the chip 16 times over for single tokens, whose requests' lengths differ (64 tokens over
+// their caches: 768 pieces 263, 1536 252, 2048 231, 4096 219 to 227, 8192 235), twice
+// for more rows, whose sums are written and read again (512 over 5000 keys: 512 pieces
+// 66, 1024 79, 4096 107), of 64 blocks at least where there is work for 1024 such
+// (32 x 4 queries over 5000 keys in pieces of 16 blocks 80, of 39 63).
 struct Plan {
-  int tiles16, splits, piece;  // rows of a tile / 16; most pieces of a tile, and the blocks of 32 keys of one
+  int rows, splits, piece;  // rows of a tile; most pieces of a tile, and the blocks of 32 keys of one
 };
 Plan plan_of(const nemo_attention_config& c, int count, int64_t q_rows, int64_t max_kv) {
-  if (count == 0 || q_rows == 0) return {1, 1, 1};
+  if (count == 0 || q_rows == 0) return {16, 1, 1};
   const int64_t rows = q_rows * (c.q_heads / c.kv_heads);
-  const int tiles16 = rows / count <= 16 ? 1 : 4;
-  const int64_t tiles = std::max<int64_t>(rows / (16 * tiles16), count) * c.kv_heads;
+  auto tiles_of = [&](int n) { return std::max<int64_t>(rows / n, count) * c.kv_heads; };
   int64_t keys = max_kv;
   if (c.left >= 0 && c.right >= 0) keys = std::min(keys, (int64_t)c.left + c.right + 1 + c.sinks);
   const int64_t blocks = std::min<int64_t>(keys, 1 << 30) / 32 + 1;
-  const int64_t places = tiles16 == 1 ? 4096 : 512, least = tiles16 == 1 ? 64 : 32;
-  const int64_t piece = std::max<int64_t>({least, (blocks * tiles + places - 1) / places, (blocks + 63) / 64});
-  return {tiles16, (int)((blocks + piece - 1) / piece), (int)piece};
+  int tile = rows / count <= 32 ? 16 : 32;
+  if (rows / count >= 256 && (tiles_of(128) >= 512 || blocks * tiles_of(128) >= 512 * 64)) tile = 128;
+  const int64_t work = blocks * tiles_of(tile);
+  if (blocks <= 72) return {tile, 1, (int)blocks};
+  const int64_t piece = std::max<int64_t>({16, std::min<int64_t>(64, work / 1024), work / (tile == 16 ? 4096 : 512) + 1,
+                                           (blocks + 63) / 64});
+  return {tile, (int)((blocks + piece - 1) / piece), (int)piece};
 }
 
 }  // namespace
@@ -614,9 +961,15 @@ hipError_t launch_cache4_attention(const nemo_cache4_config& cache, const nemo_a
   auto launch = [&](auto type, auto d) {
     constexpr int D = decltype(d)::value;
     typedef decltype(type) T;
-    if (plan.tiles16 == 1) cache4_attention_kernel<T, D, 1, 4><<<dim3(tiles(16), splits), 256, 0, stream>>>(a, part);
-    else cache4_attention_kernel<T, D, 4, 4><<<dim3(tiles(64), splits), 256, 0, stream>>>(a, part);
-    if (splits > 1) cache4_join_kernel<T, D><<<tiles(1), 256, 0, stream>>>(a, part, 16 * plan.tiles16);
+    const dim3 grid(tiles(plan.rows), splits);
+    if (plan.rows == 16) cache4_attention_kernel<T, D, 1, 4><<<grid, 256, 0, stream>>>(a, part);
+    else if (plan.rows == 32) cache4_attention_kernel<T, D, 2, 4><<<grid, 256, 0, stream>>>(a, part);
+    else cache4_tile_kernel<T, D><<<grid, 256, 0, stream>>>(a, part);
+    if (splits == 1) return;
+    // a workgroup a row for few of them, else a wave
+    const int items = (int)tiles(1);
+    if (items <= 2048) cache4_join_kernel<T, D, 4><<<items, 256, 0, stream>>>(a, part, plan.rows, items);
+    else cache4_join_kernel<T, D, 1><<<(items + 3) / 4, 256, 0, stream>>>(a, part, plan.rows, items);
   };
   auto typed = [&](auto type) {
     if (c.head_dim == 64) launch(type, std::integral_constant<int, 64>{});

@@ -334,6 +334,32 @@ def test_append_turns_keys(torch_cuda, dtype, dim, half, rotary, given):
         assert not (differ & (margin > 2.0 ** -32)).any()
 
 
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("layout", ["interleaved", "half", "half, no vectors"])
+def test_append_turns_by_nothing_at_borders(torch_cuda, dtype, dim, layout):
+    """At position 0 a rotation changes nothing, and values on borders between
+    codes and between powers of two are theirs: the rotation's error in 32
+    bits may not decide them."""
+    g = torch.Generator().manual_seed(3)
+    borders = torch.tensor([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0, 7.0, 0.0, 6.0])
+    rows, heads = 9, 5
+    pad = 1 if "no" in layout else 0
+    x = borders[torch.randint(0, 10, (rows, heads, dim + pad), generator=g)] * (1 - 2 * torch.randint(0, 2, (rows, heads, dim + pad), generator=g))
+    x = (x * torch.exp2(torch.randint(-6, 6, (rows, heads, 1), generator=g).float())).to(dtype)
+    rope = ops.Rope(ops.rope_config(dim, layout=ops.ROPE_INTERLEAVED if layout == "interleaved" else ops.ROPE_HALF))
+    pages = Pages(heads, dim, 32, [rows])
+    dx, pos, start = x.cuda(), torch.zeros(rows, dtype=torch.int64, device="cuda"), starts([rows])
+    pages.cache.append(pages.pages, ops.cache4_rows(CODE[dtype], rows, start.data_ptr(), side(dx), side(dx), pos.data_ptr()),
+                       rope, stream=stream())
+    out = torch.empty(2, rows, heads, dim, device="cuda")
+    pages.cache.read(pages.pages, ops.cache4_rows(ops.TYPE_F32, rows, start.data_ptr(), side(out[0]), side(out[1])), stream=stream())
+    torch.cuda.synchronize()
+    codes, scales, _ = lref.encode4(x[..., :dim].double())
+    want = lref.decode4(codes, scales)
+    assert torch.equal(out[0].cpu().double(), want) and torch.equal(out[1].cpu().double(), want)
+
+
 def test_append_of_values_at_the_ends(torch_cuda):
     """Ties, the largest and the smallest values, infinities and NaN."""
     x = torch.zeros(4, 1, 64)
@@ -467,11 +493,16 @@ def attend(pages, q, q_lens, left=-1, right=0, sinks=0, scale=0.0, workspace=Tru
     return out, need
 
 
-def check(out, held, q, q_lens, left=-1, right=0, sinks=0, scale=0.0):
+def check(out, held, q, q_lens, left=-1, right=0, sinks=0, scale=0.0, kv_heads=None):
+    """All heads, or those of the given KV heads."""
     row = 0
     for (k, v), n in zip(held, q_lens):
-        want, tol = ref.attention(q[row:row + n], k, v, left, right, sinks, scale or k.shape[-1] ** -0.5)
-        close(out[row:row + n], want, tol, f"rows {row} to {row + n}")
+        kv = range(k.shape[1]) if kv_heads is None else kv_heads
+        group = q.shape[1] // k.shape[1]
+        heads = [h * group + i for h in kv for i in range(group)]
+        want, tol = ref.attention(q[row:row + n, heads], k[:, list(kv)], v[:, list(kv)], left, right, sinks,
+                                  scale or k.shape[-1] ** -0.5)
+        close(out[row:row + n, heads], want, tol, f"rows {row} to {row + n}")
         row += n
 
 
@@ -511,6 +542,85 @@ def test_attention_over_long_caches(torch_cuda, dtype, dim, workspace, q_lens, k
     out, need = attend(pages, q, q_lens, workspace=workspace)
     assert not workspace or need > 0
     check(out, held, q, q_lens)
+
+
+# (tiles of 128 rows are taken from 256 rows a request on, where there are 512 tiles, or with 32768 blocks of 32 keys
+# in all of them; those of the last cases are split into pieces)
+MANY = [
+    (64, 4, 128, [128], [300], -1, 0, 0),
+    (128, 1, 256, [250, 262], [250, 700], -1, 0, 0),
+    (64, 2, 256, [129], [129], 33, 0, 40),
+    (64, 1, 256, [256], [150], -1, -1, 0),
+    (64, 1, 512, [256], [97], 20, 5, 2),             # more queries than keys
+    (128, 3, 64, [400], [395], 100, 0, 3),
+    (64, 1, 128, [256], [4100], -1, 0, 0),
+    (128, 1, 128, [256], [4500], 4200, 0, 70),
+]
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("dim,group,kv,q_lens,kv_lens,left,right,sinks", MANY)
+def test_attention_of_many_rows(torch_cuda, dtype, dim, group, kv, q_lens, kv_lens, left, right, sinks):
+    pages, held = random_cache(sum(kv_lens), kv_lens, kv, dim, 64)
+    q = rand(7, sum(q_lens), kv * group, dim, dtype=dtype)
+    out, _ = attend(pages, q, q_lens, left, right, sinks)
+    check(out, held, q, q_lens, left, right, sinks, kv_heads=[0, 1, kv - 1])
+    assert torch.isfinite(out.float()).all()
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("dim,kv,n,keys,left,right", [(64, 512, 256, 200, 60, 0), (128, 256, 256, 200, 40, 3),
+                                                      (64, 128, 256, 4100, 2000, 0)])
+def test_many_rows_and_nan_that_some_do_not_see(torch_cuda, dtype, dim, kv, n, keys, left, right):
+    pages, held = random_cache(5, [keys], kv, dim, 32)
+    base = keys - n
+    spots = [(max(0, base + 30), 0, 0), (keys - 60, 1, dim // 32 - 1), (5, kv - 1, 0)]
+    for what in ("k", "v"):
+        k, v = (t.clone() for t in held[0])
+        for t, h, b in spots:
+            page, i = int(pages.table[0, t // 32]), t % 32
+            at = h * 32 * (dim + dim // 16) + 32 * dim + (32 * dim // 32 if what == "v" else 0) + i // 8 * (dim // 4) + b * 8 + i % 8
+            was = int(pages.data[page, at])
+            pages.data[page, at] = 255
+            q = rand(10, n, kv, dim, dtype=dtype)
+            out, _ = attend(pages, q, [n], left, right, 2)
+            pages.data[page, at] = was
+            out = out.cpu()
+            see = ref.visible(n, keys, left, right, 2)[:, t]
+            want, tol = ref.attention(q[:, h:h + 1], k[:, h:h + 1], v[:, h:h + 1], left, right, 2, dim ** -0.5)
+            got = out[:, h:h + 1]
+            bad = torch.zeros(got.shape, dtype=torch.bool)
+            bad[see, :, slice(None) if what == "k" else slice(32 * b, 32 * b + 32)] = True
+            assert torch.isnan(got[bad]).all()
+            close(torch.where(bad, want.to(dtype), got), want, tol)
+            others = torch.ones(kv, dtype=torch.bool)
+            others[h] = False
+            assert torch.isfinite(out[:, others].float()).all()
+
+
+@pytest.mark.parametrize("kv,n,keys", [(512, 256, 300), (128, 256, 4200)])
+def test_many_rows_over_pages_that_are_not_there(torch_cuda, kv, n, keys):
+    pages, held = random_cache(13, [keys], kv, 64, 32)
+    gone = [1, 3, (keys - 1) // 32] if keys < 1000 else [0, 70, 100]
+    for i, p in enumerate(gone):
+        pages.table[0, p] = [-1, pages.count, 1 << 30][i]
+    pages.upload()
+    q = rand(12, n, kv, 64, dtype=F16)
+    out, _ = attend(pages, q, [n], 130 if keys < 1000 else -1, 0, 40)
+    k, v = (t.clone() for t in held[0])
+    # keys that are not there: no query sees them
+    there = torch.ones(keys, dtype=torch.bool)
+    for p in gone:
+        there[32 * p:32 * p + 32] = False
+    see = ref.visible(n, keys, 130 if keys < 1000 else -1, 0, 40) & there
+    for h in (0, kv - 1):
+        s = (q[:, h].double() @ k[:, h].T / 8).masked_fill(~see, -math.inf)
+        p = torch.nan_to_num(torch.softmax(s, -1))
+        want = p @ v[:, h]
+        mag = (q[:, h].double().abs() @ k[:, h].abs().T / 8).amax(-1, keepdim=True)
+        tol = (p @ v[:, h].abs()) * (2 * mag * 68 * 2.0 ** -24 + 2.0 ** -11 + (keys / 16 + 32) * 2.0 ** -24)
+        tol += 2.0 ** -11 * want.abs() + 2.0 ** -25 * (1 + see.double() @ v[:, h].abs() + see.sum(1, keepdim=True) * want.abs())
+        close(out[:, h], want, tol)
 
 
 @pytest.mark.parametrize("max_kv", [0, 1, 1 << 40])
