@@ -502,7 +502,8 @@ typedef struct nemo_cache4_pages {
   void* data;                  /* device, 16-byte aligned */
   const int32_t* table;        /* device [count][table_row] */
   int64_t table_row;           /* pages of a request's row of the table: 0..2^23 */
-  const int32_t* kv_len;       /* device [count]: tokens of each request, those of this call's rows among them */
+  const int32_t* kv_len;       /* device [count]: tokens of each request, at most 2^30, those of this call's rows
+                                  among them */
 } nemo_cache4_pages;
 
 /* Key and value rows of requests' last tokens: rows q_start[b] .. q_start[b + 1]
@@ -534,8 +535,9 @@ nemo_status nemo_cache4_read(nemo_ctx* ctx, const nemo_cache4_config* config, co
 /* nemo_window_attention over a cache in pages: request b's queries are rows
  * q_start[b] .. q_start[b + 1] - 1 of q and out, its keys the kv_len[b] tokens of
  * the cache, and what a query sees goes by nemo_attention_config, whose kv_heads
- * and head_dim are the cache's. Keys and values are read as `type`, exactly
- * (F16 from 2^-14 to 65504; what lies above is infinite). Softmax sums and
+ * and head_dim are the cache's. Keys and values are read as `type`, exactly in
+ * BF16, and in F16 from 2^-14 on and to 65504 (rows that see what lies above are
+ * not finite). Softmax sums and
  * outputs are in 32 bits, the probabilities rounded to `type` for the product
  * with v. Keys and values that a query does not see reach its result in no
  * form, NaN neither. A request's rows are left as they were where it has none. */

@@ -56,7 +56,7 @@ struct Seen {
 // first request. A wave looks at 64 requests at a time, evenly over those that
 // it may be.
 struct Request {
-  int i, tile, q0, queries, keys;
+  int i, tile, q0, queries, behind, keys;  // behind: position of query 0; keys: tokens that the table has room for
   __device__ __forceinline__ Request(const AttendArgs& a, int t, int ROWS) {
     const int lane = threadIdx.x & 63;
     auto row = [&](int at) { return min(max(a.b.q_start[at], 0), (int)a.b.q_rows); };
@@ -69,7 +69,7 @@ struct Request {
       left = min(step, a.c.count - from);
     }
     const int at = min(from + lane, a.c.count - 1), begin = row(at), end = row(at + 1);
-    const int len = (int)min((int64_t)max(a.c.kv_len[at], 0), min(a.c.table_row << a.c.shift, (int64_t)1 << 30));
+    const int len = min(max(a.c.kv_len[at], 0), 1 << 30);
     const int first = number(begin, at);
     const int n = (int)__popcll(__builtin_amdgcn_ballot_w64(lane < left && first <= t));
     i = from + n - 1;
@@ -78,7 +78,9 @@ struct Request {
     tile = __builtin_amdgcn_readlane(first, of);
     q0 = __builtin_amdgcn_readlane(begin, of);
     queries = max(__builtin_amdgcn_readlane(end, of) - q0, 0);
-    keys = __builtin_amdgcn_readlane(len, of);
+    const int tokens = __builtin_amdgcn_readlane(len, of);
+    behind = tokens - queries;
+    keys = (int)min((int64_t)tokens, a.c.table_row << a.c.shift);
   }
 };
 
@@ -449,8 +451,7 @@ __global__ __launch_bounds__(64 * WAVES, QT == 1 ? 3 : 2) void cache4_attention_
   const int rows = r.queries * a.group, row0 = (tile_no - r.tile) * 16 * QT;
   if ((unsigned)row0 >= (unsigned)rows) return;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 4;
-  const int behind = r.keys - r.queries;  // position of query 0
-  auto window = [&](int row) { return Seen(a, behind + a.query(row), r.keys); };
+  auto window = [&](int row) { return Seen(a, r.behind + a.query(row), r.keys); };
   const Seen first = window(row0), last = window(min(row0 + 16 * QT, rows) - 1);
   const Blocks blocks(a, first, last);
   const int size = part.size(blocks.n), block0 = size * split, block1 = min(blocks.n, block0 + size);
@@ -465,7 +466,7 @@ __global__ __launch_bounds__(64 * WAVES, QT == 1 ? 3 : 2) void cache4_attention_
 #pragma unroll
   for (int i = 0; i < QT; ++i) {
     const int row = min(row0 + 16 * i + (lane & 15), rows - 1), query = a.query(row);
-    const Seen s(a, behind + query, r.keys);
+    const Seen s(a, r.behind + query, r.keys);
     lo[i] = s.lo;
     hi[i] = s.hi;
     if constexpr (!Rows16<T, D, QT>::IMAGE) {
@@ -554,9 +555,9 @@ __global__ __launch_bounds__(256) void cache4_join_kernel(AttendArgs a, Partials
   if (r.i < 0) return;
   const int row = tile_no - r.tile;
   if ((unsigned)row >= (unsigned)(r.queries * a.group)) return;
-  const int row0 = row / of * of, behind = r.keys - r.queries;
-  const Blocks blocks(a, Seen(a, behind + a.query(row0), r.keys),
-                      Seen(a, behind + a.query(min(row0 + of, r.queries * a.group) - 1), r.keys));
+  const int row0 = row / of * of;
+  const Blocks blocks(a, Seen(a, r.behind + a.query(row0), r.keys),
+                      Seen(a, r.behind + a.query(min(row0 + of, r.queries * a.group) - 1), r.keys));
   const int size = part.size(blocks.n), pieces = (blocks.n + size - 1) / size;
   if (pieces <= 1) return;  // the row is written
   const int i = a.query(row), head = kvh * a.group + (row - i * a.group);
@@ -621,7 +622,7 @@ __device__ __forceinline__ void careful_rows(const AttendArgs& a, const Partials
   typedef typename Mma16<T>::frag frag;
   const int lane = threadIdx.x & 63, h = lane >> 4;
   const int row = min(begin + (lane & 15), rows - 1), query = a.query(row), head = kvh * a.group + row - query * a.group;
-  const Seen mine(a, r.keys - r.queries + query, r.keys);
+  const Seen mine(a, r.behind + query, r.keys);
   const int lo[1] = {mine.lo}, hi[1] = {mine.hi};
   Rows16<T, D, 1> acc;
   const T* q = (const T*)a.b.q + (int64_t)(r.q0 + query) * a.b.q_row + (int64_t)head * a.b.q_head + h * (D / 4);
@@ -729,8 +730,7 @@ __global__ __launch_bounds__(256, 2) void cache4_tile_kernel(AttendArgs a, Parti
   const int rows = r.queries * a.group, row0 = (tile_no - r.tile) * ROWS;
   if ((unsigned)row0 >= (unsigned)rows) return;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), hl = lane >> 5;
-  const int behind = r.keys - r.queries;  // position of query 0
-  auto window = [&](int row) { return Seen(a, behind + a.query(row), r.keys); };
+  auto window = [&](int row) { return Seen(a, r.behind + a.query(row), r.keys); };
   const Seen all_first = window(row0), all_last = window(min(row0 + ROWS, rows) - 1);
   const Blocks blocks(a, all_first, all_last);
   const int size = part.size(blocks.n), block0 = size * blockIdx.y, block1 = min(blocks.n, block0 + size);

@@ -712,6 +712,30 @@ def test_pages_that_are_not_there_hold_no_keys(torch_cuda):
     assert not out[2].any()
 
 
+@pytest.mark.parametrize("heads,queries", [(4, 3), (256, 300)])
+def test_queries_behind_the_end_of_the_table(torch_cuda, heads, queries):
+    """A request of more tokens than its row of the table has room for: its
+    queries stand at its last tokens, and see what is there."""
+    dim, room, tokens = 64, 96, 100
+    pages, held = random_cache(17, [room], heads, dim, 32)
+    pages.kv_lens = [tokens]
+    pages.upload()
+    q = rand(18, queries, heads, dim, dtype=F16)
+    for left in (-1, 7):
+        out, _ = attend(pages, q, [queries], left, 0, 0)
+        k, v = (torch.cat([t, torch.zeros(tokens - room, *t.shape[1:])]) for t in held[0])
+        see = ref.visible(queries, tokens, left, 0, 0)
+        see[:, room:] = False
+        for h in (0, heads - 1):
+            s = (q[:, h].double() @ k[:, h].T / 8).masked_fill(~see, -math.inf)
+            p = torch.nan_to_num(torch.softmax(s, -1))
+            want = p @ v[:, h]
+            mag = (q[:, h].double().abs() @ k[:, h].abs().T / 8).amax(-1, keepdim=True)
+            tol = (p @ v[:, h].abs()) * (2 * mag * 68 * 2.0 ** -24 + 2.0 ** -11 + (tokens / 16 + 32) * 2.0 ** -24)
+            tol += 2.0 ** -11 * want.abs() + 2.0 ** -25 * (1 + see.double() @ v[:, h].abs() + see.sum(1, keepdim=True) * want.abs())
+            close(out[:, h], want, tol)
+
+
 def test_a_strong_key_and_a_long_even_cache(torch_cuda):
     """f16's probabilities far below the largest keep their share: one key some
     17 above 4000 even ones."""
@@ -877,3 +901,50 @@ def test_results_do_not_change_from_call_to_call(torch_cuda):
     for _ in range(3):
         again, _ = attend(pages, q, [20, 20])
         assert torch.equal(first, again)
+
+
+def test_captured_calls_equal_eager_ones(torch_cuda):
+    """A product, an append and a split attention in one graph, replayed with
+    other contents and lengths, eager work between the replays."""
+    pages, _ = random_cache(33, [6000, 4000], 2, 128, 64)
+    pages.data[pages.data == 255] = 0
+    x, xs = rows8(34, 2, 512)
+    w, ws = rows8(35, 12 * 128, 512)
+    dx, dxs, dw, dws = (t.cuda() for t in (x, xs, w, ws))
+    rope = ops.Rope(ops.rope_config(128))
+    config = ops.attention_config(8, 2, 128, ops.TYPE_F16, right=0)
+    start, qkv = starts([1, 1]), torch.zeros(2, 12, 128, dtype=F16, device="cuda")
+    out = torch.zeros(2, 8, 128, dtype=F16, device="cuda")
+    need = pages.cache.workspace_bytes(config, 2, 2, 6000)
+    space = torch.empty(need, dtype=torch.uint8, device="cuda")
+    assert need
+    args = ops.matmul8_args(ops.TYPE_F16, 2, 1536, 512, dx.data_ptr(), dxs.data_ptr(), dw.data_ptr(), dws.data_ptr(), qkv.data_ptr())
+    matmul8 = ops.Matmul8()
+
+    def step():
+        s = stream()
+        matmul8.run(args, stream=s)
+        pages.cache.append(pages.pages, ops.cache4_rows(ops.TYPE_F16, 2, start.data_ptr(), side(qkv[:, 8:10]), side(qkv[:, 10:])),
+                           rope, stream=s)
+        pages.cache.attention(config, pages.pages, ops.cache4_queries(2, 6000, start.data_ptr(), side(qkv[:, :8]), side(out),
+                                                                      space.data_ptr(), need), stream=s)
+
+    step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    before = pages.data.clone()
+    for i in range(4):
+        dx.copy_(rows8(40 + i, 2, 512)[0])
+        pages.d_len.copy_(ints(6000 - 700 * i, 4000 - 1300 * i))
+        pages.data.copy_(before)
+        space.fill_(255)
+        out.fill_(7.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        replayed = out.clone(), pages.data.clone()
+        pages.data.copy_(before)
+        step()
+        torch.cuda.synchronize()
+        assert torch.equal(replayed[0], out) and torch.equal(replayed[1], pages.data) and torch.isfinite(out.float()).all()
