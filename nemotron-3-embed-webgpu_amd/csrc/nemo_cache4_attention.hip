@@ -905,8 +905,9 @@ __global__ __launch_bounds__(256, 2) void cache4_tile_kernel(AttendArgs a, Parti
 //  187 : 149).
 //  Between: 32 (32 x 32, 5000 keys 172 : 136 : 190; 512 of 512 15 : 12.5 : 18; 64 over 5000
 //  keys 27 : 24 : 28; 128 over 5000 34 : 31 : 35; 512 over 5000 83 : 66 : 68).
-// A split costs a second launch and is taken from 72 blocks on (one token: 5000 keys
-// 19.6 whole, 12 in pieces of 16 blocks; 1028 keys 8.5 and 11.3), into pieces that fill
+// A split costs a second launch and is taken from 48 blocks on, 72 where there are 128
+// tiles (one token: 5000 keys 19.6 whole, 12.4 in pieces of 16 blocks, 2000 keys 16.0 and
+// 12.4, 1400 12.3 and 12.7; 200 queries, 2000 keys 23 and 33), into pieces that fill
 // the chip 16 times over for single tokens, whose requests' lengths differ (64 tokens over
 // their caches: 768 pieces 263, 1536 252, 2048 231, 4096 219 to 227, 8192 235), twice
 // for more rows, whose sums are written and read again (512 over 5000 keys: 512 pieces
@@ -925,7 +926,7 @@ Plan plan_of(const nemo_attention_config& c, int count, int64_t q_rows, int64_t 
   int tile = rows / count <= 32 ? 16 : 32;
   if (rows / count >= 256 && (tiles_of(128) >= 512 || blocks * tiles_of(128) >= 512 * 64)) tile = 128;
   const int64_t work = blocks * tiles_of(tile);
-  if (blocks <= 72) return {tile, 1, (int)blocks};
+  if (blocks <= (tiles_of(tile) < 128 ? 48 : 72)) return {tile, 1, (int)blocks};
   const int64_t piece = std::max<int64_t>({16, std::min<int64_t>(64, work / 1024), work / (tile == 16 ? 4096 : 512) + 1,
                                            (blocks + 63) / 64});
   return {tile, (int)((blocks + piece - 1) / piece), (int)piece};
