@@ -398,20 +398,18 @@ __device__ __forceinline__ void attend_blocks(const AttendArgs& a, Rows16<T, D, 
     }
     attend<CAREFUL>(acc, raw, a.scale2, hide, seen, any);
   };
-  // AHEAD steps are in flight behind the one that is worked on.
-  constexpr int AHEAD = QT == 1 && !CAREFUL ? 2 : 1;
-  Raw<D> raw[AHEAD + 1];
-  bool there[AHEAD + 1];
-#pragma unroll
-  for (int i = 0; i < AHEAD; ++i) there[i] = load(raw[i], i);
-  for (int n = 0; n < steps; ++n) {
-    there[AHEAD] = load(raw[AHEAD], n + AHEAD);
+  // The next step's codes are in flight while one is worked on. (Two steps ahead, with
+  // registers moved from step to step, 64 tokens over their caches took 222 us, one
+  // ahead 218, without the moves 213.)
+  Raw<D> raw[2];
+  bool there[2];
+  there[0] = load(raw[0], 0);
+  for (int n = 0; n < steps; n += 2) {
+    there[1] = load(raw[1], n + 1);
     if (there[0]) step(raw[0], n);
-#pragma unroll
-    for (int i = 0; i < AHEAD; ++i) {
-      raw[i] = raw[i + 1];
-      there[i] = there[i + 1];
-    }
+    if (n + 1 >= steps) break;
+    there[0] = load(raw[0], n + 2);
+    if (there[1]) step(raw[1], n + 1);
   }
 }
 
@@ -433,8 +431,8 @@ struct Partials {
 // whose sums they add in LDS. Where a tile has more blocks than a piece, each piece
 // is a workgroup, and a second kernel joins their sums.
 //
-// Bound by memory over long caches: 64 tokens over 1.08 GB of 4-bit keys and values 218
-// us (4.9 TB/s; a copy reaches 4.9 to 5.2), one over 131072 keys 28 us (5.1 TB/s) and
+// Bound by memory over long caches: 64 tokens over 1.08 GB of 4-bit keys and values 213
+// us (5.1 TB/s; a copy reaches 4.9 to 5.2), one over 131072 keys 27 us (5.3 TB/s) and
 // its join 4 to 5; by latency below. With one step in flight, a wait for each
 // page's number and registers copied between the two files it was 408. The split
 // by pieces and not by shares of each request's keys gave 293 -> 227.
