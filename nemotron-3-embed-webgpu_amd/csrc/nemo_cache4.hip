@@ -9,9 +9,9 @@
 // So both ends of 2^-20 around it are coded, and where two codes or powers differ
 // (about one in fifty) the wave takes the rotation again in 64 bits.
 //
-// Bound by memory and by its instructions in equal parts: 31846 tokens of 8 KV
-// heads of 128 f16, 165 MB of rows and codes, 54 us (3.1 TB/s) to append and 31
-// (5.3 TB/s) to read. In 64 bits throughout they took 103 and, with codes taken
+// Appending is bound by its instructions, 70 % of the cycles, and then by memory:
+// 31846 tokens of 8 KV heads of 128 f16, 165 MB of rows and codes, 52 us (3.2 TB/s)
+// to append and 31 (5.3 TB/s) to read. In 64 bits throughout they took 103 and, with codes taken
 // apart bit by bit, 40.
 //
 // A wave takes a token. Lane l computes the angle of pair l, which the 16 lanes
