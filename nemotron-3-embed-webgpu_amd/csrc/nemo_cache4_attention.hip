@@ -762,7 +762,9 @@ __global__ __launch_bounds__(256, 2) void cache4_tile_kernel(AttendArgs a, Parti
   if (count) {
     for (int b = lane << per; b < count + (1 << per); b += 64 << per)
       if ((unsigned)page_of(b) >= (unsigned)a.c.pages) missing = true;
-    if ((unsigned)page_of(blocks.sinks - block0) >= (unsigned)a.c.pages) missing = true;  // the window's first
+    // the sinks' last and the window's first, which those steps may pass over
+    if ((unsigned)page_of(blocks.sinks - 1 - block0) >= (unsigned)a.c.pages) missing = true;
+    if ((unsigned)page_of(blocks.sinks - block0) >= (unsigned)a.c.pages) missing = true;
   }
   missing = __builtin_amdgcn_ballot_w64(missing) != 0;
   uint8_t* const rows_image = lds[wave >> 1][1] + (wave & 1) * IMG;

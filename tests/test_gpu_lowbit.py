@@ -623,6 +623,32 @@ def test_many_rows_over_pages_that_are_not_there(torch_cuda, kv, n, keys):
         close(out[:, h], want, tol)
 
 
+@pytest.mark.parametrize("sinks", [2944, 2976, 3104])
+def test_pieces_that_begin_inside_a_page_of_the_sinks(torch_cuda, sinks):
+    """Two pieces of a tile's keys, the second from inside a page of the sinks
+    on, whose last page is not there."""
+    kv, n, keys, left = 128, 256, 5601, 2000
+    pages, held = random_cache(19, [keys], kv, 64, 128)
+    gone = (sinks - 1) // 128
+    pages.table[0, gone] = 1 << 30
+    pages.upload()
+    q = rand(20, n, kv, 64, dtype=F16)
+    out, need = attend(pages, q, [n], left, 0, sinks)
+    assert need > 0
+    there = torch.ones(keys, dtype=torch.bool)
+    there[128 * gone:128 * gone + 128] = False
+    see = ref.visible(n, keys, left, 0, sinks) & there
+    k, v = held[0]
+    for h in (0, kv - 1):
+        s = (q[:, h].double() @ k[:, h].T / 8).masked_fill(~see, -math.inf)
+        p = torch.softmax(s, -1)
+        want = p @ v[:, h]
+        mag = (q[:, h].double().abs() @ k[:, h].abs().T / 8).amax(-1, keepdim=True)
+        tol = (p @ v[:, h].abs()) * (2 * mag * 68 * 2.0 ** -24 + 2.0 ** -11 + (keys / 16 + 32) * 2.0 ** -24)
+        tol += 2.0 ** -11 * want.abs() + 2.0 ** -25 * (1 + see.double() @ v[:, h].abs() + see.sum(1, keepdim=True) * want.abs())
+        close(out[:, h], want, tol)
+
+
 @pytest.mark.parametrize("max_kv", [0, 1, 1 << 40])
 def test_max_kv_is_a_hint(torch_cuda, max_kv):
     pages, held = random_cache(4, [700, 5], 1, 64, 32)
