@@ -6,13 +6,16 @@
 // bits. A rotation is not: an angle's remainder and its sine in 32 bits, the
 // factor and two products leave it some 10 2^-24 of |a| + |b| off, and next to a
 // border between codes it is decided wrongly a few times in a million values.
-// So both ends of 2^-20 around it are coded, and where two codes or powers differ
-// (about one in fifty) the wave takes the rotation again in 64 bits.
+// So both ends of 2^-20 around it are coded, and from the first heads on whose codes
+// or powers differ the wave takes the token's rotation again in 64 bits, behind the
+// others: beside them it held registers for all, and its sines were taken by all.
 //
-// Appending is bound by its instructions, 70 % of the cycles, and then by memory:
-// 31846 tokens of 8 KV heads of 128 f16, 165 MB of rows and codes, 52 us (3.2 TB/s)
-// to append and 31 (5.3 TB/s) to read. In 64 bits throughout they took 103 and, with codes taken
-// apart bit by bit, 40.
+// Appending is bound by its instructions, half of the cycles, and by memory: 31846
+// tokens of 8 KV heads of 128 f16, 165 MB of rows and codes, 45 us (3.7 TB/s), and 31
+// (5.3 TB/s) to read. On the way: in 64 bits throughout 103; bounds in 32 bits, the rare
+// path among them 52; values to codes by one conversion, without a product 48; the
+// token looked up while its rows are on their way 45. (Several tokens a wave, which
+// share the lookup, took more registers than it returned.)
 //
 // A wave takes a token. Lane l computes the angle of pair l, which the 16 lanes
 // of a head pick up from LDS: lane l's head is l / 16 (of four at a time), its
@@ -30,16 +33,17 @@ struct RowsArgs {
   nemo_cache4_rows r;
   Cache4 c;
   RopeAngles angles;  // turns null: keys as they are
-  bool wide;          // a lane's D / 16 values may be read and written as one vector
 };
 
 // A row's token of its request, none (-1) for rows before the first request and
 // behind the last and for those before token 0, and the token's page, none (-1)
 // for those that are not there. A wave looks at 64 requests at a time, evenly over
-// those that it may be.
+// those that it may be; what `meanwhile` loads is not waited for.
 struct Token {
   int at, page;
-  __device__ __forceinline__ Token(const Cache4& c, const int32_t* q_start, int64_t rows, int64_t t) {
+  template <typename Meanwhile>
+  __device__ __forceinline__ Token(const Cache4& c, const int32_t* q_start, int64_t rows, int64_t t,
+                                   Meanwhile&& meanwhile) {
     const int lane = threadIdx.x & 63;
     auto row = [&](int at) { return (int64_t)min((int64_t)max(q_start[at], 0), rows); };
     int from = 0, left = c.count;
@@ -50,7 +54,12 @@ struct Token {
       left = min(step, c.count - from);
     }
     const int i = min(from + lane, c.count - 1);
-    const int begin = (int)row(i), end = (int)row(i + 1), len = c.kv_len[i];
+    const int starts = q_start[i], ends = q_start[i + 1], len = c.kv_len[i];
+    __builtin_amdgcn_sched_barrier(0);
+    meanwhile();
+    __builtin_amdgcn_sched_barrier(0);
+    auto cut = [&](int at) { return (int)min((int64_t)max(at, 0), rows); };
+    const int begin = cut(starts), end = cut(ends);
     const int n = (int)__popcll(__builtin_amdgcn_ballot_w64(lane < left && begin <= t));
     const int of = max(n - 1, 0);
     const int end_of = __builtin_amdgcn_readlane(end, of);
@@ -89,34 +98,56 @@ __device__ __forceinline__ float odd(double v) {
   return __uint_as_float(bits);
 }
 
-// Codes of N values, two a byte.
-template <int N>
-__device__ __forceinline__ uint32_t codes_of(const float (&u)[N]) {
-  uint32_t c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(0u, u[0], u[1], 1.0f, 0);
-  c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, u[2], u[3], 1.0f, 1);
-  if constexpr (N == 8) {
-    c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, u[4], u[5], 1.0f, 2);
-    c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, u[6], u[7], 1.0f, 3);
-  }
+// Codes of N values over the power of two `scale`, two a byte: one division and one
+// rounding, from 16 and 32 bits alike.
+template <int B>
+__device__ __forceinline__ uint32_t code_pair(uint32_t c, float a, float b, float scale) {
+  return __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, a, b, scale, B);
+}
+template <int B>
+__device__ __forceinline__ uint32_t code_pair(uint32_t c, half_t a, half_t b, float scale) {
+  return __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(c, half2v{a, b}, scale, B);
+}
+template <int B>
+__device__ __forceinline__ uint32_t code_pair(uint32_t c, bf16_t a, bf16_t b, float scale) {
+  typedef bf16_t pair __attribute__((ext_vector_type(2)));
+  return __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(c, pair{a, b}, scale, B);
+}
+template <typename T, int N>
+using Vec = T __attribute__((ext_vector_type(N)));
+template <int N, typename V>
+__device__ __forceinline__ uint32_t codes_of(const V& u, float scale) {
+  uint32_t c = code_pair<1>(code_pair<0>(0u, u[0], u[1], scale), u[2], u[3], scale);
+  if constexpr (N == 8) c = code_pair<3>(code_pair<2>(c, u[4], u[5], scale), u[6], u[7], scale);
   return c;
+}
+
+// The bits of the largest |value| in 32 bits; those of NaN are larger than any.
+template <typename T, int N>
+__device__ __forceinline__ uint32_t peak_of(const Vec<T, N>& x) {
+  if constexpr (std::is_same<T, float>::value) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) m = max(m, __float_as_uint(x[i]) & 0x7fffffffu);
+    return m;
+  } else {
+    const Vec<unsigned short, N> bits = __builtin_bit_cast(Vec<unsigned short, N>, x) & (unsigned short)0x7fff;
+    Vec<unsigned short, 2> m = bits.xy;
+#pragma unroll
+    for (int i = 2; i < N; i += 2) m = __builtin_elementwise_max(m, Vec<unsigned short, 2>{bits[i], bits[i + 1]});
+    return __float_as_uint((float)__builtin_bit_cast(T, m[0] > m[1] ? m[0] : m[1]));
+  }
 }
 
 // s of 32 values whose largest has exponent e, biased by `bias`, and a fraction of
 // 1.75 or less or more: 2^(e - bias) (1 + f) is at most 7 2^s = 1.75 2^(s + 2).
 __device__ __forceinline__ int power_of(int e, int bias, bool more) { return min(max(e - bias - 2 + more, -126), 125); }
-__device__ __forceinline__ float inverse(int s) { return __uint_as_float((uint32_t)(127 - s) << 23); }
+__device__ __forceinline__ float two_to(int s) { return __uint_as_float((uint32_t)(127 + s) << 23); }
 
 template <typename T, int N>
-__device__ __forceinline__ void load_piece(const T* x, bool wide, T (&v)[N]) {
-  typedef T vec __attribute__((ext_vector_type(N)));
-  if (wide) {
-    const vec t = *(const vec*)x;
+__device__ __forceinline__ void load_piece(const T* x, Vec<T, N>& v) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = t[i];
-  } else {
-#pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = x[i];
-  }
+  for (int i = 0; i < N; ++i) v[i] = x[i];  // (one load: the card takes any address)
 }
 
 // How keys are turned: not; neighbouring pairs; halves of which a lane has values
@@ -133,40 +164,47 @@ __global__ __launch_bounds__(256) void cache4_append_kernel(RowsArgs a) {
   const int64_t t = (int64_t)blockIdx.x * 4 + wave;
   if (t >= a.r.rows) return;  // (no barrier follows: a wave has its own angles)
   const int n = lane & 15, pairs = TURN == kPlain ? 0 : a.angles.rotary / 2, heads = a.c.kv_heads;
-  // Of a turned value: whether it is its pair's second, and where the first is.
-  auto second = [&](int d) { return TURN == kPairs ? d & 1 : (TURN == kHalves ? N * n : d) >= pairs; };
-  auto pair_of = [&](int d) { return TURN == kPairs ? d >> 1 : second(d) ? d - pairs : d; };
-  struct Piece {
-    T x[N], other[N];
+  // Of value i of the lane's: whether it is turned, and if so, whether it is its pair's second and which
+  // pair (else any).
+  const int half = N * n >= pairs ? N * n - pairs : N * n;
+  auto is_turned = [&](int i) { return N * n + (TURN == kPairs ? i & ~1 : TURN == kHalves ? 0 : i) < 2 * pairs; };
+  auto second = [&](int i) { return TURN == kPairs ? i & 1 : N * n + (TURN == kHalves ? 0 : i) >= pairs; };
+  auto pair_of = [&](int i) {
+    return TURN == kPairs ? N / 2 * n + i / 2 : TURN == kHalves ? min(half, 64 - N) + i
+                                                                : min(N * n + i - (second(i) ? pairs : 0), 63);
   };
+  struct Piece {
+    Vec<T, N> x, other;
+  };
+  // (Lanes past the last head load its values too, and write nothing.)
   auto load_key = [&](Piece& p, int h) {
-    if (h >= heads) return;
-    const T* x = (const T*)a.r.k + t * a.r.k_row + h * a.r.k_head;
-    load_piece<T, N>(x + N * n, a.wide, p.x);
+    const T* x = (const T*)a.r.k + t * a.r.k_row + min(h, heads - 1) * a.r.k_head;
+    load_piece<T, N>(x + N * n, p.x);
     if constexpr (TURN == kHalves) {
-      if (N * n < 2 * pairs) load_piece<T, N>(x + (N * n >= pairs ? N * n - pairs : N * n + pairs), true, p.other);
+      load_piece<T, N>(x + (!is_turned(0) ? N * n : second(0) ? half : N * n + pairs), p.other);
     } else if constexpr (TURN == kHalvesAny) {
 #pragma unroll
       for (int i = 0; i < N; ++i) {
         const int d = N * n + i;
-        if (d < 2 * pairs) p.other[i] = x[d >= pairs ? d - pairs : d + pairs];
+        p.other[i] = x[!is_turned(i) ? d : second(i) ? d - pairs : d + pairs];
       }
     }
   };
   auto load_value = [&](Piece& p, int h) {
-    if (h < heads) load_piece<T, N>((const T*)a.r.v + t * a.r.v_row + h * a.r.v_head + N * n, a.wide, p.x);
+    load_piece<T, N>((const T*)a.r.v + t * a.r.v_row + min(h, heads - 1) * a.r.v_head + N * n, p.x);
   };
   Piece key, value, next;
   int h0 = 4 * blockIdx.y, h = h0 + (lane >> 4);
-  load_key(key, h);
-  load_value(value, h);
   double turns = 0;  // whole turns of pair `lane` a position, then at the token's, less the whole ones
   int64_t position = 0;
   if constexpr (TURN != kPlain) {
-    if (lane < pairs) turns = a.angles.turns[lane];
+    turns = a.angles.turns[min(lane, pairs - 1)];
     if (a.r.positions) position = a.r.positions[t];
   }
-  const Token token(a.c, a.r.q_start, a.r.rows, t);
+  const Token token(a.c, a.r.q_start, a.r.rows, t, [&] {
+    load_key(key, h);
+    load_value(value, h);
+  });
   if (token.at < 0 || token.page < 0) return;
   const int in = token.at & ((1 << a.c.shift) - 1);
   if constexpr (TURN != kPlain) {
@@ -190,103 +228,100 @@ __global__ __launch_bounds__(256) void cache4_append_kernel(RowsArgs a) {
     if (n % LANES == 0) to[Head::scale(a.c.shift, is_value, in, n / LANES)] = bad ? 255 : (uint8_t)(s + 127);
   };
   auto power32 = [](uint32_t bits) { return power_of((int)(bits >> 23), 127, (bits & 0x7fffff) > 0x600000); };
-  // Values that are in 32 bits what they are.
+  // Values as they are.
   auto plain = [&](const Piece& piece, bool is_value, bool real) {
-    float u[N];
-    uint32_t peak = 0;
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      u[i] = real ? (float)piece.x[i] : 0.f;
-      peak = max(peak, __float_as_uint(u[i]) & 0x7fffffffu);
-    }
-    peak = lanes_max<LANES>(peak);
+    const uint32_t peak = lanes_max<LANES>(peak_of<T, N>(piece.x));
     const int s = power32(peak);
-    const float inv = inverse(s);
-#pragma unroll
-    for (int i = 0; i < N; ++i) u[i] *= inv;
-    const uint32_t codes = codes_of<N>(u);
+    const uint32_t codes = codes_of<N>(piece.x, two_to(s));
     if (real) write(is_value, codes, s, peak >= 0x7f800000u);
   };
-  bool exact = false;  // whether angles64 holds the token's
-  auto turned = [&](const Piece& piece, bool real) {
-    float u[N], most[N], peak = 0.f, error = 0.f, finite = 0.f;
+  const float rel = fabsf(a.angles.magnitude) * 0x1p-20f;
+  // In 32 bits; whether that is enough. `whole`: every value is turned.
+  auto turned = [&](const Piece& piece, bool real, auto whole) {
+    // `all`: at least any |a| + |b|, and not finite where a value is not
+    float u[N], low[N], high[N], peak = 0.f, all = 0.f;
+    asm volatile("" ::: "memory");  // read the angles here: for all heads they would take 2 N registers
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const int d = N * n + i;
-      const float own = real ? (float)piece.x[i] : 0.f;
-      u[i] = own;
-      most[i] = 0.f;
-      if (d < 2 * pairs) {
-        const float other = real ? (float)(TURN == kPairs ? piece.x[i ^ 1] : piece.other[i]) : 0.f;
-        const float2 cs = angles[wave][pair_of(d)];
-        u[i] = fmaf(other, second(d) ? cs.y : -cs.y, own * cs.x);
-        most[i] = fabsf(own) + fabsf(other);
+      const float own = (float)piece.x[i];
+      const float other = (float)(TURN == kPairs ? piece.x[i ^ 1] : piece.other[i]);
+      const float2 by = angles[wave][pair_of(i)];
+      float most = fabsf(own) + fabsf(other), add = TURN == kPairs && i & 1 ? 0.f : most;
+      u[i] = fmaf(other, second(i) ? by.y : -by.y, own * by.x);
+      if (!decltype(whole)::value && !is_turned(i)) {
+        most = 0.f;
+        add = fabsf(own);
+        u[i] = own;
       }
+      all += add;
       peak = fmaxf(peak, fabsf(u[i]));
-      error = fmaxf(error, most[i]);
-      finite = fmaf(u[i], 0.f, finite);
+      low[i] = fmaf(-most, rel, u[i]);
+      high[i] = fmaf(most, rel, u[i]);
     }
-    const float rel = fabsf(a.angles.magnitude) * 0x1p-20f;
     peak = __uint_as_float(lanes_max<LANES>(__float_as_uint(peak)));
-    error = __uint_as_float(lanes_max<LANES>(__float_as_uint(error))) * rel;
-    int s = power32(__float_as_uint(peak));
-    const float inv = inverse(s), off = rel * inv;
-    float low[N], high[N];
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const float v = u[i] * inv;
-      low[i] = fmaf(-most[i], off, v);
-      high[i] = fmaf(most[i], off, v);
-    }
-    uint32_t codes = codes_of<N>(low);
-    bool unsure = codes != codes_of<N>(high) || !(peak + error < INFINITY) || finite != 0.f ||
+    all = __uint_as_float(lanes_max<LANES>(__float_as_uint(all)));
+    const float error = all * rel;
+    const int s = power32(__float_as_uint(peak));
+    const uint32_t codes = codes_of<N>(low, two_to(s));
+    // (what is small enough to lose bits in 32 is taken again too)
+    const bool unsure = codes != codes_of<N>(high, two_to(s)) || !(peak + error < INFINITY) || (peak < 0x1p-100f && all != 0.f) ||
                   power32(__float_as_uint(fmaxf(peak - error, 0.f))) != power32(__float_as_uint(peak + error));
-    bool bad = false;
-    if (__builtin_amdgcn_ballot_w64(unsure)) {
-      asm volatile("");  // keeps the rare path a branch
-      if (!exact) {
-        if (lane < pairs) {
-          double s64, c64;
-          sincospi(2.0 * turns, &s64, &c64);
-          angles64[wave][lane] = make_double2(c64 * a.angles.magnitude, s64 * a.angles.magnitude);
-        }
-        __builtin_amdgcn_wave_barrier();
-        exact = true;
-      }
-      double v[N];
-      uint64_t m = 0;
-#pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const int d = N * n + i;
-        const double own = real ? (double)(float)piece.x[i] : 0.0;
-        v[i] = own;
-        if (d < 2 * pairs) {
-          const double other = real ? (double)(float)(TURN == kPairs ? piece.x[i ^ 1] : piece.other[i]) : 0.0;
-          const double2 cs = angles64[wave][pair_of(d)];
-          v[i] = fma(other, second(d) ? cs.y : -cs.y, own * cs.x);
-        }
-        m = max(m, __builtin_bit_cast(uint64_t, v[i]) & 0x7fffffffffffffffull);
-      }
-      m = lanes_max<LANES>(m);
-      bad = m >= 0x7ff0000000000000ull;
-      s = power_of((int)(m >> 52), 1023, (m & 0xfffffffffffffull) > 0xc000000000000ull);
-      const double inv64 = __builtin_bit_cast(double, (uint64_t)(1023 - s) << 52);
-#pragma unroll
-      for (int i = 0; i < N; ++i) u[i] = odd(v[i] * inv64);
-      codes = codes_of<N>(u);
-    }
-    if (real) write(false, codes, s, bad);
+    if (real) write(false, codes, s, false);
+    return !unsure;
   };
   // (All lanes stay in the loops: a wave votes, and lanes exchange. Those past the last head write nothing.)
+  int again = heads;  // where heads begin that 32 bits are not enough for
   for (; h0 < heads; h0 += by, h += by) {
+    const bool more = h0 + by < heads;
     load_key(next, h + by);
-    if constexpr (TURN == kPlain) plain(key, false, h < heads);
-    else turned(key, h < heads);
+    if constexpr (TURN == kPlain) {
+      plain(key, false, h < heads);
+    } else {
+      const bool enough = 2 * pairs == D ? turned(key, h < heads, std::true_type{})
+                                         : turned(key, h < heads, std::false_type{});
+      if (__builtin_amdgcn_ballot_w64(!enough)) again = min(again, h0);
+    }
     key = next;
     load_value(next, h + by);
     plain(value, true, h < heads);
     value = next;
     to += step;
+  }
+  if constexpr (TURN != kPlain) {
+    if (again >= heads) return;
+    asm volatile("" : "+v"(turns));  // keeps the rare path's sines off the others' way
+    if (lane < pairs) {
+      double s, c;
+      sincospi(2.0 * turns, &s, &c);
+      angles64[wave][lane] = make_double2(c * a.angles.magnitude, s * a.angles.magnitude);
+    }
+    __builtin_amdgcn_wave_barrier();
+    h = again + (lane >> 4);
+    to = a.c.data + a.c.head<D>(token.page, h);
+    for (h0 = again; h0 < heads; h0 += by, h += by, to += step) {
+      load_key(key, h);
+      double v[N];
+      uint64_t m = 0;
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        asm volatile("" ::: "memory");  // one by one: fewer registers
+        const double own = (double)(float)key.x[i];
+        v[i] = own;
+        if (is_turned(i)) {
+          const double other = (double)(float)(TURN == kPairs ? key.x[i ^ 1] : key.other[i]);
+          const double2 cs = angles64[wave][pair_of(i)];
+          v[i] = fma(other, second(i) ? cs.y : -cs.y, own * cs.x);
+        }
+        m = max(m, __builtin_bit_cast(uint64_t, v[i]) & 0x7fffffffffffffffull);
+      }
+      m = lanes_max<LANES>(m);
+      const int s = power_of((int)(m >> 52), 1023, (m & 0xfffffffffffffull) > 0xc000000000000ull);
+      const double inv = __builtin_bit_cast(double, (uint64_t)(1023 - s) << 52);
+      float u[N];
+#pragma unroll
+      for (int i = 0; i < N; ++i) u[i] = odd(v[i] * inv);
+      if (h < heads) write(false, codes_of<N>(u, 1.f), s, m >= 0x7ff0000000000000ull);
+    }
   }
 }
 
@@ -309,11 +344,10 @@ template <typename T, int D>
 __global__ __launch_bounds__(256) void cache4_read_kernel(RowsArgs a) {
   typedef Cache4Head<D> Head;
   constexpr int N = D / 16;
-  typedef T vec __attribute__((ext_vector_type(N)));
   const int lane = threadIdx.x & 63;
   const int64_t t = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (t >= a.r.rows) return;
-  const Token token(a.c, a.r.q_start, a.r.rows, t);
+  const Token token(a.c, a.r.q_start, a.r.rows, t, [] {});
   if (token.at < 0) return;
   const int in = token.at & ((1 << a.c.shift) - 1), n = lane & 15;
 #pragma unroll 2
@@ -336,21 +370,9 @@ __global__ __launch_bounds__(256) void cache4_read_kernel(RowsArgs a) {
       decode<T, 3>(codes, power, v[6], v[7]);
     }
     T* x = (value ? (T*)a.r.v + t * a.r.v_row + kvh * a.r.v_head : (T*)a.r.k + t * a.r.k_row + kvh * a.r.k_head) + N * n;
-    if (a.wide) {
-      vec w;
 #pragma unroll
-      for (int i = 0; i < N; ++i) w[i] = v[i];
-      *(vec*)x = w;
-    } else {
-#pragma unroll
-      for (int i = 0; i < N; ++i) x[i] = v[i];
-    }
+    for (int i = 0; i < N; ++i) x[i] = v[i];  // (one store, as load_piece)
   }
-}
-
-bool wide(const nemo_cache4_config& c, const nemo_cache4_rows& r) {
-  const int n = c.head_dim / 16, bytes = n * (r.type == NEMO_TYPE_F32 ? 4 : 2);
-  return (((uintptr_t)r.k | (uintptr_t)r.v) & (bytes - 1)) == 0 && (r.k_row | r.k_head | r.v_row | r.v_head) % n == 0;
 }
 
 // Waves of a token: one, but for few tokens one for every 4 of `heads` heads (64 tokens of 8 KV
@@ -376,14 +398,14 @@ hipError_t by_type(int type, int head_dim, Launch&& launch) {
 hipError_t launch_cache4_append(const nemo_cache4_config& c, const nemo_cache4_pages& p, const nemo_cache4_rows& r,
                                 const RopeAngles* angles, hipStream_t stream) {
   if (p.count == 0 || r.rows == 0) return hipSuccess;
-  const RowsArgs a{r, Cache4(c, p), angles ? *angles : RopeAngles{}, wide(c, r)};
+  const RowsArgs a{r, Cache4(c, p), angles ? *angles : RopeAngles{}};
   return by_type(r.type, c.head_dim, [&](auto t, auto d) {
     const dim3 grid = grid_of(r.rows, c.kv_heads);
     typedef decltype(t) T;
     constexpr int D = decltype(d)::value;
     if (!angles) cache4_append_kernel<T, D, kPlain><<<grid, 256, 0, stream>>>(a);
     else if (!angles->half) cache4_append_kernel<T, D, kPairs><<<grid, 256, 0, stream>>>(a);
-    else if (a.wide && angles->rotary / 2 % (D / 16) == 0) cache4_append_kernel<T, D, kHalves><<<grid, 256, 0, stream>>>(a);
+    else if (angles->rotary / 2 % (D / 16) == 0) cache4_append_kernel<T, D, kHalves><<<grid, 256, 0, stream>>>(a);
     else cache4_append_kernel<T, D, kHalvesAny><<<grid, 256, 0, stream>>>(a);
   });
 }
@@ -391,7 +413,7 @@ hipError_t launch_cache4_append(const nemo_cache4_config& c, const nemo_cache4_p
 hipError_t launch_cache4_read(const nemo_cache4_config& c, const nemo_cache4_pages& p, const nemo_cache4_rows& r,
                               hipStream_t stream) {
   if (p.count == 0 || r.rows == 0) return hipSuccess;
-  const RowsArgs a{r, Cache4(c, p), RopeAngles{}, wide(c, r)};
+  const RowsArgs a{r, Cache4(c, p), RopeAngles{}};
   return by_type(r.type, c.head_dim, [&](auto t, auto d) {
     cache4_read_kernel<decltype(t), decltype(d)::value><<<grid_of(r.rows, 2 * c.kv_heads), 256, 0, stream>>>(a);
   });
