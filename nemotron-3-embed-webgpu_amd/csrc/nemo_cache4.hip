@@ -263,16 +263,14 @@ __global__ __launch_bounds__(256) void cache4_append_kernel(RowsArgs a) {
     const float error = all * rel;
     const int s = power32(__float_as_uint(peak));
     const uint32_t codes = codes_of<N>(low, two_to(s));
-    // (what is small enough to lose bits in 32 is taken again too)
-    const bool unsure = codes != codes_of<N>(high, two_to(s)) || !(peak + error < INFINITY) || (peak < 0x1p-100f && all != 0.f) ||
-                  power32(__float_as_uint(fmaxf(peak - error, 0.f))) != power32(__float_as_uint(peak + error));
     if (real) write(false, codes, s, false);
-    return !unsure;
+    // (what is small enough to lose bits in 32 is taken again too)
+    return codes == codes_of<N>(high, two_to(s)) && peak + error < INFINITY && !(peak < 0x1p-100f && all != 0.f) &&
+           power32(__float_as_uint(fmaxf(peak - error, 0.f))) == power32(__float_as_uint(peak + error));
   };
   // (All lanes stay in the loops: a wave votes, and lanes exchange. Those past the last head write nothing.)
   int again = heads;  // where heads begin that 32 bits are not enough for
   for (; h0 < heads; h0 += by, h += by) {
-    const bool more = h0 + by < heads;
     load_key(next, h + by);
     if constexpr (TURN == kPlain) {
       plain(key, false, h < heads);
