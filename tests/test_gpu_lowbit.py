@@ -386,6 +386,40 @@ def test_append_of_values_at_the_ends(torch_cuda):
 
 
 @pytest.mark.parametrize("dtype", [F16, BF16, F32])
+@pytest.mark.parametrize("dim,half,rotary,pad", [(64, False, 0, 0), (128, False, 40, 1), (128, True, 0, 0), (128, True, 40, 0),
+                                                 (64, True, 24, 3), (64, True, 64, 0)])
+def test_append_turns_many_heads_of_all_sizes(torch_cuda, dtype, dim, half, rotary, pad):
+    """Heads from the smallest to the largest, zeros, an infinity and a NaN,
+    several times a wave's four heads. A code may be another one only within
+    2^-32 of a border, as above (positions below 2^11: the angles of both sides
+    are off by less than 2^-40)."""
+    heads, rows = 9, 1100
+    g = torch.Generator().manual_seed(dim + rotary)
+    low, high = (-18, 10) if dtype == F16 else (-135, 121)
+    k = rand(5, rows, heads, dim + pad) * torch.exp2(torch.randint(low, high, (rows, heads, 1), generator=g).float())
+    k[torch.randint(0, 20, (rows, heads), generator=g) == 0] = 0
+    k[:, :, 32:][torch.randint(0, 9, (rows, heads), generator=g) == 0] = 0
+    k[4, 6, 1], k[9, 8, 33], k[11, 0, dim - 1] = math.inf, math.nan, -math.inf
+    k = k.to(dtype)
+    rope = ops.Rope(ops.rope_config(dim, rotary_dim=rotary, theta=1e4, layout=ops.ROPE_HALF if half else ops.ROPE_INTERLEAVED))
+    freq = ref.rope_frequencies(rotary or dim, 1e4, "none")
+    pages = Pages(heads, dim, 64, [rows])
+    dk, start = k.cuda(), starts([rows])
+    pages.cache.append(pages.pages, ops.cache4_rows(CODE[dtype], rows, start.data_ptr(), side(dk), side(dk)), rope, stream=stream())
+    out = torch.empty(2, rows, heads, dim, device="cuda")
+    pages.cache.read(pages.pages, ops.cache4_rows(ops.TYPE_F32, rows, start.data_ptr(), side(out[0]), side(out[1])),
+                     stream=stream())
+    torch.cuda.synchronize()
+    k = k[..., :dim].double()
+    for got, x in ((out[0], lref.turn(k, torch.arange(rows), freq, half)), (out[1], k)):
+        codes, scales, margin = lref.encode4(x)
+        want, got = lref.decode4(codes, scales), got.cpu().double()
+        assert torch.equal(torch.isnan(got), torch.isnan(want))
+        differ = (got != want) & ~torch.isnan(want)
+        assert not (differ & (margin > 2.0 ** -32)).any()
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
 @pytest.mark.parametrize("dim", [64, 128])
 def test_read_of_every_code_and_scale(torch_cuda, dtype, dim):
     """All bytes that a cache may hold, appended or not."""
