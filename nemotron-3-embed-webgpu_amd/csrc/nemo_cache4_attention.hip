@@ -103,7 +103,8 @@ template <>
 struct Mma16<half_t> {
   typedef half8v frag;
   typedef half2v pair;
-  static constexpr int kFinite = 140;  // largest scale byte with finite values
+  static constexpr int kFinite = 140;  // largest scale byte under which every code is finite
+  static constexpr uint32_t kExponent = 0x7c00, kOne = 0x3c00;
   static __device__ __forceinline__ float add(pair p, float sum) {
     return __builtin_amdgcn_fdot2(p, pair{(half_t)1.f, (half_t)1.f}, sum, false);
   }
@@ -120,6 +121,7 @@ struct Mma16<bf16_t> {
   typedef bf16_t frag __attribute__((ext_vector_type(8)));
   typedef bf16_t pair __attribute__((ext_vector_type(2)));
   static constexpr int kFinite = 252;
+  static constexpr uint32_t kExponent = 0x7f80, kOne = 0x3f80;
   static __device__ __forceinline__ float add(pair p, float sum) {
     return __builtin_amdgcn_fdot2_f32_bf16(p, pair{(bf16_t)1.f, (bf16_t)1.f}, sum, false);
   }
@@ -252,16 +254,71 @@ __device__ __forceinline__ uint32_t seen8(int j, const Seen& s, int sinks) {
   return below(s.hi) & (~below(s.lo) | below(sinks));
 }
 
+// Takes out of a block what its V holds that is not finite: the rows that see such a
+// value become NaN in its column, and its code is zero afterwards. Under a large scale
+// byte smaller codes are finite, but for byte 255.
+template <typename T, int D, int QT>
+__device__ __forceinline__ void take_out(Rows16<T, D, QT>& a, Raw<D>& raw, bool hide, const uint32_t (&seen)[QT],
+                                         uint32_t any) {
+  typedef Mma16<T> M;
+  typedef typename M::frag frag;
+  auto byte = [&](int e) { return (int)(raw.v_scales[e >> 2] >> (8 * (e & 3)) & 255); };
+  bool above = false;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) above |= byte(e) > M::kFinite && any >> e & 1;
+  if (!__builtin_amdgcn_ballot_w64(above)) return;
+  // Columns 2 b, 2 b + 1 of the lane's piece: byte b of a key's codes, D / 32 bytes.
+  auto columns = [&](auto at) {
+    constexpr int B = decltype(at)::value;
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      asm volatile("" : "+v"(raw.v_scales[0]), "+v"(raw.v_scales[1]));  // nothing is kept from one to the next
+      u32x4 bad = {0, 0, 0, 0};  // ones in the places of such values
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        constexpr int b[2] = {B, D == 128 ? B : B + 2};
+        const int word = D == 128 ? e & 3 : e >> 1 & 1;
+        const uint32_t codes = raw.v[e >> 2][word];
+        const uint32_t pair = e & 1 ? M::template decode<b[1]>(codes, power(raw.v_scales, e))
+                                    : M::template decode<b[0]>(codes, power(raw.v_scales, e));
+        if (!(any >> e & 1) || (pair >> (16 * half) & M::kExponent) != M::kExponent) continue;
+        bad[e >> 1] |= M::kOne << (16 * (e & 1));
+        raw.v[e >> 2][word] = codes & ~(15u << (8 * b[e & 1] + 4 * half));
+      }
+#pragma unroll
+      for (int i = 0; i < QT; ++i) {
+        frag sees;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sees[e] = (T)(!hide || (seen[i] >> e & 1) ? 1.f : 0.f);
+        const float4v n = M::mma(__builtin_bit_cast(frag, bad), sees, float4v{0.f, 0.f, 0.f, 0.f});
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (n[e] > 0.f) a.o[i][2 * B + half][e] = __uint_as_float(0x7fc00000u);
+      }
+    }
+  };
+  columns(std::integral_constant<int, 0>{});
+  columns(std::integral_constant<int, 1>{});
+  if constexpr (D == 128) {
+    columns(std::integral_constant<int, 2>{});
+    columns(std::integral_constant<int, 3>{});
+  }
+#pragma unroll
+  for (int e = 0; e < 8; ++e)
+    if (byte(e) == 255) raw.v_scales[e >> 2] &= ~(255u << (8 * (e & 3)));
+}
+
 // One block of 32 keys from key j0 on. `hide`: not every row sees all of them;
-// `seen`: what its lane's rows see. CAREFUL: values that are not finite are met
-// one by one, those of keys that a row does not see left out.
+// `seen`: what its lane's rows see, `any`: what some row of the tile sees. CAREFUL: V's values
+// that are not finite are taken out first and reach the rows that see them alone.
 template <bool CAREFUL, typename T, int D, int QT>
-__device__ __forceinline__ void attend(Rows16<T, D, QT>& a, const Raw<D>& raw, float scale2, bool hide,
+__device__ __forceinline__ void attend(Rows16<T, D, QT>& a, Raw<D>& raw, float scale2, bool hide,
                                        const uint32_t (&seen)[QT], uint32_t any) {
   constexpr int W = D / 32;
   typedef Mma16<T> M;
   typedef typename M::frag frag;
   const int lane = threadIdx.x & 63;
+  if constexpr (CAREFUL) take_out(a, raw, hide, seen, any);
   float4v s[QT][2];
   const float powers[2] = {__uint_as_float((raw.k_scales[0] >> (8 * (lane & 3))) << 23),
                            __uint_as_float((raw.k_scales[1] >> (8 * (lane & 3))) << 23)};
@@ -304,29 +361,6 @@ __device__ __forceinline__ void attend(Rows16<T, D, QT>& a, const Raw<D>& raw, f
       for (int e = 0; e < 8; ++e) v[e] = seen[i] >> e & 1 ? v[e] : -INFINITY;
     }
     a.settle(i, v, scale2, p[i]);
-  }
-  if constexpr (CAREFUL) {
-    // values that are not finite: their place holds 2^-127, and the rows that see
-    // one become NaN in its 32 columns
-    frag bad;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const uint32_t byte = scales[e >> 2] >> (8 * (e & 3)) & 255;
-      bad[e] = (T)(byte > M::kFinite ? 1.f : 0.f);
-      if (byte > M::kFinite) scales[e >> 2] &= ~(255u << (8 * (e & 3)));
-    }
-#pragma unroll
-    for (int i = 0; i < QT; ++i) {
-      frag sees;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) sees[e] = (T)(!hide || (seen[i] >> e & 1) ? 1.f : 0.f);
-      const float4v n = M::mma(bad, sees, float4v{0.f, 0.f, 0.f, 0.f});
-#pragma unroll
-      for (int t = 0; t < D / 16; ++t)
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (n[e] > 0.f) a.o[i][t][e] = __uint_as_float(0x7fc00000u);
-    }
   }
   // V: columns 2 b, 2 b + 1 of the lane's piece, for each of its 8 keys in one register
   float power[8];
@@ -387,7 +421,7 @@ __device__ __forceinline__ void attend_blocks(const AttendArgs& a, Rows16<T, D, 
     raw.load(a.c.data + a.c.head<D>(max(page, 0), kvh), a.c.shift, (block_of(n) & ((1 << per) - 1)) << 5, lane);
     return page >= 0;
   };
-  auto step = [&](const Raw<D>& raw, int n) {
+  auto step = [&](Raw<D>& raw, int n) {
     const int j0 = block_of(n) << 5;
     const bool hide = j0 + 32 > first.hi || (j0 < last.lo && j0 + 32 > a.sinks);
     uint32_t seen[QT] = {}, any = 255;
