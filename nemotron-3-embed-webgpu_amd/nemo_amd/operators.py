@@ -228,8 +228,11 @@ class Cache4:
         self._attention = _lib.load().nemo_cache4_attention
 
     def append(self, pages: Cache4Pages, rows: Cache4Rows, rope: Rope | None = None, stream: int = 0) -> None:
-        """Write the rows of requests' last tokens, keys turned by ``rope``."""
-        check(self._append(self.ctx.ptr, self.config, pages, rows, rope._ptr if rope else None, stream))
+        """Write the rows of requests' last tokens, keys turned by ``rope``
+        (None: as they are)."""
+        if rope is not None and not rope._ptr:  # (to the library it would be none)
+            raise _lib.NemoError(1, "rope was destroyed")
+        check(self._append(self.ctx.ptr, self.config, pages, rows, rope._ptr if rope is not None else None, stream))
 
     def read(self, pages: Cache4Pages, rows: Cache4Rows, stream: int = 0) -> None:
         """The values of requests' last tokens into rows."""

@@ -58,3 +58,28 @@ for heads, kv, dim in ((1, 1, 64), (32, 8, 128), (1024, 1, 64), (1024, 1024, 128
                 assert most_threads.value < 1 << 32, (heads, kv, dim, count, max_kv, rows, most_threads.value)
 print("ok")
 """)
+
+
+def test_a_destroyed_rope_does_not_append_keys_as_they_are(on_host):  # noqa: F811
+    """Without a rope keys go in unturned; one that is no longer there is refused, and
+    nothing is launched."""
+    on_host("""
+A = 1 << 40
+cache = ops.Cache4(ops.cache4_config(2, 64, 32))
+pages = ops.cache4_pages(1, 1, A, A, 1, A)
+rows = ops.cache4_rows(ops.TYPE_F16, 1, A, (A, 128, 64), (A, 128, 64))
+rope = ops.Rope(ops.rope_config(64))
+cache.append(pages, rows, rope)
+cache.append(pages, rows)
+rope.destroy()
+before = launches.value
+for call in (lambda: cache.append(pages, rows, rope), lambda: cache.append(pages, rows, rope=rope)):
+    try:
+        call()
+    except rt.NemoError as e:
+        assert "destroyed" in str(e), e
+    else:
+        raise AssertionError("appended")
+assert launches.value == before
+print("ok")
+""")
