@@ -297,6 +297,38 @@ def test_a_table_past_4_gib(gigabytes, queries):
     check(out, held, q, q_lens)
 
 
+# ---- many requests ---------------------------------------------------------------------
+
+def test_more_requests_than_two_searches_find(torch_cuda):
+    """5000 requests, empty ones among them and rows that are nobody's at both ends: a wave
+    looks at 64 at a time, here three times."""
+    g = torch.Generator().manual_seed(3)
+    count, dim, before = 5000, 64, 3
+    kv_lens = torch.randint(0, 40, (count,), generator=g).tolist()
+    q_lens = [min(n, m) for n, m in zip(torch.randint(0, 3, (count,), generator=g).tolist(), kv_lens)]
+    pages = Pages(1, dim, 32, kv_lens)
+    tokens, queries = sum(kv_lens), sum(q_lens)
+    starts_of = [torch.cat([torch.zeros(1, dtype=torch.int64), torch.tensor(n).cumsum(0)]) + before for n in (kv_lens, q_lens)]
+    starts_on = [t.int().cuda() for t in starts_of]
+    x = rand(4, 2, tokens + 2 * before, 1, dim, dtype=F16)
+    dx, back = x.cuda(), torch.full((2, tokens + 2 * before, 1, dim), 7.0, device="cuda")
+    for call, kind, t in ((pages.cache.append, ops.TYPE_F16, dx), (pages.cache.read, ops.TYPE_F32, back)):
+        call(pages.pages, ops.cache4_rows(kind, tokens + 2 * before, starts_on[0].data_ptr(), side(t[0]), side(t[1])),
+             stream=stream())
+    q = rand(5, queries + 2 * before, 2, dim, dtype=F16)
+    out = torch.full(q.shape, 7.0, dtype=F16, device="cuda")
+    attend(pages, q, None, out=out, start=starts_on[1])
+    out, back = out.cpu(), back.cpu()
+    for t in (out.unsqueeze(0), back):
+        assert (t[:, :before] == 7.0).all() and (t[:, -before:] == 7.0).all()
+    for b in [0, 1, 2, count - 2, count - 1] + torch.randperm(count, generator=g)[:200].tolist():
+        (k0, k1), (q0, q1) = (t[b:b + 2].tolist() for t in starts_of)
+        codes, scales, _ = lref.encode4(x[:, k0:k1].double())
+        held = lref.decode4(codes, scales)
+        assert torch.equal(back[:, k0:k1].double(), held)
+        check(out[q0:q1], [(held[0], held[1])], q[q0:q1], [q1 - q0])
+
+
 # ---- hints and streams -----------------------------------------------------------------
 
 @pytest.mark.parametrize("dim,kv,group,q_lens,kv_lens,max_kv", [
