@@ -102,6 +102,28 @@ def test_large_values_beside_a_row_that_is_not_finite(torch_cuda, dtype, dim, kv
     close(torch.where(few, want.to(dtype), out), want, tol)
 
 
+# ---- norms of heads --------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("d", [64, 1024])
+@pytest.mark.parametrize("power", [-55, 0, 58])
+def test_norms_of_small_and_large_heads(torch_cuda, dtype, d, power):
+    """Largest values from 2^-55, without an epsilon, to below 2^59."""
+    rows, heads = 5, 3
+    x = (torch.rand(rows, heads, d, generator=torch.Generator().manual_seed(power + 60)) * 1.8 - 0.9)
+    x[..., 7], x[0] = 1.0, 1.9375
+    x = (x.double() * 2.0 ** power).to(dtype)
+    w = 1 + rand(2, d) / 4
+    dx, dw = x.cuda(), w.cuda()
+    out = torch.empty_like(dx)
+    rope = ops.Rope(ops.rope_config(d, theta=1e4))
+    rope.norm_apply(CODE[dtype], ops.rope_heads(dx.data_ptr(), out.data_ptr(), heads, d), None,
+                    ops.head_norm(dw.data_ptr(), epsilon=0.0), rows, stream=stream())
+    torch.cuda.synchronize()
+    y, tol = lref.head_norm(x, w, 0.0, torch.arange(rows), ref.rope_frequencies(d, 1e4), False, 1.0)
+    close(out, y, tol + ref.HALF[dtype] * y.abs() + ref.TINY[dtype])
+
+
 # ---- pages -----------------------------------------------------------------------------
 
 @pytest.mark.parametrize("dtype,dim", [(F16, 64), (BF16, 128), (F32, 128)])

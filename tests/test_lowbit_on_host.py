@@ -83,3 +83,11 @@ for call in (lambda: cache.append(pages, rows, rope), lambda: cache.append(pages
 assert launches.value == before
 print("ok")
 """)
+
+
+def test_page_bytes_of_a_cache(on_host):  # noqa: F811
+    on_host("""
+for heads, dim, page, want in ((1, 64, 32, 32 * 68), (8, 128, 64, 8 * 64 * 136), (1024, 128, 1024, 1024 * 1024 * 136)):
+    assert ops.Cache4(ops.cache4_config(heads, dim, page)).page_bytes == want
+print("ok")
+""")
