@@ -437,7 +437,9 @@ nemo_status nemo_plan_token_states8(nemo_plan* plan, int32_t type8, int32_t grou
 /* RMSNorm of each query and key head, then its rotation, in one pass:
  *   h = x / sqrt(mean over the head of x^2 + epsilon) * weight,  y = h turned
  * by nemo_rope_apply's angles (values that it copies are normed only), in 32
- * bits with one rounding at the end. Head h's weight begins at
+ * bits, the sum of squares too (a head whose largest value is 2^59 or more, or below
+ * 2^-55 with an epsilon of 0, is not normed rightly), with one rounding at the
+ * end. Head h's weight begins at
  * weight + h weight_head; 0: one weight for all heads. */
 typedef struct nemo_head_norm {
   const float* q_weight;       /* [head_dim] each; NULL: 1 */
@@ -452,9 +454,9 @@ nemo_status nemo_rope_norm_apply(nemo_rope* rope, int32_t type, const nemo_rope_
 /* Products of 8-bit rows, as nemo_rmsnorm writes them with group 0, and 8-bit
  * weights with a scale for each output channel:
  *   y[i][j] = type(x_scale[i] w_scale[j] (sum over k of x[i][k] w[j][k]) + bias[j])
- * The sum is exact (32-bit integers); it is rounded to 32 bits, scaled by
- * x_scale, then by w_scale, and the bias is added, in 32 bits. k 0 leaves the
- * bias. x and w are 16-byte aligned, their row strides multiples of 16 and at
+ * The sum is exact (32-bit integers); it is rounded to 32 bits and scaled by
+ * x_scale; w_scale's product and the bias's addition round once, in 32 bits. k 0
+ * leaves the bias. x and w are 16-byte aligned, their row strides multiples of 16 and at
  * least k (for more than one row); bytes of a row behind k may hold anything.
  * y overlaps no other buffer. */
 typedef struct nemo_matmul8_args {
@@ -521,9 +523,11 @@ typedef struct nemo_cache4_rows {
 /* Append rows to a cache: keys are turned by `rope` (NULL: as they are; its
  * head_dim is the cache's), keys and values rounded to 4 bits: the smallest
  * power of two 2^s with max |x| <= 7 2^s, s in [-126, 125], and the nearest
- * code, to an even one on ties, up to 6. All of it is computed in 64 bits, so
- * a code is that of the exact value. 32 values with a NaN or an infinity
- * become NaN. k and v are only read. Rows of a call that share a page write
+ * code, to an even one on ties, up to 6. Values as they are get the code of the
+ * exact value, turned ones that of their rotation in 64 bits (in 32 where a bound on
+ * its error shows that to be the same): next to a border between two codes, where
+ * the angle's own rounding of about 2^-53 of it decides, the other may be taken. 32
+ * values with a NaN or an infinity become NaN. k and v are only read. Rows of a call that share a page write
  * bytes of their own. */
 nemo_status nemo_cache4_append(nemo_ctx* ctx, const nemo_cache4_config* config, const nemo_cache4_pages* pages,
                                const nemo_cache4_rows* rows, nemo_rope* rope, void* stream);
@@ -536,11 +540,13 @@ nemo_status nemo_cache4_read(nemo_ctx* ctx, const nemo_cache4_config* config, co
  * q_start[b] .. q_start[b + 1] - 1 of q and out, its keys the kv_len[b] tokens of
  * the cache, and what a query sees goes by nemo_attention_config, whose kv_heads
  * and head_dim are the cache's. Keys and values are read as `type`, exactly in
- * BF16, and in F16 from 2^-14 on and to 65504 (rows that see what lies above are
- * not finite). Softmax sums and
- * outputs are in 32 bits, the probabilities rounded to `type` for the product
- * with v. Keys and values that a query does not see reach its result in no
- * form, NaN neither. A request's rows are left as they were where it has none. */
+ * BF16, and in F16 from 2^-14 on and to 65504 (what lies above is an infinity; in
+ * v it makes its column of the rows that see it NaN). Softmax sums and outputs are in
+ * 32 bits, the probabilities rounded to `type` for the product with v; they are taken
+ * against a reference that may lie 2^15 below the largest, so the sums of BF16 values of
+ * 2^85 and more may overflow. Keys and values that a query does not see reach its result in no
+ * form, NaN neither. Rows of `out` that belong to no request are left as they
+ * were. `out` and the workspace overlap no other buffer. */
 typedef struct nemo_cache4_queries {
   int64_t q_rows;              /* rows of q and out, times q_heads at most 2^26 */
   int64_t max_kv;              /* the longest kv_len, or more: a hint for the split of the keys over the chip */

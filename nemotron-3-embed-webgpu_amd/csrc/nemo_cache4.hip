@@ -10,8 +10,10 @@
 // or powers differ the wave takes the token's rotation again in 64 bits, behind the
 // others: beside them it held registers for all, and its sines were taken by all.
 //
-// Appending is bound by its instructions, half of the cycles, and by memory: 31846
-// tokens of 8 KV heads of 128 f16, 165 MB of rows and codes, 45 us (3.7 TB/s), and 31
+// Appending is bound by a wave's chain of loads before its first write (the requests'
+// bounds, the table's page, while the first rows come) and between its turns: a wave
+// waits for 63 % of its cycles, and the vector units work for half. 31846
+// tokens of 8 KV heads of 128 f16, 165 MB of rows and codes, take 45 us (3.7 TB/s), and 31
 // (5.3 TB/s) to read. On the way: in 64 bits throughout 103; bounds in 32 bits, the rare
 // path among them 52; values to codes by one conversion, without a product 48; the
 // token looked up while its rows are on their way 45. (Several tokens a wave, which

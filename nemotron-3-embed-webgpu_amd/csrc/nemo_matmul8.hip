@@ -322,10 +322,12 @@ __global__ __launch_bounds__(64 * WM * WN) void matmul8_tile_kernel(nemo_matmul8
     for (int t = 0; t < NT; ++t) out.store(row_of(j), column(t), c[t][j], scales[j], columns[t]);
 }
 
-// A variant's tile, and its time in microseconds as a model of what 1 to 8192 rows,
-// 700 to 12288 columns and 100 to 8192 k took: `begin`, and `step` for each 128 k
+// A variant's tile, and its price, to be compared with the others': in microseconds of
+// what 33 sizes of 1 to 8192 rows, 700 to 12288 columns and 100 to 8192 k took: `begin`,
+// and `step` for each 128 k
 // and four times for the sums' way out, as often as its workgroups have to
-// follow each other on 256 CUs; `whole`: in whole rounds. Over 33 sizes the
+// follow each other on 256 CUs; `whole`: in whole rounds. (No time where all CUs work for
+// long and the clock falls: 8192 x 8192 x 8192 is priced at 317 and takes 455.) Over the 33 the
 // choice takes 1 % more than the fastest on average (few kernel of 16 x 16, 16 x 32,
 // 32 x 32, 32 x 64 : tiles of 64 x 64, 128 x 64, 256 x 128, 256 x 256; 1 x 2048 x
 // 6144 4.6, 5.7, 6.2, 8.2 : 11.6; 77 x 2048 x 6144 9.7, 9.0, 6.9, 9.4 : 12.3; 150 x 5120
