@@ -542,10 +542,9 @@ nemo_status nemo_cache4_read(nemo_ctx* ctx, const nemo_cache4_config* config, co
  * and head_dim are the cache's. Keys and values are read as `type`, exactly in
  * BF16, and in F16 from 2^-14 on and to 65504 (what lies above is an infinity; in
  * v it makes its column of the rows that see it NaN). Softmax sums and outputs are in
- * 32 bits, the probabilities rounded to `type` for the product with v; they are taken
- * against a reference that may lie 2^15 below the largest, so the sums of BF16 values of
- * 2^85 and more may overflow. Keys and values that a query does not see reach its result in no
- * form, NaN neither. Rows of `out` that belong to no request are left as they
+ * 32 bits, the probabilities rounded to `type` for the product with v. Keys and values
+ * that a query does not see, and other queries, reach its result in no form, NaN
+ * neither. Rows of `out` that belong to no request are left as they
  * were. `out` and the workspace overlap no other buffer. */
 typedef struct nemo_cache4_queries {
   int64_t q_rows;              /* rows of q and out, times q_heads at most 2^26 */

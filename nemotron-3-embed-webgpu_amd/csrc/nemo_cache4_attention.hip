@@ -199,8 +199,12 @@ struct Rows16 {
   // lane's 8 passes MOST, as in window attention: f16's largest is 2^BELOW and
   // more, so that what lies far below it keeps its share among f16's smallest
   // values.
+  //
+  // Sums of bf16's largest values leave 32 bits that way: a row whose sums do is
+  // taken again 2^42 lower, where the probabilities of 2^30 keys add up to 1 at
+  // most. Only such a row, since probabilities end 2^42 earlier too.
   static constexpr bool HALF = std::is_same<T, half_t>::value;
-  static constexpr float BELOW = HALF ? 8.f : 0.f, MOST = HALF ? 0x1p20f : 0x1p15f;
+  float low[QT];  // by how much in units of log2, CAREFUL
   static __device__ __forceinline__ float exponentials(const float (&s)[8], float scale2, float m, frag& p) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) p[i] = (T)__builtin_amdgcn_exp2f(fmaf(s[i], scale2, -m));
@@ -209,21 +213,24 @@ struct Rows16 {
     for (int i = 0; i < 8; i += 2) v = M::add(pair{p[i], p[i + 1]}, v);
     return v;
   }
+  template <bool CAREFUL>
   __device__ __forceinline__ void settle(int i, const float (&s)[8], float scale2, frag& p) {
+    const bool lower = CAREFUL && !HALF && low[i] > 0.f;
+    const float below = HALF ? 8.f : lower ? -low[i] : 0.f, most = HALF ? 0x1p20f : lower ? 0x1p-27f : 0x1p15f;
     float add = exponentials(s, scale2, m[i], p);
-    if (__builtin_amdgcn_ballot_w64(!(add <= MOST))) {
+    if (__builtin_amdgcn_ballot_w64(!(add <= most))) {
       asm volatile("");  // keeps the rare path a branch
       float top = s[0];
 #pragma unroll
       for (int r = 1; r < 8; ++r) top = fmaxf(top, s[r]);
       top *= scale2;
-      int raise = !(add <= MOST);
+      int raise = !(add <= most);
 #pragma unroll
       for (int x = 16; x < 64; x *= 2) {
         raise |= __shfl_xor(raise, x, 64);  // only the rows that ask: none depends on another
         top = fmaxf(top, __shfl_xor(top, x, 64));
       }
-      const float raised = raise ? fmaxf(m[i], top - BELOW) : m[i];
+      const float raised = raise ? fmaxf(m[i], top - below) : m[i];
       const float alpha = m[i] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[i] - raised);
       l[i] *= alpha;
 #pragma unroll
@@ -233,18 +240,22 @@ struct Rows16 {
     }
     l[i] += add;
   }
-  // Whether a value of the lane's rows is not finite.
-  __device__ __forceinline__ bool spoilt() const {
-    float z = 0.f;
+  // Whether a value of the wave's rows is not finite, and how much lower each row is taken
+  // again then.
+  __device__ __forceinline__ bool spoilt(int lane) {
+    uint64_t any = 0;
 #pragma unroll
     for (int i = 0; i < QT; ++i) {
-      z = fmaf(l[i], 0.f, z);
+      float z = l[i] * 0.f;
 #pragma unroll
       for (int t = 0; t < C; ++t)
 #pragma unroll
         for (int e = 0; e < 4; ++e) z = fmaf(o[i][t][e], 0.f, z);
+      const uint64_t lanes = __builtin_amdgcn_ballot_w64(z != 0.f);
+      low[i] = lanes >> (lane & 15) & 0x0001000100010001ull ? 42.f : 0.f;  // (a row's four)
+      any |= lanes;
     }
-    return z != 0.f;
+    return any != 0;
   }
 };
 
@@ -360,7 +371,7 @@ __device__ __forceinline__ void attend(Rows16<T, D, QT>& a, Raw<D>& raw, float s
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[e] = seen[i] >> e & 1 ? v[e] : -INFINITY;
     }
-    a.settle(i, v, scale2, p[i]);
+    a.template settle<CAREFUL>(i, v, scale2, p[i]);
   }
   // V: columns 2 b, 2 b + 1 of the lane's piece, for each of its 8 keys in one register
   float power[8];
@@ -447,6 +458,10 @@ __device__ __forceinline__ void attend_blocks(const AttendArgs& a, Rows16<T, D, 
   }
 }
 
+// Sums of waves and pieces, 64 at most, are joined as shares of 2^-kJoined and less, so
+// that finite ones add up to a finite one.
+constexpr float kJoined = 7.f;
+
 // Sums of a piece of a tile's keys: the rows' references and sums, and their
 // output values.
 struct Partials {
@@ -518,8 +533,7 @@ __global__ __launch_bounds__(64 * WAVES, QT == 1 ? 3 : 2) void cache4_attention_
   // (without pages there are no keys)
   const int from = block0 + wave, end = a.c.pages ? block1 : 0;
   attend_blocks<false>(a, acc, r, blocks, first, last, lo, hi, kvh, from, WAVES, end);
-  if (__builtin_amdgcn_ballot_w64(acc.spoilt()))
-    attend_blocks<true>(a, acc, r, blocks, first, last, lo, hi, kvh, from, WAVES, end);
+  if (acc.spoilt(lane)) attend_blocks<true>(a, acc, r, blocks, first, last, lo, hi, kvh, from, WAVES, end);
   // The waves' sums, 16 rows at a time.
   constexpr int THREADS = 64 * WAVES, PER = 16 * D / THREADS;  // columns of a thread
   static_assert(PER >= 4 && D % PER == 0, "whole vectors of one row");
@@ -541,6 +555,7 @@ __global__ __launch_bounds__(64 * WAVES, QT == 1 ? 3 : 2) void cache4_attention_
     float m = -INFINITY, l = 0.f, v[PER] = {};
 #pragma unroll
     for (int w = 0; w < WAVES; ++w) m = fmaxf(m, ml[w][row].x);
+    m += kJoined;
 #pragma unroll
     for (int w = 0; w < WAVES; ++w) {
       const float2 s = ml[w][row];
@@ -608,6 +623,7 @@ __global__ __launch_bounds__(256) void cache4_join_kernel(AttendArgs a, Partials
   float m = ml.x;
 #pragma unroll
   for (int x = 32; x > 0; x >>= 1) m = fmaxf(m, __shfl_xor(m, x, 64));
+  m += kJoined;
   const bool empty = ml.x == -INFINITY && ml.y == 0.f;  // saw nothing
   const float f = empty ? 0.f : ml.x == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(ml.x - m);
   float l = empty ? 0.f : f * ml.y;
@@ -645,11 +661,12 @@ __global__ __launch_bounds__(256) void cache4_join_kernel(AttendArgs a, Partials
 }
 
 // 16 rows from `begin` on over the blocks [block0, block1) of a tile's list, by one wave;
-// those whose bit of `mask` is set are written.
+// those whose bit of `mask` is set are written. `low`: what spoilt rows begin with.
 template <typename T, int D>
 __device__ __forceinline__ void careful_rows(const AttendArgs& a, const Partials& part, const Request& r,
                                              const Blocks& blocks, const Seen& first, const Seen& last, int kvh,
-                                             int begin, int rows, uint32_t mask, int block0, int block1, bool whole) {
+                                             int begin, int rows, uint32_t mask, int block0, int block1, bool whole,
+                                             float low) {
   constexpr int C = D / 16, W = D / 32;
   typedef typename Mma16<T>::frag frag;
   const int lane = threadIdx.x & 63, h = lane >> 4;
@@ -660,7 +677,12 @@ __device__ __forceinline__ void careful_rows(const AttendArgs& a, const Partials
   const T* q = (const T*)a.b.q + (int64_t)(r.q0 + query) * a.b.q_row + (int64_t)head * a.b.q_head + h * (D / 4);
 #pragma unroll
   for (int w = 0; w < W; ++w) acc.held[w] = *(const frag*)(q + 8 * w);
-  attend_blocks<true>(a, acc, r, blocks, first, last, lo, hi, kvh, block0, 1, a.c.pages ? block1 : 0);
+  acc.low[0] = low;
+  while (true) {
+    attend_blocks<true>(a, acc, r, blocks, first, last, lo, hi, kvh, block0, 1, a.c.pages ? block1 : 0);
+    if (acc.HALF || low > 0.f || !acc.spoilt(lane)) break;
+    low = 42.f;
+  }
   acc.l[0] += __shfl_xor(acc.l[0], 16, 64);
   acc.l[0] += __shfl_xor(acc.l[0], 32, 64);
   if (begin + (lane & 15) >= rows || !(mask >> (lane & 15) & 1)) return;
@@ -927,7 +949,8 @@ __global__ __launch_bounds__(256, 2) void cache4_tile_kernel(AttendArgs a, Parti
       const uint32_t mask = again >> (16 * i) & 0xffff;
       const int begin = w0 + 16 * i;
       if (mask && begin < rows)
-        careful_rows<T, D>(a, part, r, blocks, all_first, all_last, kvh, begin, rows, mask, block0, block1, whole);
+        careful_rows<T, D>(a, part, r, blocks, all_first, all_last, kvh, begin, rows, mask, block0, block1, whole,
+                           missing ? 0.f : 42.f);
     }
   }
 }

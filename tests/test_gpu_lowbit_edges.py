@@ -102,6 +102,44 @@ def test_large_values_beside_a_row_that_is_not_finite(torch_cuda, dtype, dim, kv
     close(torch.where(few, want.to(dtype), out), want, tol)
 
 
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("dim,kv,group,queries,keys,left", SHAPES)
+def test_a_nan_in_a_query_changes_no_other_row(torch_cuda, dtype, dim, kv, group, queries, keys, left):
+    """Not in one bit, also where probabilities are far below the largest."""
+    pages, _ = random_cache(keys + 1, [keys], kv, dim, 32)
+    q = 3 * rand(3, queries, kv * group, dim).to(dtype)
+    clean, _ = attend(pages, q, [queries], left, 0, 2)
+    q[queries // 2, 0, 5] = math.nan
+    out, _ = attend(pages, q, [queries], left, 0, 2)
+    assert torch.isnan(out[queries // 2, 0]).all()
+    out[queries // 2, 0] = clean[queries // 2, 0]
+    assert torch.isfinite(clean.float()).all() and torch.equal(out, clean)
+
+
+@pytest.mark.parametrize("dim,kv,group,queries,keys,left", SHAPES)
+def test_the_largest_values(torch_cuda, dim, kv, group, queries, keys, left):
+    """Every value of bf16's last two powers of two, all of one sign in half of the
+    columns: each result is finite, the sums in front of the division are far above
+    what 32 bits hold. (A lane's 8 keys, a wave's, and those of waves and pieces.)"""
+    g = torch.Generator().manual_seed(keys)
+    kc = torch.randint(0, 16, (keys, kv, dim), generator=g).to(torch.uint8)
+    ks = torch.randint(118, 122, (keys, kv, dim // 32), generator=g).to(torch.uint8)
+    vs = torch.randint(253, 255, (keys, kv, dim // 32), generator=g).to(torch.uint8)
+    most = torch.where(vs == 253, largest_code(BF16, 253), largest_code(BF16, 254)).repeat_interleave(32, -1)
+    vc = (torch.rand(keys, kv, dim, generator=g) * (most + 1)).floor().long()
+    vc = torch.where(torch.arange(dim) % 2 == 0, most, vc + 8 * torch.randint(0, 2, vc.shape, generator=g)).to(torch.uint8)
+    pages = Pages(kv, dim, 32, [keys])
+    pages.put(0, kc, ks, vc, vs)
+    some = sorted({0, kv - 1})
+    k, v = lref.decode4(kc[:, some], ks[:, some]), lref.decode4(vc[:, some], vs[:, some])
+    q = (rand(3, queries, kv * group, dim) / 64).to(BF16)
+    heads = [h * group + i for h in some for i in range(group)]
+    out, need = attend(pages, q, [queries], left, 0, 2)
+    assert (need > 0) == (keys > 4000)
+    want, tol = ref.attention(q[:, heads], k, v, left, 0, 2, dim ** -0.5)
+    close(out[:, heads], want, tol + ref.HALF[BF16] * want.abs())  # (the sum's rounding, as above)
+
+
 # ---- norms of heads --------------------------------------------------------------------
 
 @pytest.mark.parametrize("dtype", [BF16, F32])
