@@ -709,7 +709,7 @@ __device__ __forceinline__ void careful_rows(const AttendArgs& a, const Partials
 //
 // Bound by no unit alone: MFMAs take 45 % of the cycles, vector instructions 44, LDS 39,
 // and two waves a SIMD (its registers and images leave no third) do not cover one another,
-// which wait for 36 % of their cycles to issue. 2048 queries of 32 heads of 128
+// which wait for a third of their cycles to issue. 2048 queries of 32 heads of 128
 // behind 16000 keys (8 KV heads) and three small requests, 575 GFLOP, take 534 to 574 us by
 // the card, 1.0 PFLOP/s. Waves that decode all keys for
 // 64 rows of their own, without LDS, took 775: decoding is then half of their
